@@ -1,0 +1,732 @@
+// Selective state space scan, forward and backward.
+//
+// Per sequence and channel, N states with decays that depend on the input:
+// h[t][n] = exp(step[t] A[n]) h[t-1][n] + step[t] x[t] B[t][n], y = C.h.  Four
+// neighbouring lanes share a channel and hold N/4 states each (padded: A = B =
+// C = 0), so a wave has 16 channels and a workgroup of four waves 64.  The
+// four lanes take four frames at a time: each evaluates softplus, gate and
+// loads of one of the four, and the others read its step by a quad
+// permutation; y is summed over the quad the same way.  B and C, which all
+// channels share, go through LDS.  What bounds it is the vector unit: per
+// (frame, channel, state) one exponential (quarter rate) and four fp32
+// operations forward, about four times that backward.
+//
+// Where the sequences and channels alone do not fill the chip, time is cut
+// into chunks: the chunks' end states from zero and their summed steps (which
+// give the decay over a chunk, exp(A sum step)), then the states that enter
+// each chunk, then the chunks again from those.  The adjoint g[t] = C[t] dy[t] +
+// exp(step[t+1] A) g[t+1] is cut in the same way.
+//
+// The backward pass first runs a chunk forward and stores the state before
+// every tile of 16 frames, then takes the tiles from the last: a tile's
+// states and decays are formed again in registers, and the adjoint steps down
+// through them.  Sums over channels (gradients of B and C) go over the wave's
+// 16 channels in registers, over the four waves in LDS, and over workgroups in
+// a fixed order afterwards; no atomics.
+#include "seq.h"
+
+namespace dgen {
+
+namespace {
+
+constexpr int kWaves = 4, kThreads = 64 * kWaves, kChannels = 16 * kWaves;
+constexpr int kTile = 32;  // frames staged at a time, forward
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Frames of a backward tile: its states and decays are 2 S registers a frame.
+template <int S>
+constexpr int bwd_tile() { return S <= 4 ? 16 : 64 / S; }
+
+template <class E>
+struct Rows {  // [batch][time][.], contiguous last axis
+  E* p;
+  int64_t b, t;
+};
+
+template <class E>
+struct ScanP {
+  Rows<const E> x, dt, z, B, C, dy;
+  Rows<E> y, dx, ddt, dz;
+  const float *A, *skip, *bias, *state;
+  const int32_t* lengths;
+  float* state_out;
+  int64_t T, D, N, chunk, chunks, nd;  // nd: blocks of 64 channels
+  float* sums;                         // [batch][chunks][D]: summed steps
+  float* ends;                         // [batch][chunks][D][NP]: end states, then the states entering
+  float* gends;                        // the same of the adjoint
+  float* ckpt;                         // [batch][tiles][D][NP]: states before each backward tile
+  float* shared;                       // [nd][batch][T][2 N]: dB | dC per block of channels
+  float* parts;                        // [batch chunks][D (N + 2)]: dA | dskip | ddt_bias
+  int64_t batch;
+};
+
+__device__ __forceinline__ int64_t live_of(const int32_t* __restrict__ lengths, int64_t b, int64_t T) {
+  if (!lengths) return T;
+  const int64_t n = lengths[b];
+  return n < 0 ? 0 : n < T ? n : T;
+}
+
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
+// The value that lane J of each quad holds.
+template <int J>
+__device__ __forceinline__ float quad(float v) { return dpp<J * 0x55>(v); }
+// Sum over the quad, in every lane of it.
+__device__ __forceinline__ float quad_sum(float v) {
+  v += dpp<0xB1>(v);
+  return v + dpp<0x4E>(v);
+}
+
+template <int S>
+__device__ __forceinline__ void read_states(const float* __restrict__ p, float (&o)[S]) {
+  if constexpr (S % 4 == 0) {
+#pragma unroll
+    for (int s = 0; s < S; s += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(p + s);
+      o[s] = v.x, o[s + 1] = v.y, o[s + 2] = v.z, o[s + 3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int s = 0; s < S; ++s) o[s] = p[s];
+  }
+}
+
+template <int S>
+__device__ __forceinline__ void write_states(float* __restrict__ p, const float (&v)[S]) {
+  if constexpr (S % 4 == 0) {
+#pragma unroll
+    for (int s = 0; s < S; s += 4) *reinterpret_cast<float4*>(p + s) = make_float4(v[s], v[s + 1], v[s + 2], v[s + 3]);
+  } else {
+#pragma unroll
+    for (int s = 0; s < S; ++s) p[s] = v[s];
+  }
+}
+
+// A workgroup's place: channel block, chunk, sequence.
+struct Place {
+  int64_t b, c, d;
+  int lane, wave, q;
+  bool on;
+  int64_t begin, end, live;  // the chunk's frames, and how far they are inside the sequence
+};
+template <class E>
+__device__ __forceinline__ Place place_of(const ScanP<E>& p) {
+  Place w;
+  const uint32_t nd = (uint32_t)p.nd, nc = (uint32_t)p.chunks, i = blockIdx.x / nd;
+  w.lane = threadIdx.x & 63;
+  w.wave = threadIdx.x >> 6;
+  w.q = w.lane & 3;
+  w.d = (int64_t)(blockIdx.x % nd) * kChannels + w.wave * 16 + (w.lane >> 2);
+  w.on = w.d < p.D;
+  w.c = i % nc;
+  w.b = i / nc;
+  w.begin = w.c * p.chunk;
+  w.end = w.begin + p.chunk < p.T ? w.begin + p.chunk : p.T;
+  const int64_t n = live_of(p.lengths, w.b, p.T);
+  w.live = n < w.end ? n : w.end;
+  return w;
+}
+
+// The tile's rows of B and C that a thread carries from memory to LDS:
+// element i + 256 k of [FRAMES][2][NP].
+template <class E, int FRAMES, int NP>
+struct Shared {
+  static constexpr int K = (FRAMES * 2 * NP + kThreads - 1) / kThreads;
+  float v[K];
+  __device__ __forceinline__ void load(const ScanP<E>& p, const Place& w, int64_t t0, int frames) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int i = threadIdx.x + k * kThreads, row = i / (2 * NP), col = i % (2 * NP), n = col % NP;
+      const int64_t t = t0 + row;
+      v[k] = 0.f;
+      if (row < frames && t < w.live && n < p.N) {
+        const Rows<const E>& m = col < NP ? p.B : p.C;
+        v[k] = to_f32(m.p[w.b * m.b + t * m.t + n]);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(float* lds) const {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int i = threadIdx.x + k * kThreads;
+      if (i < FRAMES * 2 * NP) lds[i] = v[k];
+    }
+  }
+};
+
+// One lane's frames of a tile: frame 4 g + q of the tile for g < G.
+template <class E, int G>
+__device__ __forceinline__ void load_frames(const Rows<const E>& m, const Place& w, int64_t t0, float (&o)[G]) {
+  const E* p = m.p + w.b * m.b + w.d;
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    const int64_t t = t0 + 4 * g + w.q;
+    o[g] = w.on && t < w.live ? to_f32(p[t * m.t]) : 0.f;
+  }
+}
+
+enum Mode { kWhole, kSummary, kReplay, kSummaryBoth };
+
+// Forward: kWhole (one chunk: state to state_out), kReplay (from the state
+// that enters the chunk); kSummary: end state from zero and summed steps;
+// kSummaryBoth: the adjoint's too, accumulated forwards with the running
+// product of decays.
+template <class E, int S, int MODE>
+__global__ __launch_bounds__(kThreads) void k_scan(ScanP<E> p) {
+  constexpr int NP = 4 * S, G = kTile / 4;
+  constexpr bool OUT = MODE == kWhole || MODE == kReplay, ADJ = MODE == kSummaryBoth;
+  __shared__ __align__(16) float bc[2][kTile * 2 * NP];
+  const Place w = place_of(p);
+  if (!OUT && w.begin >= w.live) return;  // a chunk past the sequence: the carry leaves it out
+
+  float h[S], a2[S], prod[S], adj[S];
+  const float bias = p.bias && w.on ? p.bias[w.d] : 0.f, skip = p.skip && w.on ? p.skip[w.d] : 0.f;
+  const int64_t at = ((w.b * p.chunks + w.c) * p.D + w.d) * NP + w.q * S;
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    const int n = w.q * S + s;
+    const bool real = w.on && n < p.N;
+    a2[s] = real ? p.A[w.d * p.N + n] * kLog2e : 0.f;
+    h[s] = 0.f;
+    if (MODE == kWhole && p.state && real) h[s] = p.state[(w.b * p.D + w.d) * p.N + n];
+    prod[s] = 1.f;
+    adj[s] = 0.f;
+  }
+  if (MODE == kReplay && w.on) read_states<S>(p.ends + at, h);
+
+  float sum = 0.f;
+  float x[G], dt[G], z[G], dy[G];
+  Shared<E, kTile, NP> bcv;
+  auto fetch = [&](int64_t t0) {
+    bcv.load(p, w, t0, kTile);
+    load_frames<E, G>(p.x, w, t0, x);
+    load_frames<E, G>(p.dt, w, t0, dt);
+    if ((OUT || ADJ) && p.z.p) load_frames<E, G>(p.z, w, t0, z);
+    if (ADJ) load_frames<E, G>(p.dy, w, t0, dy);
+  };
+  fetch(w.begin);
+  int buf = 0;
+  for (int64_t t0 = w.begin; t0 < w.live; t0 += kTile, buf ^= 1) {
+    float* lds = bc[buf];
+    bcv.store(lds);
+    float cx[G], cdt[G], cz[G], cdy[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) cx[g] = x[g], cdt[g] = dt[g], cz[g] = z[g], cdy[g] = dy[g];
+    __syncthreads();
+    if (t0 + kTile < w.live) fetch(t0 + kTile);
+    const int groups = (int)(w.live - t0 < kTile ? (w.live - t0 + 3) / 4 : G);
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      if (g >= groups) continue;
+      const int64_t t = t0 + 4 * g + w.q;
+      const bool ok = w.on && t < w.live;
+      float slope;
+      const float step = ok ? softplus_accurate(cdt[g] + bias, slope) : 0.f, u = step * cx[g];
+      float gate = 1.f, up = 0.f;
+      if ((OUT || ADJ) && p.z.p) gate = silu(cz[g]);
+      if (ADJ) up = cdy[g] * gate;
+      if (!OUT) sum += step;
+      float y = 0.f;
+      auto frame = [&](auto jc) {
+        constexpr int J = decltype(jc)::value;
+        const float sj = quad<J>(step), uj = quad<J>(u), dj = ADJ ? quad<J>(up) : 0.f;
+        const float* row = lds + (4 * g + J) * 2 * NP + w.q * S;
+        float bv[S], cv[S], yj = 0.f;
+        read_states<S>(row, bv);
+        if (OUT || ADJ) read_states<S>(row + NP, cv);
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+          const float a = __builtin_amdgcn_exp2f(sj * a2[s]);
+          h[s] = fmaf(a, h[s], uj * bv[s]);
+          if (OUT) yj = fmaf(cv[s], h[s], yj);
+          if (ADJ) {
+            prod[s] *= a;
+            adj[s] = fmaf(prod[s] * cv[s], dj, adj[s]);
+          }
+        }
+        if (OUT) {
+          yj = quad_sum(yj);
+          y = w.q == J ? yj : y;
+        }
+      };
+      frame(std::integral_constant<int, 0>{});
+      frame(std::integral_constant<int, 1>{});
+      frame(std::integral_constant<int, 2>{});
+      frame(std::integral_constant<int, 3>{});
+      if (OUT && ok) p.y.p[w.b * p.y.b + t * p.y.t + w.d] = from_f32<E>(fmaf(skip, cx[g], y) * gate);
+    }
+  }
+  if (!w.on) return;
+  if (OUT)
+    for (int64_t t = (w.live > w.begin ? w.live : w.begin) + w.q; t < w.end; t += 4)
+      p.y.p[w.b * p.y.b + t * p.y.t + w.d] = from_f32<E>(0.f);
+  if (MODE == kWhole && p.state_out) {
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+      if (w.q * S + s < p.N) p.state_out[(w.b * p.D + w.d) * p.N + w.q * S + s] = h[s];
+  }
+  if (!OUT) {
+    write_states<S>(p.ends + at, h);
+    if (ADJ) write_states<S>(p.gends + at, adj);
+    sum = quad_sum(sum);
+    if (w.q == 0) p.sums[(w.b * p.chunks + w.c) * p.D + w.d] = sum;
+  }
+}
+
+// States entering each chunk, in place of the chunks' end states (reverse:
+// the adjoints entering from the chunks after).  64 states a workgroup, 16
+// threads over the chunks: each joins its run of chunks, the runs are joined
+// in LDS, and each walks its run again.
+template <class E>
+__global__ __launch_bounds__(1024) void k_scan_carry(ScanP<E> p, float* ends, int np, bool reverse) {
+  __shared__ float rsum[16][65], rend[16][65];
+  const int col = threadIdx.x & 63, seg = threadIdx.x >> 6;
+  const int64_t per = p.D * np, blocks = (per + 63) / 64;
+  const int64_t b = blockIdx.x / blocks, j = (blockIdx.x % blocks) * 64 + col;
+  const bool on = j < per;
+  const int64_t d = on ? j / np : 0;
+  const int n = on ? (int)(j % np) : 0;
+  const bool real = on && n < p.N;
+  const float a2 = real ? p.A[d * p.N + n] * kLog2e : 0.f;
+  const int64_t live = live_of(p.lengths, b, p.T), used = (live + p.chunk - 1) / p.chunk;
+  const int64_t run = (p.chunks + 15) / 16, lo = seg * run, hi = lo + run < used ? lo + run : used;
+  float* e = ends + b * p.chunks * per + j;
+  const float* sm = p.sums + b * p.chunks * p.D + d;
+  auto chunk = [&](int64_t k) { return reverse ? used - 1 - k : k; };  // k-th in walking order
+  float sum = 0.f, end = 0.f;
+  if (on)
+#pragma unroll 8
+    for (int64_t k = lo; k < hi; ++k) {
+      const float s = sm[chunk(k) * p.D];
+      end = fmaf(__builtin_amdgcn_exp2f(s * a2), end, e[chunk(k) * per]);
+      sum += s;
+    }
+  rsum[seg][col] = sum;
+  rend[seg][col] = end;
+  float h = 0.f;
+  if (!reverse && real && p.state) h = p.state[(b * p.D + d) * p.N + n];
+  __syncthreads();
+  for (int k = 0; k < seg; ++k) h = fmaf(__builtin_amdgcn_exp2f(rsum[k][col] * a2), h, rend[k][col]);
+  if (!on) return;
+#pragma unroll 8
+  for (int64_t k = lo; k < hi; ++k) {
+    const float s = sm[chunk(k) * p.D], v = e[chunk(k) * per];
+    e[chunk(k) * per] = h;
+    h = fmaf(__builtin_amdgcn_exp2f(s * a2), h, v);
+  }
+  // the thread past the last run has the state after all chunks
+  if (!reverse && seg == 15 && real && p.state_out) p.state_out[(b * p.D + d) * p.N + n] = h;
+}
+
+// Sum over the wave's 16 channels (lane bits 2..5) of V values per lane, by
+// exchange: after the half-wave and row swaps a lane holds a quarter of the
+// values; those are summed over lane bits 2 and 3 by row rotations.  w[k] is
+// value index 4 k + 2 (lane bit 4) + (lane bit 5) (V = 2: lane bit 5).
+__device__ __forceinline__ float swap_add32(float a, float b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float swap_add16(float a, float b) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+template <int V>
+constexpr int kept() { return V >= 4 ? V / 4 : 1; }
+template <int V>
+__device__ __forceinline__ void channel_sum(const float (&v)[V], float (&w)[kept<V>()]) {
+  float r[V / 2];
+#pragma unroll
+  for (int i = 0; i < V / 2; ++i) r[i] = swap_add32(v[2 * i], v[2 * i + 1]);
+  if constexpr (V >= 4) {
+#pragma unroll
+    for (int k = 0; k < V / 4; ++k) w[k] = swap_add16(r[2 * k], r[2 * k + 1]);
+  } else {
+    w[0] = swap_add16(r[0], r[0]);
+  }
+#pragma unroll
+  for (int k = 0; k < kept<V>(); ++k) {
+    w[k] += dpp<0x124>(w[k]);  // row_ror:4
+    w[k] += dpp<0x128>(w[k]);  // row_ror:8
+  }
+}
+
+template <class E, int S>
+__global__ __launch_bounds__(kThreads) void k_scan_bwd(ScanP<E> p) {
+  constexpr int NP = 4 * S, TL = bwd_tile<S>(), G = TL / 4;
+  __shared__ __align__(16) float bc[2][TL * 2 * NP];
+  __shared__ float red[TL][kWaves][2 * NP];
+  const Place w = place_of(p);
+  const int64_t tiles_all = (p.T + TL - 1) / TL, tile0 = w.begin / TL;
+  const int64_t tiles = w.live > w.begin ? (w.live - w.begin + TL - 1) / TL : 0;
+
+  float h[S], a[S], g[S], dA[S];
+  const float bias = p.bias && w.on ? p.bias[w.d] : 0.f, skip = p.skip && w.on ? p.skip[w.d] : 0.f;
+  const int64_t at = ((w.b * p.chunks + w.c) * p.D + w.d) * NP + w.q * S;
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    const int n = w.q * S + s;
+    const bool real = w.on && n < p.N;
+    a[s] = real ? p.A[w.d * p.N + n] : 0.f;
+    h[s] = p.chunks == 1 && p.state && real ? p.state[(w.b * p.D + w.d) * p.N + n] : 0.f;
+    g[s] = 0.f;
+    dA[s] = 0.f;
+  }
+  if (p.chunks > 1 && tiles > 0 && w.on) {
+    read_states<S>(p.ends + at, h);
+    read_states<S>(p.gends + at, g);
+  }
+  float dskip = 0.f, dbias = 0.f;
+  float* ck = p.ckpt + ((w.b * tiles_all + tile0) * p.D + w.d) * NP + w.q * S;
+  Shared<E, TL, NP> bcv;
+
+  // forward over the chunk: the state before every tile
+  {
+    float x[G], dt[G];
+    auto fetch = [&](int64_t t0) {
+      bcv.load(p, w, t0, TL);
+      load_frames<E, G>(p.x, w, t0, x);
+      load_frames<E, G>(p.dt, w, t0, dt);
+    };
+    if (tiles > 0) fetch(w.begin);
+    for (int64_t i = 0; i < tiles; ++i) {
+      if (w.on) write_states<S>(ck + i * p.D * NP, h);
+      if (i + 1 == tiles) break;
+      float* lds = bc[i & 1];
+      bcv.store(lds);
+      float cx[G], cdt[G];
+#pragma unroll
+      for (int k = 0; k < G; ++k) cx[k] = x[k], cdt[k] = dt[k];
+      __syncthreads();
+      fetch(w.begin + (i + 1) * TL);
+#pragma unroll
+      for (int k = 0; k < G; ++k) {
+        float slope;
+        // (every frame of a tile that another follows is inside the sequence)
+        const float step = w.on ? softplus_accurate(cdt[k] + bias, slope) : 0.f, u = step * cx[k];
+        auto frame = [&](auto jc) {
+          constexpr int J = decltype(jc)::value;
+          const float sj = quad<J>(step) * kLog2e, uj = quad<J>(u);
+          float bv[S];
+          read_states<S>(lds + (4 * k + J) * 2 * NP + w.q * S, bv);
+#pragma unroll
+          for (int s = 0; s < S; ++s) h[s] = fmaf(__builtin_amdgcn_exp2f(sj * a[s]), h[s], uj * bv[s]);
+        };
+        frame(std::integral_constant<int, 0>{});
+        frame(std::integral_constant<int, 1>{});
+        frame(std::integral_constant<int, 2>{});
+        frame(std::integral_constant<int, 3>{});
+      }
+    }
+    __syncthreads();
+  }
+
+  float x[G], dt[G], z[G], dy[G], hn[S];
+  auto fetch = [&](int64_t i) {
+    const int64_t t0 = w.begin + i * TL;
+    bcv.load(p, w, t0, TL);
+    load_frames<E, G>(p.x, w, t0, x);
+    load_frames<E, G>(p.dt, w, t0, dt);
+    if (p.z.p) load_frames<E, G>(p.z, w, t0, z);
+    load_frames<E, G>(p.dy, w, t0, dy);
+    if (w.on) read_states<S>(ck + i * p.D * NP, hn);
+  };
+#pragma unroll
+  for (int s = 0; s < S; ++s) hn[s] = 0.f;
+  if (tiles > 0) fetch(tiles - 1);
+  for (int64_t i = tiles - 1; i >= 0; --i) {
+    const int64_t t0 = w.begin + i * TL;
+    float* lds = bc[i & 1];
+    bcv.store(lds);
+    float cx[G], cz[G], cdy[G], step[G], slope[G], u[G], up[G], y[G];
+#pragma unroll
+    for (int s = 0; s < S; ++s) h[s] = hn[s];
+#pragma unroll
+    for (int k = 0; k < G; ++k) {
+      const bool ok = w.on && t0 + 4 * k + w.q < w.live;
+      cx[k] = x[k], cz[k] = z[k], cdy[k] = dy[k];
+      step[k] = softplus_accurate(dt[k] + bias, slope[k]);
+      if (!ok) step[k] = slope[k] = 0.f;
+      u[k] = step[k] * cx[k];
+      up[k] = p.z.p ? cdy[k] * silu(cz[k]) : cdy[k];
+    }
+    __syncthreads();
+    if (i > 0) fetch(i - 1);
+
+    // the tile's states and decays
+    float hs[TL][S], as[TL][S];
+#pragma unroll
+    for (int k = 0; k < G; ++k) {
+      y[k] = 0.f;
+      auto frame = [&](auto jc) {
+        constexpr int J = decltype(jc)::value;
+        const float sj = quad<J>(step[k]) * kLog2e, uj = quad<J>(u[k]);
+        const float* row = lds + (4 * k + J) * 2 * NP + w.q * S;
+        float bv[S], cv[S], yj = 0.f;
+        read_states<S>(row, bv);
+        read_states<S>(row + NP, cv);
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+          const float e = __builtin_amdgcn_exp2f(sj * a[s]);
+          hs[4 * k + J][s] = h[s];
+          as[4 * k + J][s] = e;
+          h[s] = fmaf(e, h[s], uj * bv[s]);
+          yj = fmaf(cv[s], h[s], yj);
+        }
+        yj = quad_sum(yj);
+        y[k] = w.q == J ? yj : y[k];
+      };
+      frame(std::integral_constant<int, 0>{});
+      frame(std::integral_constant<int, 1>{});
+      frame(std::integral_constant<int, 2>{});
+      frame(std::integral_constant<int, 3>{});
+    }
+    // down through the tile: h is the state after the frame
+#pragma unroll
+    for (int k = G - 1; k >= 0; --k) {
+      float gb = 0.f, ga = 0.f;
+      auto frame = [&](auto jc) {
+        constexpr int J = decltype(jc)::value, F = 4 * 0 + J;
+        const int f = 4 * k + F;
+        const float sj = quad<J>(step[k]), uj = quad<J>(u[k]), dj = quad<J>(up[k]);
+        const float* row = lds + f * 2 * NP + w.q * S;
+        float bv[S], cv[S], v[2 * S], gbj = 0.f, gaj = 0.f;
+        read_states<S>(row, bv);
+        read_states<S>(row + NP, cv);
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+          g[s] = fmaf(cv[s], dj, g[s]);
+          v[s] = g[s] * uj;       // dB
+          v[S + s] = h[s] * dj;   // dC
+          gbj = fmaf(g[s], bv[s], gbj);
+          g[s] *= as[f][s];       // the adjoint of the state before
+          h[s] = hs[f][s];
+          const float gh = g[s] * h[s];
+          gaj = fmaf(gh, a[s], gaj);
+          dA[s] = fmaf(gh, sj, dA[s]);
+        }
+        gbj = quad_sum(gbj);
+        gaj = quad_sum(gaj);
+        gb = w.q == J ? gbj : gb;
+        ga = w.q == J ? gaj : ga;
+        float sums[kept<2 * S>()];
+        channel_sum<2 * S>(v, sums);
+        if ((w.lane & 12) == 0) {
+#pragma unroll
+          for (int m = 0; m < kept<2 * S>(); ++m) {
+            const int idx = S >= 2 ? 4 * m + 2 * ((w.lane >> 4) & 1) + (w.lane >> 5) : w.lane >> 5;
+            red[f][w.wave][(idx / S) * NP + w.q * S + idx % S] = sums[m];
+          }
+        }
+      };
+      frame(std::integral_constant<int, 3>{});
+      frame(std::integral_constant<int, 2>{});
+      frame(std::integral_constant<int, 1>{});
+      frame(std::integral_constant<int, 0>{});
+      const int64_t t = t0 + 4 * k + w.q;
+      if (w.on && t < w.live) {
+        const float draw = fmaf(gb, cx[k], ga) * slope[k];
+        dbias += draw;
+        dskip = fmaf(up[k], cx[k], dskip);
+        p.dx.p[w.b * p.dx.b + t * p.dx.t + w.d] = from_f32<E>(fmaf(step[k], gb, skip * up[k]));
+        p.ddt.p[w.b * p.ddt.b + t * p.ddt.t + w.d] = from_f32<E>(draw);
+        if (p.z.p)
+          p.dz.p[w.b * p.dz.b + t * p.dz.t + w.d] =
+              from_f32<E>(cdy[k] * fmaf(skip, cx[k], y[k]) * silu_grad(cz[k], sigmoid(cz[k])));
+      }
+    }
+    __syncthreads();
+    // dB | dC of the block's channels
+    float* out = p.shared + (((blockIdx.x % (uint32_t)p.nd) * p.batch + w.b) * p.T + t0) * 2 * p.N;
+    for (int o = threadIdx.x; o < TL * 2 * NP; o += kThreads) {
+      const int f = o / (2 * NP), col = o % (2 * NP), n = col % NP;
+      if (t0 + f < w.live && n < p.N) {
+        float t = 0.f;
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) t += red[f][k][col];
+        out[f * 2 * p.N + (col < NP ? 0 : p.N) + n] = t;
+      }
+    }
+  }
+  if (!w.on) return;
+  for (int64_t t = (w.live > w.begin ? w.live : w.begin) + w.q; t < w.end; t += 4) {
+    p.dx.p[w.b * p.dx.b + t * p.dx.t + w.d] = from_f32<E>(0.f);
+    p.ddt.p[w.b * p.ddt.b + t * p.ddt.t + w.d] = from_f32<E>(0.f);
+    if (p.z.p) p.dz.p[w.b * p.dz.b + t * p.dz.t + w.d] = from_f32<E>(0.f);
+  }
+  float* part = p.parts + (w.b * p.chunks + w.c) * p.D * (p.N + 2);
+#pragma unroll
+  for (int s = 0; s < S; ++s)
+    if (w.q * S + s < p.N) part[w.d * p.N + w.q * S + s] = dA[s];
+  dskip = quad_sum(dskip);
+  dbias = quad_sum(dbias);
+  if (w.q == 0) {
+    part[p.D * p.N + w.d] = dskip;
+    part[p.D * (p.N + 1) + w.d] = dbias;
+  }
+}
+
+// dB and dC: the channel blocks' sums added in order.
+template <class E>
+__global__ __launch_bounds__(256) void k_scan_shared(const float* __restrict__ shared, const int32_t* __restrict__ lengths,
+                                                     Rows<E> dB, Rows<E> dC, int64_t nd, int64_t batch, int64_t T,
+                                                     int64_t N) {
+  const int64_t total = batch * T * 2 * N, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= total) return;
+  const int64_t row = i / (2 * N), col = i - row * 2 * N, b = row / T, t = row - b * T;
+  float v = 0.f;
+  if (t < live_of(lengths, b, T))
+    for (int64_t k = 0; k < nd; ++k) v += shared[k * total + i];
+  const Rows<E>& m = col < N ? dB : dC;
+  m.p[b * m.b + t * m.t + (col < N ? col : col - N)] = from_f32<E>(v);
+}
+
+struct ScanShape {
+  int S;
+  int64_t NP, nd, chunk, chunks;
+  // workspace, in floats
+  int64_t sums, ends, ckpt, shared, parts, total;
+};
+
+// Chunks: as many as give every CU two workgroups (two waves a SIMD), none
+// shorter than 64 frames, and none where the sequences and channel blocks
+// come near that alone: a chunked pass evaluates every decay twice.
+constexpr int64_t kFill = 512, kFillAlone = 320, kMinChunk = 64, kMaxChunks = 512;
+
+ScanShape scan_shape(const dgen_hip_scan& a, bool backward) {
+  ScanShape s{};
+  s.S = a.N <= 4 ? 1 : a.N <= 8 ? 2 : a.N <= 16 ? 4 : a.N <= 32 ? 8 : 16;
+  s.NP = 4 * s.S;
+  s.nd = (a.D + kChannels - 1) / kChannels;
+  const int64_t blocks = std::max<int64_t>(1, a.batch * s.nd);
+  int64_t chunks = 1;
+  if (blocks < kFillAlone)
+    chunks = std::min({(kFill + blocks - 1) / blocks, (a.T + kMinChunk - 1) / kMinChunk, kMaxChunks});
+  s.chunk = (a.T + chunks - 1) / chunks;
+  s.chunk = (s.chunk + kTile - 1) / kTile * kTile;
+  s.chunks = (a.T + s.chunk - 1) / s.chunk;
+  const int64_t lanes = a.batch * a.D;
+  auto up = [](int64_t n) { return (n + 63) & ~int64_t(63); };
+  if (s.chunks > 1) {
+    s.sums = up(s.chunks * lanes);
+    s.ends = up(s.chunks * lanes * s.NP);
+  }
+  if (backward) {
+    const int64_t tl = s.S <= 4 ? 16 : 64 / s.S;
+    s.ckpt = up((a.T + tl - 1) / tl * lanes * s.NP);
+    s.shared = up(s.nd * a.batch * a.T * 2 * a.N);
+    s.parts = up(a.batch * s.chunks * a.D * (a.N + 2));
+  }
+  s.total = s.sums + s.ends * (backward ? 2 : 1) + s.ckpt + s.shared + s.parts;
+  return s;
+}
+
+template <class E>
+Rows<const E> in_rows(const dgen_hip_seq& v) { return {(const E*)v.data, v.stride_b, v.stride_t}; }
+template <class E>
+Rows<E> out_rows(const dgen_hip_seq& v) { return {(E*)v.data, v.stride_b, v.stride_t}; }
+
+template <class E, int S>
+void scan_launch(const dgen_hip_scan& a, bool backward, const ScanShape& s, hipStream_t st) {
+  float* ws = (float*)a.workspace;
+  ScanP<E> p{};
+  p.x = in_rows<E>(a.x), p.dt = in_rows<E>(a.dt), p.z = in_rows<E>(a.z), p.B = in_rows<E>(a.B), p.C = in_rows<E>(a.C);
+  p.A = a.A, p.skip = a.skip, p.bias = a.dt_bias, p.state = a.state, p.lengths = a.lengths;
+  p.T = a.T, p.D = a.D, p.N = a.N, p.chunk = s.chunk, p.chunks = s.chunks, p.nd = s.nd, p.batch = a.batch;
+  p.sums = ws, p.ends = p.sums + s.sums, p.gends = p.ends + s.ends;
+  if (!backward) p.y = out_rows<E>(a.y), p.state_out = a.state_out;
+  const dim3 grid((unsigned)(s.nd * s.chunks * a.batch));
+  const dim3 carry((unsigned)((a.D * s.NP + 63) / 64 * a.batch));
+  if (!backward) {
+    if (s.chunks == 1) {
+      k_scan<E, S, kWhole><<<grid, kThreads, 0, st>>>(p);
+    } else {
+      k_scan<E, S, kSummary><<<grid, kThreads, 0, st>>>(p);
+      k_scan_carry<E><<<carry, 1024, 0, st>>>(p, p.ends, (int)s.NP, false);
+      k_scan<E, S, kReplay><<<grid, kThreads, 0, st>>>(p);
+    }
+    return;
+  }
+  p.dy = in_rows<E>(a.dy), p.dx = out_rows<E>(a.dx), p.ddt = out_rows<E>(a.ddt), p.dz = out_rows<E>(a.dz);
+  p.ckpt = p.gends + s.ends, p.shared = p.ckpt + s.ckpt, p.parts = p.shared + s.shared;
+  if (s.chunks > 1) {
+    k_scan<E, S, kSummaryBoth><<<grid, kThreads, 0, st>>>(p);
+    k_scan_carry<E><<<carry, 1024, 0, st>>>(p, p.ends, (int)s.NP, false);
+    k_scan_carry<E><<<carry, 1024, 0, st>>>(p, p.gends, (int)s.NP, true);
+  }
+  k_scan_bwd<E, S><<<grid, kThreads, 0, st>>>(p);
+  k_scan_shared<E><<<dim3((unsigned)((a.batch * a.T * 2 * a.N + 255) / 256)), 256, 0, st>>>(
+      p.shared, a.lengths, out_rows<E>(a.dB), out_rows<E>(a.dC), s.nd, a.batch, a.T, a.N);
+  enqueue_sum_parts(st, p.parts, a.batch * s.chunks, {{a.dA, a.dskip, a.ddt_bias}, {a.D * a.N, a.D, a.D}});
+}
+
+template <class E>
+void scan_states(const dgen_hip_scan& a, bool backward, const ScanShape& s, hipStream_t st) {
+  switch (s.S) {
+    case 1: return scan_launch<E, 1>(a, backward, s, st);
+    case 2: return scan_launch<E, 2>(a, backward, s, st);
+    case 4: return scan_launch<E, 4>(a, backward, s, st);
+    case 8: return scan_launch<E, 8>(a, backward, s, st);
+    default: return scan_launch<E, 16>(a, backward, s, st);
+  }
+}
+
+}  // namespace
+
+int64_t scan_workspace(const dgen_hip_scan& a, bool backward) {
+  return align256(scan_shape(a, backward).total * (int64_t)sizeof(float));
+}
+
+int scan_run(const dgen_hip_scan& a, bool backward, hipStream_t st, bool dry) {
+  const char* what = backward ? "selective_scan_backward" : "selective_scan";
+  DGEN_REQUIRE(a.struct_size == sizeof(a), "%s: struct_size %u, expected %zu", what, a.struct_size, sizeof(a));
+  DGEN_REQUIRE(a.type == DGEN_HIP_F32 || a.type == DGEN_HIP_BF16, "%s: type %d", what, a.type);
+  DGEN_REQUIRE(a.N >= 1 && a.N <= 64, "%s: N %lld outside [1, 64]", what, (long long)a.N);
+  DGEN_REQUIRE(a.batch >= 0 && a.batch <= (1 << 20), "%s: batch %lld outside [0, 2^20]", what, (long long)a.batch);
+  DGEN_REQUIRE(a.T >= 1 && a.T <= (1 << 24), "%s: T %lld outside [1, 2^24]", what, (long long)a.T);
+  DGEN_REQUIRE(a.D >= 1 && a.D <= (1 << 20), "%s: D %lld outside [1, 2^20]", what, (long long)a.D);
+  const ScanShape s = scan_shape(a, backward);
+  // (a launch takes fewer than 2^32 threads)
+  DGEN_REQUIRE(s.nd * s.chunks * a.batch < (int64_t(1) << 23) && (a.D * s.NP + 63) / 64 * a.batch < (int64_t(1) << 21) &&
+                   (!backward || a.batch * a.T * 2 * a.N < (int64_t(1) << 31)),
+               "%s: batch %lld x T %lld x D %lld x N %lld is too large for one call", what, (long long)a.batch,
+               (long long)a.T, (long long)a.D, (long long)a.N);
+  DGEN_REQUIRE(a.A, "%s: null A", what);
+  const bool empty = a.batch == 0;
+  for (const dgen_hip_seq* v : {&a.x, &a.dt, &a.B, &a.C})
+    DGEN_REQUIRE((v->data || empty) && seq_readable(*v), "%s: x, dt, B or C missing or with a negative stride", what);
+  DGEN_REQUIRE(!a.z.data || seq_readable(a.z), "%s: z has a negative stride", what);
+  if (!backward) {
+    DGEN_REQUIRE((a.y.data || empty) && seq_writable(a.y, a.batch, a.T, a.D), "%s: y missing or overlapping itself",
+                 what);
+  } else {
+    DGEN_REQUIRE((a.dy.data || empty) && seq_readable(a.dy), "%s: dy missing or with a negative stride", what);
+    for (const dgen_hip_seq* v : {&a.dx, &a.ddt})
+      DGEN_REQUIRE((v->data || empty) && seq_writable(*v, a.batch, a.T, a.D),
+                   "%s: dx or ddt missing or overlapping itself", what);
+    for (const dgen_hip_seq* v : {&a.dB, &a.dC})
+      DGEN_REQUIRE((v->data || empty) && seq_writable(*v, a.batch, a.T, a.N),
+                   "%s: dB or dC missing or overlapping itself", what);
+    DGEN_REQUIRE(!a.z.data || (a.dz.data && seq_writable(a.dz, a.batch, a.T, a.D)),
+                 "%s: dz missing or overlapping itself", what);
+    DGEN_REQUIRE(a.dA && (!a.skip || a.dskip) && (!a.dt_bias || a.ddt_bias), "%s: null dA, dskip or ddt_bias", what);
+  }
+  const int64_t need = scan_workspace(a, backward);
+  DGEN_REQUIRE(need == 0 || (a.workspace && a.workspace_bytes >= (uint64_t)need && (uintptr_t)a.workspace % 256 == 0),
+               "%s: workspace of %llu bytes, %lld needed (256-byte aligned)", what,
+               (unsigned long long)a.workspace_bytes, (long long)need);
+  if (dry) return 0;
+  if (empty) {
+    if (!backward) return 0;
+    enqueue_sum_parts(st, a.A, 0, {{a.dA, a.dskip, a.ddt_bias}, {a.D * a.N, a.D, a.D}});  // zeros
+  } else if (a.type == DGEN_HIP_BF16) {
+    scan_states<bf16>(a, backward, s, st);
+  } else {
+    scan_states<float>(a, backward, s, st);
+  }
+  DGEN_LAUNCH_CHECK(what);
+  return 0;
+}
+
+}  // namespace dgen

@@ -70,6 +70,9 @@ KERNEL_NAMES = {v: k[2:].lower() for k, v in globals().items() if k.startswith("
 EPI_NONE, EPI_BIAS, EPI_BIAS_TANH, EPI_TANH_GRAD = 0, 1, 2, 3
 OP_STATIC, OP_SIDE, OP_JOIN, OP_FORK = 1, 2, 4, 8
 
+# the operators on device tensors (sequence.py)
+SEQUENCE_OPS = ("rms_norm", "causal_conv", "selective_scan", "gated_mlp")
+
 EXPORTED_SYMBOLS = (
     "dgen_hip_abi_version", "dgen_hip_device_count", "dgen_hip_create", "dgen_hip_destroy",
     "dgen_hip_last_error", "dgen_hip_configure", "dgen_hip_host_memory", "dgen_hip_upload",
@@ -79,7 +82,7 @@ EXPORTED_SYMBOLS = (
     "dgen_hip_host_outputs", "dgen_hip_set_sample_rate", "dgen_hip_biquad_forward_noalloc",
     "dgen_hip_set_process_ports", "dgen_hip_process_v1", "dgen_hip_process_bind", "dgen_hip_process_memory_size",
     "dgen_hip_set_blocks", "dgen_hip_render_blocks",
-)
+) + tuple(f"dgen_hip_{op}{entry}" for op in SEQUENCE_OPS for entry in ("", "_backward", "_workspace"))
 # the reference-named process-function exports (include/dgen_process_v1.h)
 PROCESS_V1_SYMBOLS = ("dgen_process_v1", "dgen_set_param_value_v1")
 DGEN_ABI_VERSION_V1 = 1
@@ -163,6 +166,9 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
         "dgen_hip_render_blocks": ([vp, u32, i32, ctypes.c_char_p, ctypes.c_size_t, ctypes.POINTER(ctypes.c_size_t)],
                                    i32),
     }
+    for op in SEQUENCE_OPS:
+        sig[f"dgen_hip_{op}"] = sig[f"dgen_hip_{op}_backward"] = ([i32, vp, vp], i32)
+        sig[f"dgen_hip_{op}_workspace"] = ([i32, vp, i32, ctypes.POINTER(u64)], i32)
     for name, (args, res) in sig.items():
         fn = getattr(L, name)
         fn.argtypes = args

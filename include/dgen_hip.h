@@ -804,6 +804,164 @@ int dgen_hip_time_op_alone(dgen_hip_ctx* ctx, uint32_t frame_count, uint32_t op_
 int dgen_hip_biquad_forward_noalloc(int device, const float* x, const float* mod, const float* params, float* y,
                                     uint32_t B, uint32_t T, uint32_t chunk, void* stream);
 
+/* ---- sequence operators on device tensors ----------------------------------
+ * No counterpart in the reference, whose decoder sees one control frame at a
+ * time: the parts of a recurrent control decoder (norm with the residual's
+ * addition, short causal convolution, selective state space scan, gated
+ * feed-forward block), each with its backward pass and its form for single
+ * frames, on device buffers the caller owns.
+ *
+ * Every entry takes the device, a descriptor (struct_size = sizeof of it) and
+ * a stream (a hipStream_t, or NULL for the null stream), checks the
+ * descriptor, enqueues its kernels on the stream and returns without waiting.
+ * Nothing is allocated: an operator that needs scratch says how much
+ * (..._workspace, which depends on the sizes and on which pointers are set)
+ * and takes it in `workspace`, 256-byte aligned, free again once the call's
+ * work is done; two calls that can overlap need two.  Workspaces are written
+ * before they are read and their contents do not matter.  The caller's
+ * current device is restored.
+ *
+ * Types: DGEN_HIP_F32 or DGEN_HIP_BF16 for the tensors that say so; states,
+ * norm statistics and all sums are fp32 whatever the types.  A sequence
+ * tensor is [batch][time][channel] with contiguous channels and its own batch
+ * and time strides in elements (a view of a wider tensor is fine).  Outputs
+ * must not overlap one another or an input, except where a field says so.
+ *
+ * lengths (optional, [batch] int32): sequence b is frames [0, lengths[b])
+ * (clamped to [0, T]); the frames after it are not read, their outputs and
+ * gradients are 0, and the state that a call leaves is that after the last
+ * frame of the sequence. */
+enum dgen_hip_type { DGEN_HIP_F32 = 0, DGEN_HIP_BF16 = 1 };
+
+typedef struct dgen_hip_seq {
+  void* data;       /* NULL: not given, where optional */
+  int64_t stride_b; /* elements between sequences */
+  int64_t stride_t; /* elements between frames */
+} dgen_hip_seq;
+
+/* Root-mean-square norm: s = x + residual, y = s / sqrt(mean(s^2) + eps) *
+ * weight over the `width` columns of each of `rows` rows; the sum is stored
+ * in `s`, rounded to its type, for the next layer's residual.  Without a
+ * residual, s = x and nothing but y is stored.
+ * Backward (dy, s, weight -> dx, dweight): dx is the gradient of the sum,
+ * hence of x and of the residual alike, with ds (optional: the gradient that
+ * reaches the stored sum from elsewhere) added. */
+typedef struct dgen_hip_norm {
+  uint32_t struct_size;
+  int32_t x_type;  /* x, y, dy */
+  int32_t s_type;  /* residual, s, ds, dx */
+  float eps;
+  int64_t rows;
+  int64_t width;   /* 1 .. 32768 */
+  const float* weight;
+  const void* x;        int64_t x_stride;        /* forward; elements between rows */
+  const void* residual; int64_t residual_stride; /* forward, optional */
+  void* y;              int64_t y_stride;        /* forward */
+  void* s;              int64_t s_stride;        /* forward: out, with a residual (may be the residual itself);
+                                                    backward: in */
+  const void* dy;       int64_t dy_stride;       /* backward */
+  const void* ds;       int64_t ds_stride;       /* backward, optional */
+  void* dx;             int64_t dx_stride;       /* backward (may be ds itself) */
+  float* dweight;                                /* backward, [width] */
+  void* workspace;
+  uint64_t workspace_bytes;
+} dgen_hip_norm;
+int dgen_hip_rms_norm(int device, const dgen_hip_norm* n, void* stream);
+int dgen_hip_rms_norm_backward(int device, const dgen_hip_norm* n, void* stream);
+int dgen_hip_rms_norm_workspace(int device, const dgen_hip_norm* n, int backward, uint64_t* bytes);
+
+/* Depthwise causal convolution with optional SiLU: u[t][c] = bias[c] +
+ * sum_i weight[c][i] x[t - W + 1 + i][c], y = silu(u) or u.  Frames before
+ * the first are those of `state` ([batch][W-1][D], oldest first, x's type) or
+ * 0; `state_out` receives the W-1 frames before the sequence's end (it may
+ * be `state` itself).
+ * Backward (dy, x -> dx, dweight, dbias): the state counts as given, no
+ * gradient reaches it. */
+typedef struct dgen_hip_conv {
+  uint32_t struct_size;
+  int32_t type;    /* x, y, dy, dx and the states */
+  int32_t silu;    /* 0: y = u */
+  int32_t width;   /* W, 1 .. 8 */
+  int64_t batch, T, D;
+  const float* weight;    /* [D][W] */
+  const float* bias;      /* [D], optional */
+  const int32_t* lengths; /* optional */
+  dgen_hip_seq x;
+  dgen_hip_seq y;         /* forward */
+  const void* state;      /* optional */
+  void* state_out;        /* forward, optional */
+  dgen_hip_seq dy, dx;    /* backward */
+  float* dweight;         /* backward, [D][W] */
+  float* dbias;           /* backward, [D]; with a bias */
+  void* workspace;
+  uint64_t workspace_bytes;
+} dgen_hip_conv;
+int dgen_hip_causal_conv(int device, const dgen_hip_conv* c, void* stream);
+int dgen_hip_causal_conv_backward(int device, const dgen_hip_conv* c, void* stream);
+int dgen_hip_causal_conv_workspace(int device, const dgen_hip_conv* c, int backward, uint64_t* bytes);
+
+/* Selective state space scan.  Per sequence and channel d, with N states:
+ *   step[t] = softplus(dt[t][d] + dt_bias[d])
+ *   h[t][n] = exp(step[t] A[d][n]) h[t-1][n] + step[t] x[t][d] B[t][n]
+ *   y[t][d] = (sum_n C[t][n] h[t][n] + D[d] x[t][d]) * silu(z[t][d])
+ * dt_bias, D and z are optional (left out: 0, 0 and a factor of 1).  h[-1] is
+ * `state` ([batch][D][N] fp32) or 0; `state_out` receives the last h (it may
+ * be `state` itself).  A must be negative or 0 for a bounded state.
+ * Backward: every gradient that has a pointer's input given is required
+ * (ddt_bias with dt_bias, dD with D, dz with z); the state counts as given, no
+ * gradient reaches it, and no gradient enters through state_out. */
+typedef struct dgen_hip_scan {
+  uint32_t struct_size;
+  int32_t type;           /* x, dt, z, B, C, y and the gradients of these */
+  int64_t batch, T, D;
+  int64_t N;              /* states per channel, 1 .. 64 */
+  const float* A;         /* [D][N] */
+  const float* skip;      /* D[d], optional */
+  const float* dt_bias;   /* [D], optional */
+  const int32_t* lengths; /* optional */
+  const float* state;     /* optional */
+  float* state_out;       /* forward, optional */
+  dgen_hip_seq x, dt, z;  /* z optional */
+  dgen_hip_seq B, C;      /* [batch][T][N] */
+  dgen_hip_seq y;         /* forward */
+  dgen_hip_seq dy, dx, ddt, dz, dB, dC; /* backward */
+  float* dA;              /* backward, [D][N] */
+  float* dskip;           /* backward, [D] */
+  float* ddt_bias;        /* backward, [D] */
+  void* workspace;
+  uint64_t workspace_bytes;
+} dgen_hip_scan;
+int dgen_hip_selective_scan(int device, const dgen_hip_scan* s, void* stream);
+int dgen_hip_selective_scan_backward(int device, const dgen_hip_scan* s, void* stream);
+int dgen_hip_selective_scan_workspace(int device, const dgen_hip_scan* s, int backward, uint64_t* bytes);
+
+/* Gated feed-forward block: h = act(x w_gate) * (x w_up), x [rows][width],
+ * the weights [width][hidden] (rows contiguous, row strides given), h
+ * [rows][hidden]; act is SiLU or GELU (tanh form).
+ * Backward (dh, x -> dx, dw_gate, dw_up) forms the projections again instead
+ * of reading them: no tensor is kept between the passes. */
+enum dgen_hip_act { DGEN_HIP_SILU = 0, DGEN_HIP_GELU = 1 };
+typedef struct dgen_hip_mlp {
+  uint32_t struct_size;
+  int32_t type;
+  int32_t act;   /* enum dgen_hip_act */
+  int32_t reserved;
+  int64_t rows, width, hidden;
+  const void* x;       int64_t x_stride;
+  const void* w_gate;  int64_t w_gate_stride;
+  const void* w_up;    int64_t w_up_stride;
+  void* h;             int64_t h_stride;        /* forward */
+  const void* dh;      int64_t dh_stride;       /* backward */
+  void* dx;            int64_t dx_stride;       /* backward */
+  void* dw_gate;       int64_t dw_gate_stride;  /* backward */
+  void* dw_up;         int64_t dw_up_stride;    /* backward */
+  void* workspace;
+  uint64_t workspace_bytes;
+} dgen_hip_mlp;
+int dgen_hip_gated_mlp(int device, const dgen_hip_mlp* m, void* stream);
+int dgen_hip_gated_mlp_backward(int device, const dgen_hip_mlp* m, void* stream);
+int dgen_hip_gated_mlp_workspace(int device, const dgen_hip_mlp* m, int backward, uint64_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif
