@@ -1,5 +1,588 @@
+// Gated feed-forward block: h = act(x Wg) * (x Wu), forward and backward, on
+// the bf16 matrix cores.
+//
+// One product kernel serves four uses.  A workgroup of four waves owns a tile
+// of the output; operand tiles go from memory through registers to LDS, where
+// they lie k-contiguous whatever their layout in memory (an operand that is
+// contiguous along its rows is transposed on the way: a thread loads 8 k's of a
+// few neighbouring rows and packs them with one byte permutation a dword).
+//
+// - forward: the tile's columns are 32- or 64-wide groups of gate and up
+//   columns side by side, so a wave holds both projections of the same outputs
+//   and applies the activation and the product in registers;
+// - backward, projections again: the same, but the epilogue reads dh and
+//   writes dg = dh u act'(g) and du = dh act(g), in the operands' type;
+// - dx = dg Wg^T + du Wu^T: one product over 2 x hidden;
+// - dWg = x^T dg, dWu = x^T du: products over the rows, split over row ranges
+//   where the tiles alone do not fill the chip; the parts are added in order.
+//
+// bfloat16 operands multiply as they are, accumulated in fp32.  fp32 operands
+// are split exactly into three bfloat16 parts on the way to LDS and the six
+// partial products down to 2^-16 are accumulated in fp32, as accurate as fp32
+// products (see k_gemm.hip).
+//
+// The matrix instruction's row index is the output's column, so a lane ends
+// with four consecutive columns of one output row.
 #include "seq.h"
+
 namespace dgen {
-int64_t mlp_workspace(const dgen_hip_mlp&, bool) { return 0; }
-int mlp_run(const dgen_hip_mlp&, bool, hipStream_t, bool) { return fail(DGEN_HIP_E_INVALID, "not yet"); }
+
+namespace {
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kThreads = 256;
+
+enum Use { kForward, kProject, kDx, kDw };
+
+template <class E>
+struct GluP {
+  // operand rows along the output's columns (n) and rows (m): two matrices
+  // each (gate, up), used as columns side by side, as segments of the reduction
+  // or as two products
+  const E *n0, *n1, *m0, *m1;
+  int64_t nld0, nld1, mld0, mld1;
+  int64_t M, N, K;  // output rows, columns (of one matrix), reduction length
+  E *out0, *out1;
+  int64_t old0, old1;
+  const E* dh;
+  int64_t dhld;
+  float* parts;     // [splits][2][M][N]
+  int64_t span;     // reduction length of a split
+  int act;
+  uint32_t tiles_n, tiles_m, splits;
+};
+
+// ------------------------------------------------------------- activation
+// GELU, tanh form: 0.5 v (1 + tanh(k (v + c v^3))) = v sigmoid(2 k (v + c v^3)).
+constexpr float kGeluA = 1.5957691216057308f, kGeluB = 0.044715f;
+__device__ __forceinline__ float act_of(int act, float v, float& slope) {
+  if (act == DGEN_HIP_SILU) {
+    const float p = sigmoid(v);
+    slope = silu_grad(v, p);
+    return v * p;
+  }
+  const float v2 = v * v, p = sigmoid(kGeluA * v * fmaf(kGeluB, v2, 1.f));
+  slope = p * fmaf(v * (1.f - p), kGeluA * fmaf(3.f * kGeluB, v2, 1.f), 1.f);
+  return v * p;
 }
+
+// ---------------------------------------------------------------- staging
+// 8 consecutive k of one row as a 16-byte chunk per plane.
+template <class E>
+constexpr int planes() { return sizeof(E) == 2 ? 1 : 3; }
+
+struct Chunk {
+  uint32_t w[4];
+};
+
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  return (uint32_t)from_f32<bf16>(a).v | (uint32_t)from_f32<bf16>(b).v << 16;
+}
+__device__ __forceinline__ float part_of(uint32_t w, int hi) { return __uint_as_float(hi ? w & 0xffff0000u : w << 16); }
+
+// v = h + m + l exactly in bfloat16 parts, two values at a time.
+__device__ __forceinline__ void split2(float a, float b, uint32_t& h, uint32_t& m, uint32_t& l) {
+  h = pack2(a, b);
+  const float ra = a - part_of(h, 0), rb = b - part_of(h, 1);
+  m = pack2(ra, rb);
+  l = pack2(ra - part_of(m, 0), rb - part_of(m, 1));
+}
+
+template <class E, int V>
+struct __attribute__((packed, aligned(alignof(E)))) Vec {
+  E e[V];
+};
+
+// LDS place of chunk c (8 k's) of row r, in chunks of 16 bytes: rows of BK
+// k's, the chunks of a row permuted so that neither the fragments' reads (32
+// consecutive rows, one chunk) nor the transposing writes (rows 4 or 8 apart)
+// meet in a bank.
+template <int BK>
+__device__ __forceinline__ int place(int r, int c) {
+  constexpr int C = BK / 8;
+  if constexpr (C == 8) return r * 8 + (c ^ ((r ^ (r >> 3)) & 7));
+  else return r * C + (c ^ (((r >> 1) ^ (r >> 3)) & (C - 1)));
+}
+
+// One operand's tile of R rows x BK, between memory and LDS.  KC: k is the
+// contiguous axis in memory.
+template <class E, int R, int BK, bool KC>
+struct Stage {
+  static constexpr int P = planes<E>();
+  static constexpr int kPer = R * BK / kThreads;                     // elements a thread carries
+  static constexpr int kMaxV = 16 / (int)sizeof(E);
+  static constexpr int V = KC ? 8 : (kPer / 8 < kMaxV ? kPer / 8 : kMaxV);  // elements of a load
+  static constexpr int U = kPer / (8 * (KC ? 1 : V));                // chunks (KC) or 8 x V blocks a thread
+  static_assert(kPer % 8 == 0 && V >= 1 && U >= 1, "tile too small");
+  E v[U][KC ? 1 : 8][V];
+
+  // row(r): the address of row r of the tile (KC) or of element (r, k = 0)
+  // (!KC), and how many rows from r on are inside the operand.
+  template <class Row>
+  __device__ __forceinline__ void load(Row row, int64_t ld, int64_t k0, int64_t kend) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = threadIdx.x + u * kThreads;
+      if constexpr (KC) {
+        const int r = i / (BK / 8);
+        const int64_t k = k0 + (i % (BK / 8)) * 8;
+        const E* p;
+        const bool in = row(r, p) > 0;
+        get<V>(p + k, in ? kend - k : 0, v[u][0]);
+      } else {
+        const int r = (i % (R / V)) * V;
+        const int64_t k = k0 + (i / (R / V)) * 8;
+        const E* p;
+        const int64_t in = row(r, p);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) get<V>(p + (k + q) * ld, k + q < kend ? in : 0, v[u][q]);
+      }
+    }
+  }
+
+  template <int W>
+  __device__ __forceinline__ static void get(const E* p, int64_t valid, E (&o)[W]) {
+    if (valid >= W) {
+      const Vec<E, W> t = *reinterpret_cast<const Vec<E, W>*>(p);
+#pragma unroll
+      for (int e = 0; e < W; ++e) o[e] = t.e[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < W; ++e) o[e] = e < valid ? p[e] : E{};
+    }
+  }
+
+  __device__ __forceinline__ void store(Chunk* lds) const {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = threadIdx.x + u * kThreads;
+#pragma unroll
+      for (int b = 0; b < (KC ? 1 : V); ++b) {
+        const int r = KC ? i / (BK / 8) : (i % (R / V)) * V + b;
+        const int c = KC ? i % (BK / 8) : i / (R / V);
+        Chunk o[P];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const E lo = KC ? v[u][0][KC ? 2 * q : 0] : v[u][KC ? 0 : 2 * q][KC ? 0 : b];
+          const E hi = KC ? v[u][0][KC ? 2 * q + 1 : 0] : v[u][KC ? 0 : 2 * q + 1][KC ? 0 : b];
+          if constexpr (P == 1) o[0].w[q] = (uint32_t)lo.v | (uint32_t)hi.v << 16;
+          else split2(lo, hi, o[0].w[q], o[1].w[q], o[2].w[q]);
+        }
+#pragma unroll
+        for (int pl = 0; pl < P; ++pl) lds[pl * (R * BK / 8) + place<BK>(r, c)] = o[pl];
+      }
+    }
+  }
+};
+
+template <class E, int W>
+__device__ __forceinline__ void put_four(E* p, int64_t valid, const float (&o)[W]) {
+  store_four(p, (int)(valid < 4 ? valid : 4), o);
+}
+
+// ----------------------------------------------------------------- kernel
+// BM x BN: output rows and operand columns of a tile; WM x WN: of a wave.
+template <class E, int BM, int BN, int WM, int WN, int BK, int BUF, int USE>
+__global__ __launch_bounds__(kThreads) void k_glu(GluP<E> p) {
+  constexpr int P = planes<E>(), NF = WN / 32, MF = WM / 32;
+  constexpr bool PAIR = USE == kForward || USE == kProject;
+  constexpr bool NKC = USE == kDx, MKC = USE != kDw;
+  static_assert((BM / WM) * (BN / WN) == kThreads / 64, "four waves");
+  constexpr int NCH = P * BN * BK / 8, MCH = P * BM * BK / 8;
+  __shared__ Chunk lds[BUF][NCH + MCH];
+
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wn = wave % (BN / WN), wm = wave / (BN / WN);
+  // Tile of this workgroup.  Consecutive workgroups go to the eight XCDs in
+  // turn; each XCD takes a run of consecutive tiles (n fastest), which share
+  // their operand rows in its L2.
+  const uint32_t total = gridDim.x;
+  uint32_t id = blockIdx.x;
+  if (total % 8 == 0) id = (id & 7) * (total / 8) + (id >> 3);
+  const uint32_t tn = id % p.tiles_n, tr = id / p.tiles_n, tm = tr % p.tiles_m, rest = tr / p.tiles_m;
+  const uint32_t split = USE == kDw ? rest % p.splits : 0, mat = USE == kDw ? rest / p.splits : 0;
+  constexpr int COLS = PAIR ? BN / 2 : BN;  // output columns of a tile
+  const int64_t n0 = (int64_t)tn * COLS, m0 = (int64_t)tm * BM;
+  const int64_t kfrom = USE == kDw ? split * p.span : 0;
+  const int64_t kend = USE == kDw && kfrom + p.span < p.K ? kfrom + p.span : p.K;
+  const int64_t kblocks = kend > kfrom ? (kend - kfrom + BK - 1) / BK : 0;
+  const int64_t steps = USE == kDx ? 2 * kblocks : kblocks;
+
+  Stage<E, BN, BK, NKC> sn;
+  Stage<E, BM, BK, MKC> sm;
+  auto load = [&](int64_t step) {
+    const bool second = USE == kDx && step >= kblocks;
+    const int64_t k0 = kfrom + (second ? step - kblocks : step) * BK;
+    const bool n_second = second || (USE == kDw && mat), m_second = second;
+    const E* nb = n_second ? p.n1 : p.n0;
+    const int64_t nld = n_second ? p.nld1 : p.nld0;
+    const E* mb = m_second ? p.m1 : p.m0;
+    const int64_t mld = m_second ? p.mld1 : p.mld0;
+    auto nrow = [&](int r, const E*& at) -> int64_t {
+      if constexpr (PAIR) {
+        // a wave's WN columns: WN / 2 of gate, then the same of up
+        const bool up = (r % WN) >= WN / 2;
+        const int64_t f = n0 + r / WN * (WN / 2) + r % (WN / 2);
+        at = (up ? p.n1 : p.n0) + f;
+        return p.N - f;
+      } else {
+        const int64_t n = n0 + r;
+        at = NKC ? nb + n * nld : nb + n;
+        return p.N - n;
+      }
+    };
+    auto mrow = [&](int r, const E*& at) -> int64_t {
+      const int64_t m = m0 + r;
+      at = MKC ? mb + m * mld : mb + m;
+      return p.M - m;
+    };
+    if constexpr (PAIR) {
+      // (the two matrices may have different strides: the block's own is used)
+      const bool up = ((threadIdx.x % (BN / Stage<E, BN, BK, NKC>::V)) * Stage<E, BN, BK, NKC>::V) % WN >= WN / 2;
+      sn.load(nrow, up ? p.nld1 : p.nld0, k0, kend);
+    } else {
+      sn.load(nrow, nld, k0, kend);
+    }
+    sm.load(mrow, mld, k0, kend);
+  };
+
+  floatx16 acc[NF][MF] = {};
+  auto compute = [&](const Chunk* b) {
+#pragma unroll
+    for (int ks = 0; ks < BK / 16; ++ks) {
+      bf16x8 nf[NF][P], mf[MF][P];
+      const int c = ks * 2 + (lane >> 5), r = lane & 31;
+#pragma unroll
+      for (int i = 0; i < NF; ++i)
+#pragma unroll
+        for (int pl = 0; pl < P; ++pl)
+          nf[i][pl] = __builtin_bit_cast(bf16x8, b[pl * (BN * BK / 8) + place<BK>(wn * WN + i * 32 + r, c)]);
+#pragma unroll
+      for (int j = 0; j < MF; ++j)
+#pragma unroll
+        for (int pl = 0; pl < P; ++pl)
+          mf[j][pl] = __builtin_bit_cast(bf16x8, b[NCH + pl * (BM * BK / 8) + place<BK>(wm * WM + j * 32 + r, c)]);
+#pragma unroll
+      for (int i = 0; i < NF; ++i)
+#pragma unroll
+        for (int j = 0; j < MF; ++j) {
+          if constexpr (P == 1) {
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(nf[i][0], mf[j][0], acc[i][j], 0, 0, 0);
+          } else {
+            // smallest products first
+#define DGEN_PART(a, b2) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(nf[i][a], mf[j][b2], acc[i][j], 0, 0, 0)
+            DGEN_PART(2, 0);
+            DGEN_PART(0, 2);
+            DGEN_PART(1, 1);
+            DGEN_PART(1, 0);
+            DGEN_PART(0, 1);
+            DGEN_PART(0, 0);
+#undef DGEN_PART
+          }
+        }
+    }
+  };
+
+  if (steps > 0) load(0);
+  if constexpr (BUF == 2) {
+    if (steps > 0) {
+      sn.store(lds[0]);
+      sm.store(lds[0] + NCH);
+    }
+    __syncthreads();
+    for (int64_t s = 0; s < steps; ++s) {
+      if (s + 1 < steps) load(s + 1);
+      compute(lds[s & 1]);
+      if (s + 1 < steps) {
+        sn.store(lds[(s + 1) & 1]);
+        sm.store(lds[(s + 1) & 1] + NCH);
+      }
+      __syncthreads();
+    }
+  } else {
+    for (int64_t s = 0; s < steps; ++s) {
+      __syncthreads();
+      sn.store(lds[0]);
+      sm.store(lds[0] + NCH);
+      __syncthreads();
+      if (s + 1 < steps) load(s + 1);
+      compute(lds[0]);
+    }
+  }
+
+  // register 4 q + e of acc[i][j]: output column 8 q + 4 (lane / 32) + e of
+  // the fragment's 32, row lane % 32
+  const int r = lane & 31, h = lane >> 5;
+#pragma unroll
+  for (int j = 0; j < MF; ++j) {
+    const int64_t m = m0 + wm * WM + j * 32 + r;
+    if (m >= p.M) continue;
+#pragma unroll
+    for (int i = 0; i < (PAIR ? NF / 2 : NF); ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int64_t n = n0 + (PAIR ? wn * (WN / 2) : wn * WN) + i * 32 + 8 * q + 4 * h;
+        if (n >= p.N) continue;
+        float a[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = acc[i][j][4 * q + e];
+        if constexpr (PAIR) {
+          float u[4], slope;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) u[e] = acc[i + NF / 2][j][4 * q + e];
+          if constexpr (USE == kForward) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[e] = act_of(p.act, a[e], slope) * u[e];
+            put_four(p.out0 + m * p.old0 + n, p.N - n, a);
+          } else {
+            float d[4];
+            load_four(p.dh + m * p.dhld + n, (int)(p.N - n < 4 ? p.N - n : 4), d);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float v = act_of(p.act, a[e], slope);
+              a[e] = d[e] * u[e] * slope;
+              u[e] = d[e] * v;
+            }
+            put_four(p.out0 + m * p.old0 + n, p.N - n, a);
+            put_four(p.out1 + m * p.old1 + n, p.N - n, u);
+          }
+        } else if constexpr (USE == kDx) {
+          put_four(p.out0 + m * p.old0 + n, p.N - n, a);
+        } else {
+          if (p.splits > 1) {
+            put_four(p.parts + ((int64_t)split * 2 + mat) * p.M * p.N + m * p.N + n, p.N - n, a);
+          } else {
+            put_four(mat ? p.out1 + m * p.old1 + n : p.out0 + m * p.old0 + n, p.N - n, a);
+          }
+        }
+      }
+  }
+}
+
+// dW from the row ranges' parts.
+template <class E>
+__global__ __launch_bounds__(256) void k_glu_join(const float* __restrict__ parts, uint32_t splits, int64_t M, int64_t N,
+                                                  E* out0, int64_t ld0, E* out1, int64_t ld1) {
+  const int64_t groups = (N + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= 2 * M * groups) return;
+  const int64_t mat = i / (M * groups), at = i - mat * M * groups, m = at / groups, n = (at - m * groups) * 4;
+  float t[4] = {0.f, 0.f, 0.f, 0.f};
+  const int valid = (int)(N - n < 4 ? N - n : 4);
+  for (uint32_t s = 0; s < splits; ++s) {
+    float v[4];
+    load_four(parts + ((int64_t)s * 2 + mat) * M * N + m * N + n, valid, v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) t[e] += v[e];
+  }
+  store_four(mat ? out1 + m * ld1 + n : out0 + m * ld0 + n, valid, t);
+}
+
+// Forward for a few rows (single frames of some voices): the weights' reading
+// is all that counts, so the vector unit multiplies.  A workgroup owns 64
+// columns; 32 lanes x 2 columns, the half-waves of eight waves take every
+// 16th k, and the sixteen sums meet in LDS.
+constexpr int kFewRows = 8, kFewThreads = 512, kFewCols = 64, kFewK = 512;
+template <class E>
+__global__ __launch_bounds__(kFewThreads) void k_glu_few(GluP<E> p) {
+  __shared__ float xs[kFewK][kFewRows];
+  __shared__ float red[8][kFewCols][2][kFewRows + 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+  const int64_t m0 = (int64_t)blockIdx.y * kFewRows, f = (int64_t)blockIdx.x * kFewCols + (lane & 31) * 2;
+  const int valid = (int)(p.N - f < 0 ? 0 : p.N - f < 2 ? p.N - f : 2);
+  float acc[2][2][kFewRows] = {};
+  for (int64_t k0 = 0; k0 < p.K; k0 += kFewK) {
+    const int kn = (int)(p.K - k0 < kFewK ? p.K - k0 : kFewK);
+    __syncthreads();
+    for (int i = threadIdx.x; i < kFewK * kFewRows; i += kFewThreads) {
+      const int m = i / kFewK, k = i % kFewK;
+      xs[k][m] = k < kn && m0 + m < p.M ? to_f32(p.m0[(m0 + m) * p.mld0 + k0 + k]) : 0.f;
+    }
+    __syncthreads();
+#pragma unroll 8
+    for (int k = wave * 2 + half; k < kn; k += 16) {
+      Vec<E, 2> w[2] = {};
+      const E *g = p.n0 + (k0 + k) * p.nld0 + f, *u = p.n1 + (k0 + k) * p.nld1 + f;
+      if (valid == 2) {
+        w[0] = *reinterpret_cast<const Vec<E, 2>*>(g);
+        w[1] = *reinterpret_cast<const Vec<E, 2>*>(u);
+      } else if (valid == 1) {
+        w[0].e[0] = *g;
+        w[1].e[0] = *u;
+      }
+#pragma unroll
+      for (int m = 0; m < kFewRows; ++m) {
+        const float x = xs[k][m];
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+          for (int b = 0; b < 2; ++b) acc[a][b][m] = fmaf(x, to_f32(w[a].e[b]), acc[a][b][m]);
+      }
+    }
+  }
+#pragma unroll
+  for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int m = 0; m < kFewRows; ++m) {
+        const float t = acc[a][b][m] + __shfl_xor(acc[a][b][m], 32, 64);
+        if (half == 0) red[wave][lane * 2 + b][a][m] = t;
+      }
+  __syncthreads();
+  const int c = threadIdx.x % kFewCols, m = threadIdx.x / kFewCols;  // 64 columns x 8 rows
+  const int64_t n = (int64_t)blockIdx.x * kFewCols + c;
+  float s[2] = {0.f, 0.f}, slope;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    s[0] += red[w][c][0][m];
+    s[1] += red[w][c][1][m];
+  }
+  if (m0 + m < p.M && n < p.N) p.out0[(m0 + m) * p.old0 + n] = from_f32<E>(act_of(p.act, s[0], slope) * s[1]);
+}
+
+// ------------------------------------------------------------------ shapes
+struct Tile {
+  int bm, bn;
+};
+// Large tiles where they fill the chip's 256 CUs, else small ones.
+template <class E>
+bool large_tiles(int64_t M, int64_t cols) {
+  const int64_t bm = sizeof(E) == 2 ? 256 : 128;
+  return ((M + bm - 1) / bm) * ((cols + bm - 1) / bm) >= 128;
+}
+
+template <class E, int USE>
+void product(GluP<E> p, int64_t cols, hipStream_t st) {
+  // cols: operand columns of the tiles (gate and up side by side in PAIR uses)
+  constexpr bool PAIR = USE == kForward || USE == kProject;
+  constexpr int L = sizeof(E) == 2 ? 256 : 128;
+  const bool large = large_tiles<E>(p.M, cols);
+  const int bm = large ? L : 64, bn = large ? L : 128, per = PAIR ? bn / 2 : bn;
+  p.tiles_m = (uint32_t)((p.M + bm - 1) / bm);
+  p.tiles_n = (uint32_t)((p.N + per - 1) / per);
+  const dim3 grid(p.tiles_m * p.tiles_n * (USE == kDw ? 2 * p.splits : 1));
+  if (large) {
+    if constexpr (sizeof(E) == 2) k_glu<E, 256, 256, 128, 128, 64, 2, USE><<<grid, kThreads, 0, st>>>(p);
+    else k_glu<E, 128, 128, 64, 64, 32, 1, USE><<<grid, kThreads, 0, st>>>(p);
+  } else {
+    k_glu<E, 64, 128, 32, 64, sizeof(E) == 2 ? 64 : 32, 1, USE><<<grid, kThreads, 0, st>>>(p);
+  }
+}
+
+// Row ranges of the weight gradients' products.
+template <class E>
+void dw_splits(const dgen_hip_mlp& a, uint32_t& splits, int64_t& span) {
+  const int64_t L = sizeof(E) == 2 ? 256 : 128;
+  const bool large = large_tiles<E>(a.width, 2 * a.hidden);
+  const int64_t bm = large ? L : 64, bn = large ? L : 128;
+  const int64_t tiles = 2 * ((a.width + bm - 1) / bm) * ((a.hidden + bn - 1) / bn);
+  // about two workgroups a CU, none with fewer than 512 rows
+  int64_t s = std::max<int64_t>(1, std::min<int64_t>((512 + tiles - 1) / tiles, (a.rows + 511) / 512));
+  span = std::max<int64_t>(64, ((a.rows + s - 1) / s + 63) / 64 * 64);
+  splits = (uint32_t)std::max<int64_t>(1, (a.rows + span - 1) / span);
+}
+
+struct MlpWs {
+  int64_t dg, du, parts, total;  // bytes
+};
+MlpWs mlp_ws(const dgen_hip_mlp& a) {
+  MlpWs w{};
+  const int64_t es = a.type == DGEN_HIP_BF16 ? 2 : 4;
+  uint32_t splits;
+  int64_t span;
+  if (a.type == DGEN_HIP_BF16) dw_splits<bf16>(a, splits, span);
+  else dw_splits<float>(a, splits, span);
+  w.dg = w.du = align256(a.rows * a.hidden * es);
+  w.parts = splits > 1 ? align256((int64_t)splits * 2 * a.width * a.hidden * 4) : 0;
+  w.total = w.dg + w.du + w.parts;
+  return w;
+}
+
+template <class E>
+void mlp_launch(const dgen_hip_mlp& a, bool backward, hipStream_t st) {
+  GluP<E> p{};
+  p.act = a.act;
+  p.splits = 1;
+  p.n0 = (const E*)a.w_gate, p.n1 = (const E*)a.w_up, p.nld0 = a.w_gate_stride, p.nld1 = a.w_up_stride;
+  p.m0 = p.m1 = (const E*)a.x, p.mld0 = p.mld1 = a.x_stride;
+  p.M = a.rows, p.N = a.hidden, p.K = a.width;
+  if (!backward) {
+    p.out0 = (E*)a.h, p.old0 = a.h_stride;
+    if (a.rows <= 2 * kFewRows) {
+      k_glu_few<E><<<dim3((unsigned)((a.hidden + kFewCols - 1) / kFewCols), (unsigned)((a.rows + kFewRows - 1) / kFewRows)),
+                     kFewThreads, 0, st>>>(p);
+    } else {
+      product<E, kForward>(p, 2 * a.hidden, st);
+    }
+    return;
+  }
+  const MlpWs w = mlp_ws(a);
+  E* dg = (E*)a.workspace;
+  E* du = (E*)((char*)a.workspace + w.dg);
+  float* parts = (float*)((char*)a.workspace + w.dg + w.du);
+  if (a.rows > 0) {
+    GluP<E> q = p;
+    q.out0 = dg, q.out1 = du, q.old0 = q.old1 = a.hidden;
+    q.dh = (const E*)a.dh, q.dhld = a.dh_stride;
+    product<E, kProject>(q, 2 * a.hidden, st);
+    q = p;
+    q.m0 = dg, q.m1 = du, q.mld0 = q.mld1 = a.hidden;
+    q.N = a.width, q.K = a.hidden;
+    q.out0 = (E*)a.dx, q.old0 = a.dx_stride;
+    product<E, kDx>(q, a.width, st);
+  }
+  GluP<E> q = p;
+  q.n0 = dg, q.n1 = du, q.nld0 = q.nld1 = a.hidden;
+  q.M = a.width, q.N = a.hidden, q.K = a.rows;
+  q.out0 = (E*)a.dw_gate, q.old0 = a.dw_gate_stride, q.out1 = (E*)a.dw_up, q.old1 = a.dw_up_stride;
+  q.parts = parts;
+  dw_splits<E>(a, q.splits, q.span);
+  product<E, kDw>(q, 2 * a.hidden, st);
+  if (q.splits > 1) {
+    const int64_t n = 2 * a.width * ((a.hidden + 3) / 4);
+    k_glu_join<E><<<dim3((unsigned)((n + 255) / 256)), 256, 0, st>>>(parts, q.splits, a.width, a.hidden, q.out0, q.old0,
+                                                                     q.out1, q.old1);
+  }
+}
+
+}  // namespace
+
+int64_t mlp_workspace(const dgen_hip_mlp& a, bool backward) { return backward ? mlp_ws(a).total : 0; }
+
+int mlp_run(const dgen_hip_mlp& a, bool backward, hipStream_t st, bool dry) {
+  const char* what = backward ? "gated_mlp_backward" : "gated_mlp";
+  DGEN_REQUIRE(a.struct_size == sizeof(a), "%s: struct_size %u, expected %zu", what, a.struct_size, sizeof(a));
+  DGEN_REQUIRE(a.type == DGEN_HIP_F32 || a.type == DGEN_HIP_BF16, "%s: type %d", what, a.type);
+  DGEN_REQUIRE(a.act == DGEN_HIP_SILU || a.act == DGEN_HIP_GELU, "%s: activation %d", what, a.act);
+  DGEN_REQUIRE(a.width >= 1 && a.width <= (1 << 17) && a.hidden >= 1 && a.hidden <= (1 << 17),
+               "%s: width %lld or hidden %lld outside [1, 2^17]", what, (long long)a.width, (long long)a.hidden);
+  // (tiles, of 64 rows at least, times threads stay below 2^32)
+  DGEN_REQUIRE(a.rows >= 0 && (a.rows + 63) / 64 * ((2 * a.hidden + 127) / 128 + (a.width + 127) / 128) < (1 << 23),
+               "%s: rows %lld too many for one call", what, (long long)a.rows);
+  DGEN_REQUIRE(a.w_gate && a.w_up, "%s: null w_gate or w_up", what);
+  DGEN_REQUIRE(a.w_gate_stride >= 0 && a.w_up_stride >= 0 && a.x_stride >= 0, "%s: negative stride", what);
+  const bool empty = a.rows == 0;
+  DGEN_REQUIRE(a.x || empty, "%s: null x", what);
+  if (!backward) {
+    DGEN_REQUIRE((a.h || empty) && (a.rows <= 1 || a.h_stride >= a.hidden), "%s: h missing or overlapping itself", what);
+  } else {
+    DGEN_REQUIRE((a.dh || empty) && a.dh_stride >= 0, "%s: dh missing or with a negative stride", what);
+    DGEN_REQUIRE((a.dx || empty) && (a.rows <= 1 || a.dx_stride >= a.width), "%s: dx missing or overlapping itself",
+                 what);
+    DGEN_REQUIRE(a.dw_gate && a.dw_up && (a.width <= 1 || (a.dw_gate_stride >= a.hidden && a.dw_up_stride >= a.hidden)),
+                 "%s: dw_gate or dw_up missing or overlapping itself", what);
+    const int64_t need = mlp_workspace(a, true);
+    DGEN_REQUIRE(need == 0 || (a.workspace && a.workspace_bytes >= (uint64_t)need && (uintptr_t)a.workspace % 256 == 0),
+                 "%s: workspace of %llu bytes, %lld needed (256-byte aligned)", what,
+                 (unsigned long long)a.workspace_bytes, (long long)need);
+  }
+  if (dry || (empty && !backward)) return 0;
+  if (a.type == DGEN_HIP_BF16) mlp_launch<bf16>(a, backward, st);
+  else mlp_launch<float>(a, backward, st);
+  DGEN_LAUNCH_CHECK(what);
+  return 0;
+}
+
+}  // namespace dgen
