@@ -182,7 +182,77 @@ __device__ __forceinline__ void put_four(E* p, int64_t valid, const float (&o)[W
   store_four(p, (int)(valid < 4 ? valid : 4), o);
 }
 
+// A wave's accumulators to memory; its tile starts at output row mb, column nb.
+template <class E, int USE, int NF, int MF>
+__device__ __forceinline__ void finish(const GluP<E>& p, const floatx16 (&acc)[NF][MF], int64_t mb, int64_t nb,
+                                       uint32_t split, uint32_t mat) {
+  constexpr bool PAIR = USE == kForward || USE == kProject;
+  const int lane = threadIdx.x & 63;
+  // register 4 q + e of acc[i][j]: output column 8 q + 4 (lane / 32) + e of
+  // the fragment's 32, row lane % 32
+  const int r = lane & 31, h = lane >> 5;
+#pragma unroll
+  for (int j = 0; j < MF; ++j) {
+    const int64_t m = mb + j * 32 + r;
+    if (m >= p.M) continue;
+#pragma unroll
+    for (int i = 0; i < (PAIR ? NF / 2 : NF); ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int64_t n = nb + i * 32 + 8 * q + 4 * h;
+        if (n >= p.N) continue;
+        float a[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = acc[i][j][4 * q + e];
+        if constexpr (PAIR) {
+          float u[4], slope;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) u[e] = acc[i + NF / 2][j][4 * q + e];
+          if constexpr (USE == kForward) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[e] = act_of(p.act, a[e], slope) * u[e];
+            put_four(p.out0 + m * p.old0 + n, p.N - n, a);
+          } else {
+            float d[4];
+            load_four(p.dh + m * p.dhld + n, (int)(p.N - n < 4 ? p.N - n : 4), d);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float v = act_of(p.act, a[e], slope);
+              a[e] = d[e] * u[e] * slope;
+              u[e] = d[e] * v;
+            }
+            put_four(p.out0 + m * p.old0 + n, p.N - n, a);
+            put_four(p.out1 + m * p.old1 + n, p.N - n, u);
+          }
+        } else if constexpr (USE == kDx) {
+          put_four(p.out0 + m * p.old0 + n, p.N - n, a);
+        } else {
+          if (p.parts) {
+            put_four(p.parts + ((int64_t)split * 2 + mat) * p.M * p.N + m * p.N + n, p.N - n, a);
+          } else {
+            put_four(mat ? p.out1 + m * p.old1 + n : p.out0 + m * p.old0 + n, p.N - n, a);
+          }
+        }
+      }
+  }
+}
+
 // ----------------------------------------------------------------- kernel
+// Tile of this workgroup.  Consecutive workgroups go to the eight XCDs in
+// turn; each XCD takes a run of consecutive tiles (n fastest), which share
+// their operand rows in its L2.
+struct TileAt {
+  uint32_t n, m, split, mat;
+};
+template <int USE, class E>
+__device__ __forceinline__ TileAt tile_at(const GluP<E>& p) {
+  const uint32_t total = gridDim.x;
+  uint32_t id = blockIdx.x;
+  if (total % 8 == 0) id = (id & 7) * (total / 8) + (id >> 3);
+  const uint32_t tr = id / p.tiles_n, rest = tr / p.tiles_m;
+  return {id % p.tiles_n, tr % p.tiles_m, USE == kDw ? rest % p.splits : 0, USE == kDw ? rest / p.splits : 0};
+}
+
 // BM x BN: output rows and operand columns of a tile; WM x WN: of a wave.
 template <class E, int BM, int BN, int WM, int WN, int BK, int BUF, int USE>
 __global__ __launch_bounds__(kThreads) void k_glu(GluP<E> p) {
@@ -195,16 +265,10 @@ __global__ __launch_bounds__(kThreads) void k_glu(GluP<E> p) {
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wn = wave % (BN / WN), wm = wave / (BN / WN);
-  // Tile of this workgroup.  Consecutive workgroups go to the eight XCDs in
-  // turn; each XCD takes a run of consecutive tiles (n fastest), which share
-  // their operand rows in its L2.
-  const uint32_t total = gridDim.x;
-  uint32_t id = blockIdx.x;
-  if (total % 8 == 0) id = (id & 7) * (total / 8) + (id >> 3);
-  const uint32_t tn = id % p.tiles_n, tr = id / p.tiles_n, tm = tr % p.tiles_m, rest = tr / p.tiles_m;
-  const uint32_t split = USE == kDw ? rest % p.splits : 0, mat = USE == kDw ? rest / p.splits : 0;
+  const TileAt t = tile_at<USE>(p);
+  const uint32_t split = t.split, mat = t.mat;
   constexpr int COLS = PAIR ? BN / 2 : BN;  // output columns of a tile
-  const int64_t n0 = (int64_t)tn * COLS, m0 = (int64_t)tm * BM;
+  const int64_t n0 = (int64_t)t.n * COLS, m0 = (int64_t)t.m * BM;
   const int64_t kfrom = USE == kDw ? split * p.span : 0;
   const int64_t kend = USE == kDw && kfrom + p.span < p.K ? kfrom + p.span : p.K;
   const int64_t kblocks = kend > kfrom ? (kend - kfrom + BK - 1) / BK : 0;
@@ -312,53 +376,165 @@ __global__ __launch_bounds__(kThreads) void k_glu(GluP<E> p) {
     }
   }
 
-  // register 4 q + e of acc[i][j]: output column 8 q + 4 (lane / 32) + e of
-  // the fragment's 32, row lane % 32
-  const int r = lane & 31, h = lane >> 5;
-#pragma unroll
-  for (int j = 0; j < MF; ++j) {
-    const int64_t m = m0 + wm * WM + j * 32 + r;
-    if (m >= p.M) continue;
-#pragma unroll
-    for (int i = 0; i < (PAIR ? NF / 2 : NF); ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int64_t n = n0 + (PAIR ? wn * (WN / 2) : wn * WN) + i * 32 + 8 * q + 4 * h;
-        if (n >= p.N) continue;
-        float a[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) a[e] = acc[i][j][4 * q + e];
-        if constexpr (PAIR) {
-          float u[4], slope;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) u[e] = acc[i + NF / 2][j][4 * q + e];
-          if constexpr (USE == kForward) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) a[e] = act_of(p.act, a[e], slope) * u[e];
-            put_four(p.out0 + m * p.old0 + n, p.N - n, a);
-          } else {
-            float d[4];
-            load_four(p.dh + m * p.dhld + n, (int)(p.N - n < 4 ? p.N - n : 4), d);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float v = act_of(p.act, a[e], slope);
-              a[e] = d[e] * u[e] * slope;
-              u[e] = d[e] * v;
-            }
-            put_four(p.out0 + m * p.old0 + n, p.N - n, a);
-            put_four(p.out1 + m * p.old1 + n, p.N - n, u);
-          }
-        } else if constexpr (USE == kDx) {
-          put_four(p.out0 + m * p.old0 + n, p.N - n, a);
-        } else {
-          if (p.splits > 1) {
-            put_four(p.parts + ((int64_t)split * 2 + mat) * p.M * p.N + m * p.N + n, p.N - n, a);
-          } else {
-            put_four(mat ? p.out1 + m * p.old1 + n : p.out0 + m * p.old0 + n, p.N - n, a);
-          }
-        }
-      }
+  finish<E, USE, NF, MF>(p, acc, m0 + wm * WM, n0 + (PAIR ? wn * (WN / 2) : wn * WN), split, mat);
+}
+
+// ------------------------------------------------- bf16, aligned operands
+// The same product with operand tiles copied global -> LDS by the load-to-LDS
+// instructions, as they lie in memory: 256 x 256 outputs a workgroup, 128 x 128
+// a wave (256 accumulators a lane), stages of 32 k's in four LDS buffers, two
+// to three of them in flight.  An operand that is contiguous along its rows is
+// read with the transposing LDS load.  Chunks of 16 bytes are permuted within
+// their LDS rows through the global addresses, so that the fragments' reads
+// spread over the banks: k-contiguous rows (four chunks) by row / 2, row-
+// contiguous k's (32 chunks) by twice the k.
+constexpr int kDT = 256, kDK = 32, kDBufs = 4, kDChunks = kDT * kDK / 8;  // chunks of one operand's stage
+
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) short4v lds_short4;
+
+// 16 bytes a lane from `g` to LDS byte `at` + 16 lane (at: uniform).  In
+// assembly, since the compiler would wait for every copy in flight before any
+// transposing LDS read; the kernel waits for its copies itself.  (M0 has no
+// other use in it.)
+__device__ __forceinline__ void copy_to_lds(const bf16* g, uint32_t at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(g) : "memory");
+}
+
+template <bool KC>
+__device__ __forceinline__ int chunk_swizzle(int row) { return KC ? (row >> 1) & 3 : (row & 3) << 1; }
+
+// Fragment of 32 rows from `r0` on at k-step ks of a stage.
+template <bool KC>
+__device__ __forceinline__ bf16x8 fragment(const uint4* b, int r0, int ks, int lane) {
+  if constexpr (KC) {
+    const int r = r0 + (lane & 31), c = ks * 2 + (lane >> 5);
+    return __builtin_bit_cast(bf16x8, b[r * 4 + (c ^ chunk_swizzle<true>(r))]);
+  } else {
+    // lane group g = lane / 16: rows 16 (g & 1) + lane % 16, k's 8 (g / 2) ..;
+    // each lane addresses four rows of one k and receives four k's of one row
+    const int g = lane >> 4, k = ks * 16 + 8 * (g >> 1) + ((lane & 15) >> 2);
+    const int r = r0 + 16 * (g & 1) + 4 * (lane & 3);
+    struct Two {
+      short4v a, b;
+    } o;
+    const int c = r >> 3, half = (r >> 2) & 1;
+    // k + 4 has the same swizzle (k & 3)
+    const uint4* p = b + k * 32 + (c ^ chunk_swizzle<false>(k));
+    o.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)((const short*)p + half * 4));
+    o.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)((const short*)(p + 4 * 32) + half * 4));
+    return __builtin_bit_cast(bf16x8, o);
   }
+}
+
+template <int USE>
+__global__ __launch_bounds__(kThreads, 1) void k_glu_direct(GluP<bf16> p) {
+  constexpr bool PAIR = USE == kForward || USE == kProject;
+  constexpr bool NKC = USE == kDx, MKC = USE != kDw;
+  __shared__ __align__(1024) uint4 lds[kDBufs][2][kDChunks];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wn = wave & 1, wm = wave >> 1;
+  const TileAt t = tile_at<USE>(p);
+  const int64_t n0 = (int64_t)t.n * (PAIR ? kDT / 2 : kDT), m0 = (int64_t)t.m * kDT;
+  const int64_t kfrom = USE == kDw ? t.split * p.span : 0;
+  const int64_t kend = USE == kDw && kfrom + p.span < p.K ? kfrom + p.span : p.K;
+  const int64_t len = kend > kfrom ? kend - kfrom : 0;
+  const int blocks = (int)(len / kDK);  // (len is a multiple of kDK)
+  const int stages = USE == kDx ? 2 * blocks : blocks;
+
+  // This lane's sources of the copies: chunk 64 (4 wave + j) + lane of a stage.
+  const bf16 *na[4], *ma[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int id = (wave * 4 + j) * 64 + lane;
+    auto source = [&](bool kc, const bf16* base, int64_t ld, int64_t first, int64_t limit, bool pair) {
+      if (kc) {
+        const int row = id >> 2, c = (id & 3) ^ chunk_swizzle<true>(row);
+        const int64_t r = first + row < limit ? first + row : limit - 1;  // (rows past the end are not stored)
+        return base + r * ld + kfrom + c * 8;
+      }
+      // pair: a wave's 128 columns are 64 of gate, then the same 64 of up
+      const int k = id >> 5, c = (id & 31) ^ chunk_swizzle<false>(k);
+      const int64_t r = first + (pair ? (c >> 4) * 64 + (c & 7) * 8 : c * 8);
+      return base + (kfrom + k) * ld + (r < limit ? r : limit - 8);
+    };
+    const bool up = (USE == kDw && t.mat) || (PAIR && (id & 8));
+    na[j] = source(NKC, up ? p.n1 : p.n0, p.nld0, n0, p.N, PAIR);
+    ma[j] = source(MKC, p.m0, p.mld0, m0, p.M, false);
+  }
+  // to the next stage, and (dx) from the last one of the first segment to the
+  // first of the second
+  const int64_t nstep = NKC ? kDK : kDK * p.nld0, mstep = MKC ? kDK : kDK * p.mld0;
+  const int64_t nturn = USE == kDx ? p.n1 - p.n0 - (int64_t)(blocks - 1) * kDK : 0;
+  const int64_t mturn = USE == kDx ? p.m1 - p.m0 - (int64_t)(blocks - 1) * kDK : 0;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&lds[0][0][0];
+  auto issue = [&](int stage) {
+    const uint32_t at = lds0 + (uint32_t)((stage & 3) * 2 * kDChunks + wave * 256) * 16;
+    const bool turn = USE == kDx && stage + 1 == blocks;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      copy_to_lds(na[j], at + j * 1024);
+      na[j] += turn ? nturn : nstep;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      copy_to_lds(ma[j], at + kDChunks * 16 + j * 1024);
+      ma[j] += turn ? mturn : mstep;
+    }
+  };
+
+  floatx16 acc[4][4] = {};
+  bf16x8 nf[2][4], mf[2][4];
+  auto read = [&](int stage, int ks) {
+    const uint4 *nb = lds[stage & 3][0], *mb = lds[stage & 3][1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) nf[ks][i] = fragment<NKC>(nb, wn * 128 + i * 32, ks, lane);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) mf[ks][j] = fragment<MKC>(mb, wm * 128 + j * 32, ks, lane);
+  };
+  auto multiply = [&](int ks) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(nf[ks][i], mf[ks][j], acc[i][j], 0, 0, 0);
+  };
+
+  // Stage s + 1 is waited for in the middle of stage s: each wave for its own
+  // copies, then for the other waves; after that the buffer of stage s - 1 is
+  // free, which every wave has left.
+  if (stages > 0) {
+    issue(0);
+    if (stages > 1) issue(1);
+    if (stages > 2) {
+      issue(2);
+      asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    asm volatile("s_barrier" ::: "memory");
+    read(0, 0);
+    int s = 0;
+    for (; s + 3 < stages; ++s) {
+      read(s, 1);
+      __builtin_amdgcn_sched_barrier(0);  // the reads first: they land behind the products
+      multiply(0);
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("s_waitcnt vmcnt(8)\n\ts_barrier" ::: "memory");
+      issue(s + 3);
+      read(s + 1, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(1);
+    }
+    for (; s < stages; ++s) {
+      read(s, 1);
+      multiply(0);
+      asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+      read(s + 1 < stages ? s + 1 : s, 0);
+      multiply(1);
+    }
+  }
+  finish<bf16, USE, 4, 4>(p, acc, m0 + wm * 128, n0 + (PAIR ? wn * 64 : wn * 128), t.split, t.mat);
 }
 
 // dW from the row ranges' parts.
@@ -443,46 +619,78 @@ __global__ __launch_bounds__(kFewThreads) void k_glu_few(GluP<E> p) {
 }
 
 // ------------------------------------------------------------------ shapes
-struct Tile {
-  int bm, bn;
-};
-// Large tiles where they fill the chip's 256 CUs, else small ones.
+// Large tiles where they come near to filling the chip's 256 CUs, else small
+// ones.
 template <class E>
 bool large_tiles(int64_t M, int64_t cols) {
   const int64_t bm = sizeof(E) == 2 ? 256 : 128;
   return ((M + bm - 1) / bm) * ((cols + bm - 1) / bm) >= 128;
 }
 
+bool aligned16(const void* p, int64_t ld) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0; }
+
 template <class E, int USE>
-void product(GluP<E> p, int64_t cols, hipStream_t st) {
-  // cols: operand columns of the tiles (gate and up side by side in PAIR uses)
+void product(GluP<E> p, bool large, hipStream_t st) {
   constexpr bool PAIR = USE == kForward || USE == kProject;
   constexpr int L = sizeof(E) == 2 ? 256 : 128;
-  const bool large = large_tiles<E>(p.M, cols);
   const int bm = large ? L : 64, bn = large ? L : 128, per = PAIR ? bn / 2 : bn;
   p.tiles_m = (uint32_t)((p.M + bm - 1) / bm);
   p.tiles_n = (uint32_t)((p.N + per - 1) / per);
   const dim3 grid(p.tiles_m * p.tiles_n * (USE == kDw ? 2 * p.splits : 1));
-  if (large) {
-    if constexpr (sizeof(E) == 2) k_glu<E, 256, 256, 128, 128, 64, 2, USE><<<grid, kThreads, 0, st>>>(p);
-    else k_glu<E, 128, 128, 64, 64, 32, 1, USE><<<grid, kThreads, 0, st>>>(p);
-  } else {
+  if (!large) {
     k_glu<E, 64, 128, 32, 64, sizeof(E) == 2 ? 64 : 32, 1, USE><<<grid, kThreads, 0, st>>>(p);
+  } else if constexpr (sizeof(E) == 4) {
+    k_glu<E, 128, 128, 64, 64, 32, 1, USE><<<grid, kThreads, 0, st>>>(p);
+  } else {
+    // whole chunks and stages: every row (k-contiguous) or k (row-contiguous)
+    // starts at 16 bytes, row-contiguous operands have a multiple of 8 rows,
+    // the reduction is a multiple of 32, and the two matrices share a stride
+    const bool direct = aligned16(p.n0, p.nld0) && aligned16(p.n1, p.nld1) && aligned16(p.m0, p.mld0) &&
+                        aligned16(p.m1, p.mld1) && p.nld0 == p.nld1 && p.mld0 == p.mld1 &&
+                        (USE == kDx || p.N % 8 == 0) && (USE != kDw || p.M % 8 == 0) && p.K % kDK == 0;
+    if (direct) k_glu_direct<USE><<<grid, kThreads, 0, st>>>(p);
+    else k_glu<E, 256, 256, 128, 128, 64, 2, USE><<<grid, kThreads, 0, st>>>(p);
   }
 }
 
-// Row ranges of the weight gradients' products.
+// The weight gradients' products: tiles and row ranges.  As many ranges, of 512
+// rows or more, as make the rounds over the 256 CUs full, against the time
+// that the partial sums take: a tile's 512 rows take a CU about `unit`, and a
+// tile's part takes the whole chip about `join` to write and read.
+struct DwShape {
+  bool large;
+  int64_t rows;     // in the ranges; the rest (bf16 stages are whole) is a part of its own
+  int64_t span;     // rows of a range
+  uint32_t ranges, parts;
+};
 template <class E>
-void dw_splits(const dgen_hip_mlp& a, uint32_t& splits, int64_t& span) {
-  const int64_t L = sizeof(E) == 2 ? 256 : 128;
-  const bool large = large_tiles<E>(a.width, 2 * a.hidden);
-  const int64_t bm = large ? L : 64, bn = large ? L : 128;
-  const int64_t tiles = 2 * ((a.width + bm - 1) / bm) * ((a.hidden + bn - 1) / bn);
-  // about two workgroups a CU, none with fewer than 512 rows
-  int64_t s = std::max<int64_t>(1, std::min<int64_t>((512 + tiles - 1) / tiles, (a.rows + 511) / 512));
-  span = std::max<int64_t>(64, ((a.rows + s - 1) / s + 63) / 64 * 64);
-  splits = (uint32_t)std::max<int64_t>(1, (a.rows + span - 1) / span);
+DwShape dw_shape(const dgen_hip_mlp& a) {
+  constexpr bool kHalf = sizeof(E) == 2;
+  const int64_t L = kHalf ? 256 : 128;
+  auto count = [&](int64_t bm, int64_t bn) {
+    return 2 * ((a.width + bm - 1) / bm) * ((a.hidden + bn - 1) / bn);
+  };
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(a.rows / 512, 32));
+  DwShape d{};
+  d.large = count(L, L) * most >= 128;
+  d.rows = kHalf && d.large ? a.rows / kDK * kDK : a.rows;
+  const int64_t tiles = d.large ? count(L, L) : count(64, 128);
+  const double unit = !d.large ? 4e-6 : kHalf ? 14e-6 : 21e-6, join = d.large ? 0.13e-6 : 0.02e-6;
+  int64_t best = 1;
+  double least = 0;
+  for (int64_t s = 1; s <= most; ++s) {
+    const double rounds = (double)((tiles * s + 255) / 256);
+    const double cost = rounds * ((double)a.rows / (512.0 * (double)s)) * unit + (s > 1 ? (double)(s * tiles) * join : 0);
+    if (s == 1 || cost < least) best = s, least = cost;
+  }
+  d.span = std::max<int64_t>(64, ((d.rows + best - 1) / best + 63) / 64 * 64);
+  d.ranges = (uint32_t)std::max<int64_t>(1, (d.rows + d.span - 1) / d.span);
+  d.parts = d.ranges + (d.rows < a.rows ? 1 : 0);
+  return d;
 }
+
+// Rows of dg and du start at 16 bytes.
+int64_t dg_stride(const dgen_hip_mlp& a) { return (a.hidden + 7) & ~int64_t(7); }
 
 struct MlpWs {
   int64_t dg, du, parts, total;  // bytes
@@ -490,12 +698,9 @@ struct MlpWs {
 MlpWs mlp_ws(const dgen_hip_mlp& a) {
   MlpWs w{};
   const int64_t es = a.type == DGEN_HIP_BF16 ? 2 : 4;
-  uint32_t splits;
-  int64_t span;
-  if (a.type == DGEN_HIP_BF16) dw_splits<bf16>(a, splits, span);
-  else dw_splits<float>(a, splits, span);
-  w.dg = w.du = align256(a.rows * a.hidden * es);
-  w.parts = splits > 1 ? align256((int64_t)splits * 2 * a.width * a.hidden * 4) : 0;
+  const DwShape d = a.type == DGEN_HIP_BF16 ? dw_shape<bf16>(a) : dw_shape<float>(a);
+  w.dg = w.du = align256(a.rows * dg_stride(a) * es);
+  w.parts = d.parts > 1 ? align256((int64_t)d.parts * 2 * a.width * a.hidden * 4) : 0;
   w.total = w.dg + w.du + w.parts;
   return w;
 }
@@ -514,7 +719,7 @@ void mlp_launch(const dgen_hip_mlp& a, bool backward, hipStream_t st) {
       k_glu_few<E><<<dim3((unsigned)((a.hidden + kFewCols - 1) / kFewCols), (unsigned)((a.rows + kFewRows - 1) / kFewRows)),
                      kFewThreads, 0, st>>>(p);
     } else {
-      product<E, kForward>(p, 2 * a.hidden, st);
+      product<E, kForward>(p, large_tiles<E>(a.rows, 2 * a.hidden), st);
     }
     return;
   }
@@ -524,25 +729,34 @@ void mlp_launch(const dgen_hip_mlp& a, bool backward, hipStream_t st) {
   float* parts = (float*)((char*)a.workspace + w.dg + w.du);
   if (a.rows > 0) {
     GluP<E> q = p;
-    q.out0 = dg, q.out1 = du, q.old0 = q.old1 = a.hidden;
+    q.out0 = dg, q.out1 = du, q.old0 = q.old1 = dg_stride(a);
     q.dh = (const E*)a.dh, q.dhld = a.dh_stride;
-    product<E, kProject>(q, 2 * a.hidden, st);
+    product<E, kProject>(q, large_tiles<E>(a.rows, 2 * a.hidden), st);
     q = p;
-    q.m0 = dg, q.m1 = du, q.mld0 = q.mld1 = a.hidden;
+    q.m0 = dg, q.m1 = du, q.mld0 = q.mld1 = dg_stride(a);
     q.N = a.width, q.K = a.hidden;
     q.out0 = (E*)a.dx, q.old0 = a.dx_stride;
-    product<E, kDx>(q, a.width, st);
+    product<E, kDx>(q, large_tiles<E>(a.rows, a.width), st);
   }
   GluP<E> q = p;
-  q.n0 = dg, q.n1 = du, q.nld0 = q.nld1 = a.hidden;
-  q.M = a.width, q.N = a.hidden, q.K = a.rows;
+  const DwShape d = dw_shape<E>(a);
+  q.n0 = dg, q.n1 = du, q.nld0 = q.nld1 = dg_stride(a);
+  q.M = a.width, q.N = a.hidden, q.K = d.rows;
   q.out0 = (E*)a.dw_gate, q.old0 = a.dw_gate_stride, q.out1 = (E*)a.dw_up, q.old1 = a.dw_up_stride;
-  q.parts = parts;
-  dw_splits<E>(a, q.splits, q.span);
-  product<E, kDw>(q, 2 * a.hidden, st);
-  if (q.splits > 1) {
+  q.parts = d.parts > 1 ? parts : nullptr;
+  q.splits = d.ranges, q.span = d.span;
+  product<E, kDw>(q, d.large, st);
+  if (d.rows < a.rows) {
+    GluP<E> r = q;
+    r.n0 += d.rows * r.nld0, r.n1 += d.rows * r.nld1, r.m0 += d.rows * r.mld0, r.m1 = r.m0;
+    r.K = r.span = a.rows - d.rows;
+    r.splits = 1;
+    r.parts += (int64_t)d.ranges * 2 * a.width * a.hidden;
+    product<E, kDw>(r, d.large, st);
+  }
+  if (d.parts > 1) {
     const int64_t n = 2 * a.width * ((a.hidden + 3) / 4);
-    k_glu_join<E><<<dim3((unsigned)((n + 255) / 256)), 256, 0, st>>>(parts, q.splits, a.width, a.hidden, q.out0, q.old0,
+    k_glu_join<E><<<dim3((unsigned)((n + 255) / 256)), 256, 0, st>>>(parts, d.parts, a.width, a.hidden, q.out0, q.old0,
                                                                      q.out1, q.old1);
   }
 }

@@ -122,7 +122,7 @@ def test_backward(gpu, rows, width, hidden, ty, act):
     check_backward(rows, width, hidden, ty, act)
 
 
-@pytest.mark.parametrize("rows,width,hidden", [(2500, 520, 900), (3001, 1100, 300)])
+@pytest.mark.parametrize("rows,width,hidden", [(2500, 520, 900), (3001, 1100, 300), (2085, 512, 992)])
 @pytest.mark.parametrize("ty", TYPES)
 def test_backward_large(gpu, rows, width, hidden, ty):
     """Large tiles and row ranges; repeated calls give the same bits."""
@@ -131,6 +131,28 @@ def test_backward_large(gpu, rows, width, hidden, ty):
     once = Q.gated_mlp_backward(dh.cuda(), x.cuda(), wg.cuda(), wu.cuda())
     for a, b, c in zip(first, again, once):
         assert torch.equal(a, b) and torch.equal(b, c)
+
+
+@pytest.mark.parametrize("rows,width,hidden", [(4096, 64, 1024), (2100, 96, 1920), (9000, 256, 256)])
+def test_aligned_operands(gpu, rows, width, hidden):
+    """bfloat16 tensors that start at 16 bytes with sizes in multiples of 32,
+    as training batches have them, and a number of rows that has not."""
+    ty = torch.bfloat16
+    x, wg, wu, dh = make(rows, width, hidden, ty, 5)
+    h = Q.gated_mlp(x.cuda(), wg.cuda(), wu.cuda())
+    viewed = Q.gated_mlp(view(x), view(wg), view(wu))  # the same by unaligned loads
+    a, b, c = (t.to(F64) for t in (x, wg, wu))
+    f, _ = act64("silu", a @ b)
+    want, mag = f * (a @ c), (a.abs() @ b.abs()) * (a @ c).abs() * 1.2 + f.abs() * (a.abs() @ c.abs())
+    bound = (width + 32) * EPS32 * mag + EPS16 * 1.01 * want.abs() + 1e-30
+    within(h, want, bound, "h")
+    within(viewed, want, bound, "h of views")
+    got = Q.gated_mlp_backward(dh.cuda(), x.cuda(), wg.cuda(), wu.cuda())
+    ref = Q.gated_mlp_backward(view(dh), view(x), view(wg), view(wu))
+    for p, q in zip(got, ref):
+        # both are within the bound of check_backward; between them, rounding
+        scale = q.double().abs().max().item()
+        assert (p.double() - q.double()).abs().max().item() <= 2 * EPS16 * scale
 
 
 def test_gradient_against_differences(gpu):
