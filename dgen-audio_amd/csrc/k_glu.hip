@@ -239,18 +239,21 @@ __device__ __forceinline__ void finish(const GluP<E>& p, const floatx16 (&acc)[N
 
 // ----------------------------------------------------------------- kernel
 // Tile of this workgroup.  Consecutive workgroups go to the eight XCDs in
-// turn; each XCD takes a run of consecutive tiles (n fastest), which share
-// their operand rows in its L2.
+// turn, so each XCD takes a run of consecutive tiles; a run goes through
+// groups of four column tiles, row tiles in turn, so that the tiles an XCD
+// works on at a time (32 of the large ones, one a CU) share eight row tiles
+// and four column tiles in its L2.
 struct TileAt {
   uint32_t n, m, split, mat;
 };
 template <int USE, class E>
 __device__ __forceinline__ TileAt tile_at(const GluP<E>& p) {
-  const uint32_t total = gridDim.x;
-  uint32_t id = blockIdx.x;
-  if (total % 8 == 0) id = (id & 7) * (total / 8) + (id >> 3);
-  const uint32_t tr = id / p.tiles_n, rest = tr / p.tiles_m;
-  return {id % p.tiles_n, tr % p.tiles_m, USE == kDw ? rest % p.splits : 0, USE == kDw ? rest / p.splits : 0};
+  const uint32_t total = gridDim.x, each = total / 8, more = total % 8;
+  const uint32_t xcd = blockIdx.x & 7, id = xcd * each + (xcd < more ? xcd : more) + (blockIdx.x >> 3);
+  const uint32_t plane = p.tiles_n * p.tiles_m, rest = id / plane, at = id - rest * plane;
+  const uint32_t group = at / (4 * p.tiles_m), in = at - group * 4 * p.tiles_m;
+  const uint32_t wide = p.tiles_n - group * 4 < 4 ? p.tiles_n - group * 4 : 4;
+  return {group * 4 + in % wide, in / wide, USE == kDw ? rest % p.splits : 0, USE == kDw ? rest / p.splits : 0};
 }
 
 // BM x BN: output rows and operand columns of a tile; WM x WN: of a wave.
@@ -381,14 +384,18 @@ __global__ __launch_bounds__(kThreads) void k_glu(GluP<E> p) {
 
 // ------------------------------------------------- bf16, aligned operands
 // The same product with operand tiles copied global -> LDS by the load-to-LDS
-// instructions, as they lie in memory: 256 x 256 outputs a workgroup, 128 x 128
-// a wave (256 accumulators a lane), stages of 32 k's in four LDS buffers, two
-// to three of them in flight.  An operand that is contiguous along its rows is
+// instructions, as they lie in memory: 256 x 256 outputs a workgroup of eight
+// waves, 128 x 64 a wave (128 accumulators a lane; two waves a SIMD cover each
+// other's LDS reads and barriers), stages of 32 k's in four LDS buffers, two to
+// three of them in flight.  An operand that is contiguous along its rows is
 // read with the transposing LDS load.  Chunks of 16 bytes are permuted within
 // their LDS rows through the global addresses, so that the fragments' reads
 // spread over the banks: k-contiguous rows (four chunks) by row / 2, row-
-// contiguous k's (32 chunks) by twice the k.
-constexpr int kDT = 256, kDK = 32, kDBufs = 4, kDChunks = kDT * kDK / 8;  // chunks of one operand's stage
+// contiguous k's (32 chunks) by twice the k.  Results go to memory through LDS
+// in whole rows of the tile (stored from the accumulators' layout, 8 bytes to
+// each of 32 rows, a tile took 40 us).
+constexpr int kDM = 256, kDN = 256, kDK = 32, kDBufs = 4, kDThreads = 512;
+constexpr int kDMChunks = kDM * kDK / 8, kDNChunks = kDN * kDK / 8;  // of a stage
 
 typedef short short4v __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) short4v lds_short4;
@@ -405,8 +412,9 @@ template <bool KC>
 __device__ __forceinline__ int chunk_swizzle(int row) { return KC ? (row >> 1) & 3 : (row & 3) << 1; }
 
 // Fragment of 32 rows from `r0` on at k-step ks of a stage.
-template <bool KC>
+template <bool KC, int ROWS>
 __device__ __forceinline__ bf16x8 fragment(const uint4* b, int r0, int ks, int lane) {
+  constexpr int C = ROWS / 8;
   if constexpr (KC) {
     const int r = r0 + (lane & 31), c = ks * 2 + (lane >> 5);
     return __builtin_bit_cast(bf16x8, b[r * 4 + (c ^ chunk_swizzle<true>(r))]);
@@ -420,95 +428,105 @@ __device__ __forceinline__ bf16x8 fragment(const uint4* b, int r0, int ks, int l
     } o;
     const int c = r >> 3, half = (r >> 2) & 1;
     // k + 4 has the same swizzle (k & 3)
-    const uint4* p = b + k * 32 + (c ^ chunk_swizzle<false>(k));
+    const uint4* p = b + k * C + (c ^ chunk_swizzle<false>(k));
     o.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)((const short*)p + half * 4));
-    o.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)((const short*)(p + 4 * 32) + half * 4));
+    o.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)((const short*)(p + 4 * C) + half * 4));
     return __builtin_bit_cast(bf16x8, o);
   }
 }
 
 template <int USE>
-__global__ __launch_bounds__(kThreads, 1) void k_glu_direct(GluP<bf16> p) {
+__global__ __launch_bounds__(kDThreads, 2) void k_glu_direct(GluP<bf16> p) {
   constexpr bool PAIR = USE == kForward || USE == kProject;
   constexpr bool NKC = USE == kDx, MKC = USE != kDw;
-  __shared__ __align__(1024) uint4 lds[kDBufs][2][kDChunks];
+  constexpr int NF = 2, MF = 4, NJ = kDNChunks / kDThreads, MJ = kDMChunks / kDThreads;
+  __shared__ __align__(1024) uint4 lds[kDBufs][kDNChunks + kDMChunks];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wn = wave & 1, wm = wave >> 1;
+  const int wn = wave & 3, wm = wave >> 2;
   const TileAt t = tile_at<USE>(p);
-  const int64_t n0 = (int64_t)t.n * (PAIR ? kDT / 2 : kDT), m0 = (int64_t)t.m * kDT;
+  const int64_t n0 = (int64_t)t.n * (PAIR ? kDN / 2 : kDN), m0 = (int64_t)t.m * kDM;
   const int64_t kfrom = USE == kDw ? t.split * p.span : 0;
   const int64_t kend = USE == kDw && kfrom + p.span < p.K ? kfrom + p.span : p.K;
   const int64_t len = kend > kfrom ? kend - kfrom : 0;
   const int blocks = (int)(len / kDK);  // (len is a multiple of kDK)
   const int stages = USE == kDx ? 2 * blocks : blocks;
 
-  // This lane's sources of the copies: chunk 64 (4 wave + j) + lane of a stage.
-  const bf16 *na[4], *ma[4];
+  // This lane's sources of the copies: chunk 64 (J wave + j) + lane of a stage.
+  const bf16 *na[NJ], *ma[MJ];
+  auto source = [&](bool kc, int id, int chunks, const bf16* b0, const bf16* b1, int64_t ld, int64_t first,
+                    int64_t limit, bool pair) {
+    if (kc) {
+      const int row = id >> 2, c = (id & 3) ^ chunk_swizzle<true>(row);
+      const int64_t r = first + row < limit ? first + row : limit - 1;  // (rows past the end are not stored)
+      return b0 + r * ld + kfrom + c * 8;
+    }
+    // pair: a wave's 64 columns are 32 of gate, then the same 32 of up
+    const int k = id / chunks, c = (id % chunks) ^ chunk_swizzle<false>(k);
+    const int64_t r = first + (pair ? (c >> 3) * 32 + (c & 3) * 8 : c * 8);
+    return (pair && (c & 4) ? b1 : b0) + (kfrom + k) * ld + (r < limit ? r : limit - 8);
+  };
+  const bf16* nbase = USE == kDw && t.mat ? p.n1 : p.n0;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int id = (wave * 4 + j) * 64 + lane;
-    auto source = [&](bool kc, const bf16* base, int64_t ld, int64_t first, int64_t limit, bool pair) {
-      if (kc) {
-        const int row = id >> 2, c = (id & 3) ^ chunk_swizzle<true>(row);
-        const int64_t r = first + row < limit ? first + row : limit - 1;  // (rows past the end are not stored)
-        return base + r * ld + kfrom + c * 8;
-      }
-      // pair: a wave's 128 columns are 64 of gate, then the same 64 of up
-      const int k = id >> 5, c = (id & 31) ^ chunk_swizzle<false>(k);
-      const int64_t r = first + (pair ? (c >> 4) * 64 + (c & 7) * 8 : c * 8);
-      return base + (kfrom + k) * ld + (r < limit ? r : limit - 8);
-    };
-    const bool up = (USE == kDw && t.mat) || (PAIR && (id & 8));
-    na[j] = source(NKC, up ? p.n1 : p.n0, p.nld0, n0, p.N, PAIR);
-    ma[j] = source(MKC, p.m0, p.mld0, m0, p.M, false);
-  }
+  for (int j = 0; j < NJ; ++j) na[j] = source(NKC, (wave * NJ + j) * 64 + lane, kDN / 8, nbase, p.n1, p.nld0, n0, p.N, PAIR);
+#pragma unroll
+  for (int j = 0; j < MJ; ++j) ma[j] = source(MKC, (wave * MJ + j) * 64 + lane, kDM / 8, p.m0, p.m0, p.mld0, m0, p.M, false);
   // to the next stage, and (dx) from the last one of the first segment to the
   // first of the second
   const int64_t nstep = NKC ? kDK : kDK * p.nld0, mstep = MKC ? kDK : kDK * p.mld0;
   const int64_t nturn = USE == kDx ? p.n1 - p.n0 - (int64_t)(blocks - 1) * kDK : 0;
   const int64_t mturn = USE == kDx ? p.m1 - p.m0 - (int64_t)(blocks - 1) * kDK : 0;
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&lds[0][0][0];
-  auto issue = [&](int stage) {
-    const uint32_t at = lds0 + (uint32_t)((stage & 3) * 2 * kDChunks + wave * 256) * 16;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&lds[0][0];
+  auto issue = [&](int stage, int buf) {
+    const uint32_t at = lds0 + (uint32_t)(buf * (kDNChunks + kDMChunks)) * 16;
     const bool turn = USE == kDx && stage + 1 == blocks;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      copy_to_lds(na[j], at + j * 1024);
+    for (int j = 0; j < NJ; ++j) {
+      copy_to_lds(na[j], at + (uint32_t)(wave * NJ + j) * 1024);
       na[j] += turn ? nturn : nstep;
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      copy_to_lds(ma[j], at + kDChunks * 16 + j * 1024);
+    for (int j = 0; j < MJ; ++j) {
+      copy_to_lds(ma[j], at + kDNChunks * 16 + (uint32_t)(wave * MJ + j) * 1024);
       ma[j] += turn ? mturn : mstep;
     }
   };
 
-  floatx16 acc[4][4] = {};
-  bf16x8 nf[2][4], mf[2][4];
-  auto read = [&](int stage, int ks) {
-    const uint4 *nb = lds[stage & 3][0], *mb = lds[stage & 3][1];
+  // project: the tile of dh, 128 rows to each of the two buffers that fall
+  // free before the last stages (rows of 16 chunks, permuted by row % 16)
+  auto copy_dh = [&]() {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) nf[ks][i] = fragment<NKC>(nb, wn * 128 + i * 32, ks, lane);
+    for (int k = 0; k < kDM * 16 / kDThreads; ++k) {
+      const int id = k * kDThreads + wave * 64 + lane, row = id >> 4, c = (id & 15) ^ (row & 15);
+      const int64_t m = m0 + row < p.M ? m0 + row : p.M - 1, n = n0 + c * 8 < p.N ? n0 + c * 8 : p.N - 8;
+      const int buf = (stages + (row >> 7)) & 3;
+      copy_to_lds(p.dh + m * p.dhld + n,
+                  lds0 + (uint32_t)(__builtin_amdgcn_readfirstlane(buf) * (kDNChunks + kDMChunks)) * 16 +
+                      (uint32_t)((k * kDThreads + wave * 64) & 2047) * 16);
+    }
+  };
+
+  floatx16 acc[NF][MF] = {};
+  bf16x8 nf[2][NF], mf[2][MF];
+  auto read = [&](int st, int ks) {
+    const uint4 *nb = lds[st & 3], *mb = nb + kDNChunks;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) mf[ks][j] = fragment<MKC>(mb, wm * 128 + j * 32, ks, lane);
+    for (int i = 0; i < NF; ++i) nf[ks][i] = fragment<NKC, kDN>(nb, wn * 64 + i * 32, ks, lane);
+#pragma unroll
+    for (int j = 0; j < MF; ++j) mf[ks][j] = fragment<MKC, kDM>(mb, wm * 128 + j * 32, ks, lane);
   };
   auto multiply = [&](int ks) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < NF; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int j = 0; j < MF; ++j)
         acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(nf[ks][i], mf[ks][j], acc[i][j], 0, 0, 0);
   };
-
-  // Stage s + 1 is waited for in the middle of stage s: each wave for its own
-  // copies, then for the other waves; after that the buffer of stage s - 1 is
-  // free, which every wave has left.
   if (stages > 0) {
-    issue(0);
-    if (stages > 1) issue(1);
+    issue(0, 0);
+    if (stages > 1) issue(1, 1);
     if (stages > 2) {
-      issue(2);
-      asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+      issue(2, 2);
+      asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
     } else {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
@@ -517,24 +535,113 @@ __global__ __launch_bounds__(kThreads, 1) void k_glu_direct(GluP<bf16> p) {
     int s = 0;
     for (; s + 3 < stages; ++s) {
       read(s, 1);
-      __builtin_amdgcn_sched_barrier(0);  // the reads first: they land behind the products
+      __builtin_amdgcn_sched_barrier(0);
       multiply(0);
       __builtin_amdgcn_sched_barrier(0);
-      asm volatile("s_waitcnt vmcnt(8)\n\ts_barrier" ::: "memory");
-      issue(s + 3);
+      asm volatile("s_waitcnt vmcnt(4)\n\ts_barrier" ::: "memory");
+      issue(s + 3, (s + 3) & 3);
       read(s + 1, 0);
       __builtin_amdgcn_sched_barrier(0);
       multiply(1);
     }
+    if (USE == kProject && stages == 1) copy_dh();
     for (; s < stages; ++s) {
       read(s, 1);
       multiply(0);
       asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+      if (USE == kProject && s + 2 == stages) copy_dh();
       read(s + 1 < stages ? s + 1 : s, 0);
       multiply(1);
     }
   }
-  finish<bf16, USE, 4, 4>(p, acc, m0 + wm * 128, n0 + (PAIR ? wn * 64 : wn * 128), t.split, t.mat);
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+
+  // The tile's rows in LDS: chunk c of row r (of C chunks) at r C + (c ^ r % 16).
+  // Register 4 q + e of acc[i][j]: column 8 q + 4 (lane / 32) + e of fragment
+  // i's 32, row lane % 32 of fragment j's.
+  const int r32 = lane & 31, hi = lane >> 5;
+  uint4* tile = lds[0];
+  if constexpr (USE == kDw) {
+    // fp32 parts, 128 rows at a time
+    float* out = p.parts + ((int64_t)t.split * 2 + t.mat) * p.M * p.N;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      if (half) __syncthreads();
+      if (wm == half) {
+#pragma unroll
+        for (int j = 0; j < MF; ++j)
+#pragma unroll
+          for (int i = 0; i < NF; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int r = j * 32 + r32, c = wn * 16 + i * 8 + 2 * q + hi;
+              const floatx16& v = acc[i][j];
+              tile[r * 64 + (c ^ (r & 15))] = __builtin_bit_cast(
+                  uint4, make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]));
+            }
+      }
+      __syncthreads();
+#pragma unroll 4
+      for (int k = 0; k < 128 * 64 / kDThreads; ++k) {
+        const int id = threadIdx.x + k * kDThreads, r = id >> 6, c = id & 63;
+        const int64_t m = m0 + half * 128 + r, n = n0 + c * 4;
+        if (m < p.M && n < p.N) *reinterpret_cast<uint4*>(out + m * p.N + n) = tile[r * 64 + (c ^ (r & 15))];
+      }
+    }
+  } else {
+    constexpr int C = PAIR ? 16 : 32;  // chunks of a row
+    // project: dh lies where dg goes, du in the other two buffers
+    uint4* second = PAIR ? lds[(stages + 2) & 3] : nullptr;
+    uint4* third = PAIR ? lds[(stages + 3) & 3] : nullptr;
+    uint4 *first0 = USE == kProject ? lds[stages & 3] : tile, *first1 = USE == kProject ? lds[(stages + 1) & 3] : tile + 128 * C;
+#pragma unroll
+    for (int j = 0; j < MF; ++j)
+#pragma unroll
+      for (int i = 0; i < (PAIR ? 1 : NF); ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int r = j * 32 + r32, c = (PAIR ? wn * 4 : wn * 8 + i * 4) + q;
+          const int at = r * C + (c ^ (r & 15));
+          Four<bf16>* o = reinterpret_cast<Four<bf16>*>((wm ? first1 : first0) + at) + hi;
+          Four<bf16> w;
+          if constexpr (PAIR) {
+            float slope;
+            if constexpr (USE == kForward) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float v = act_of(p.act, acc[0][j][4 * q + e], slope);
+                w.e[e] = from_f32<bf16>(v * acc[NF / 2][j][4 * q + e]);
+              }
+            } else {
+              const Four<bf16> d4 = *o;
+              Four<bf16> x;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float v = act_of(p.act, acc[0][j][4 * q + e], slope), d = to_f32(d4.e[e]);
+                w.e[e] = from_f32<bf16>(d * acc[NF / 2][j][4 * q + e] * slope);
+                x.e[e] = from_f32<bf16>(d * v);
+              }
+              *(reinterpret_cast<Four<bf16>*>((wm ? third : second) + at) + hi) = x;
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w.e[e] = from_f32<bf16>(acc[i][j][4 * q + e]);
+          }
+          *o = w;
+        }
+    __syncthreads();
+    auto put = [&](const uint4* lo, const uint4* up, bf16* out, int64_t ld) {
+#pragma unroll 4
+      for (int k = 0; k < kDM * C / kDThreads; ++k) {
+        const int id = threadIdx.x + k * kDThreads, row = id / C, c = id % C, r = row & 127;
+        const int64_t m = m0 + row, n = n0 + c * 8;
+        const uint4 v = (row >> 7 ? up : lo)[r * C + (c ^ (r & 15))];
+        if (m < p.M && n < p.N) *reinterpret_cast<Vec<bf16, 8>*>(out + m * ld + n) = __builtin_bit_cast(Vec<bf16, 8>, v);
+      }
+    };
+    put(first0, first1, p.out0, p.old0);
+    if (USE == kProject) put(second, third, p.out1, p.old1);
+  }
 }
 
 // dW from the row ranges' parts.
@@ -644,12 +751,19 @@ void product(GluP<E> p, bool large, hipStream_t st) {
   } else {
     // whole chunks and stages: every row (k-contiguous) or k (row-contiguous)
     // starts at 16 bytes, row-contiguous operands have a multiple of 8 rows,
-    // the reduction is a multiple of 32, and the two matrices share a stride
+    // results a multiple of 8 columns, the reduction is a multiple of 32, and
+    // the two matrices share a stride
     const bool direct = aligned16(p.n0, p.nld0) && aligned16(p.n1, p.nld1) && aligned16(p.m0, p.mld0) &&
                         aligned16(p.m1, p.mld1) && p.nld0 == p.nld1 && p.mld0 == p.mld1 &&
-                        (USE == kDx || p.N % 8 == 0) && (USE != kDw || p.M % 8 == 0) && p.K % kDK == 0;
-    if (direct) k_glu_direct<USE><<<grid, kThreads, 0, st>>>(p);
-    else k_glu<E, 256, 256, 128, 128, 64, 2, USE><<<grid, kThreads, 0, st>>>(p);
+                        p.N % 8 == 0 && (USE != kDw || p.M % 8 == 0) && p.K % kDK == 0 && p.K > 0 &&
+                        (USE != kProject || aligned16(p.dh, p.dhld)) && (USE != kDw || p.parts);
+    if (direct) {
+      p.tiles_m = (uint32_t)((p.M + kDM - 1) / kDM);
+      p.tiles_n = (uint32_t)((p.N + (PAIR ? kDN / 2 : kDN) - 1) / (PAIR ? kDN / 2 : kDN));
+      k_glu_direct<USE><<<dim3(p.tiles_m * p.tiles_n * (USE == kDw ? 2 * p.splits : 1)), kDThreads, 0, st>>>(p);
+    } else {
+      k_glu<E, 256, 256, 128, 128, 64, 2, USE><<<grid, kThreads, 0, st>>>(p);
+    }
   }
 }
 
@@ -662,6 +776,7 @@ struct DwShape {
   int64_t rows;     // in the ranges; the rest (bf16 stages are whole) is a part of its own
   int64_t span;     // rows of a range
   uint32_t ranges, parts;
+  bool in_parts;    // the products leave fp32 parts (else they write the gradients)
 };
 template <class E>
 DwShape dw_shape(const dgen_hip_mlp& a) {
@@ -686,6 +801,7 @@ DwShape dw_shape(const dgen_hip_mlp& a) {
   d.span = std::max<int64_t>(64, ((d.rows + best - 1) / best + 63) / 64 * 64);
   d.ranges = (uint32_t)std::max<int64_t>(1, (d.rows + d.span - 1) / d.span);
   d.parts = d.ranges + (d.rows < a.rows ? 1 : 0);
+  d.in_parts = d.parts > 1 || (kHalf && d.large);
   return d;
 }
 
@@ -700,7 +816,7 @@ MlpWs mlp_ws(const dgen_hip_mlp& a) {
   const int64_t es = a.type == DGEN_HIP_BF16 ? 2 : 4;
   const DwShape d = a.type == DGEN_HIP_BF16 ? dw_shape<bf16>(a) : dw_shape<float>(a);
   w.dg = w.du = align256(a.rows * dg_stride(a) * es);
-  w.parts = d.parts > 1 ? align256((int64_t)d.parts * 2 * a.width * a.hidden * 4) : 0;
+  w.parts = d.in_parts ? align256((int64_t)d.parts * 2 * a.width * a.hidden * 4) : 0;
   w.total = w.dg + w.du + w.parts;
   return w;
 }
@@ -743,7 +859,7 @@ void mlp_launch(const dgen_hip_mlp& a, bool backward, hipStream_t st) {
   q.n0 = dg, q.n1 = du, q.nld0 = q.nld1 = dg_stride(a);
   q.M = a.width, q.N = a.hidden, q.K = d.rows;
   q.out0 = (E*)a.dw_gate, q.old0 = a.dw_gate_stride, q.out1 = (E*)a.dw_up, q.old1 = a.dw_up_stride;
-  q.parts = d.parts > 1 ? parts : nullptr;
+  q.parts = d.in_parts ? parts : nullptr;
   q.splits = d.ranges, q.span = d.span;
   product<E, kDw>(q, d.large, st);
   if (d.rows < a.rows) {
@@ -754,7 +870,7 @@ void mlp_launch(const dgen_hip_mlp& a, bool backward, hipStream_t st) {
     r.parts += (int64_t)d.ranges * 2 * a.width * a.hidden;
     product<E, kDw>(r, d.large, st);
   }
-  if (d.parts > 1) {
+  if (d.in_parts) {
     const int64_t n = 2 * a.width * ((a.hidden + 3) / 4);
     k_glu_join<E><<<dim3((unsigned)((n + 255) / 256)), 256, 0, st>>>(parts, d.parts, a.width, a.hidden, q.out0, q.old0,
                                                                      q.out1, q.old1);
