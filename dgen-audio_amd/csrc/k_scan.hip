@@ -33,7 +33,8 @@ constexpr int kWaves = 4, kThreads = 64 * kWaves, kChannels = 16 * kWaves;
 constexpr int kTile = 32;  // frames staged at a time, forward
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Frames of a backward tile: its states and decays are 2 S registers a frame.
+// Frames of a backward tile: its decays are S registers a frame, its states S
+// LDS words a lane and frame (64 KB a workgroup at S = 4, two workgroups a CU).
 template <int S>
 constexpr int bwd_tile() { return S <= 4 ? 16 : 64 / S; }
 
@@ -135,16 +136,17 @@ template <class E, int FRAMES, int NP>
 struct Shared {
   static constexpr int K = (FRAMES * 2 * NP + kThreads - 1) / kThreads;
   float v[K];
-  __device__ __forceinline__ void load(const ScanP<E>& p, const Place& w, int64_t t0, int frames) {
+  __device__ __forceinline__ void load(const ScanP<E>& p, const Place& w, int64_t t0) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int i = threadIdx.x + k * kThreads, row = i / (2 * NP), col = i % (2 * NP), n = col % NP;
-      const int64_t t = t0 + row;
-      v[k] = 0.f;
-      if (row < frames && t < w.live && n < p.N) {
-        const Rows<const E>& m = col < NP ? p.B : p.C;
-        v[k] = to_f32(m.p[w.b * m.b + t * m.t + n]);
-      }
+      // (without a branch: what lies outside is loaded from inside and zeroed)
+      const int64_t left = w.live - 1 - t0;
+      const bool in = row <= left && n < p.N;
+      const uint32_t r = row < left ? row : (uint32_t)left, c = n < p.N ? n : 0;
+      const Rows<const E>& m = col < NP ? p.B : p.C;
+      const float x = to_f32((m.p + w.b * m.b + t0 * m.t)[r * (uint32_t)m.t + c]);
+      v[k] = in ? x : 0.f;
     }
   }
   __device__ __forceinline__ void store(float* lds) const {
@@ -156,16 +158,40 @@ struct Shared {
   }
 };
 
-// One lane's frames of a tile: frame 4 g + q of the tile for g < G.
-template <class E, int G>
-__device__ __forceinline__ void load_frames(const Rows<const E>& m, const Place& w, int64_t t0, float (&o)[G]) {
-  const E* p = m.p + w.b * m.b + w.d;
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-    const int64_t t = t0 + 4 * g + w.q;
-    o[g] = w.on && t < w.live ? to_f32(p[t * m.t]) : 0.f;
+// One lane's place in a tile of a sequence tensor: its channel and the first
+// of its frames, as an offset from the tile's first frame (the host checks
+// that it fits).  Frames 4 g + q of the tile are loaded for g < G without any
+// branch: past the sequence's end the last frame is loaded again, and lanes
+// past the last channel take that one; both are left out by their steps and
+// gradients being set to 0.
+template <class E>
+struct Lane {
+  const E* seq;  // the sequence's first frame
+  int64_t t;     // elements between frames
+  uint32_t at;   // q t + d
+  uint32_t d;
+  __device__ __forceinline__ Lane(const Rows<const E>& m, const Place& w, int64_t D) {
+    seq = m.p + w.b * m.b;
+    t = m.t;
+    d = (uint32_t)(w.on ? w.d : D - 1);
+    at = (uint32_t)w.q * (uint32_t)m.t + d;
   }
-}
+  template <int G>
+  __device__ __forceinline__ void load(const Place& w, int64_t t0, float (&o)[G]) const {
+    const E* p = seq + t0 * t;
+    if (t0 + 4 * G <= w.live) {
+#pragma unroll
+      for (int g = 0; g < G; ++g) o[g] = to_f32((p + 4 * g * t)[at]);
+    } else {
+      const uint32_t last = (uint32_t)(w.live - 1 - t0);
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const uint32_t f = 4 * g + w.q;
+        o[g] = to_f32(p[(f < last ? f : last) * (uint32_t)t + d]);
+      }
+    }
+  }
+};
 
 enum Mode { kWhole, kSummary, kReplay, kSummaryBoth };
 
@@ -199,14 +225,17 @@ __global__ __launch_bounds__(kThreads) void k_scan(ScanP<E> p) {
   float sum = 0.f;
   float x[G], dt[G], z[G], dy[G];
   Shared<E, kTile, NP> bcv;
+  const Lane<E> lx(p.x, w, p.D), ldt(p.dt, w, p.D), lz(p.z, w, p.D), ldy(p.dy, w, p.D);
   auto fetch = [&](int64_t t0) {
-    bcv.load(p, w, t0, kTile);
-    load_frames<E, G>(p.x, w, t0, x);
-    load_frames<E, G>(p.dt, w, t0, dt);
-    if ((OUT || ADJ) && p.z.p) load_frames<E, G>(p.z, w, t0, z);
-    if (ADJ) load_frames<E, G>(p.dy, w, t0, dy);
+    bcv.load(p, w, t0);
+    lx.load(w, t0, x);
+    ldt.load(w, t0, dt);
+    if ((OUT || ADJ) && p.z.p) lz.load(w, t0, z);
+    if (ADJ) ldy.load(w, t0, dy);
   };
-  fetch(w.begin);
+  if (w.begin < w.live) fetch(w.begin);
+  E* const yrow = p.y.p + w.b * p.y.b;
+  const uint32_t yat = (uint32_t)w.q * (uint32_t)p.y.t + (uint32_t)w.d;
   int buf = 0;
   for (int64_t t0 = w.begin; t0 < w.live; t0 += kTile, buf ^= 1) {
     float* lds = bc[buf];
@@ -223,10 +252,11 @@ __global__ __launch_bounds__(kThreads) void k_scan(ScanP<E> p) {
       const int64_t t = t0 + 4 * g + w.q;
       const bool ok = w.on && t < w.live;
       float slope;
-      const float step = ok ? softplus_accurate(cdt[g] + bias, slope) : 0.f, u = step * cx[g];
+      const float soft = softplus_accurate(cdt[g] + bias, slope);
+      const float step = ok ? soft : 0.f, u = ok ? soft * cx[g] : 0.f;
       float gate = 1.f, up = 0.f;
       if ((OUT || ADJ) && p.z.p) gate = silu(cz[g]);
-      if (ADJ) up = cdy[g] * gate;
+      if (ADJ) up = ok ? cdy[g] * gate : 0.f;
       if (!OUT) sum += step;
       float y = 0.f;
       auto frame = [&](auto jc) {
@@ -255,7 +285,7 @@ __global__ __launch_bounds__(kThreads) void k_scan(ScanP<E> p) {
       frame(std::integral_constant<int, 1>{});
       frame(std::integral_constant<int, 2>{});
       frame(std::integral_constant<int, 3>{});
-      if (OUT && ok) p.y.p[w.b * p.y.b + t * p.y.t + w.d] = from_f32<E>(fmaf(skip, cx[g], y) * gate);
+      if (OUT && ok) (yrow + (t0 + 4 * g) * p.y.t)[yat] = from_f32<E>(fmaf(skip, cx[g], y) * gate);
     }
   }
   if (!w.on) return;
@@ -353,10 +383,12 @@ __device__ __forceinline__ void channel_sum(const float (&v)[V], float (&w)[kept
 }
 
 template <class E, int S>
-__global__ __launch_bounds__(kThreads) void k_scan_bwd(ScanP<E> p) {
+__global__ __launch_bounds__(kThreads, 2) void k_scan_bwd(ScanP<E> p) {
   constexpr int NP = 4 * S, TL = bwd_tile<S>(), G = TL / 4;
   __shared__ __align__(16) float bc[2][TL * 2 * NP];
   __shared__ float red[TL][kWaves][2 * NP];
+  // the tile's states before each frame, a lane's own
+  __shared__ __align__(16) float hs[TL][kThreads][S];
   const Place w = place_of(p);
   const int64_t tiles_all = (p.T + TL - 1) / TL, tile0 = w.begin / TL;
   const int64_t tiles = w.live > w.begin ? (w.live - w.begin + TL - 1) / TL : 0;
@@ -378,16 +410,18 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(ScanP<E> p) {
     read_states<S>(p.gends + at, g);
   }
   float dskip = 0.f, dbias = 0.f;
-  float* ck = p.ckpt + ((w.b * tiles_all + tile0) * p.D + w.d) * NP + w.q * S;
+  // (lanes past the last channel read that one's states and store none)
+  float* ck = p.ckpt + ((w.b * tiles_all + tile0) * p.D + (w.on ? w.d : p.D - 1)) * NP + w.q * S;
   Shared<E, TL, NP> bcv;
+  const Lane<E> lx(p.x, w, p.D), ldt(p.dt, w, p.D), lz(p.z, w, p.D), ldy(p.dy, w, p.D);
 
   // forward over the chunk: the state before every tile
   {
     float x[G], dt[G];
     auto fetch = [&](int64_t t0) {
-      bcv.load(p, w, t0, TL);
-      load_frames<E, G>(p.x, w, t0, x);
-      load_frames<E, G>(p.dt, w, t0, dt);
+      bcv.load(p, w, t0);
+      lx.load(w, t0, x);
+      ldt.load(w, t0, dt);
     };
     if (tiles > 0) fetch(w.begin);
     for (int64_t i = 0; i < tiles; ++i) {
@@ -404,7 +438,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(ScanP<E> p) {
       for (int k = 0; k < G; ++k) {
         float slope;
         // (every frame of a tile that another follows is inside the sequence)
-        const float step = w.on ? softplus_accurate(cdt[k] + bias, slope) : 0.f, u = step * cx[k];
+        const float step = softplus_accurate(cdt[k] + bias, slope), u = step * cx[k];
         auto frame = [&](auto jc) {
           constexpr int J = decltype(jc)::value;
           const float sj = quad<J>(step) * kLog2e, uj = quad<J>(u);
@@ -422,15 +456,18 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(ScanP<E> p) {
     __syncthreads();
   }
 
+  E *const dxr = p.dx.p + w.b * p.dx.b, *const ddtr = p.ddt.p + w.b * p.ddt.b, *const dzr = p.dz.p + w.b * p.dz.b;
+  const uint32_t q = w.q, d = (uint32_t)w.d, dxat = q * (uint32_t)p.dx.t + d, ddtat = q * (uint32_t)p.ddt.t + d,
+                 dzat = q * (uint32_t)p.dz.t + d;
   float x[G], dt[G], z[G], dy[G], hn[S];
   auto fetch = [&](int64_t i) {
     const int64_t t0 = w.begin + i * TL;
-    bcv.load(p, w, t0, TL);
-    load_frames<E, G>(p.x, w, t0, x);
-    load_frames<E, G>(p.dt, w, t0, dt);
-    if (p.z.p) load_frames<E, G>(p.z, w, t0, z);
-    load_frames<E, G>(p.dy, w, t0, dy);
-    if (w.on) read_states<S>(ck + i * p.D * NP, hn);
+    bcv.load(p, w, t0);
+    lx.load(w, t0, x);
+    ldt.load(w, t0, dt);
+    if (p.z.p) lz.load(w, t0, z);
+    ldy.load(w, t0, dy);
+    read_states<S>(ck + i * p.D * NP, hn);
   };
 #pragma unroll
   for (int s = 0; s < S; ++s) hn[s] = 0.f;
@@ -447,15 +484,15 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(ScanP<E> p) {
       const bool ok = w.on && t0 + 4 * k + w.q < w.live;
       cx[k] = x[k], cz[k] = z[k], cdy[k] = dy[k];
       step[k] = softplus_accurate(dt[k] + bias, slope[k]);
-      if (!ok) step[k] = slope[k] = 0.f;
       u[k] = step[k] * cx[k];
       up[k] = p.z.p ? cdy[k] * silu(cz[k]) : cdy[k];
+      if (!ok) step[k] = slope[k] = u[k] = up[k] = 0.f;
     }
     __syncthreads();
     if (i > 0) fetch(i - 1);
 
     // the tile's states and decays
-    float hs[TL][S], as[TL][S];
+    float as[TL][S];
 #pragma unroll
     for (int k = 0; k < G; ++k) {
       y[k] = 0.f;
@@ -466,10 +503,10 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(ScanP<E> p) {
         float bv[S], cv[S], yj = 0.f;
         read_states<S>(row, bv);
         read_states<S>(row + NP, cv);
+        write_states<S>(hs[4 * k + J][threadIdx.x], h);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
           const float e = __builtin_amdgcn_exp2f(sj * a[s]);
-          hs[4 * k + J][s] = h[s];
           as[4 * k + J][s] = e;
           h[s] = fmaf(e, h[s], uj * bv[s]);
           yj = fmaf(cv[s], h[s], yj);
@@ -487,13 +524,14 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(ScanP<E> p) {
     for (int k = G - 1; k >= 0; --k) {
       float gb = 0.f, ga = 0.f;
       auto frame = [&](auto jc) {
-        constexpr int J = decltype(jc)::value, F = 4 * 0 + J;
-        const int f = 4 * k + F;
+        constexpr int J = decltype(jc)::value;
+        const int f = 4 * k + J;
         const float sj = quad<J>(step[k]), uj = quad<J>(u[k]), dj = quad<J>(up[k]);
         const float* row = lds + f * 2 * NP + w.q * S;
-        float bv[S], cv[S], v[2 * S], gbj = 0.f, gaj = 0.f;
+        float bv[S], cv[S], hb[S], v[2 * S], gbj = 0.f, gaj = 0.f;
         read_states<S>(row, bv);
         read_states<S>(row + NP, cv);
+        read_states<S>(hs[f][threadIdx.x], hb);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
           g[s] = fmaf(cv[s], dj, g[s]);
@@ -501,7 +539,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(ScanP<E> p) {
           v[S + s] = h[s] * dj;   // dC
           gbj = fmaf(g[s], bv[s], gbj);
           g[s] *= as[f][s];       // the adjoint of the state before
-          h[s] = hs[f][s];
+          h[s] = hb[s];
           const float gh = g[s] * h[s];
           gaj = fmaf(gh, a[s], gaj);
           dA[s] = fmaf(gh, sj, dA[s]);
@@ -529,10 +567,10 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(ScanP<E> p) {
         const float draw = fmaf(gb, cx[k], ga) * slope[k];
         dbias += draw;
         dskip = fmaf(up[k], cx[k], dskip);
-        p.dx.p[w.b * p.dx.b + t * p.dx.t + w.d] = from_f32<E>(fmaf(step[k], gb, skip * up[k]));
-        p.ddt.p[w.b * p.ddt.b + t * p.ddt.t + w.d] = from_f32<E>(draw);
+        (dxr + (t0 + 4 * k) * p.dx.t)[dxat] = from_f32<E>(fmaf(step[k], gb, skip * up[k]));
+        (ddtr + (t0 + 4 * k) * p.ddt.t)[ddtat] = from_f32<E>(draw);
         if (p.z.p)
-          p.dz.p[w.b * p.dz.b + t * p.dz.t + w.d] =
+          (dzr + (t0 + 4 * k) * p.dz.t)[dzat] =
               from_f32<E>(cdy[k] * fmaf(skip, cx[k], y[k]) * silu_grad(cz[k], sigmoid(cz[k])));
       }
     }
@@ -693,6 +731,9 @@ int scan_run(const dgen_hip_scan& a, bool backward, hipStream_t st, bool dry) {
                "%s: batch %lld x T %lld x D %lld x N %lld is too large for one call", what, (long long)a.batch,
                (long long)a.T, (long long)a.D, (long long)a.N);
   DGEN_REQUIRE(a.A, "%s: null A", what);
+  for (const dgen_hip_seq* v : {&a.x, &a.dt, &a.z, &a.B, &a.C, &a.y, &a.dy, &a.dx, &a.ddt, &a.dz, &a.dB, &a.dC})
+    DGEN_REQUIRE(v->stride_t < (1 << 26), "%s: stride of %lld between frames, at most 2^26", what,
+                 (long long)v->stride_t);  // (a tile's offsets are 32 bits: 32 frames)
   const bool empty = a.batch == 0;
   for (const dgen_hip_seq* v : {&a.x, &a.dt, &a.B, &a.C})
     DGEN_REQUIRE((v->data || empty) && seq_readable(*v), "%s: x, dt, B or C missing or with a negative stride", what);
