@@ -41,7 +41,8 @@ constexpr int bwd_tile() { return S <= 4 ? 16 : 64 / S; }
 template <class E>
 struct Rows {  // [batch][time][.], contiguous last axis
   E* p;
-  int64_t b, t;
+  int64_t b;
+  int t;
 };
 
 template <class E>
@@ -51,19 +52,18 @@ struct ScanP {
   const float *A, *skip, *bias, *state;
   const int32_t* lengths;
   float* state_out;
-  int64_t T, D, N, chunk, chunks, nd;  // nd: blocks of 64 channels
+  int T, D, N, chunk, chunks, nd, batch;  // nd: blocks of 64 channels
   float* sums;                         // [batch][chunks][D]: summed steps
   float* ends;                         // [batch][chunks][D][NP]: end states, then the states entering
   float* gends;                        // the same of the adjoint
   float* ckpt;                         // [batch][tiles][D][NP]: states before each backward tile
   float* shared;                       // [nd][batch][T][2 N]: dB | dC per block of channels
   float* parts;                        // [batch chunks][D (N + 2)]: dA | dskip | ddt_bias
-  int64_t batch;
 };
 
-__device__ __forceinline__ int64_t live_of(const int32_t* __restrict__ lengths, int64_t b, int64_t T) {
+__device__ __forceinline__ int live_of(const int32_t* __restrict__ lengths, int b, int T) {
   if (!lengths) return T;
-  const int64_t n = lengths[b];
+  const int n = lengths[b];
   return n < 0 ? 0 : n < T ? n : T;
 }
 
@@ -78,6 +78,13 @@ __device__ __forceinline__ float quad(float v) { return dpp<J * 0x55>(v); }
 __device__ __forceinline__ float quad_sum(float v) {
   v += dpp<0xB1>(v);
   return v + dpp<0x4E>(v);
+}
+
+// Sums over the quad of four values: lane q of each quad gets that of v[q].
+__device__ __forceinline__ float quad_sums(const float (&v)[4], bool odd, bool upper) {
+  const float a = (odd ? v[1] : v[0]) + dpp<0xB1>(odd ? v[0] : v[1]);
+  const float b = (odd ? v[3] : v[2]) + dpp<0xB1>(odd ? v[2] : v[3]);
+  return (upper ? b : a) + dpp<0x4E>(upper ? a : b);
 }
 
 template <int S>
@@ -107,10 +114,9 @@ __device__ __forceinline__ void write_states(float* __restrict__ p, const float 
 
 // A workgroup's place: channel block, chunk, sequence.
 struct Place {
-  int64_t b, c, d;
-  int lane, wave, q;
+  int b, c, d, lane, wave, q;
   bool on;
-  int64_t begin, end, live;  // the chunk's frames, and how far they are inside the sequence
+  int begin, end, live;  // the chunk's frames, and how far they are inside the sequence
 };
 template <class E>
 __device__ __forceinline__ Place place_of(const ScanP<E>& p) {
@@ -119,13 +125,13 @@ __device__ __forceinline__ Place place_of(const ScanP<E>& p) {
   w.lane = threadIdx.x & 63;
   w.wave = threadIdx.x >> 6;
   w.q = w.lane & 3;
-  w.d = (int64_t)(blockIdx.x % nd) * kChannels + w.wave * 16 + (w.lane >> 2);
+  w.d = (int)(blockIdx.x % nd) * kChannels + w.wave * 16 + (w.lane >> 2);
   w.on = w.d < p.D;
   w.c = i % nc;
   w.b = i / nc;
   w.begin = w.c * p.chunk;
   w.end = w.begin + p.chunk < p.T ? w.begin + p.chunk : p.T;
-  const int64_t n = live_of(p.lengths, w.b, p.T);
+  const int n = live_of(p.lengths, w.b, p.T);
   w.live = n < w.end ? n : w.end;
   return w;
 }
@@ -136,16 +142,16 @@ template <class E, int FRAMES, int NP>
 struct Shared {
   static constexpr int K = (FRAMES * 2 * NP + kThreads - 1) / kThreads;
   float v[K];
-  __device__ __forceinline__ void load(const ScanP<E>& p, const Place& w, int64_t t0) {
+  __device__ __forceinline__ void load(const ScanP<E>& p, const Place& w, int t0) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int i = threadIdx.x + k * kThreads, row = i / (2 * NP), col = i % (2 * NP), n = col % NP;
       // (without a branch: what lies outside is loaded from inside and zeroed)
-      const int64_t left = w.live - 1 - t0;
+      const int left = w.live - 1 - t0;
       const bool in = row <= left && n < p.N;
-      const uint32_t r = row < left ? row : (uint32_t)left, c = n < p.N ? n : 0;
+      const uint32_t r = row < left ? row : left, c = n < p.N ? n : 0;
       const Rows<const E>& m = col < NP ? p.B : p.C;
-      const float x = to_f32((m.p + w.b * m.b + t0 * m.t)[r * (uint32_t)m.t + c]);
+      const float x = to_f32((m.p + w.b * m.b + (int64_t)t0 * m.t)[r * (uint32_t)m.t + c]);
       v[k] = in ? x : 0.f;
     }
   }
@@ -167,21 +173,21 @@ struct Shared {
 template <class E>
 struct Lane {
   const E* seq;  // the sequence's first frame
-  int64_t t;     // elements between frames
+  int t;         // elements between frames
   uint32_t at;   // q t + d
   uint32_t d;
-  __device__ __forceinline__ Lane(const Rows<const E>& m, const Place& w, int64_t D) {
+  __device__ __forceinline__ Lane(const Rows<const E>& m, const Place& w, int D) {
     seq = m.p + w.b * m.b;
     t = m.t;
     d = (uint32_t)(w.on ? w.d : D - 1);
     at = (uint32_t)w.q * (uint32_t)m.t + d;
   }
   template <int G>
-  __device__ __forceinline__ void load(const Place& w, int64_t t0, float (&o)[G]) const {
-    const E* p = seq + t0 * t;
+  __device__ __forceinline__ void load(const Place& w, int t0, float (&o)[G]) const {
+    const E* p = seq + (int64_t)t0 * t;
     if (t0 + 4 * G <= w.live) {
 #pragma unroll
-      for (int g = 0; g < G; ++g) o[g] = to_f32((p + 4 * g * t)[at]);
+      for (int g = 0; g < G; ++g) o[g] = to_f32((p + (int64_t)(4 * g) * t)[at]);
     } else {
       const uint32_t last = (uint32_t)(w.live - 1 - t0);
 #pragma unroll
@@ -209,24 +215,25 @@ __global__ __launch_bounds__(kThreads) void k_scan(ScanP<E> p) {
 
   float h[S], a2[S], prod[S], adj[S];
   const float bias = p.bias && w.on ? p.bias[w.d] : 0.f, skip = p.skip && w.on ? p.skip[w.d] : 0.f;
-  const int64_t at = ((w.b * p.chunks + w.c) * p.D + w.d) * NP + w.q * S;
+  const int64_t at = ((int64_t)(w.b * p.chunks + w.c) * p.D + w.d) * NP + w.q * S;
 #pragma unroll
   for (int s = 0; s < S; ++s) {
     const int n = w.q * S + s;
     const bool real = w.on && n < p.N;
-    a2[s] = real ? p.A[w.d * p.N + n] * kLog2e : 0.f;
+    a2[s] = real ? p.A[(int64_t)w.d * p.N + n] * kLog2e : 0.f;
     h[s] = 0.f;
-    if (MODE == kWhole && p.state && real) h[s] = p.state[(w.b * p.D + w.d) * p.N + n];
+    if (MODE == kWhole && p.state && real) h[s] = p.state[((int64_t)w.b * p.D + w.d) * p.N + n];
     prod[s] = 1.f;
     adj[s] = 0.f;
   }
   if (MODE == kReplay && w.on) read_states<S>(p.ends + at, h);
 
+  const bool odd = w.q & 1, upper = w.q & 2;
   float sum = 0.f;
   float x[G], dt[G], z[G], dy[G];
   Shared<E, kTile, NP> bcv;
   const Lane<E> lx(p.x, w, p.D), ldt(p.dt, w, p.D), lz(p.z, w, p.D), ldy(p.dy, w, p.D);
-  auto fetch = [&](int64_t t0) {
+  auto fetch = [&](int t0) {
     bcv.load(p, w, t0);
     lx.load(w, t0, x);
     ldt.load(w, t0, dt);
@@ -237,7 +244,7 @@ __global__ __launch_bounds__(kThreads) void k_scan(ScanP<E> p) {
   E* const yrow = p.y.p + w.b * p.y.b;
   const uint32_t yat = (uint32_t)w.q * (uint32_t)p.y.t + (uint32_t)w.d;
   int buf = 0;
-  for (int64_t t0 = w.begin; t0 < w.live; t0 += kTile, buf ^= 1) {
+  for (int t0 = w.begin; t0 < w.live; t0 += kTile, buf ^= 1) {
     float* lds = bc[buf];
     bcv.store(lds);
     float cx[G], cdt[G], cz[G], cdy[G];
@@ -245,11 +252,11 @@ __global__ __launch_bounds__(kThreads) void k_scan(ScanP<E> p) {
     for (int g = 0; g < G; ++g) cx[g] = x[g], cdt[g] = dt[g], cz[g] = z[g], cdy[g] = dy[g];
     __syncthreads();
     if (t0 + kTile < w.live) fetch(t0 + kTile);
-    const int groups = (int)(w.live - t0 < kTile ? (w.live - t0 + 3) / 4 : G);
+    const int groups = w.live - t0 < kTile ? (w.live - t0 + 3) / 4 : G;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       if (g >= groups) continue;
-      const int64_t t = t0 + 4 * g + w.q;
+      const int t = t0 + 4 * g + w.q;
       const bool ok = w.on && t < w.live;
       float slope;
       const float soft = softplus_accurate(cdt[g] + bias, slope);
@@ -258,7 +265,7 @@ __global__ __launch_bounds__(kThreads) void k_scan(ScanP<E> p) {
       if ((OUT || ADJ) && p.z.p) gate = silu(cz[g]);
       if (ADJ) up = ok ? cdy[g] * gate : 0.f;
       if (!OUT) sum += step;
-      float y = 0.f;
+      float y4[4];
       auto frame = [&](auto jc) {
         constexpr int J = decltype(jc)::value;
         const float sj = quad<J>(step), uj = quad<J>(u), dj = ADJ ? quad<J>(up) : 0.f;
@@ -276,34 +283,34 @@ __global__ __launch_bounds__(kThreads) void k_scan(ScanP<E> p) {
             adj[s] = fmaf(prod[s] * cv[s], dj, adj[s]);
           }
         }
-        if (OUT) {
-          yj = quad_sum(yj);
-          y = w.q == J ? yj : y;
-        }
+        y4[J] = yj;
       };
       frame(std::integral_constant<int, 0>{});
       frame(std::integral_constant<int, 1>{});
       frame(std::integral_constant<int, 2>{});
       frame(std::integral_constant<int, 3>{});
-      if (OUT && ok) (yrow + (t0 + 4 * g) * p.y.t)[yat] = from_f32<E>(fmaf(skip, cx[g], y) * gate);
+      const float y = OUT ? quad_sums(y4, odd, upper) : 0.f;
+      if (OUT && ok) (yrow + (int64_t)(t0 + 4 * g) * p.y.t)[yat] = from_f32<E>(fmaf(skip, cx[g], y) * gate);
     }
   }
   if (!w.on) return;
   if (OUT)
-    for (int64_t t = (w.live > w.begin ? w.live : w.begin) + w.q; t < w.end; t += 4)
-      p.y.p[w.b * p.y.b + t * p.y.t + w.d] = from_f32<E>(0.f);
+    for (int t = (w.live > w.begin ? w.live : w.begin) + w.q; t < w.end; t += 4)
+      p.y.p[w.b * p.y.b + (int64_t)t * p.y.t + w.d] = from_f32<E>(0.f);
   if (MODE == kWhole && p.state_out) {
 #pragma unroll
     for (int s = 0; s < S; ++s)
-      if (w.q * S + s < p.N) p.state_out[(w.b * p.D + w.d) * p.N + w.q * S + s] = h[s];
+      if (w.q * S + s < p.N) p.state_out[((int64_t)w.b * p.D + w.d) * p.N + w.q * S + s] = h[s];
   }
   if (!OUT) {
     write_states<S>(p.ends + at, h);
     if (ADJ) write_states<S>(p.gends + at, adj);
     sum = quad_sum(sum);
-    if (w.q == 0) p.sums[(w.b * p.chunks + w.c) * p.D + w.d] = sum;
+    if (w.q == 0) p.sums[(int64_t)(w.b * p.chunks + w.c) * p.D + w.d] = sum;
   }
 }
+
+constexpr int kMaxChunks = 512, kMaxRun = kMaxChunks / 16;
 
 // States entering each chunk, in place of the chunks' end states (reverse:
 // the adjoints entering from the chunks after).  64 states a workgroup, 16
@@ -313,41 +320,58 @@ template <class E>
 __global__ __launch_bounds__(1024) void k_scan_carry(ScanP<E> p, float* ends, int np, bool reverse) {
   __shared__ float rsum[16][65], rend[16][65];
   const int col = threadIdx.x & 63, seg = threadIdx.x >> 6;
-  const int64_t per = p.D * np, blocks = (per + 63) / 64;
-  const int64_t b = blockIdx.x / blocks, j = (blockIdx.x % blocks) * 64 + col;
+  const int64_t per = (int64_t)p.D * np, blocks = (per + 63) / 64;
+  const int b = (int)(blockIdx.x / blocks);
+  const int64_t j = (blockIdx.x % blocks) * 64 + col;
   const bool on = j < per;
   const int64_t d = on ? j / np : 0;
   const int n = on ? (int)(j % np) : 0;
   const bool real = on && n < p.N;
   const float a2 = real ? p.A[d * p.N + n] * kLog2e : 0.f;
-  const int64_t live = live_of(p.lengths, b, p.T), used = (live + p.chunk - 1) / p.chunk;
-  const int64_t run = (p.chunks + 15) / 16, lo = seg * run, hi = lo + run < used ? lo + run : used;
-  float* e = ends + b * p.chunks * per + j;
-  const float* sm = p.sums + b * p.chunks * p.D + d;
-  auto chunk = [&](int64_t k) { return reverse ? used - 1 - k : k; };  // k-th in walking order
+  const int live = live_of(p.lengths, b, p.T), used = (live + p.chunk - 1) / p.chunk;
+  const int run = (p.chunks + 15) / 16, lo = seg * run, hi = lo + run < used ? lo + run : used;
+  float* e = ends + (int64_t)b * p.chunks * per + j;
+  const float* sm = p.sums + (int64_t)b * p.chunks * p.D + d;
+  auto chunk = [&](int k) { return (int64_t)(reverse ? used - 1 - k : k); };  // k-th in walking order
+  // the run in registers, loaded at once (past its end: its first chunk again)
+  float rs[kMaxRun], re[kMaxRun];
+#pragma unroll
+  for (int i = 0; i < kMaxRun; i += 8)
+    if (i < run)
+#pragma unroll
+      for (int k = i; k < i + 8; ++k) {
+        const int64_t c = on && lo + k < hi ? chunk(lo + k) : 0;
+        const float x = on ? sm[c * p.D] : 0.f, y = on ? e[c * per] : 0.f;
+        rs[k] = lo + k < hi ? x : 0.f;
+        re[k] = lo + k < hi ? y : 0.f;
+      }
   float sum = 0.f, end = 0.f;
-  if (on)
-#pragma unroll 8
-    for (int64_t k = lo; k < hi; ++k) {
-      const float s = sm[chunk(k) * p.D];
-      end = fmaf(__builtin_amdgcn_exp2f(s * a2), end, e[chunk(k) * per]);
-      sum += s;
-    }
+#pragma unroll
+  for (int i = 0; i < kMaxRun; i += 8)
+    if (i < run)
+#pragma unroll
+      for (int k = i; k < i + 8; ++k) {
+        // (step 0 and state 0 past the end: the decay is 1)
+        end = fmaf(__builtin_amdgcn_exp2f(rs[k] * a2), end, re[k]);
+        sum += rs[k];
+      }
   rsum[seg][col] = sum;
   rend[seg][col] = end;
   float h = 0.f;
-  if (!reverse && real && p.state) h = p.state[(b * p.D + d) * p.N + n];
+  if (!reverse && real && p.state) h = p.state[((int64_t)b * p.D + d) * p.N + n];
   __syncthreads();
   for (int k = 0; k < seg; ++k) h = fmaf(__builtin_amdgcn_exp2f(rsum[k][col] * a2), h, rend[k][col]);
   if (!on) return;
-#pragma unroll 8
-  for (int64_t k = lo; k < hi; ++k) {
-    const float s = sm[chunk(k) * p.D], v = e[chunk(k) * per];
-    e[chunk(k) * per] = h;
-    h = fmaf(__builtin_amdgcn_exp2f(s * a2), h, v);
-  }
+#pragma unroll
+  for (int i = 0; i < kMaxRun; i += 8)
+    if (i < run)
+#pragma unroll
+      for (int k = i; k < i + 8; ++k) {
+        if (lo + k < hi) e[chunk(lo + k) * per] = h;
+        h = fmaf(__builtin_amdgcn_exp2f(rs[k] * a2), h, re[k]);
+      }
   // the thread past the last run has the state after all chunks
-  if (!reverse && seg == 15 && real && p.state_out) p.state_out[(b * p.D + d) * p.N + n] = h;
+  if (!reverse && seg == 15 && real && p.state_out) p.state_out[((int64_t)b * p.D + d) * p.N + n] = h;
 }
 
 // Sum over the wave's 16 channels (lane bits 2..5) of V values per lane, by
@@ -390,18 +414,18 @@ __global__ __launch_bounds__(kThreads, 2) void k_scan_bwd(ScanP<E> p) {
   // the tile's states before each frame, a lane's own
   __shared__ __align__(16) float hs[TL][kThreads][S];
   const Place w = place_of(p);
-  const int64_t tiles_all = (p.T + TL - 1) / TL, tile0 = w.begin / TL;
-  const int64_t tiles = w.live > w.begin ? (w.live - w.begin + TL - 1) / TL : 0;
+  const int tiles_all = (p.T + TL - 1) / TL, tile0 = w.begin / TL;
+  const int tiles = w.live > w.begin ? (w.live - w.begin + TL - 1) / TL : 0;
 
   float h[S], a[S], g[S], dA[S];
   const float bias = p.bias && w.on ? p.bias[w.d] : 0.f, skip = p.skip && w.on ? p.skip[w.d] : 0.f;
-  const int64_t at = ((w.b * p.chunks + w.c) * p.D + w.d) * NP + w.q * S;
+  const int64_t at = ((int64_t)(w.b * p.chunks + w.c) * p.D + w.d) * NP + w.q * S;
 #pragma unroll
   for (int s = 0; s < S; ++s) {
     const int n = w.q * S + s;
     const bool real = w.on && n < p.N;
-    a[s] = real ? p.A[w.d * p.N + n] : 0.f;
-    h[s] = p.chunks == 1 && p.state && real ? p.state[(w.b * p.D + w.d) * p.N + n] : 0.f;
+    a[s] = real ? p.A[(int64_t)w.d * p.N + n] : 0.f;
+    h[s] = p.chunks == 1 && p.state && real ? p.state[((int64_t)w.b * p.D + w.d) * p.N + n] : 0.f;
     g[s] = 0.f;
     dA[s] = 0.f;
   }
@@ -409,23 +433,24 @@ __global__ __launch_bounds__(kThreads, 2) void k_scan_bwd(ScanP<E> p) {
     read_states<S>(p.ends + at, h);
     read_states<S>(p.gends + at, g);
   }
+  const bool odd = w.q & 1, upper = w.q & 2;
   float dskip = 0.f, dbias = 0.f;
   // (lanes past the last channel read that one's states and store none)
-  float* ck = p.ckpt + ((w.b * tiles_all + tile0) * p.D + (w.on ? w.d : p.D - 1)) * NP + w.q * S;
+  float* ck = p.ckpt + ((int64_t)(w.b * tiles_all + tile0) * p.D + (w.on ? w.d : p.D - 1)) * NP + w.q * S;
   Shared<E, TL, NP> bcv;
   const Lane<E> lx(p.x, w, p.D), ldt(p.dt, w, p.D), lz(p.z, w, p.D), ldy(p.dy, w, p.D);
 
   // forward over the chunk: the state before every tile
   {
     float x[G], dt[G];
-    auto fetch = [&](int64_t t0) {
+    auto fetch = [&](int t0) {
       bcv.load(p, w, t0);
       lx.load(w, t0, x);
       ldt.load(w, t0, dt);
     };
     if (tiles > 0) fetch(w.begin);
-    for (int64_t i = 0; i < tiles; ++i) {
-      if (w.on) write_states<S>(ck + i * p.D * NP, h);
+    for (int i = 0; i < tiles; ++i) {
+      if (w.on) write_states<S>(ck + (int64_t)i * p.D * NP, h);
       if (i + 1 == tiles) break;
       float* lds = bc[i & 1];
       bcv.store(lds);
@@ -438,10 +463,10 @@ __global__ __launch_bounds__(kThreads, 2) void k_scan_bwd(ScanP<E> p) {
       for (int k = 0; k < G; ++k) {
         float slope;
         // (every frame of a tile that another follows is inside the sequence)
-        const float step = softplus_accurate(cdt[k] + bias, slope), u = step * cx[k];
+        const float step = softplus_accurate(cdt[k] + bias, slope), u = step * cx[k], step2 = step * kLog2e;
         auto frame = [&](auto jc) {
           constexpr int J = decltype(jc)::value;
-          const float sj = quad<J>(step) * kLog2e, uj = quad<J>(u);
+          const float sj = quad<J>(step2), uj = quad<J>(u);
           float bv[S];
           read_states<S>(lds + (4 * k + J) * 2 * NP + w.q * S, bv);
 #pragma unroll
@@ -460,20 +485,20 @@ __global__ __launch_bounds__(kThreads, 2) void k_scan_bwd(ScanP<E> p) {
   const uint32_t q = w.q, d = (uint32_t)w.d, dxat = q * (uint32_t)p.dx.t + d, ddtat = q * (uint32_t)p.ddt.t + d,
                  dzat = q * (uint32_t)p.dz.t + d;
   float x[G], dt[G], z[G], dy[G], hn[S];
-  auto fetch = [&](int64_t i) {
-    const int64_t t0 = w.begin + i * TL;
+  auto fetch = [&](int i) {
+    const int t0 = w.begin + i * TL;
     bcv.load(p, w, t0);
     lx.load(w, t0, x);
     ldt.load(w, t0, dt);
     if (p.z.p) lz.load(w, t0, z);
     ldy.load(w, t0, dy);
-    read_states<S>(ck + i * p.D * NP, hn);
+    read_states<S>(ck + (int64_t)i * p.D * NP, hn);
   };
 #pragma unroll
   for (int s = 0; s < S; ++s) hn[s] = 0.f;
   if (tiles > 0) fetch(tiles - 1);
-  for (int64_t i = tiles - 1; i >= 0; --i) {
-    const int64_t t0 = w.begin + i * TL;
+  for (int i = tiles - 1; i >= 0; --i) {
+    const int t0 = w.begin + i * TL;
     float* lds = bc[i & 1];
     bcv.store(lds);
     float cx[G], cz[G], cdy[G], step[G], slope[G], u[G], up[G], y[G];
@@ -495,10 +520,11 @@ __global__ __launch_bounds__(kThreads, 2) void k_scan_bwd(ScanP<E> p) {
     float as[TL][S];
 #pragma unroll
     for (int k = 0; k < G; ++k) {
-      y[k] = 0.f;
+      float y4[4];
+      const float step2 = step[k] * kLog2e;
       auto frame = [&](auto jc) {
         constexpr int J = decltype(jc)::value;
-        const float sj = quad<J>(step[k]) * kLog2e, uj = quad<J>(u[k]);
+        const float sj = quad<J>(step2), uj = quad<J>(u[k]);
         const float* row = lds + (4 * k + J) * 2 * NP + w.q * S;
         float bv[S], cv[S], yj = 0.f;
         read_states<S>(row, bv);
@@ -511,18 +537,18 @@ __global__ __launch_bounds__(kThreads, 2) void k_scan_bwd(ScanP<E> p) {
           h[s] = fmaf(e, h[s], uj * bv[s]);
           yj = fmaf(cv[s], h[s], yj);
         }
-        yj = quad_sum(yj);
-        y[k] = w.q == J ? yj : y[k];
+        y4[J] = yj;
       };
       frame(std::integral_constant<int, 0>{});
       frame(std::integral_constant<int, 1>{});
       frame(std::integral_constant<int, 2>{});
       frame(std::integral_constant<int, 3>{});
+      y[k] = quad_sums(y4, odd, upper);
     }
     // down through the tile: h is the state after the frame
 #pragma unroll
     for (int k = G - 1; k >= 0; --k) {
-      float gb = 0.f, ga = 0.f;
+      float gb4[4], ga4[4];
       auto frame = [&](auto jc) {
         constexpr int J = decltype(jc)::value;
         const int f = 4 * k + J;
@@ -544,10 +570,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_scan_bwd(ScanP<E> p) {
           gaj = fmaf(gh, a[s], gaj);
           dA[s] = fmaf(gh, sj, dA[s]);
         }
-        gbj = quad_sum(gbj);
-        gaj = quad_sum(gaj);
-        gb = w.q == J ? gbj : gb;
-        ga = w.q == J ? gaj : ga;
+        gb4[J] = gbj;
+        ga4[J] = gaj;
         float sums[kept<2 * S>()];
         channel_sum<2 * S>(v, sums);
         if ((w.lane & 12) == 0) {
@@ -562,21 +586,22 @@ __global__ __launch_bounds__(kThreads, 2) void k_scan_bwd(ScanP<E> p) {
       frame(std::integral_constant<int, 2>{});
       frame(std::integral_constant<int, 1>{});
       frame(std::integral_constant<int, 0>{});
-      const int64_t t = t0 + 4 * k + w.q;
+      const float gb = quad_sums(gb4, odd, upper), ga = quad_sums(ga4, odd, upper);
+      const int t = t0 + 4 * k + w.q;
       if (w.on && t < w.live) {
         const float draw = fmaf(gb, cx[k], ga) * slope[k];
         dbias += draw;
         dskip = fmaf(up[k], cx[k], dskip);
-        (dxr + (t0 + 4 * k) * p.dx.t)[dxat] = from_f32<E>(fmaf(step[k], gb, skip * up[k]));
-        (ddtr + (t0 + 4 * k) * p.ddt.t)[ddtat] = from_f32<E>(draw);
+        (dxr + (int64_t)(t0 + 4 * k) * p.dx.t)[dxat] = from_f32<E>(fmaf(step[k], gb, skip * up[k]));
+        (ddtr + (int64_t)(t0 + 4 * k) * p.ddt.t)[ddtat] = from_f32<E>(draw);
         if (p.z.p)
-          (dzr + (t0 + 4 * k) * p.dz.t)[dzat] =
+          (dzr + (int64_t)(t0 + 4 * k) * p.dz.t)[dzat] =
               from_f32<E>(cdy[k] * fmaf(skip, cx[k], y[k]) * silu_grad(cz[k], sigmoid(cz[k])));
       }
     }
     __syncthreads();
     // dB | dC of the block's channels
-    float* out = p.shared + (((blockIdx.x % (uint32_t)p.nd) * p.batch + w.b) * p.T + t0) * 2 * p.N;
+    float* out = p.shared + ((int64_t)((int)(blockIdx.x % (uint32_t)p.nd) * p.batch + w.b) * p.T + t0) * 2 * p.N;
     for (int o = threadIdx.x; o < TL * 2 * NP; o += kThreads) {
       const int f = o / (2 * NP), col = o % (2 * NP), n = col % NP;
       if (t0 + f < w.live && n < p.N) {
@@ -588,20 +613,20 @@ __global__ __launch_bounds__(kThreads, 2) void k_scan_bwd(ScanP<E> p) {
     }
   }
   if (!w.on) return;
-  for (int64_t t = (w.live > w.begin ? w.live : w.begin) + w.q; t < w.end; t += 4) {
-    p.dx.p[w.b * p.dx.b + t * p.dx.t + w.d] = from_f32<E>(0.f);
-    p.ddt.p[w.b * p.ddt.b + t * p.ddt.t + w.d] = from_f32<E>(0.f);
-    if (p.z.p) p.dz.p[w.b * p.dz.b + t * p.dz.t + w.d] = from_f32<E>(0.f);
+  for (int t = (w.live > w.begin ? w.live : w.begin) + w.q; t < w.end; t += 4) {
+    p.dx.p[w.b * p.dx.b + (int64_t)t * p.dx.t + w.d] = from_f32<E>(0.f);
+    p.ddt.p[w.b * p.ddt.b + (int64_t)t * p.ddt.t + w.d] = from_f32<E>(0.f);
+    if (p.z.p) p.dz.p[w.b * p.dz.b + (int64_t)t * p.dz.t + w.d] = from_f32<E>(0.f);
   }
-  float* part = p.parts + (w.b * p.chunks + w.c) * p.D * (p.N + 2);
+  float* part = p.parts + (int64_t)(w.b * p.chunks + w.c) * p.D * (p.N + 2);
 #pragma unroll
   for (int s = 0; s < S; ++s)
-    if (w.q * S + s < p.N) part[w.d * p.N + w.q * S + s] = dA[s];
+    if (w.q * S + s < p.N) part[(int64_t)w.d * p.N + w.q * S + s] = dA[s];
   dskip = quad_sum(dskip);
   dbias = quad_sum(dbias);
   if (w.q == 0) {
-    part[p.D * p.N + w.d] = dskip;
-    part[p.D * (p.N + 1) + w.d] = dbias;
+    part[(int64_t)p.D * p.N + w.d] = dskip;
+    part[(int64_t)p.D * (p.N + 1) + w.d] = dbias;
   }
 }
 
@@ -614,10 +639,10 @@ __global__ __launch_bounds__(256) void k_scan_shared(const float* __restrict__ s
   if (i >= total) return;
   const int64_t row = i / (2 * N), col = i - row * 2 * N, b = row / T, t = row - b * T;
   float v = 0.f;
-  if (t < live_of(lengths, b, T))
+  if (t < live_of(lengths, (int)b, (int)T))
     for (int64_t k = 0; k < nd; ++k) v += shared[k * total + i];
   const Rows<E>& m = col < N ? dB : dC;
-  m.p[b * m.b + t * m.t + (col < N ? col : col - N)] = from_f32<E>(v);
+  m.p[b * m.b + t * (int64_t)m.t + (col < N ? col : col - N)] = from_f32<E>(v);
 }
 
 struct ScanShape {
@@ -630,7 +655,7 @@ struct ScanShape {
 // Chunks: as many as give every CU two workgroups (two waves a SIMD), none
 // shorter than 64 frames, and none where the sequences and channel blocks
 // come near that alone: a chunked pass evaluates every decay twice.
-constexpr int64_t kFill = 512, kFillAlone = 320, kMinChunk = 64, kMaxChunks = 512;
+constexpr int64_t kFill = 512, kFillAlone = 320, kMinChunk = 64;
 
 ScanShape scan_shape(const dgen_hip_scan& a, bool backward) {
   ScanShape s{};
@@ -640,7 +665,7 @@ ScanShape scan_shape(const dgen_hip_scan& a, bool backward) {
   const int64_t blocks = std::max<int64_t>(1, a.batch * s.nd);
   int64_t chunks = 1;
   if (blocks < kFillAlone)
-    chunks = std::min({(kFill + blocks - 1) / blocks, (a.T + kMinChunk - 1) / kMinChunk, kMaxChunks});
+    chunks = std::min({(kFill + blocks - 1) / blocks, (a.T + kMinChunk - 1) / kMinChunk, (int64_t)kMaxChunks});
   s.chunk = (a.T + chunks - 1) / chunks;
   s.chunk = (s.chunk + kTile - 1) / kTile * kTile;
   s.chunks = (a.T + s.chunk - 1) / s.chunk;
@@ -661,9 +686,9 @@ ScanShape scan_shape(const dgen_hip_scan& a, bool backward) {
 }
 
 template <class E>
-Rows<const E> in_rows(const dgen_hip_seq& v) { return {(const E*)v.data, v.stride_b, v.stride_t}; }
+Rows<const E> in_rows(const dgen_hip_seq& v) { return {(const E*)v.data, v.stride_b, (int)v.stride_t}; }
 template <class E>
-Rows<E> out_rows(const dgen_hip_seq& v) { return {(E*)v.data, v.stride_b, v.stride_t}; }
+Rows<E> out_rows(const dgen_hip_seq& v) { return {(E*)v.data, v.stride_b, (int)v.stride_t}; }
 
 template <class E, int S>
 void scan_launch(const dgen_hip_scan& a, bool backward, const ScanShape& s, hipStream_t st) {
@@ -671,7 +696,8 @@ void scan_launch(const dgen_hip_scan& a, bool backward, const ScanShape& s, hipS
   ScanP<E> p{};
   p.x = in_rows<E>(a.x), p.dt = in_rows<E>(a.dt), p.z = in_rows<E>(a.z), p.B = in_rows<E>(a.B), p.C = in_rows<E>(a.C);
   p.A = a.A, p.skip = a.skip, p.bias = a.dt_bias, p.state = a.state, p.lengths = a.lengths;
-  p.T = a.T, p.D = a.D, p.N = a.N, p.chunk = s.chunk, p.chunks = s.chunks, p.nd = s.nd, p.batch = a.batch;
+  p.T = (int)a.T, p.D = (int)a.D, p.N = (int)a.N, p.chunk = (int)s.chunk, p.chunks = (int)s.chunks, p.nd = (int)s.nd;
+  p.batch = (int)a.batch;
   p.sums = ws, p.ends = p.sums + s.sums, p.gends = p.ends + s.ends;
   if (!backward) p.y = out_rows<E>(a.y), p.state_out = a.state_out;
   const dim3 grid((unsigned)(s.nd * s.chunks * a.batch));
@@ -726,7 +752,8 @@ int scan_run(const dgen_hip_scan& a, bool backward, hipStream_t st, bool dry) {
   DGEN_REQUIRE(a.D >= 1 && a.D <= (1 << 20), "%s: D %lld outside [1, 2^20]", what, (long long)a.D);
   const ScanShape s = scan_shape(a, backward);
   // (a launch takes fewer than 2^32 threads)
-  DGEN_REQUIRE(s.nd * s.chunks * a.batch < (int64_t(1) << 23) && (a.D * s.NP + 63) / 64 * a.batch < (int64_t(1) << 21) &&
+  DGEN_REQUIRE(s.nd * s.chunks * a.batch < (int64_t(1) << 23) && a.batch * ((a.T + 3) / 4) < (int64_t(1) << 31) &&
+                   s.nd * a.batch < (int64_t(1) << 31) && (a.D * s.NP + 63) / 64 * a.batch < (int64_t(1) << 21) &&
                    (!backward || a.batch * a.T * 2 * a.N < (int64_t(1) << 31)),
                "%s: batch %lld x T %lld x D %lld x N %lld is too large for one call", what, (long long)a.batch,
                (long long)a.T, (long long)a.D, (long long)a.N);
