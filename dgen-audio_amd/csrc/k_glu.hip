@@ -663,44 +663,51 @@ __global__ __launch_bounds__(256) void k_glu_join(const float* __restrict__ part
 }
 
 // Forward for a few rows (single frames of some voices): the weights' reading
-// is all that counts, so the vector unit multiplies.  A workgroup owns 64
-// columns; 32 lanes x 2 columns, the half-waves of eight waves take every
-// 16th k, and the sixteen sums meet in LDS.
-constexpr int kFewRows = 8, kFewThreads = 512, kFewCols = 64, kFewK = 512;
+// is all that counts, and its latency, so the vector unit multiplies.  A
+// workgroup owns 64 columns (32 lanes x 2: whole cache lines); the half-waves
+// of 16 waves take every 32nd k, each with all of its 16 loads of a round of
+// 512 k's in flight at once; the 32 sums meet in LDS.
+constexpr int kFewRows = 8, kFewThreads = 1024, kFewCols = 64, kFewK = 512, kFewLoads = kFewK / 32;
 template <class E>
 __global__ __launch_bounds__(kFewThreads) void k_glu_few(GluP<E> p) {
-  __shared__ float xs[kFewK][kFewRows];
-  __shared__ float red[8][kFewCols][2][kFewRows + 1];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+  __shared__ __align__(16) float xs[kFewK][kFewRows];
+  __shared__ float red[16][kFewCols][2][kFewRows + 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, slice = wave * 2 + (lane >> 5);
   const int64_t m0 = (int64_t)blockIdx.y * kFewRows, f = (int64_t)blockIdx.x * kFewCols + (lane & 31) * 2;
-  const int valid = (int)(p.N - f < 0 ? 0 : p.N - f < 2 ? p.N - f : 2);
+  const bool two = f + 1 < p.N;
+  const int64_t col = two ? f : f < p.N ? f : p.N - 1;  // (columns past the end are not stored)
   float acc[2][2][kFewRows] = {};
   for (int64_t k0 = 0; k0 < p.K; k0 += kFewK) {
-    const int kn = (int)(p.K - k0 < kFewK ? p.K - k0 : kFewK);
-    __syncthreads();
+    Vec<E, 2> w[kFewLoads][2];
+    const E *g = p.n0 + col, *u = p.n1 + col;
+#pragma unroll
+    for (int i = 0; i < kFewLoads; ++i) {
+      const int64_t k = k0 + slice + 32 * i, kc = k < p.K ? k : p.K - 1;  // (x is 0 past the end)
+      if (two) {
+        w[i][0] = *reinterpret_cast<const Vec<E, 2>*>(g + kc * p.nld0);
+        w[i][1] = *reinterpret_cast<const Vec<E, 2>*>(u + kc * p.nld1);
+      } else {
+        w[i][0].e[0] = w[i][0].e[1] = g[kc * p.nld0];
+        w[i][1].e[0] = w[i][1].e[1] = u[kc * p.nld1];
+      }
+    }
+    if (k0 > 0) __syncthreads();
     for (int i = threadIdx.x; i < kFewK * kFewRows; i += kFewThreads) {
       const int m = i / kFewK, k = i % kFewK;
-      xs[k][m] = k < kn && m0 + m < p.M ? to_f32(p.m0[(m0 + m) * p.mld0 + k0 + k]) : 0.f;
+      xs[k][m] = k0 + k < p.K && m0 + m < p.M ? to_f32(p.m0[(m0 + m) * p.mld0 + k0 + k]) : 0.f;
     }
     __syncthreads();
-#pragma unroll 8
-    for (int k = wave * 2 + half; k < kn; k += 16) {
-      Vec<E, 2> w[2] = {};
-      const E *g = p.n0 + (k0 + k) * p.nld0 + f, *u = p.n1 + (k0 + k) * p.nld1 + f;
-      if (valid == 2) {
-        w[0] = *reinterpret_cast<const Vec<E, 2>*>(g);
-        w[1] = *reinterpret_cast<const Vec<E, 2>*>(u);
-      } else if (valid == 1) {
-        w[0].e[0] = *g;
-        w[1].e[0] = *u;
-      }
+#pragma unroll
+    for (int i = 0; i < kFewLoads; ++i) {
+      const int64_t k = k0 + slice + 32 * i;
+      if (k >= p.K) continue;
 #pragma unroll
       for (int m = 0; m < kFewRows; ++m) {
-        const float x = xs[k][m];
+        const float x = xs[slice + 32 * i][m];
 #pragma unroll
         for (int a = 0; a < 2; ++a)
 #pragma unroll
-          for (int b = 0; b < 2; ++b) acc[a][b][m] = fmaf(x, to_f32(w[a].e[b]), acc[a][b][m]);
+          for (int b = 0; b < 2; ++b) acc[a][b][m] = fmaf(x, to_f32(w[i][a].e[b]), acc[a][b][m]);
       }
     }
   }
@@ -711,14 +718,15 @@ __global__ __launch_bounds__(kFewThreads) void k_glu_few(GluP<E> p) {
 #pragma unroll
       for (int m = 0; m < kFewRows; ++m) {
         const float t = acc[a][b][m] + __shfl_xor(acc[a][b][m], 32, 64);
-        if (half == 0) red[wave][lane * 2 + b][a][m] = t;
+        if (lane < 32) red[wave][lane * 2 + b][a][m] = t;
       }
   __syncthreads();
+  if (threadIdx.x >= kFewCols * kFewRows) return;
   const int c = threadIdx.x % kFewCols, m = threadIdx.x / kFewCols;  // 64 columns x 8 rows
   const int64_t n = (int64_t)blockIdx.x * kFewCols + c;
   float s[2] = {0.f, 0.f}, slope;
 #pragma unroll
-  for (int w = 0; w < 8; ++w) {
+  for (int w = 0; w < 16; ++w) {
     s[0] += red[w][c][0][m];
     s[1] += red[w][c][1][m];
   }

@@ -313,15 +313,19 @@ __global__ __launch_bounds__(kThreads) void k_scan(ScanP<E> p) {
 constexpr int kMaxChunks = 512, kMaxRun = kMaxChunks / 16;
 
 // States entering each chunk, in place of the chunks' end states (reverse:
-// the adjoints entering from the chunks after).  64 states a workgroup, 16
+// the adjoints entering from the chunks after).  64 states a workgroup, SEGS
 // threads over the chunks: each joins its run of chunks, the runs are joined
 // in LDS, and each walks its run again.
-template <class E>
-__global__ __launch_bounds__(1024) void k_scan_carry(ScanP<E> p, float* ends, int np, bool reverse) {
-  __shared__ float rsum[16][65], rend[16][65];
+// The backward pass takes both directions in one launch: the second half of
+// the grid is the adjoint's.
+template <class E, int SEGS>
+__global__ __launch_bounds__(64 * SEGS) void k_scan_carry(ScanP<E> p, int np) {
+  __shared__ float rsum[SEGS][65], rend[SEGS][65];
   const int col = threadIdx.x & 63, seg = threadIdx.x >> 6;
   const int64_t per = (int64_t)p.D * np, blocks = (per + 63) / 64;
-  const int b = (int)(blockIdx.x / blocks);
+  const int row = (int)(blockIdx.x / blocks), b = row % p.batch;
+  const bool reverse = row >= p.batch;
+  float* const ends = reverse ? p.gends : p.ends;
   const int64_t j = (blockIdx.x % blocks) * 64 + col;
   const bool on = j < per;
   const int64_t d = on ? j / np : 0;
@@ -329,17 +333,17 @@ __global__ __launch_bounds__(1024) void k_scan_carry(ScanP<E> p, float* ends, in
   const bool real = on && n < p.N;
   const float a2 = real ? p.A[d * p.N + n] * kLog2e : 0.f;
   const int live = live_of(p.lengths, b, p.T), used = (live + p.chunk - 1) / p.chunk;
-  const int run = (p.chunks + 15) / 16, lo = seg * run, hi = lo + run < used ? lo + run : used;
+  const int run = (p.chunks + SEGS - 1) / SEGS, lo = seg * run, hi = lo + run < used ? lo + run : used;
   float* e = ends + (int64_t)b * p.chunks * per + j;
   const float* sm = p.sums + (int64_t)b * p.chunks * p.D + d;
   auto chunk = [&](int k) { return (int64_t)(reverse ? used - 1 - k : k); };  // k-th in walking order
   // the run in registers, loaded at once (past its end: its first chunk again)
   float rs[kMaxRun], re[kMaxRun];
 #pragma unroll
-  for (int i = 0; i < kMaxRun; i += 8)
+  for (int i = 0; i < kMaxRun; i += 4)
     if (i < run)
 #pragma unroll
-      for (int k = i; k < i + 8; ++k) {
+      for (int k = i; k < i + 4; ++k) {
         const int64_t c = on && lo + k < hi ? chunk(lo + k) : 0;
         const float x = on ? sm[c * p.D] : 0.f, y = on ? e[c * per] : 0.f;
         rs[k] = lo + k < hi ? x : 0.f;
@@ -347,10 +351,10 @@ __global__ __launch_bounds__(1024) void k_scan_carry(ScanP<E> p, float* ends, in
       }
   float sum = 0.f, end = 0.f;
 #pragma unroll
-  for (int i = 0; i < kMaxRun; i += 8)
+  for (int i = 0; i < kMaxRun; i += 4)
     if (i < run)
 #pragma unroll
-      for (int k = i; k < i + 8; ++k) {
+      for (int k = i; k < i + 4; ++k) {
         // (step 0 and state 0 past the end: the decay is 1)
         end = fmaf(__builtin_amdgcn_exp2f(rs[k] * a2), end, re[k]);
         sum += rs[k];
@@ -363,15 +367,15 @@ __global__ __launch_bounds__(1024) void k_scan_carry(ScanP<E> p, float* ends, in
   for (int k = 0; k < seg; ++k) h = fmaf(__builtin_amdgcn_exp2f(rsum[k][col] * a2), h, rend[k][col]);
   if (!on) return;
 #pragma unroll
-  for (int i = 0; i < kMaxRun; i += 8)
+  for (int i = 0; i < kMaxRun; i += 4)
     if (i < run)
 #pragma unroll
-      for (int k = i; k < i + 8; ++k) {
+      for (int k = i; k < i + 4; ++k) {
         if (lo + k < hi) e[chunk(lo + k) * per] = h;
         h = fmaf(__builtin_amdgcn_exp2f(rs[k] * a2), h, re[k]);
       }
   // the thread past the last run has the state after all chunks
-  if (!reverse && seg == 15 && real && p.state_out) p.state_out[((int64_t)b * p.D + d) * p.N + n] = h;
+  if (!reverse && seg == SEGS - 1 && real && p.state_out) p.state_out[((int64_t)b * p.D + d) * p.N + n] = h;
 }
 
 // Sum over the wave's 16 channels (lane bits 2..5) of V values per lane, by
@@ -653,9 +657,9 @@ struct ScanShape {
 };
 
 // Chunks: as many as give every CU two workgroups (two waves a SIMD), none
-// shorter than 64 frames, and none where the sequences and channel blocks
+// shorter than 32 frames, and none where the sequences and channel blocks
 // come near that alone: a chunked pass evaluates every decay twice.
-constexpr int64_t kFill = 512, kFillAlone = 320, kMinChunk = 64;
+constexpr int64_t kFill = 512, kFillAlone = 320, kMinChunk = 32;
 
 ScanShape scan_shape(const dgen_hip_scan& a, bool backward) {
   ScanShape s{};
@@ -701,13 +705,18 @@ void scan_launch(const dgen_hip_scan& a, bool backward, const ScanShape& s, hipS
   p.sums = ws, p.ends = p.sums + s.sums, p.gends = p.ends + s.ends;
   if (!backward) p.y = out_rows<E>(a.y), p.state_out = a.state_out;
   const dim3 grid((unsigned)(s.nd * s.chunks * a.batch));
-  const dim3 carry((unsigned)((a.D * s.NP + 63) / 64 * a.batch));
+  // (few chunks: four threads a state, with runs of up to 16)
+  auto carry = [&]() {
+    const dim3 states((unsigned)((a.D * s.NP + 63) / 64 * a.batch * (backward ? 2 : 1)));
+    if (s.chunks <= 64) k_scan_carry<E, 4><<<states, 256, 0, st>>>(p, (int)s.NP);
+    else k_scan_carry<E, 16><<<states, 1024, 0, st>>>(p, (int)s.NP);
+  };
   if (!backward) {
     if (s.chunks == 1) {
       k_scan<E, S, kWhole><<<grid, kThreads, 0, st>>>(p);
     } else {
       k_scan<E, S, kSummary><<<grid, kThreads, 0, st>>>(p);
-      k_scan_carry<E><<<carry, 1024, 0, st>>>(p, p.ends, (int)s.NP, false);
+      carry();
       k_scan<E, S, kReplay><<<grid, kThreads, 0, st>>>(p);
     }
     return;
@@ -716,8 +725,7 @@ void scan_launch(const dgen_hip_scan& a, bool backward, const ScanShape& s, hipS
   p.ckpt = p.gends + s.ends, p.shared = p.ckpt + s.ckpt, p.parts = p.shared + s.shared;
   if (s.chunks > 1) {
     k_scan<E, S, kSummaryBoth><<<grid, kThreads, 0, st>>>(p);
-    k_scan_carry<E><<<carry, 1024, 0, st>>>(p, p.ends, (int)s.NP, false);
-    k_scan_carry<E><<<carry, 1024, 0, st>>>(p, p.gends, (int)s.NP, true);
+    carry();
   }
   k_scan_bwd<E, S><<<grid, kThreads, 0, st>>>(p);
   k_scan_shared<E><<<dim3((unsigned)((a.batch * a.T * 2 * a.N + 255) / 256)), 256, 0, st>>>(
