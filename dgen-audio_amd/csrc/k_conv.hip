@@ -39,21 +39,67 @@ __device__ __forceinline__ int64_t live_frames(const int32_t* __restrict__ lengt
   return n < 0 ? 0 : n < T ? n : T;
 }
 
-// Frame t (< 0: of the state, else 0) of four channels.
-template <class T, int W>
-__device__ __forceinline__ void conv_frame(const T* __restrict__ x, int64_t ld, const T* st, int64_t D, int64_t t,
-                                           int valid, float (&o)[4]) {
-  if (t >= 0) {
-    load_four(x + t * ld, valid, o);
-  } else if (st) {
-    load_four(st + (t + W - 1) * D, valid, o);
+// Four channels of a thread: its group's, or the last four where the group
+// reaches past the last channel (so that every load is a whole one); of those
+// it owns, and stores, the ones from `skip` on.  Tensors of fewer than four
+// channels (FEW) are loaded element by element.
+struct Channels {
+  int64_t c;
+  int skip, end;  // owned: [skip, end)
+};
+template <bool FEW>
+__device__ __forceinline__ Channels channels_of(int64_t g, int64_t D) {
+  if (FEW) return {0, 0, (int)D};
+  const int64_t c = g * 4 < D - 4 ? g * 4 : D - 4;
+  const int64_t skip = g * 4 - c;
+  return {c, (int)(skip < 4 ? skip : 4), 4};
+}
+template <bool FEW, class T>
+__device__ __forceinline__ Four<T> get_four(const T* __restrict__ p, const Channels& ch) {
+  if (!FEW) return *reinterpret_cast<const Four<T>*>(p);
+  Four<T> f{};
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (e < ch.end) f.e[e] = p[e];
+  return f;
+}
+template <class T>
+__device__ __forceinline__ void put_four(T* __restrict__ p, const Channels& ch, const float (&o)[4]) {
+  if (ch.skip == 0 && ch.end == 4) {
+    store_four(p, 4, o);
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = 0.f;
+    for (int e = 0; e < 4; ++e)
+      if (e >= ch.skip && e < ch.end) p[e] = from_f32<T>(o[e]);
   }
 }
 
-template <class T, int W, bool SILU>
+// Frame t < 0: of the state, else 0.
+template <class T, int W, bool FEW>
+__device__ __forceinline__ void frame_before(const T* st, int64_t D, int64_t t, const Channels& ch, float (&o)[4]) {
+  Four<T> f{};
+  if (st) f = get_four<FEW>(st + (t + W - 1) * D, ch);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = to_f32(f.e[e]);
+}
+
+template <int W>
+struct Taps {
+  float w[W][4], bias[4];
+  __device__ __forceinline__ void load(const float* __restrict__ wt, const float* __restrict__ bs, const Channels& ch) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int64_t c = ch.c + (e < ch.end ? e : 0);
+      bias[e] = bs ? bs[c] : 0.f;
+#pragma unroll
+      for (int q = 0; q < W; ++q) w[q][e] = wt[c * W + q];
+    }
+  }
+};
+
+constexpr int kGroup = 4;  // frames a thread loads ahead of their use
+
+template <class T, int W, bool SILU, bool FEW>
 __global__ __launch_bounds__(kFwdThreads) void k_conv(ConvShape s, const T* __restrict__ x, int64_t xb, int64_t xt,
                                                       const float* __restrict__ w, const float* __restrict__ bias,
                                                       const int32_t* __restrict__ lengths, const T* state,
@@ -61,64 +107,84 @@ __global__ __launch_bounds__(kFwdThreads) void k_conv(ConvShape s, const T* __re
   const int64_t i = (int64_t)blockIdx.x * kFwdThreads + threadIdx.x;
   if (i >= s.B * s.tiles * s.G) return;
   const int64_t b = i / (s.tiles * s.G), r = i - b * (s.tiles * s.G), tile = r / s.G;
-  const int64_t c = (r - tile * s.G) * 4;
-  const int valid = (int)(s.D - c < 4 ? s.D - c : 4);
+  const Channels ch = channels_of<FEW>(r - tile * s.G, s.D);
   const int64_t n = live_frames(lengths, b, s.T), t0 = tile * s.tile, t1 = t0 + s.tile < s.T ? t0 + s.tile : s.T;
-  const T* xp = x + b * xb + c;
-  const T* sp = state ? state + b * (W - 1) * s.D + c : nullptr;
-  T* yp = y + b * yb + c;
+  const int64_t last = n > 0 ? n - 1 : 0;
+  const T* xp = x + b * xb + ch.c;
+  const T* sp = state ? state + b * (W - 1) * s.D + ch.c : nullptr;
+  T* yp = y + b * yb + ch.c;
 
-  float wt[W][4], bs[4], past[W > 1 ? W - 1 : 1][4];
+  Four<T> next[kGroup];
+  auto fetch = [&](int64_t t) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    bs[e] = bias && e < valid ? bias[c + e] : 0.f;
-#pragma unroll
-    for (int q = 0; q < W; ++q) wt[q][e] = e < valid ? w[(c + e) * W + q] : 0.f;
-  }
+    for (int k = 0; k < kGroup; ++k) next[k] = get_four<FEW>(xp + (t + k < last ? t + k : last) * xt, ch);
+  };
+  fetch(t0);
+  Taps<W> taps;
+  taps.load(w, bias, ch);
+  // win[q]: frame t - (W-1) + q of the group's first frame t
+  float win[W - 1 + kGroup][4];
 #pragma unroll
   for (int q = 0; q < W - 1; ++q) {
     const int64_t t = t0 - (W - 1) + q;
-    conv_frame<T, W>(xp, xt, sp, s.D, t, t < n ? valid : 0, past[q]);
+    if (t < 0) {
+      frame_before<T, W, FEW>(sp, s.D, t, ch, win[q]);
+    } else {
+      const Four<T> f = get_four<FEW>(xp + (t < last ? t : last) * xt, ch);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) win[q][e] = to_f32(f.e[e]);
+    }
   }
   if (state_out && tile == 0) {
     // The frames before the sequence's end.  The first tile is the only
     // reader of the state (no tile is shorter than the window), and has read
-    // all that it needs of it before it stores over it.
+    // all that it needs of its channels before it stores over them.
     float left[W > 1 ? W - 1 : 1][4];
 #pragma unroll
-    for (int q = 0; q < W - 1; ++q) conv_frame<T, W>(xp, xt, sp, s.D, n - (W - 1) + q, valid, left[q]);
-    T* so = state_out + b * (W - 1) * s.D + c;
+    for (int q = 0; q < W - 1; ++q) {
+      const int64_t t = n - (W - 1) + q;
+      if (t < 0) {
+        frame_before<T, W, FEW>(sp, s.D, t, ch, left[q]);
+      } else {
+        const Four<T> f = get_four<FEW>(xp + t * xt, ch);
 #pragma unroll
-    for (int q = 0; q < W - 1; ++q) store_four(so + q * s.D, valid, left[q]);
-  }
-  for (int64_t t = t0; t < t1; ++t) {
-    float o[4] = {0.f, 0.f, 0.f, 0.f};
-    if (t < n) {
-      float v[4];
-      load_four(xp + t * xt, valid, v);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float u = bs[e];
-#pragma unroll
-        for (int q = 0; q < W - 1; ++q) u = fmaf(wt[q][e], past[q][e], u);
-        u = fmaf(wt[W - 1][e], v[e], u);
-        o[e] = SILU ? silu(u) : u;
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-#pragma unroll
-        for (int q = 0; q + 1 < W - 1; ++q) past[q][e] = past[q + 1][e];
-        if (W > 1) past[W > 1 ? W - 2 : 0][e] = v[e];
+        for (int e = 0; e < 4; ++e) left[q][e] = to_f32(f.e[e]);
       }
     }
-    store_four(yp + t * yt, valid, o);
+    T* so = state_out + b * (W - 1) * s.D + ch.c;
+#pragma unroll
+    for (int q = 0; q < W - 1; ++q) put_four(so + q * s.D, ch, left[q]);
+  }
+  for (int64_t t = t0; t < t1; t += kGroup) {
+#pragma unroll
+    for (int k = 0; k < kGroup; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) win[W - 1 + k][e] = to_f32(next[k].e[e]);
+    if (t + kGroup < t1) fetch(t + kGroup);
+#pragma unroll
+    for (int k = 0; k < kGroup; ++k) {
+      if (t + k >= t1) break;
+      float o[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float u = taps.bias[e];
+#pragma unroll
+        for (int q = 0; q < W; ++q) u = fmaf(taps.w[q][e], win[k + q][e], u);
+        o[e] = t + k < n ? (SILU ? silu(u) : u) : 0.f;
+      }
+      put_four(yp + (t + k) * yt, ch, o);
+    }
+#pragma unroll
+    for (int q = 0; q < W - 1; ++q)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) win[q][e] = win[q + kGroup][e];
   }
 }
 
 // Workgroup: a tile quad (four tiles) of sequence blockIdx.y and 64 channel
 // groups, blockIdx.x = quad * ceil(G / 64) + block of groups; its partial row
 // is (sequence, quad).
-template <class T, int W, bool SILU>
+template <class T, int W, bool SILU, bool FEW>
 __global__ __launch_bounds__(kBwdGroups* kBwdTiles) void k_conv_bwd(
     ConvShape s, const T* __restrict__ x, int64_t xb, int64_t xt, const T* __restrict__ dy, int64_t gb, int64_t gt,
     const float* __restrict__ w, const float* __restrict__ bias, const int32_t* __restrict__ lengths,
@@ -127,75 +193,94 @@ __global__ __launch_bounds__(kBwdGroups* kBwdTiles) void k_conv_bwd(
   const uint32_t gx = (uint32_t)((s.G + kBwdGroups - 1) / kBwdGroups);
   const int64_t b = blockIdx.y, quad = blockIdx.x / gx;
   const int lane = threadIdx.x & 63, sub = threadIdx.x >> 6;
-  const int64_t g = (int64_t)(blockIdx.x % gx) * kBwdGroups + lane, c = g * 4;
-  const int valid = (int)(c >= s.D ? 0 : s.D - c < 4 ? s.D - c : 4);
-  const int64_t n = live_frames(lengths, b, s.T);
+  const int64_t g = (int64_t)(blockIdx.x % gx) * kBwdGroups + lane;
+  const Channels ch = channels_of<FEW>(g < s.G ? g : s.G - 1, s.D);
+  const int64_t n = live_frames(lengths, b, s.T), last = n > 0 ? n - 1 : 0;
   const int64_t t0 = (quad * kBwdTiles + sub) * s.tile, t1 = t0 + s.tile < s.T ? t0 + s.tile : s.T;
-  float wt[W][4], bs[4], dw[W][4] = {}, dbs[4] = {};
+  float dw[W][4] = {}, dbs[4] = {};
+  if (t0 < s.T && g < s.G) {
+    const T* xp = x + b * xb + ch.c;
+    const T* gp = dy + b * gb + ch.c;
+    const T* sp = state ? state + b * (W - 1) * s.D + ch.c : nullptr;
+    T* op = dx + b * db + ch.c;
+    Four<T> nextx[kGroup], nextg[kGroup];
+    auto fetch = [&](int64_t t) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    bs[e] = bias && e < valid ? bias[c + e] : 0.f;
-#pragma unroll
-    for (int q = 0; q < W; ++q) wt[q][e] = e < valid ? w[(c + e) * W + q] : 0.f;
-  }
-  if (valid && t0 < s.T) {
-    const T* xp = x + b * xb + c;
-    const T* gp = dy + b * gb + c;
-    const T* sp = state ? state + b * (W - 1) * s.D + c : nullptr;
-    T* op = dx + b * db + c;
-    // win[q]: frame t - (W-1) + q; du[q]: du of frame t - q
-    float win[W][4], du[W][4];
-#pragma unroll
-    for (int q = 0; q < W; ++q)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) win[q][e] = du[q][e] = 0.f;
+      for (int k = 0; k < kGroup; ++k) {
+        const int64_t at = t + k < last ? t + k : last;
+        nextx[k] = get_four<FEW>(xp + at * xt, ch);
+        nextg[k] = get_four<FEW>(gp + at * gt, ch);
+      }
+    };
+    fetch(t0);
+    Taps<W> taps;
+    taps.load(w, bias, ch);
+    // win[q]: frame t - (W-1) + q, du[q]: du of frame t - (W-1) + q
+    float win[W - 1 + kGroup][4], du[W - 1 + kGroup][4];
 #pragma unroll
     for (int q = 0; q < W - 1; ++q) {
       const int64_t t = t0 - (W - 1) + q;
-      conv_frame<T, W>(xp, xt, sp, s.D, t, t < n ? valid : 0, win[q + 1]);
+      if (t < 0) {
+        frame_before<T, W, FEW>(sp, s.D, t, ch, win[q]);
+      } else {
+        const Four<T> f = get_four<FEW>(xp + (t < last ? t : last) * xt, ch);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) win[q][e] = t < n ? to_f32(f.e[e]) : 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) du[q][e] = 0.f;
     }
-    for (int64_t t = t0; t < t1 + W - 1; ++t) {
+    for (int64_t t = t0; t < t1 + W - 1; t += kGroup) {
 #pragma unroll
-      for (int q = 0; q + 1 < W; ++q)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) win[q][e] = win[q + 1][e];
-#pragma unroll
-      for (int q = W - 1; q > 0; --q)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) du[q][e] = du[q - 1][e];
-      float d[4];
-      load_four(xp + t * xt, t < n ? valid : 0, win[W - 1]);
-      load_four(gp + t * gt, t < n ? valid : 0, d);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (SILU) {
-          float u = bs[e];
-#pragma unroll
-          for (int q = 0; q < W; ++q) u = fmaf(wt[q][e], win[q][e], u);
-          d[e] = t < n ? d[e] * silu_grad(u, sigmoid(u)) : 0.f;
-        }
-        du[0][e] = d[e];
-      }
-      if (t < t1) {
+      for (int k = 0; k < kGroup; ++k)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          dbs[e] += d[e];
-#pragma unroll
-          for (int q = 0; q < W; ++q) dw[q][e] = fmaf(d[e], win[q][e], dw[q][e]);
+          const bool in = t + k < n;
+          win[W - 1 + k][e] = in ? to_f32(nextx[k].e[e]) : 0.f;
+          du[W - 1 + k][e] = in ? to_f32(nextg[k].e[e]) : 0.f;
         }
-      }
-      const int64_t to = t - (W - 1);
-      if (to >= t0) {
-        float o[4];
+      if (t + kGroup < t1 + W - 1) fetch(t + kGroup);
+#pragma unroll
+      for (int k = 0; k < kGroup; ++k) {
+        const bool own = t + k < t1;  // (frames past the tile only for the gradients before them)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          o[e] = 0.f;
+          float d = du[W - 1 + k][e];
+          if (SILU) {
+            float u = taps.bias[e];
 #pragma unroll
-          for (int q = 0; q < W; ++q) o[e] = fmaf(wt[q][e], du[q][e], o[e]);
-          if (to >= n) o[e] = 0.f;
+            for (int q = 0; q < W; ++q) u = fmaf(taps.w[q][e], win[k + q][e], u);
+            const float sl = silu_grad(u, sigmoid(u));
+            d = t + k < n ? d * sl : 0.f;
+            du[W - 1 + k][e] = d;
+          }
+          const float mine = own ? d : 0.f;
+          dbs[e] += mine;
+#pragma unroll
+          for (int q = 0; q < W; ++q) dw[q][e] = fmaf(mine, win[k + q][e], dw[q][e]);
         }
-        store_four(op + to * dt, valid, o);
+        // the frame that has all of its du now
+        const int64_t to = t + k - (W - 1);
+        if (to >= t0 && to < t1) {
+          float o[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            o[e] = 0.f;
+            // dx[to] = sum_q w[q] du[to + W-1-q]
+#pragma unroll
+            for (int q = 0; q < W; ++q) o[e] = fmaf(taps.w[q][e], du[W - 1 + k - q][e], o[e]);
+            if (to >= n) o[e] = 0.f;
+          }
+          put_four(op + to * dt, ch, o);
+        }
       }
+#pragma unroll
+      for (int q = 0; q < W - 1; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          win[q][e] = win[q + kGroup][e];
+          du[q][e] = du[q + kGroup][e];
+        }
     }
   }
   // [D][W] weight gradients, then [D] bias gradients
@@ -206,52 +291,57 @@ __global__ __launch_bounds__(kBwdGroups* kBwdTiles) void k_conv_bwd(
 #pragma unroll
     for (int e = 0; e < 4; ++e) red[sub][lane][e] = q < W ? dw[q < W ? q : 0][e] : dbs[e];
     __syncthreads();
-    // thread (sub, lane): channel 4 lane + sub
-    if (sub < valid) {
+    // thread (sub, lane): channel `sub` of the lane's four
+    if (g < s.G && sub >= ch.skip && sub < ch.end) {
       float t = 0.f;
 #pragma unroll
       for (int k = 0; k < kBwdTiles; ++k) t += red[k][lane][sub];
-      if (q < W) out[(c + sub) * W + q] = t;
-      else out[s.D * W + c + sub] = t;
+      if (q < W) out[(ch.c + sub) * W + q] = t;
+      else out[s.D * W + ch.c + sub] = t;
     }
   }
 }
 
 int64_t conv_quads(const ConvShape& s) { return (s.tiles + kBwdTiles - 1) / kBwdTiles; }
 
-template <class T, int W, bool SILU>
+template <class T, int W, bool SILU, bool FEW>
 void conv_launch(const dgen_hip_conv& a, bool backward, hipStream_t st) {
   const ConvShape s = conv_shape(a, backward);
   if (!backward) {
     const int64_t threads = s.B * s.tiles * s.G;
-    k_conv<T, W, SILU><<<dim3((unsigned)((threads + kFwdThreads - 1) / kFwdThreads)), kFwdThreads, 0, st>>>(
+    k_conv<T, W, SILU, FEW><<<dim3((unsigned)((threads + kFwdThreads - 1) / kFwdThreads)), kFwdThreads, 0, st>>>(
         s, (const T*)a.x.data, a.x.stride_b, a.x.stride_t, a.weight, a.bias, a.lengths, (const T*)a.state,
         (T*)a.state_out, (T*)a.y.data, a.y.stride_b, a.y.stride_t);
   } else {
     const int64_t quads = conv_quads(s);
     float* parts = (float*)a.workspace;
-    k_conv_bwd<T, W, SILU>
+    k_conv_bwd<T, W, SILU, FEW>
         <<<dim3((unsigned)((s.G + kBwdGroups - 1) / kBwdGroups * quads), (unsigned)s.B), kBwdGroups * kBwdTiles, 0,
-           st>>>(s, (const T*)a.x.data, a.x.stride_b, a.x.stride_t, (const T*)a.dy.data,
-                                            a.dy.stride_b, a.dy.stride_t, a.weight, a.bias, a.lengths,
-                                            (const T*)a.state, (T*)a.dx.data, a.dx.stride_b, a.dx.stride_t, parts,
-                                            quads);
+           st>>>(s, (const T*)a.x.data, a.x.stride_b, a.x.stride_t, (const T*)a.dy.data, a.dy.stride_b, a.dy.stride_t,
+                 a.weight, a.bias, a.lengths, (const T*)a.state, (T*)a.dx.data, a.dx.stride_b, a.dx.stride_t, parts,
+                 quads);
     enqueue_sum_parts(st, parts, s.B * quads, {{a.dweight, a.dbias, nullptr}, {s.D * W, s.D, 0}});
   }
 }
 
-template <class T, bool SILU>
+template <class T, bool SILU, bool FEW>
 void conv_taps(const dgen_hip_conv& a, bool backward, hipStream_t st) {
   switch (a.width) {
-    case 1: return conv_launch<T, 1, SILU>(a, backward, st);
-    case 2: return conv_launch<T, 2, SILU>(a, backward, st);
-    case 3: return conv_launch<T, 3, SILU>(a, backward, st);
-    case 4: return conv_launch<T, 4, SILU>(a, backward, st);
-    case 5: return conv_launch<T, 5, SILU>(a, backward, st);
-    case 6: return conv_launch<T, 6, SILU>(a, backward, st);
-    case 7: return conv_launch<T, 7, SILU>(a, backward, st);
-    default: return conv_launch<T, 8, SILU>(a, backward, st);
+    case 1: return conv_launch<T, 1, SILU, FEW>(a, backward, st);
+    case 2: return conv_launch<T, 2, SILU, FEW>(a, backward, st);
+    case 3: return conv_launch<T, 3, SILU, FEW>(a, backward, st);
+    case 4: return conv_launch<T, 4, SILU, FEW>(a, backward, st);
+    case 5: return conv_launch<T, 5, SILU, FEW>(a, backward, st);
+    case 6: return conv_launch<T, 6, SILU, FEW>(a, backward, st);
+    case 7: return conv_launch<T, 7, SILU, FEW>(a, backward, st);
+    default: return conv_launch<T, 8, SILU, FEW>(a, backward, st);
   }
+}
+
+template <class T>
+void conv_form(const dgen_hip_conv& a, bool backward, hipStream_t st) {
+  if (a.D < 4) a.silu ? conv_taps<T, true, true>(a, backward, st) : conv_taps<T, false, true>(a, backward, st);
+  else a.silu ? conv_taps<T, true, false>(a, backward, st) : conv_taps<T, false, false>(a, backward, st);
 }
 
 }  // namespace
@@ -299,9 +389,9 @@ int conv_run(const dgen_hip_conv& a, bool backward, hipStream_t st, bool dry) {
     if (!backward) return 0;
     enqueue_sum_parts(st, a.weight, 0, {{a.dweight, a.dbias, nullptr}, {a.D * a.width, a.D, 0}});  // zeros
   } else if (a.type == DGEN_HIP_BF16) {
-    a.silu ? conv_taps<bf16, true>(a, backward, st) : conv_taps<bf16, false>(a, backward, st);
+    conv_form<bf16>(a, backward, st);
   } else {
-    a.silu ? conv_taps<float, true>(a, backward, st) : conv_taps<float, false>(a, backward, st);
+    conv_form<float>(a, backward, st);
   }
   DGEN_LAUNCH_CHECK(what);
   return 0;

@@ -664,25 +664,33 @@ __global__ __launch_bounds__(256) void k_glu_join(const float* __restrict__ part
 
 // Forward for a few rows (single frames of some voices): the weights' reading
 // is all that counts, and its latency, so the vector unit multiplies.  A
-// workgroup owns 64 columns (32 lanes x 2: whole cache lines); the half-waves
-// of 16 waves take every 32nd k, each with all of its 16 loads of a round of
-// 512 k's in flight at once; the 32 sums meet in LDS.
-constexpr int kFewRows = 8, kFewThreads = 1024, kFewCols = 64, kFewK = 512, kFewLoads = kFewK / 32;
+// workgroup owns 32 columns (16 lanes x 2); the quarter-waves of 16 waves take
+// every 64th k, each with all of its 8 loads of a round of 512 k's in flight
+// at once; the 64 sums meet in registers, then in LDS.  (64 columns a workgroup
+// leave most CUs idle: 512 x 1408, 8 rows: 11.8 us against 9.8.)
+constexpr int kFewRows = 8, kFewThreads = 1024, kFewCols = 32, kFewK = 512;
+constexpr int kFewLanes = kFewCols / 2, kFewSlices = kFewThreads / kFewLanes, kFewLoads = kFewK / kFewSlices;
 template <class E>
 __global__ __launch_bounds__(kFewThreads) void k_glu_few(GluP<E> p) {
   __shared__ __align__(16) float xs[kFewK][kFewRows];
   __shared__ float red[16][kFewCols][2][kFewRows + 1];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, slice = wave * 2 + (lane >> 5);
-  const int64_t m0 = (int64_t)blockIdx.y * kFewRows, f = (int64_t)blockIdx.x * kFewCols + (lane & 31) * 2;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, slice = threadIdx.x / kFewLanes;
+  const int64_t m0 = (int64_t)blockIdx.y * kFewRows, f = (int64_t)blockIdx.x * kFewCols + (lane % kFewLanes) * 2;
   const bool two = f + 1 < p.N;
   const int64_t col = two ? f : f < p.N ? f : p.N - 1;  // (columns past the end are not stored)
   float acc[2][2][kFewRows] = {};
   for (int64_t k0 = 0; k0 < p.K; k0 += kFewK) {
+    float xv[kFewK * kFewRows / kFewThreads];
+#pragma unroll
+    for (int i = 0; i < kFewK * kFewRows / kFewThreads; ++i) {
+      const int id = threadIdx.x + i * kFewThreads, m = id / kFewK, k = id % kFewK;
+      xv[i] = k0 + k < p.K && m0 + m < p.M ? to_f32(p.m0[(m0 + m) * p.mld0 + k0 + k]) : 0.f;
+    }
     Vec<E, 2> w[kFewLoads][2];
     const E *g = p.n0 + col, *u = p.n1 + col;
 #pragma unroll
     for (int i = 0; i < kFewLoads; ++i) {
-      const int64_t k = k0 + slice + 32 * i, kc = k < p.K ? k : p.K - 1;  // (x is 0 past the end)
+      const int64_t k = k0 + slice + kFewSlices * i, kc = k < p.K ? k : p.K - 1;  // (x is 0 past the end)
       if (two) {
         w[i][0] = *reinterpret_cast<const Vec<E, 2>*>(g + kc * p.nld0);
         w[i][1] = *reinterpret_cast<const Vec<E, 2>*>(u + kc * p.nld1);
@@ -692,18 +700,19 @@ __global__ __launch_bounds__(kFewThreads) void k_glu_few(GluP<E> p) {
       }
     }
     if (k0 > 0) __syncthreads();
-    for (int i = threadIdx.x; i < kFewK * kFewRows; i += kFewThreads) {
-      const int m = i / kFewK, k = i % kFewK;
-      xs[k][m] = k0 + k < p.K && m0 + m < p.M ? to_f32(p.m0[(m0 + m) * p.mld0 + k0 + k]) : 0.f;
+#pragma unroll
+    for (int i = 0; i < kFewK * kFewRows / kFewThreads; ++i) {
+      const int id = threadIdx.x + i * kFewThreads;
+      xs[id % kFewK][id / kFewK] = xv[i];
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kFewLoads; ++i) {
-      const int64_t k = k0 + slice + 32 * i;
-      if (k >= p.K) continue;
+      // (past the end the weights are a row inside, which may hold anything)
+      if (k0 + slice + kFewSlices * i >= p.K) continue;
 #pragma unroll
       for (int m = 0; m < kFewRows; ++m) {
-        const float x = xs[slice + 32 * i][m];
+        const float x = xs[slice + kFewSlices * i][m];
 #pragma unroll
         for (int a = 0; a < 2; ++a)
 #pragma unroll
@@ -717,12 +726,14 @@ __global__ __launch_bounds__(kFewThreads) void k_glu_few(GluP<E> p) {
     for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int m = 0; m < kFewRows; ++m) {
-        const float t = acc[a][b][m] + __shfl_xor(acc[a][b][m], 32, 64);
-        if (lane < 32) red[wave][lane * 2 + b][a][m] = t;
+        float t = acc[a][b][m];
+        t += __shfl_xor(t, 16, 64);
+        t += __shfl_xor(t, 32, 64);
+        if (lane < kFewLanes) red[wave][lane * 2 + b][a][m] = t;
       }
   __syncthreads();
   if (threadIdx.x >= kFewCols * kFewRows) return;
-  const int c = threadIdx.x % kFewCols, m = threadIdx.x / kFewCols;  // 64 columns x 8 rows
+  const int c = threadIdx.x % kFewCols, m = threadIdx.x / kFewCols;
   const int64_t n = (int64_t)blockIdx.x * kFewCols + c;
   float s[2] = {0.f, 0.f}, slope;
 #pragma unroll
