@@ -1,25 +1,27 @@
 // Gated feed-forward block: h = act(x Wg) * (x Wu), forward and backward, on
 // the bf16 matrix cores.
 //
-// One product kernel serves four uses.  A workgroup of four waves owns a tile
-// of the output; operand tiles go from memory through registers to LDS, where
-// they lie k-contiguous whatever their layout in memory (an operand that is
-// contiguous along its rows is transposed on the way: a thread loads 8 k's of a
-// few neighbouring rows and packs them with one byte permutation a dword).
-//
-// - forward: the tile's columns are 32- or 64-wide groups of gate and up
-//   columns side by side, so a wave holds both projections of the same outputs
-//   and applies the activation and the product in registers;
+// Products, by use:
+// - forward: a tile's columns are groups of gate and up columns side by side,
+//   so a wave holds both projections of the same outputs and applies the
+//   activation and the product in registers;
 // - backward, projections again: the same, but the epilogue reads dh and
-//   writes dg = dh u act'(g) and du = dh act(g), in the operands' type;
+//   writes dg = dh u act'(g) and du = dh act(g);
 // - dx = dg Wg^T + du Wu^T: one product over 2 x hidden;
-// - dWg = x^T dg, dWu = x^T du: products over the rows, split over row ranges
-//   where the tiles alone do not fill the chip; the parts are added in order.
+// - dWg = x^T dg, dWu = x^T du: products over the rows.
+// Where tiles alone do not fill the chip, the reductions of dx and dW are cut
+// into runs whose parts are added in order.
 //
-// bfloat16 operands multiply as they are, accumulated in fp32.  fp32 operands
-// are split exactly into three bfloat16 parts on the way to LDS and the six
-// partial products down to 2^-16 are accumulated in fp32, as accurate as fp32
-// products (see k_gemm.hip).
+// bfloat16 operands multiply as they are, accumulated in fp32 (dg and du are
+// rounded to bfloat16 between the products, as the operands are).  fp32
+// operands are split exactly into three bfloat16 parts on the way to LDS, and
+// the six partial products down to 2^-16 are accumulated in fp32, as accurate
+// as fp32 products (see k_gemm.hip).
+//
+// Three kernels: k_glu_direct, bfloat16, 256 x 256 tiles on operands that lie
+// in whole 16-byte chunks (packed first where they do not); k_glu, operands of
+// any layout and type, 128 x 128 (fp32) or 64 x 128 tiles; k_glu_few, a few
+// rows.
 //
 // The matrix instruction's row index is the output's column, so a lane ends
 // with four consecutive columns of one output row.
@@ -118,39 +120,43 @@ struct Stage {
   static_assert(kPer % 8 == 0 && V >= 1 && U >= 1, "tile too small");
   E v[U][KC ? 1 : 8][V];
 
-  // row(r): the address of row r of the tile (KC) or of element (r, k = 0)
-  // (!KC), and how many rows from r on are inside the operand.
-  template <class Row>
-  __device__ __forceinline__ void load(Row row, int64_t ld, int64_t k0, int64_t kend) {
+  // at(r): the address of row r of the tile (KC), or of element (r, k = 0)
+  // (!KC), clamped into the operand; inside(r): how many rows from r on lie in
+  // it.  `whole`: the tile is inside the operand (uniform), so that the loads
+  // are whole and without a branch; else zeros stand for what lies outside.
+  // (Rows past the end of a k-contiguous operand repeat its last one: their
+  // results are not stored.)
+  template <class At, class Inside>
+  __device__ __forceinline__ void load(At at, Inside inside, int64_t ld, int64_t k0, int64_t kend, bool whole) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = threadIdx.x + u * kThreads;
-      if constexpr (KC) {
-        const int r = i / (BK / 8);
-        const int64_t k = k0 + (i % (BK / 8)) * 8;
-        const E* p;
-        const bool in = row(r, p) > 0;
-        get<V>(p + k, in ? kend - k : 0, v[u][0]);
-      } else {
-        const int r = (i % (R / V)) * V;
-        const int64_t k = k0 + (i / (R / V)) * 8;
-        const E* p;
-        const int64_t in = row(r, p);
+      const int r = KC ? i / (BK / 8) : (i % (R / V)) * V;
+      const int64_t k = k0 + (KC ? i % (BK / 8) : i / (R / V)) * 8;
+      const E* p = at(r);
+      if (whole) {
 #pragma unroll
-        for (int q = 0; q < 8; ++q) get<V>(p + (k + q) * ld, k + q < kend ? in : 0, v[u][q]);
+        for (int q = 0; q < (KC ? 1 : 8); ++q) {
+          const Vec<E, V> t = *reinterpret_cast<const Vec<E, V>*>(KC ? p + k : p + (k + q) * ld);
+#pragma unroll
+          for (int e = 0; e < V; ++e) v[u][q][e] = t.e[e];
+        }
+      } else {
+        const int64_t rows = inside(r);
+#pragma unroll
+        for (int q = 0; q < (KC ? 1 : 8); ++q)
+          get(KC ? p + k : p + (k + q) * ld, KC ? kend - k : k + q < kend ? rows : 0, v[u][q]);
       }
     }
   }
-
-  template <int W>
-  __device__ __forceinline__ static void get(const E* p, int64_t valid, E (&o)[W]) {
-    if (valid >= W) {
-      const Vec<E, W> t = *reinterpret_cast<const Vec<E, W>*>(p);
+  __device__ __forceinline__ static void get(const E* p, int64_t valid, E (&o)[V]) {
+    if (valid >= V) {
+      const Vec<E, V> t = *reinterpret_cast<const Vec<E, V>*>(p);
 #pragma unroll
-      for (int e = 0; e < W; ++e) o[e] = t.e[e];
+      for (int e = 0; e < V; ++e) o[e] = t.e[e];
     } else {
 #pragma unroll
-      for (int e = 0; e < W; ++e) o[e] = e < valid ? p[e] : E{};
+      for (int e = 0; e < V; ++e) o[e] = e < valid ? p[e] : E{};
     }
   }
 
@@ -225,7 +231,8 @@ __device__ __forceinline__ void finish(const GluP<E>& p, const floatx16 (&acc)[N
             put_four(p.out1 + m * p.old1 + n, p.N - n, u);
           }
         } else if constexpr (USE == kDx) {
-          put_four(p.out0 + m * p.old0 + n, p.N - n, a);
+          if (p.parts) put_four(p.parts + ((int64_t)split * p.M + m) * p.N + n, p.N - n, a);
+          else put_four(p.out0 + m * p.old0 + n, p.N - n, a);
         } else {
           if (p.parts) {
             put_four(p.parts + ((int64_t)split * 2 + mat) * p.M * p.N + m * p.N + n, p.N - n, a);
@@ -246,25 +253,25 @@ __device__ __forceinline__ void finish(const GluP<E>& p, const floatx16 (&acc)[N
 struct TileAt {
   uint32_t n, m, split, mat;
 };
-template <int USE, class E>
-__device__ __forceinline__ TileAt tile_at(const GluP<E>& p) {
+template <int USE, class Params>
+__device__ __forceinline__ TileAt tile_at(const Params& p) {
   const uint32_t total = gridDim.x, each = total / 8, more = total % 8;
   const uint32_t xcd = blockIdx.x & 7, id = xcd * each + (xcd < more ? xcd : more) + (blockIdx.x >> 3);
   const uint32_t plane = p.tiles_n * p.tiles_m, rest = id / plane, at = id - rest * plane;
   const uint32_t group = at / (4 * p.tiles_m), in = at - group * 4 * p.tiles_m;
   const uint32_t wide = p.tiles_n - group * 4 < 4 ? p.tiles_n - group * 4 : 4;
-  return {group * 4 + in % wide, in / wide, USE == kDw ? rest % p.splits : 0, USE == kDw ? rest / p.splits : 0};
+  return {group * 4 + in % wide, in / wide, USE == kDw || USE == kDx ? rest % p.splits : 0, USE == kDw ? rest / p.splits : 0};
 }
 
 // BM x BN: output rows and operand columns of a tile; WM x WN: of a wave.
-template <class E, int BM, int BN, int WM, int WN, int BK, int BUF, int USE>
+template <class E, int BM, int BN, int WM, int WN, int BK, int USE>
 __global__ __launch_bounds__(kThreads) void k_glu(GluP<E> p) {
   constexpr int P = planes<E>(), NF = WN / 32, MF = WM / 32;
   constexpr bool PAIR = USE == kForward || USE == kProject;
   constexpr bool NKC = USE == kDx, MKC = USE != kDw;
   static_assert((BM / WM) * (BN / WN) == kThreads / 64, "four waves");
   constexpr int NCH = P * BN * BK / 8, MCH = P * BM * BK / 8;
-  __shared__ Chunk lds[BUF][NCH + MCH];
+  __shared__ Chunk lds[NCH + MCH];
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wn = wave % (BN / WN), wm = wave / (BN / WN);
@@ -275,44 +282,41 @@ __global__ __launch_bounds__(kThreads) void k_glu(GluP<E> p) {
   const int64_t kfrom = USE == kDw ? split * p.span : 0;
   const int64_t kend = USE == kDw && kfrom + p.span < p.K ? kfrom + p.span : p.K;
   const int64_t kblocks = kend > kfrom ? (kend - kfrom + BK - 1) / BK : 0;
-  const int64_t steps = USE == kDx ? 2 * kblocks : kblocks;
+  const int64_t all = USE == kDx ? 2 * kblocks : kblocks;
+  // dx over few tiles: a run of the steps each
+  const int64_t first = USE == kDx ? split * p.span : 0;
+  const int64_t steps = USE == kDx && first + p.span < all ? first + p.span : all;
 
   Stage<E, BN, BK, NKC> sn;
   Stage<E, BM, BK, MKC> sm;
   auto load = [&](int64_t step) {
     const bool second = USE == kDx && step >= kblocks;
     const int64_t k0 = kfrom + (second ? step - kblocks : step) * BK;
-    const bool n_second = second || (USE == kDw && mat), m_second = second;
-    const E* nb = n_second ? p.n1 : p.n0;
-    const int64_t nld = n_second ? p.nld1 : p.nld0;
-    const E* mb = m_second ? p.m1 : p.m0;
-    const int64_t mld = m_second ? p.mld1 : p.mld0;
-    auto nrow = [&](int r, const E*& at) -> int64_t {
-      if constexpr (PAIR) {
-        // a wave's WN columns: WN / 2 of gate, then the same of up
-        const bool up = (r % WN) >= WN / 2;
-        const int64_t f = n0 + r / WN * (WN / 2) + r % (WN / 2);
-        at = (up ? p.n1 : p.n0) + f;
-        return p.N - f;
-      } else {
-        const int64_t n = n0 + r;
-        at = NKC ? nb + n * nld : nb + n;
-        return p.N - n;
-      }
+    const bool n_second = second || (USE == kDw && mat);
+    const E *nb = n_second ? p.n1 : p.n0, *mb = second ? p.m1 : p.m0;
+    const int64_t nld = n_second ? p.nld1 : p.nld0, mld = second ? p.mld1 : p.mld0;
+    // a wave's WN columns are WN / 2 of gate, then the same of up
+    auto column = [&](int r) { return PAIR ? n0 + r / WN * (WN / 2) + r % (WN / 2) : n0 + r; };
+    auto nat = [&](int r) {
+      const int64_t c = column(r), n = c < p.N ? c : p.N - 1;
+      if constexpr (PAIR) return ((r % WN) >= WN / 2 ? p.n1 : p.n0) + n;
+      else return NKC ? nb + n * nld : nb + n;
     };
-    auto mrow = [&](int r, const E*& at) -> int64_t {
-      const int64_t m = m0 + r;
-      at = MKC ? mb + m * mld : mb + m;
-      return p.M - m;
+    auto nin = [&](int r) { return p.N - column(r); };
+    auto mat_at = [&](int r) {
+      const int64_t m = m0 + r < p.M ? m0 + r : p.M - 1;
+      return MKC ? mb + m * mld : mb + m;
     };
+    auto min = [&](int r) { return p.M - (m0 + r); };
+    const bool ks = k0 + BK <= kend;
     if constexpr (PAIR) {
       // (the two matrices may have different strides: the block's own is used)
       const bool up = ((threadIdx.x % (BN / Stage<E, BN, BK, NKC>::V)) * Stage<E, BN, BK, NKC>::V) % WN >= WN / 2;
-      sn.load(nrow, up ? p.nld1 : p.nld0, k0, kend);
+      sn.load(nat, nin, up ? p.nld1 : p.nld0, k0, kend, ks && n0 + COLS <= p.N);
     } else {
-      sn.load(nrow, nld, k0, kend);
+      sn.load(nat, nin, nld, k0, kend, ks && (NKC || n0 + COLS <= p.N));
     }
-    sm.load(mrow, mld, k0, kend);
+    sm.load(mat_at, min, mld, k0, kend, ks && (MKC || m0 + BM <= p.M));
   };
 
   floatx16 acc[NF][MF] = {};
@@ -352,50 +356,50 @@ __global__ __launch_bounds__(kThreads) void k_glu(GluP<E> p) {
     }
   };
 
-  if (steps > 0) load(0);
-  if constexpr (BUF == 2) {
-    if (steps > 0) {
-      sn.store(lds[0]);
-      sm.store(lds[0] + NCH);
-    }
+  if (steps > first) load(first);
+  for (int64_t s = first; s < steps; ++s) {
     __syncthreads();
-    for (int64_t s = 0; s < steps; ++s) {
-      if (s + 1 < steps) load(s + 1);
-      compute(lds[s & 1]);
-      if (s + 1 < steps) {
-        sn.store(lds[(s + 1) & 1]);
-        sm.store(lds[(s + 1) & 1] + NCH);
-      }
-      __syncthreads();
-    }
-  } else {
-    for (int64_t s = 0; s < steps; ++s) {
-      __syncthreads();
-      sn.store(lds[0]);
-      sm.store(lds[0] + NCH);
-      __syncthreads();
-      if (s + 1 < steps) load(s + 1);
-      compute(lds[0]);
-    }
+    sn.store(lds);
+    sm.store(lds + NCH);
+    __syncthreads();
+    if (s + 1 < steps) load(s + 1);
+    __builtin_amdgcn_sched_barrier(0);  // the loads before the products, which they land behind
+    compute(lds);
   }
 
   finish<E, USE, NF, MF>(p, acc, m0 + wm * WM, n0 + (PAIR ? wn * (WN / 2) : wn * WN), split, mat);
 }
 
-// ------------------------------------------------- bf16, aligned operands
-// The same product with operand tiles copied global -> LDS by the load-to-LDS
-// instructions, as they lie in memory: 256 x 256 outputs a workgroup of eight
-// waves, 128 x 64 a wave (128 accumulators a lane; two waves a SIMD cover each
-// other's LDS reads and barriers), stages of 32 k's in four LDS buffers, two to
-// three of them in flight.  An operand that is contiguous along its rows is
-// read with the transposing LDS load.  Chunks of 16 bytes are permuted within
-// their LDS rows through the global addresses, so that the fragments' reads
-// spread over the banks: k-contiguous rows (four chunks) by row / 2, row-
-// contiguous k's (32 chunks) by twice the k.  Results go to memory through LDS
-// in whole rows of the tile (stored from the accumulators' layout, 8 bytes to
-// each of 32 rows, a tile took 40 us).
-constexpr int kDM = 256, kDN = 256, kDK = 32, kDBufs = 4, kDThreads = 512;
-constexpr int kDMChunks = kDM * kDK / 8, kDNChunks = kDN * kDK / 8;  // of a stage
+// ------------------------------------------------------- packed operands
+// Operand tiles are copied global -> LDS by the load-to-LDS instructions, as
+// they lie in memory: 256 x 256 outputs a workgroup of eight waves, 128 x 64 a
+// wave (128 accumulators a lane; two waves a SIMD cover each other's LDS reads
+// and barriers), stages of 32 k's in four LDS buffers, two to three of them in
+// flight.  An operand that is contiguous along its rows is read with the
+// transposing LDS load.  Chunks of 16 bytes are permuted within their LDS rows
+// through the global addresses, so that the fragments' reads spread over the
+// banks: k-contiguous rows (four chunks) by row / 2, row-contiguous k's (32
+// chunks) by twice the k.  Results go to memory through LDS in whole rows of
+// the tile (stored from the accumulators' layout, 8 bytes
+// to each of 32 rows, a tile took 40 us).
+constexpr int kDT = 256, kDK = 32, kDThreads = 512, kDChunks = kDT * kDK / 8;  // chunks of an operand's stage
+
+struct GluD {
+  const bf16 *n0, *n1, *m0, *m1;  // operands along columns and rows, gate and up
+  int64_t nld, mld;               // row strides
+  int64_t nx, mx;                 // readable extent of the axis that is not reduced (k-contiguous:
+                                  // rows; else columns, a multiple of 8)
+  int64_t M, N, K;                // results; reduction of a segment, a multiple of 32
+  bf16 *out0, *out1;
+  int64_t old0, old1;
+  int64_t om, on;                 // project: extent of dg and du (zero past M, N)
+  const bf16* dh;
+  int64_t dhld;
+  float* parts;                   // [splits][mats][M][N] (dx may do without: to out)
+  int64_t span;                   // of a split: rows (dW, a multiple of 32) or stages (dx)
+  int act, dh_copied;             // dh lies in whole chunks: copied to LDS too
+  uint32_t tiles_n, tiles_m, splits;
+};
 
 typedef short short4v __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) short4v lds_short4;
@@ -405,16 +409,19 @@ typedef __attribute__((address_space(3))) short4v lds_short4;
 // transposing LDS read; the kernel waits for its copies itself.  (M0 has no
 // other use in it.)
 __device__ __forceinline__ void copy_to_lds(const bf16* g, uint32_t at) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(g) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(
+                   __builtin_amdgcn_readfirstlane(at)),
+               "v"(g)
+               : "memory");
 }
 
 template <bool KC>
 __device__ __forceinline__ int chunk_swizzle(int row) { return KC ? (row >> 1) & 3 : (row & 3) << 1; }
 
 // Fragment of 32 rows from `r0` on at k-step ks of a stage.
-template <bool KC, int ROWS>
+template <bool KC>
 __device__ __forceinline__ bf16x8 fragment(const uint4* b, int r0, int ks, int lane) {
-  constexpr int C = ROWS / 8;
+  constexpr int C = kDT / 8;
   if constexpr (KC) {
     const int r = r0 + (lane & 31), c = ks * 2 + (lane >> 5);
     return __builtin_bit_cast(bf16x8, b[r * 4 + (c ^ chunk_swizzle<true>(r))]);
@@ -435,84 +442,106 @@ __device__ __forceinline__ bf16x8 fragment(const uint4* b, int r0, int ks, int l
   }
 }
 
+// Whole rows of a tile from LDS (C chunks a row, chunk c of row r at
+// r C + (c ^ r % 16)) to memory: V elements a chunk, rows below `rows` and
+// columns below `cols`.
+template <class E, int C, int ROWS>
+__device__ __forceinline__ void put_rows(const uint4* tile, E* out, int64_t ld, int64_t m0, int64_t n0, int64_t rows,
+                                         int64_t cols) {
+  constexpr int V = 16 / (int)sizeof(E);
+#pragma unroll 4
+  for (int k = 0; k < ROWS * C / kDThreads; ++k) {
+    const int id = threadIdx.x + k * kDThreads, r = id / C, c = id % C;
+    const int64_t m = m0 + r, n = n0 + c * V;
+    const Vec<E, V> v = __builtin_bit_cast(Vec<E, V>, tile[r * C + (c ^ (r & 15))]);
+    if (m < rows) {
+      if (n + V <= cols) {
+        *reinterpret_cast<Vec<E, V>*>(out + m * ld + n) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (n + e < cols) out[m * ld + n + e] = v.e[e];
+      }
+    }
+  }
+}
+
 template <int USE>
-__global__ __launch_bounds__(kDThreads, 2) void k_glu_direct(GluP<bf16> p) {
+__global__ __launch_bounds__(kDThreads, 2) void k_glu_direct(GluD p) {
   constexpr bool PAIR = USE == kForward || USE == kProject;
   constexpr bool NKC = USE == kDx, MKC = USE != kDw;
-  constexpr int NF = 2, MF = 4, NJ = kDNChunks / kDThreads, MJ = kDMChunks / kDThreads;
-  __shared__ __align__(1024) uint4 lds[kDBufs][kDNChunks + kDMChunks];
+  constexpr int NF = 2, MF = 4, J = kDChunks / kDThreads;  // copies of an operand a lane and stage
+  static_assert(J == 2, "the waits below count them");
+  __shared__ __align__(1024) uint4 lds[4][2 * kDChunks];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wn = wave & 3, wm = wave >> 2;
   const TileAt t = tile_at<USE>(p);
-  const int64_t n0 = (int64_t)t.n * (PAIR ? kDN / 2 : kDN), m0 = (int64_t)t.m * kDM;
+  const int64_t n0 = (int64_t)t.n * (PAIR ? kDT / 2 : kDT), m0 = (int64_t)t.m * kDT;
   const int64_t kfrom = USE == kDw ? t.split * p.span : 0;
   const int64_t kend = USE == kDw && kfrom + p.span < p.K ? kfrom + p.span : p.K;
-  const int64_t len = kend > kfrom ? kend - kfrom : 0;
-  const int blocks = (int)(len / kDK);  // (len is a multiple of kDK)
-  const int stages = USE == kDx ? 2 * blocks : blocks;
+  const int blocks = (int)((kend - kfrom) / kDK);  // stages of a segment
+  const int all = USE == kDx ? 2 * blocks : blocks;
+  // dx: a run of the stages
+  const int first = USE == kDx ? (int)(t.split * p.span) : 0;
+  const int stages = USE == kDx && first + p.span < all ? (int)p.span : all - first;
 
-  // This lane's sources of the copies: chunk 64 (J wave + j) + lane of a stage.
-  const bf16 *na[NJ], *ma[MJ];
-  auto source = [&](bool kc, int id, int chunks, const bf16* b0, const bf16* b1, int64_t ld, int64_t first,
-                    int64_t limit, bool pair) {
+  // This lane's sources of the copies, at k = 0: chunk 64 (J wave + j) + lane
+  // of a stage.
+  const bf16 *na[J], *ma[J];
+  auto source = [&](bool kc, int id, const bf16* b0, const bf16* b1, int64_t ld, int64_t from, int64_t extent, bool pair) {
     if (kc) {
       const int row = id >> 2, c = (id & 3) ^ chunk_swizzle<true>(row);
-      const int64_t r = first + row < limit ? first + row : limit - 1;  // (rows past the end are not stored)
-      return b0 + r * ld + kfrom + c * 8;
+      const int64_t r = from + row < extent ? from + row : extent - 1;  // (rows past the end are not stored)
+      return b0 + r * ld + c * 8;
     }
     // pair: a wave's 64 columns are 32 of gate, then the same 32 of up
-    const int k = id / chunks, c = (id % chunks) ^ chunk_swizzle<false>(k);
-    const int64_t r = first + (pair ? (c >> 3) * 32 + (c & 3) * 8 : c * 8);
-    return (pair && (c & 4) ? b1 : b0) + (kfrom + k) * ld + (r < limit ? r : limit - 8);
+    const int k = id >> 5, c = (id & 31) ^ chunk_swizzle<false>(k);
+    const int64_t r = from + (pair ? (c >> 3) * 32 + (c & 3) * 8 : c * 8);
+    return (pair && (c & 4) ? b1 : b0) + k * ld + (r < extent ? r : extent - 8);
   };
   const bf16* nbase = USE == kDw && t.mat ? p.n1 : p.n0;
 #pragma unroll
-  for (int j = 0; j < NJ; ++j) na[j] = source(NKC, (wave * NJ + j) * 64 + lane, kDN / 8, nbase, p.n1, p.nld0, n0, p.N, PAIR);
-#pragma unroll
-  for (int j = 0; j < MJ; ++j) ma[j] = source(MKC, (wave * MJ + j) * 64 + lane, kDM / 8, p.m0, p.m0, p.mld0, m0, p.M, false);
-  // to the next stage, and (dx) from the last one of the first segment to the
-  // first of the second
-  const int64_t nstep = NKC ? kDK : kDK * p.nld0, mstep = MKC ? kDK : kDK * p.mld0;
-  const int64_t nturn = USE == kDx ? p.n1 - p.n0 - (int64_t)(blocks - 1) * kDK : 0;
-  const int64_t mturn = USE == kDx ? p.m1 - p.m0 - (int64_t)(blocks - 1) * kDK : 0;
+  for (int j = 0; j < J; ++j) {
+    const int id = (wave * J + j) * 64 + lane;
+    na[j] = source(NKC, id, nbase, p.n1, p.nld, n0, p.nx, PAIR);
+    ma[j] = source(MKC, id, p.m0, p.m0, p.mld, m0, p.mx, false);
+  }
+  const int64_t nstep = NKC ? 1 : p.nld, mstep = MKC ? 1 : p.mld;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&lds[0][0];
-  auto issue = [&](int stage, int buf) {
-    const uint32_t at = lds0 + (uint32_t)(buf * (kDNChunks + kDMChunks)) * 16;
-    const bool turn = USE == kDx && stage + 1 == blocks;
+  auto issue = [&](int stage) {
+    const uint32_t at = lds0 + (uint32_t)((stage & 3) * 2 * kDChunks) * 16;
+    const int step = first + stage;
+    const bool second = USE == kDx && step >= blocks;  // du, w_up
+    const int64_t k = kfrom + (int64_t)(second ? step - blocks : step) * kDK;
+    const int64_t noff = k * nstep + (second ? p.n1 - p.n0 : 0), moff = k * mstep + (second ? p.m1 - p.m0 : 0);
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      copy_to_lds(na[j], at + (uint32_t)(wave * NJ + j) * 1024);
-      na[j] += turn ? nturn : nstep;
-    }
+    for (int j = 0; j < J; ++j) copy_to_lds(na[j] + noff, at + (uint32_t)(wave * J + j) * 1024);
 #pragma unroll
-    for (int j = 0; j < MJ; ++j) {
-      copy_to_lds(ma[j], at + kDNChunks * 16 + (uint32_t)(wave * MJ + j) * 1024);
-      ma[j] += turn ? mturn : mstep;
-    }
+    for (int j = 0; j < J; ++j) copy_to_lds(ma[j] + moff, at + kDChunks * 16 + (uint32_t)(wave * J + j) * 1024);
   };
-
   // project: the tile of dh, 128 rows to each of the two buffers that fall
   // free before the last stages (rows of 16 chunks, permuted by row % 16)
   auto copy_dh = [&]() {
 #pragma unroll
-    for (int k = 0; k < kDM * 16 / kDThreads; ++k) {
+    for (int k = 0; k < kDT * 16 / kDThreads; ++k) {
       const int id = k * kDThreads + wave * 64 + lane, row = id >> 4, c = (id & 15) ^ (row & 15);
       const int64_t m = m0 + row < p.M ? m0 + row : p.M - 1, n = n0 + c * 8 < p.N ? n0 + c * 8 : p.N - 8;
       const int buf = (stages + (row >> 7)) & 3;
       copy_to_lds(p.dh + m * p.dhld + n,
-                  lds0 + (uint32_t)(__builtin_amdgcn_readfirstlane(buf) * (kDNChunks + kDMChunks)) * 16 +
+                  lds0 + (uint32_t)(__builtin_amdgcn_readfirstlane(buf) * 2 * kDChunks) * 16 +
                       (uint32_t)((k * kDThreads + wave * 64) & 2047) * 16);
     }
   };
+  const bool dh_copied = USE == kProject && p.dh_copied;
 
   floatx16 acc[NF][MF] = {};
   bf16x8 nf[2][NF], mf[2][MF];
   auto read = [&](int st, int ks) {
-    const uint4 *nb = lds[st & 3], *mb = nb + kDNChunks;
+    const uint4 *nb = lds[st & 3], *mb = nb + kDChunks;
 #pragma unroll
-    for (int i = 0; i < NF; ++i) nf[ks][i] = fragment<NKC, kDN>(nb, wn * 64 + i * 32, ks, lane);
+    for (int i = 0; i < NF; ++i) nf[ks][i] = fragment<NKC>(nb, wn * 64 + i * 32, ks, lane);
 #pragma unroll
-    for (int j = 0; j < MF; ++j) mf[ks][j] = fragment<MKC, kDM>(mb, wm * 128 + j * 32, ks, lane);
+    for (int j = 0; j < MF; ++j) mf[ks][j] = fragment<MKC>(mb, wm * 128 + j * 32, ks, lane);
   };
   auto multiply = [&](int ks) {
 #pragma unroll
@@ -521,11 +550,14 @@ __global__ __launch_bounds__(kDThreads, 2) void k_glu_direct(GluP<bf16> p) {
       for (int j = 0; j < MF; ++j)
         acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(nf[ks][i], mf[ks][j], acc[i][j], 0, 0, 0);
   };
+  // Stage s + 1 is waited for in the middle of stage s: each wave for its own
+  // copies, then for the other waves; after that the buffer of stage s - 1 is
+  // free, which every wave has left.
   if (stages > 0) {
-    issue(0, 0);
-    if (stages > 1) issue(1, 1);
+    issue(0);
+    if (stages > 1) issue(1);
     if (stages > 2) {
-      issue(2, 2);
+      issue(2);
       asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
     } else {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -535,35 +567,38 @@ __global__ __launch_bounds__(kDThreads, 2) void k_glu_direct(GluP<bf16> p) {
     int s = 0;
     for (; s + 3 < stages; ++s) {
       read(s, 1);
-      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_sched_barrier(0);  // the reads first: they land behind the products
       multiply(0);
       __builtin_amdgcn_sched_barrier(0);
       asm volatile("s_waitcnt vmcnt(4)\n\ts_barrier" ::: "memory");
-      issue(s + 3, (s + 3) & 3);
+      issue(s + 3);
       read(s + 1, 0);
       __builtin_amdgcn_sched_barrier(0);
       multiply(1);
     }
-    if (USE == kProject && stages == 1) copy_dh();
+    if (dh_copied && stages == 1) copy_dh();
     for (; s < stages; ++s) {
       read(s, 1);
       multiply(0);
       asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-      if (USE == kProject && s + 2 == stages) copy_dh();
+      if (dh_copied && s + 2 == stages) copy_dh();
       read(s + 1 < stages ? s + 1 : s, 0);
       multiply(1);
     }
   }
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 
-  // The tile's rows in LDS: chunk c of row r (of C chunks) at r C + (c ^ r % 16).
   // Register 4 q + e of acc[i][j]: column 8 q + 4 (lane / 32) + e of fragment
   // i's 32, row lane % 32 of fragment j's.
   const int r32 = lane & 31, hi = lane >> 5;
   uint4* tile = lds[0];
-  if constexpr (USE == kDw) {
+  auto four = [&](int i, int j, int q) {
+    const floatx16& v = acc[i][j];
+    return __builtin_bit_cast(uint4, make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]));
+  };
+  if (!PAIR && (USE == kDw || p.parts)) {
     // fp32 parts, 128 rows at a time
-    float* out = p.parts + ((int64_t)t.split * 2 + t.mat) * p.M * p.N;
+    float* out = p.parts + ((int64_t)t.split * (USE == kDw ? 2 : 1) + t.mat) * p.M * p.N;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       if (half) __syncthreads();
@@ -575,87 +610,102 @@ __global__ __launch_bounds__(kDThreads, 2) void k_glu_direct(GluP<bf16> p) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
               const int r = j * 32 + r32, c = wn * 16 + i * 8 + 2 * q + hi;
-              const floatx16& v = acc[i][j];
-              tile[r * 64 + (c ^ (r & 15))] = __builtin_bit_cast(
-                  uint4, make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]));
+              tile[r * 64 + (c ^ (r & 15))] = four(i, j, q);
             }
       }
       __syncthreads();
-#pragma unroll 4
-      for (int k = 0; k < 128 * 64 / kDThreads; ++k) {
-        const int id = threadIdx.x + k * kDThreads, r = id >> 6, c = id & 63;
-        const int64_t m = m0 + half * 128 + r, n = n0 + c * 4;
-        if (m < p.M && n < p.N) *reinterpret_cast<uint4*>(out + m * p.N + n) = tile[r * 64 + (c ^ (r & 15))];
-      }
+      put_rows<float, 64, 128>(tile, out, p.N, m0 + half * 128, n0, p.M, p.N);
     }
-  } else {
-    constexpr int C = PAIR ? 16 : 32;  // chunks of a row
-    // project: dh lies where dg goes, du in the other two buffers
-    uint4* second = PAIR ? lds[(stages + 2) & 3] : nullptr;
-    uint4* third = PAIR ? lds[(stages + 3) & 3] : nullptr;
-    uint4 *first0 = USE == kProject ? lds[stages & 3] : tile, *first1 = USE == kProject ? lds[(stages + 1) & 3] : tile + 128 * C;
+    return;
+  }
+  if constexpr (USE == kProject) {
+    // dg and du in place of the projections; dh from LDS, or straight from
+    // memory.  Rows past M and columns past N give 0: what reduces over them
+    // reads whole stages.
+#pragma unroll
+    for (int j = 0; j < MF; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int r = j * 32 + r32, c = wn * 4 + q;
+        const int64_t m = m0 + wm * 128 + r, n = n0 + wn * 32 + 8 * q + 4 * hi;
+        float d[4] = {0.f, 0.f, 0.f, 0.f};
+        if (dh_copied) {
+          const Four<bf16> f = *(reinterpret_cast<const Four<bf16>*>(lds[(stages + wm) & 3] + r * 16 + (c ^ (r & 15))) + hi);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) d[e] = to_f32(f.e[e]);
+        } else if (m < p.M) {
+          load_four(p.dh + m * p.dhld + n, (int)(p.N - n < 4 ? p.N - n : 4), d);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool in = m < p.M && n + e < p.N;
+          float slope;
+          const float v = act_of(p.act, acc[0][j][4 * q + e], slope), u = acc[1][j][4 * q + e];
+          acc[0][j][4 * q + e] = in ? d[e] * u * slope : 0.f;
+          acc[1][j][4 * q + e] = in ? d[e] * v : 0.f;
+        }
+      }
+    __syncthreads();
+  }
+  // bfloat16 rows; dg and du lie side by side
+  constexpr int C = PAIR ? 16 : 32, COUNT = USE == kProject ? 2 : 1;
+#pragma unroll
+  for (int w = 0; w < COUNT; ++w)
 #pragma unroll
     for (int j = 0; j < MF; ++j)
 #pragma unroll
       for (int i = 0; i < (PAIR ? 1 : NF); ++i)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const int r = j * 32 + r32, c = (PAIR ? wn * 4 : wn * 8 + i * 4) + q;
-          const int at = r * C + (c ^ (r & 15));
-          Four<bf16>* o = reinterpret_cast<Four<bf16>*>((wm ? first1 : first0) + at) + hi;
-          Four<bf16> w;
-          if constexpr (PAIR) {
-            float slope;
-            if constexpr (USE == kForward) {
+          const int r = wm * 128 + j * 32 + r32, c = (PAIR ? wn * 4 : wn * 8 + i * 4) + q;
+          Four<bf16> o;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float v = act_of(p.act, acc[0][j][4 * q + e], slope);
-                w.e[e] = from_f32<bf16>(v * acc[NF / 2][j][4 * q + e]);
-              }
-            } else {
-              const Four<bf16> d4 = *o;
-              Four<bf16> x;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float v = act_of(p.act, acc[0][j][4 * q + e], slope), d = to_f32(d4.e[e]);
-                w.e[e] = from_f32<bf16>(d * acc[NF / 2][j][4 * q + e] * slope);
-                x.e[e] = from_f32<bf16>(d * v);
-              }
-              *(reinterpret_cast<Four<bf16>*>((wm ? third : second) + at) + hi) = x;
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w.e[e] = from_f32<bf16>(acc[i][j][4 * q + e]);
+          for (int e = 0; e < 4; ++e) {
+            float v = acc[PAIR ? w : i][j][4 * q + e], slope;
+            if constexpr (USE == kForward) v = act_of(p.act, v, slope) * acc[1][j][4 * q + e];
+            o.e[e] = from_f32<bf16>(v);
           }
-          *o = w;
+          *(reinterpret_cast<Four<bf16>*>(tile + w * kDT * C + r * C + (c ^ (r & 15))) + hi) = o;
         }
-    __syncthreads();
-    auto put = [&](const uint4* lo, const uint4* up, bf16* out, int64_t ld) {
-#pragma unroll 4
-      for (int k = 0; k < kDM * C / kDThreads; ++k) {
-        const int id = threadIdx.x + k * kDThreads, row = id / C, c = id % C, r = row & 127;
-        const int64_t m = m0 + row, n = n0 + c * 8;
-        const uint4 v = (row >> 7 ? up : lo)[r * C + (c ^ (r & 15))];
-        if (m < p.M && n < p.N) *reinterpret_cast<Vec<bf16, 8>*>(out + m * ld + n) = __builtin_bit_cast(Vec<bf16, 8>, v);
-      }
-    };
-    put(first0, first1, p.out0, p.old0);
-    if (USE == kProject) put(second, third, p.out1, p.old1);
-  }
+  __syncthreads();
+  const int64_t rows = USE == kProject ? p.om : p.M, cols = USE == kProject ? p.on : p.N;
+  put_rows<bf16, C, kDT>(tile, p.out0, p.old0, m0, n0, rows, cols);
+  if (USE == kProject) put_rows<bf16, C, kDT>(tile + kDT * C, p.out1, p.old1, m0, n0, rows, cols);
 }
 
-// dW from the row ranges' parts.
+// An operand in whole chunks: rows of `cols` elements to rows of `ld`, with
+// zeros up to `ld` columns and `prows` rows.
+__global__ __launch_bounds__(256) void k_glu_pack(const bf16* __restrict__ src, int64_t sld, int64_t rows, int64_t cols,
+                                                  bf16* __restrict__ out, int64_t ld, int64_t prows) {
+  const int64_t chunks = ld / 8, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= chunks * prows) return;
+  const int64_t r = i / chunks, c = (i - r * chunks) * 8;
+  Vec<bf16, 8> v{};
+  if (r < rows) {
+    const bf16* p = src + r * sld + c;
+    if (c + 8 <= cols) {
+      v = *reinterpret_cast<const Vec<bf16, 8>*>(p);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (c + e < cols) v.e[e] = p[e];
+    }
+  }
+  *reinterpret_cast<uint4*>(out + r * ld + c) = __builtin_bit_cast(uint4, v);
+}
+
+// dW (two matrices a part) or dx (one) from their parts, in order.
 template <class E>
-__global__ __launch_bounds__(256) void k_glu_join(const float* __restrict__ parts, uint32_t splits, int64_t M, int64_t N,
-                                                  E* out0, int64_t ld0, E* out1, int64_t ld1) {
+__global__ __launch_bounds__(256) void k_glu_join(const float* __restrict__ parts, uint32_t splits, int mats, int64_t M,
+                                                  int64_t N, E* out0, int64_t ld0, E* out1, int64_t ld1) {
   const int64_t groups = (N + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= 2 * M * groups) return;
+  if (i >= mats * M * groups) return;
   const int64_t mat = i / (M * groups), at = i - mat * M * groups, m = at / groups, n = (at - m * groups) * 4;
   float t[4] = {0.f, 0.f, 0.f, 0.f};
   const int valid = (int)(N - n < 4 ? N - n : 4);
   for (uint32_t s = 0; s < splits; ++s) {
     float v[4];
-    load_four(parts + ((int64_t)s * 2 + mat) * M * N + m * N + n, valid, v);
+    load_four(parts + ((int64_t)s * mats + mat) * M * N + m * N + n, valid, v);
 #pragma unroll
     for (int e = 0; e < 4; ++e) t[e] += v[e];
   }
@@ -745,160 +795,263 @@ __global__ __launch_bounds__(kFewThreads) void k_glu_few(GluP<E> p) {
 }
 
 // ------------------------------------------------------------------ shapes
-// Large tiles where they come near to filling the chip's 256 CUs, else small
-// ones.
-template <class E>
-bool large_tiles(int64_t M, int64_t cols) {
-  const int64_t bm = sizeof(E) == 2 ? 256 : 128;
-  return ((M + bm - 1) / bm) * ((cols + bm - 1) / bm) >= 128;
+int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+int64_t tiles(int64_t n, int64_t of) { return (n + of - 1) / of; }
+
+// bfloat16: packed operands and 256 x 256 tiles where the projections' tiles
+// come near to filling the chip's 256 CUs; else small tiles on the operands as
+// they are.  (SIDES)
+bool large(const dgen_hip_mlp& a) {
+  return a.type == DGEN_HIP_BF16 && a.rows > 2 * kFewRows && tiles(a.rows, kDT) * tiles(2 * a.hidden, kDT) >= 128;
 }
 
-bool aligned16(const void* p, int64_t ld) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0; }
+// Runs of a reduction of `steps`, as many as make the rounds of `count` tiles
+// over the CUs' `slots` full, against the time that the parts take: a step of
+// a tile takes `step`, writing and reading a tile's part `join` of the whole
+// chip, both in us.
+int64_t runs_of(int64_t count, int64_t steps, int64_t least, int64_t slots, double step, double join) {
+  int64_t best = 1;
+  double cost = 0;
+  for (int64_t r = 1; r <= std::max<int64_t>(1, std::min<int64_t>(steps / least, 64)); ++r) {
+    const double c = (double)(tiles(count * r, slots) * tiles(steps, r)) * step + (r > 1 ? (double)(r * count) * join : 0);
+    if (r == 1 || c < cost) best = r, cost = c;
+  }
+  return best;
+}
 
-template <class E, int USE>
-void product(GluP<E> p, bool large, hipStream_t st) {
-  constexpr bool PAIR = USE == kForward || USE == kProject;
-  constexpr int L = sizeof(E) == 2 ? 256 : 128;
-  const int bm = large ? L : 64, bn = large ? L : 128, per = PAIR ? bn / 2 : bn;
-  p.tiles_m = (uint32_t)((p.M + bm - 1) / bm);
-  p.tiles_n = (uint32_t)((p.N + per - 1) / per);
-  const dim3 grid(p.tiles_m * p.tiles_n * (USE == kDw ? 2 * p.splits : 1));
-  if (!large) {
-    k_glu<E, 64, 128, 32, 64, sizeof(E) == 2 ? 64 : 32, 1, USE><<<grid, kThreads, 0, st>>>(p);
-  } else if constexpr (sizeof(E) == 4) {
-    k_glu<E, 128, 128, 64, 64, 32, 1, USE><<<grid, kThreads, 0, st>>>(p);
-  } else {
-    // whole chunks and stages: every row (k-contiguous) or k (row-contiguous)
-    // starts at 16 bytes, row-contiguous operands have a multiple of 8 rows,
-    // results a multiple of 8 columns, the reduction is a multiple of 32, and
-    // the two matrices share a stride
-    const bool direct = aligned16(p.n0, p.nld0) && aligned16(p.n1, p.nld1) && aligned16(p.m0, p.mld0) &&
-                        aligned16(p.m1, p.mld1) && p.nld0 == p.nld1 && p.mld0 == p.mld1 &&
-                        p.N % 8 == 0 && (USE != kDw || p.M % 8 == 0) && p.K % kDK == 0 && p.K > 0 &&
-                        (USE != kProject || aligned16(p.dh, p.dhld)) && (USE != kDw || p.parts);
-    if (direct) {
-      p.tiles_m = (uint32_t)((p.M + kDM - 1) / kDM);
-      p.tiles_n = (uint32_t)((p.N + (PAIR ? kDN / 2 : kDN) - 1) / (PAIR ? kDN / 2 : kDN));
-      k_glu_direct<USE><<<dim3(p.tiles_m * p.tiles_n * (USE == kDw ? 2 * p.splits : 1)), kDThreads, 0, st>>>(p);
+struct Split {
+  int64_t span;  // steps or rows of a run
+  uint32_t runs;
+};
+Split split_of(int64_t n, int64_t runs, int64_t unit) {
+  const int64_t span = std::max(unit, up(tiles(n, runs), unit));
+  return {span, (uint32_t)std::max<int64_t>(1, tiles(n, span))};
+}
+
+// How a call is laid out: which operands are packed, how the reductions are
+// cut, and what lies where in the workspace (byte offsets).
+struct Plan {
+  bool large;
+  int64_t width, hidden, rows;  // padded to whole stages
+  bool pack_x, pack_w;
+  Split dx, dw;                 // stages or steps of dx's runs, rows of dW's
+  int64_t dw_rows;              // rows in the runs; the rest (of x as it is) is one more
+  int64_t x, xtail, wg, wu, dg, du, parts, total;
+};
+// k_glu's tile: 128 x 128 for fp32 products that have tiles (with the runs that
+// their reduction can be cut into) for every CU, else 64 x 128.
+template <class E>
+bool wide_tile(int64_t rows, int64_t cols, int64_t runs) {
+  return sizeof(E) == 4 && tiles(rows, 128) * tiles(cols, 128) * runs >= 256;
+}
+template <class E>
+int64_t runs_small(int64_t rows, int64_t cols, int64_t mats, int64_t steps) {
+  // (a step of a 128 x 128 fp32 tile takes about 4 us with two workgroups a
+  // CU, of a 64 x 128 tile 1 to 2 us with four; a part 0.03 and 0.02 us)
+  if (wide_tile<E>(rows, mats * cols, std::max<int64_t>(1, steps / 8)))
+    return runs_of(mats * tiles(rows, 128) * tiles(cols, 128), steps, 8, 512, 4.0, 0.03);
+  return runs_of(mats * tiles(rows, 64) * tiles(cols, 128), steps, 8, 1024, 1.5, 0.02);
+}
+template <class E>
+Plan plan_of(const dgen_hip_mlp& a, bool backward) {
+  Plan p{};
+  p.large = large(a);
+  p.rows = up(a.rows, kDK), p.width = up(a.width, kDK), p.hidden = up(a.hidden, p.large ? kDK : 8);
+  auto whole = [](const void* q, int64_t ld) { return (uintptr_t)q % 16 == 0 && ld % 8 == 0; };
+  p.pack_x = p.large && !(a.width % kDK == 0 && whole(a.x, a.x_stride));
+  p.pack_w = p.large && !(a.width % kDK == 0 && a.hidden % kDK == 0 && whole(a.w_gate, a.w_gate_stride) &&
+                          whole(a.w_up, a.w_up_stride) && a.w_gate_stride == a.w_up_stride);
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += align256(bytes);
+    return here;
+  };
+  if (p.pack_x) p.x = take(p.rows * p.width * 2);
+  if (p.pack_w) p.wg = take(p.width * p.hidden * 2), p.wu = take(p.width * p.hidden * 2);
+  if (backward) {
+    p.dg = take((p.large ? p.rows : a.rows) * p.hidden * (int64_t)sizeof(E));
+    p.du = take((p.large ? p.rows : a.rows) * p.hidden * (int64_t)sizeof(E));
+    int64_t parts = 0;
+    if (p.large) {
+      // (a 256 x 256 x 32 stage takes a CU about 0.9 us; a tile's part, 512
+      // KB to and from memory, 0.13 us)
+      const int64_t stages = 2 * p.hidden / kDK;
+      p.dx = split_of(stages, runs_of(tiles(a.rows, kDT) * tiles(a.width, kDT), stages, 16, 256, 0.9, 0.13), 1);
+      p.dw_rows = p.pack_x ? p.rows : a.rows / kDK * kDK;
+      const int64_t count = 2 * tiles(a.width, kDT) * tiles(a.hidden, kDT);
+      p.dw = split_of(p.dw_rows, runs_of(count, p.dw_rows / kDK, 16, 256, 0.9, 0.13), kDK);
+      if (p.dw_rows < a.rows) p.xtail = take(kDK * p.width * 2);
+      parts = (int64_t)(p.dw.runs + (p.dw_rows < a.rows ? 1 : 0)) * 2 * a.width * a.hidden * 4;
     } else {
-      k_glu<E, 256, 256, 128, 128, 64, 2, USE><<<grid, kThreads, 0, st>>>(p);
+      const int64_t bk = sizeof(E) == 2 ? 64 : 32, steps = 2 * tiles(a.hidden, bk);
+      p.dx = split_of(steps, runs_small<E>(a.rows, a.width, 1, steps), 1);
+      p.dw_rows = a.rows;
+      p.dw = split_of(a.rows, runs_small<E>(a.width, a.hidden, 2, tiles(a.rows, bk)), bk);
+      if (p.dw.runs > 1) parts = (int64_t)p.dw.runs * 2 * a.width * a.hidden * 4;
+    }
+    if (p.dx.runs > 1) parts = std::max(parts, (int64_t)p.dx.runs * a.rows * a.width * 4);
+    p.parts = take(parts);
+  }
+  p.total = at;
+  return p;
+}
+
+// ----------------------------------------------------------------- launches
+template <class E, int USE>
+void staged(GluP<E> p, hipStream_t st) {
+  constexpr bool PAIR = USE == kForward || USE == kProject;
+  const uint32_t more = USE == kDw ? 2 * p.splits : p.splits;
+  if constexpr (sizeof(E) == 4) {
+    if (wide_tile<E>(p.M, PAIR ? 2 * p.N : p.N, more)) {
+      p.tiles_m = (uint32_t)tiles(p.M, 128);
+      p.tiles_n = (uint32_t)tiles(p.N, PAIR ? 64 : 128);
+      k_glu<E, 128, 128, 64, 64, 32, USE><<<dim3(p.tiles_m * p.tiles_n * more), kThreads, 0, st>>>(p);
+      return;
     }
   }
+  p.tiles_m = (uint32_t)tiles(p.M, 64);
+  p.tiles_n = (uint32_t)tiles(p.N, PAIR ? 64 : 128);
+  k_glu<E, 64, 128, 32, 64, sizeof(E) == 2 ? 64 : 32, USE><<<dim3(p.tiles_m * p.tiles_n * more), kThreads, 0, st>>>(p);
 }
 
-// The weight gradients' products: tiles and row ranges.  As many ranges, of 512
-// rows or more, as make the rounds over the 256 CUs full, against the time
-// that the partial sums take: a tile's 512 rows take a CU about `unit`, and a
-// tile's part takes the whole chip about `join` to write and read.
-struct DwShape {
-  bool large;
-  int64_t rows;     // in the ranges; the rest (bf16 stages are whole) is a part of its own
-  int64_t span;     // rows of a range
-  uint32_t ranges, parts;
-  bool in_parts;    // the products leave fp32 parts (else they write the gradients)
-};
+template <int USE>
+void direct(GluD p, hipStream_t st) {
+  constexpr bool PAIR = USE == kForward || USE == kProject;
+  p.tiles_m = (uint32_t)tiles(USE == kProject ? p.om : p.M, kDT);
+  p.tiles_n = (uint32_t)tiles(USE == kProject ? p.on : p.N, PAIR ? kDT / 2 : kDT);
+  const uint32_t more = USE == kDw ? 2 * p.splits : p.splits;
+  k_glu_direct<USE><<<dim3(p.tiles_m * p.tiles_n * more), kDThreads, 0, st>>>(p);
+}
+
+void pack(const void* src, int64_t sld, int64_t rows, int64_t cols, bf16* out, int64_t ld, int64_t prows, hipStream_t st) {
+  const int64_t n = ld / 8 * prows;
+  k_glu_pack<<<dim3((unsigned)((n + 255) / 256)), 256, 0, st>>>((const bf16*)src, sld, rows, cols, out, ld, prows);
+}
+
 template <class E>
-DwShape dw_shape(const dgen_hip_mlp& a) {
-  constexpr bool kHalf = sizeof(E) == 2;
-  const int64_t L = kHalf ? 256 : 128;
-  auto count = [&](int64_t bm, int64_t bn) {
-    return 2 * ((a.width + bm - 1) / bm) * ((a.hidden + bn - 1) / bn);
-  };
-  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(a.rows / 512, 32));
-  DwShape d{};
-  d.large = count(L, L) * most >= 128;
-  d.rows = kHalf && d.large ? a.rows / kDK * kDK : a.rows;
-  const int64_t tiles = d.large ? count(L, L) : count(64, 128);
-  const double unit = !d.large ? 4e-6 : kHalf ? 14e-6 : 21e-6, join = d.large ? 0.13e-6 : 0.02e-6;
-  int64_t best = 1;
-  double least = 0;
-  for (int64_t s = 1; s <= most; ++s) {
-    const double rounds = (double)((tiles * s + 255) / 256);
-    const double cost = rounds * ((double)a.rows / (512.0 * (double)s)) * unit + (s > 1 ? (double)(s * tiles) * join : 0);
-    if (s == 1 || cost < least) best = s, least = cost;
-  }
-  d.span = std::max<int64_t>(64, ((d.rows + best - 1) / best + 63) / 64 * 64);
-  d.ranges = (uint32_t)std::max<int64_t>(1, (d.rows + d.span - 1) / d.span);
-  d.parts = d.ranges + (d.rows < a.rows ? 1 : 0);
-  d.in_parts = d.parts > 1 || (kHalf && d.large);
-  return d;
+void join(const float* parts, uint32_t runs, int mats, int64_t M, int64_t N, void* out0, int64_t ld0, void* out1,
+          int64_t ld1, hipStream_t st) {
+  const int64_t n = mats * M * ((N + 3) / 4);
+  k_glu_join<E><<<dim3((unsigned)((n + 255) / 256)), 256, 0, st>>>(parts, runs, mats, M, N, (E*)out0, ld0, (E*)out1, ld1);
 }
 
-// Rows of dg and du start at 16 bytes.
-int64_t dg_stride(const dgen_hip_mlp& a) { return (a.hidden + 7) & ~int64_t(7); }
+void launch_large(const dgen_hip_mlp& a, bool backward, const Plan& p, hipStream_t st) {
+  char* ws = (char*)a.workspace;
+  GluD q{};
+  q.act = a.act, q.splits = 1;
+  q.K = p.width;
+  if (p.pack_x) {
+    pack(a.x, a.x_stride, a.rows, a.width, (bf16*)(ws + p.x), p.width, p.rows, st);
+    q.m0 = (bf16*)(ws + p.x), q.mld = p.width;
+  } else {
+    q.m0 = (const bf16*)a.x, q.mld = a.x_stride;
+  }
+  if (p.pack_w) {
+    pack(a.w_gate, a.w_gate_stride, a.width, a.hidden, (bf16*)(ws + p.wg), p.hidden, p.width, st);
+    pack(a.w_up, a.w_up_stride, a.width, a.hidden, (bf16*)(ws + p.wu), p.hidden, p.width, st);
+    q.n0 = (bf16*)(ws + p.wg), q.n1 = (bf16*)(ws + p.wu), q.nld = p.hidden;
+  } else {
+    q.n0 = (const bf16*)a.w_gate, q.n1 = (const bf16*)a.w_up, q.nld = a.w_gate_stride;
+  }
+  q.nx = p.hidden, q.mx = a.rows;
+  q.M = a.rows, q.N = a.hidden;
+  if (!backward) {
+    q.out0 = (bf16*)a.h, q.old0 = a.h_stride;
+    direct<kForward>(q, st);
+    return;
+  }
+  bf16 *dg = (bf16*)(ws + p.dg), *du = (bf16*)(ws + p.du);
+  float* parts = (float*)(ws + p.parts);
+  GluD r = q;
+  r.out0 = dg, r.out1 = du, r.old0 = r.old1 = p.hidden;
+  r.om = p.rows, r.on = p.hidden;
+  r.dh = (const bf16*)a.dh, r.dhld = a.dh_stride;
+  r.dh_copied = (uintptr_t)a.dh % 16 == 0 && a.dh_stride % 8 == 0 && a.hidden % 8 == 0;
+  direct<kProject>(r, st);
 
-struct MlpWs {
-  int64_t dg, du, parts, total;  // bytes
-};
-MlpWs mlp_ws(const dgen_hip_mlp& a) {
-  MlpWs w{};
-  const int64_t es = a.type == DGEN_HIP_BF16 ? 2 : 4;
-  const DwShape d = a.type == DGEN_HIP_BF16 ? dw_shape<bf16>(a) : dw_shape<float>(a);
-  w.dg = w.du = align256(a.rows * dg_stride(a) * es);
-  w.parts = d.in_parts ? align256((int64_t)d.parts * 2 * a.width * a.hidden * 4) : 0;
-  w.total = w.dg + w.du + w.parts;
-  return w;
+  GluD x = q;
+  x.m0 = dg, x.m1 = du, x.mld = p.hidden;
+  x.N = a.width, x.K = p.hidden, x.nx = a.width;
+  x.out0 = (bf16*)a.dx, x.old0 = a.dx_stride;
+  x.splits = p.dx.runs, x.span = p.dx.span;
+  x.parts = p.dx.runs > 1 ? parts : nullptr;
+  direct<kDx>(x, st);
+  if (x.parts) join<bf16>(parts, p.dx.runs, 1, x.M, x.N, a.dx, a.dx_stride, nullptr, 0, st);
+
+  GluD w = q;
+  w.n0 = dg, w.n1 = du, w.nld = p.hidden, w.nx = p.hidden;
+  w.M = a.width, w.N = a.hidden, w.mx = p.width;
+  w.K = p.dw_rows, w.splits = p.dw.runs, w.span = p.dw.span, w.parts = parts;
+  if (p.dw_rows > 0) direct<kDw>(w, st);
+  uint32_t runs = p.dw_rows > 0 ? p.dw.runs : 0;
+  if (p.dw_rows < a.rows) {
+    // the last rows of x, less than a stage, with zeros up to it
+    bf16* tail = (bf16*)(ws + p.xtail);
+    pack((const bf16*)a.x + p.dw_rows * a.x_stride, a.x_stride, a.rows - p.dw_rows, a.width, tail, p.width, kDK, st);
+    w.m0 = tail, w.mld = p.width, w.n0 = dg + p.dw_rows * p.hidden, w.n1 = du + p.dw_rows * p.hidden;
+    w.K = w.span = kDK, w.splits = 1, w.parts = parts + (int64_t)runs * 2 * a.width * a.hidden;
+    direct<kDw>(w, st);
+    ++runs;
+  }
+  join<bf16>(parts, runs, 2, a.width, a.hidden, a.dw_gate, a.dw_gate_stride, a.dw_up, a.dw_up_stride, st);
+}
+
+template <class E>
+void launch_staged(const dgen_hip_mlp& a, bool backward, const Plan& p, hipStream_t st) {
+  GluP<E> q{};
+  q.act = a.act;
+  q.splits = 1, q.span = int64_t(1) << 40;
+  q.n0 = (const E*)a.w_gate, q.n1 = (const E*)a.w_up, q.nld0 = a.w_gate_stride, q.nld1 = a.w_up_stride;
+  q.m0 = q.m1 = (const E*)a.x, q.mld0 = q.mld1 = a.x_stride;
+  q.M = a.rows, q.N = a.hidden, q.K = a.width;
+  if (!backward) {
+    q.out0 = (E*)a.h, q.old0 = a.h_stride;
+    if (a.rows <= 2 * kFewRows) {
+      const dim3 grid((unsigned)tiles(a.hidden, kFewCols), (unsigned)tiles(a.rows, kFewRows));
+      k_glu_few<E><<<grid, kFewThreads, 0, st>>>(q);
+    } else {
+      staged<E, kForward>(q, st);
+    }
+    return;
+  }
+  E *dg = (E*)((char*)a.workspace + p.dg), *du = (E*)((char*)a.workspace + p.du);
+  float* parts = (float*)((char*)a.workspace + p.parts);
+  if (a.rows > 0) {
+    GluP<E> r = q;
+    r.out0 = dg, r.out1 = du, r.old0 = r.old1 = p.hidden;
+    r.dh = (const E*)a.dh, r.dhld = a.dh_stride;
+    staged<E, kProject>(r, st);
+    GluP<E> x = q;
+    x.m0 = dg, x.m1 = du, x.mld0 = x.mld1 = p.hidden;
+    x.N = a.width, x.K = a.hidden;
+    x.out0 = (E*)a.dx, x.old0 = a.dx_stride;
+    x.splits = p.dx.runs, x.span = p.dx.span;
+    x.parts = p.dx.runs > 1 ? parts : nullptr;
+    staged<E, kDx>(x, st);
+    if (x.parts) join<E>(parts, p.dx.runs, 1, x.M, x.N, a.dx, a.dx_stride, nullptr, 0, st);
+  }
+  GluP<E> w = q;
+  w.n0 = dg, w.n1 = du, w.nld0 = w.nld1 = p.hidden;
+  w.M = a.width, w.N = a.hidden, w.K = a.rows;
+  w.out0 = (E*)a.dw_gate, w.old0 = a.dw_gate_stride, w.out1 = (E*)a.dw_up, w.old1 = a.dw_up_stride;
+  w.splits = p.dw.runs, w.span = p.dw.span;
+  w.parts = p.dw.runs > 1 ? parts : nullptr;
+  staged<E, kDw>(w, st);
+  if (w.parts) join<E>(parts, p.dw.runs, 2, a.width, a.hidden, a.dw_gate, a.dw_gate_stride, a.dw_up, a.dw_up_stride, st);
 }
 
 template <class E>
 void mlp_launch(const dgen_hip_mlp& a, bool backward, hipStream_t st) {
-  GluP<E> p{};
-  p.act = a.act;
-  p.splits = 1;
-  p.n0 = (const E*)a.w_gate, p.n1 = (const E*)a.w_up, p.nld0 = a.w_gate_stride, p.nld1 = a.w_up_stride;
-  p.m0 = p.m1 = (const E*)a.x, p.mld0 = p.mld1 = a.x_stride;
-  p.M = a.rows, p.N = a.hidden, p.K = a.width;
-  if (!backward) {
-    p.out0 = (E*)a.h, p.old0 = a.h_stride;
-    if (a.rows <= 2 * kFewRows) {
-      k_glu_few<E><<<dim3((unsigned)((a.hidden + kFewCols - 1) / kFewCols), (unsigned)((a.rows + kFewRows - 1) / kFewRows)),
-                     kFewThreads, 0, st>>>(p);
-    } else {
-      product<E, kForward>(p, large_tiles<E>(a.rows, 2 * a.hidden), st);
-    }
-    return;
-  }
-  const MlpWs w = mlp_ws(a);
-  E* dg = (E*)a.workspace;
-  E* du = (E*)((char*)a.workspace + w.dg);
-  float* parts = (float*)((char*)a.workspace + w.dg + w.du);
-  if (a.rows > 0) {
-    GluP<E> q = p;
-    q.out0 = dg, q.out1 = du, q.old0 = q.old1 = dg_stride(a);
-    q.dh = (const E*)a.dh, q.dhld = a.dh_stride;
-    product<E, kProject>(q, large_tiles<E>(a.rows, 2 * a.hidden), st);
-    q = p;
-    q.m0 = dg, q.m1 = du, q.mld0 = q.mld1 = dg_stride(a);
-    q.N = a.width, q.K = a.hidden;
-    q.out0 = (E*)a.dx, q.old0 = a.dx_stride;
-    product<E, kDx>(q, large_tiles<E>(a.rows, a.width), st);
-  }
-  GluP<E> q = p;
-  const DwShape d = dw_shape<E>(a);
-  q.n0 = dg, q.n1 = du, q.nld0 = q.nld1 = dg_stride(a);
-  q.M = a.width, q.N = a.hidden, q.K = d.rows;
-  q.out0 = (E*)a.dw_gate, q.old0 = a.dw_gate_stride, q.out1 = (E*)a.dw_up, q.old1 = a.dw_up_stride;
-  q.parts = d.in_parts ? parts : nullptr;
-  q.splits = d.ranges, q.span = d.span;
-  product<E, kDw>(q, d.large, st);
-  if (d.rows < a.rows) {
-    GluP<E> r = q;
-    r.n0 += d.rows * r.nld0, r.n1 += d.rows * r.nld1, r.m0 += d.rows * r.mld0, r.m1 = r.m0;
-    r.K = r.span = a.rows - d.rows;
-    r.splits = 1;
-    r.parts += (int64_t)d.ranges * 2 * a.width * a.hidden;
-    product<E, kDw>(r, d.large, st);
-  }
-  if (d.in_parts) {
-    const int64_t n = 2 * a.width * ((a.hidden + 3) / 4);
-    k_glu_join<E><<<dim3((unsigned)((n + 255) / 256)), 256, 0, st>>>(parts, d.parts, a.width, a.hidden, q.out0, q.old0,
-                                                                     q.out1, q.old1);
-  }
+  const Plan p = plan_of<E>(a, backward);
+  p.large ? launch_large(a, backward, p, st) : launch_staged<E>(a, backward, p, st);
 }
 
 }  // namespace
 
-int64_t mlp_workspace(const dgen_hip_mlp& a, bool backward) { return backward ? mlp_ws(a).total : 0; }
+int64_t mlp_workspace(const dgen_hip_mlp& a, bool backward) {
+  return a.type == DGEN_HIP_BF16 ? plan_of<bf16>(a, backward).total : plan_of<float>(a, backward).total;
+}
 
 int mlp_run(const dgen_hip_mlp& a, bool backward, hipStream_t st, bool dry) {
   const char* what = backward ? "gated_mlp_backward" : "gated_mlp";
@@ -922,11 +1075,11 @@ int mlp_run(const dgen_hip_mlp& a, bool backward, hipStream_t st, bool dry) {
                  what);
     DGEN_REQUIRE(a.dw_gate && a.dw_up && (a.width <= 1 || (a.dw_gate_stride >= a.hidden && a.dw_up_stride >= a.hidden)),
                  "%s: dw_gate or dw_up missing or overlapping itself", what);
-    const int64_t need = mlp_workspace(a, true);
-    DGEN_REQUIRE(need == 0 || (a.workspace && a.workspace_bytes >= (uint64_t)need && (uintptr_t)a.workspace % 256 == 0),
-                 "%s: workspace of %llu bytes, %lld needed (256-byte aligned)", what,
-                 (unsigned long long)a.workspace_bytes, (long long)need);
   }
+  const int64_t need = mlp_workspace(a, backward);
+  DGEN_REQUIRE(need == 0 || (a.workspace && a.workspace_bytes >= (uint64_t)need && (uintptr_t)a.workspace % 256 == 0),
+               "%s: workspace of %llu bytes, %lld needed (256-byte aligned)", what, (unsigned long long)a.workspace_bytes,
+               (long long)need);
   if (dry || (empty && !backward)) return 0;
   if (a.type == DGEN_HIP_BF16) mlp_launch<bf16>(a, backward, st);
   else mlp_launch<float>(a, backward, st);

@@ -389,7 +389,8 @@ def gated_mlp(x, w_gate, w_up, activation: str = "silu", out=None):
     if out is None:
         out = torch.empty(shape, dtype=x.dtype, device=x.device)
     d.h, d.h_stride = _rows(out, "out", shape, x.dtype, x.device)
-    _op("gated_mlp")(d, x.device, False, False)  # (no scratch in this direction)
+    # (few rows take no scratch)
+    _op("gated_mlp")(d, x.device, False, d.rows > 16)
     return out
 
 

@@ -81,7 +81,7 @@ def test_forward(gpu, rows, width, hidden, ty, act):
     check_forward(rows, width, hidden, ty, act)
 
 
-@pytest.mark.parametrize("rows,width,hidden", [(2500, 72, 1700), (4100, 64, 1024)])
+@pytest.mark.parametrize("rows,width,hidden", [(2500, 72, 1700), (4100, 64, 1024), (300, 40, 8200), (9, 40, 16500)])
 @pytest.mark.parametrize("ty", TYPES)
 def test_forward_large(gpu, rows, width, hidden, ty):
     check_forward(rows, width, hidden, ty, "silu")
@@ -122,7 +122,8 @@ def test_backward(gpu, rows, width, hidden, ty, act):
     check_backward(rows, width, hidden, ty, act)
 
 
-@pytest.mark.parametrize("rows,width,hidden", [(2500, 520, 900), (3001, 1100, 300), (2085, 512, 992)])
+@pytest.mark.parametrize("rows,width,hidden", [(2500, 520, 900), (3001, 1100, 300), (2085, 512, 992), (2100, 33, 1801),
+                                               (8300, 70, 450), (300, 40, 8200)])
 @pytest.mark.parametrize("ty", TYPES)
 def test_backward_large(gpu, rows, width, hidden, ty):
     """Large tiles and row ranges; repeated calls give the same bits."""
