@@ -243,6 +243,7 @@ __global__ __launch_bounds__(kThreads) void k_scan(ScanP<E> p) {
   if (w.begin < w.live) fetch(w.begin);
   E* const yrow = p.y.p + w.b * p.y.b;
   const uint32_t yat = (uint32_t)w.q * (uint32_t)p.y.t + (uint32_t)w.d;
+  const bool whole = ((int)(blockIdx.x % (uint32_t)p.nd) + 1) * kChannels <= p.D;
   int buf = 0;
   for (int t0 = w.begin; t0 < w.live; t0 += kTile, buf ^= 1) {
     float* lds = bc[buf];
@@ -253,11 +254,9 @@ __global__ __launch_bounds__(kThreads) void k_scan(ScanP<E> p) {
     __syncthreads();
     if (t0 + kTile < w.live) fetch(t0 + kTile);
     const int groups = w.live - t0 < kTile ? (w.live - t0 + 3) / 4 : G;
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-      if (g >= groups) continue;
+    auto group = [&](int g, auto wholec) {
       const int t = t0 + 4 * g + w.q;
-      const bool ok = w.on && t < w.live;
+      const bool ok = decltype(wholec)::value || (w.on && t < w.live);
       float slope;
       const float soft = softplus_accurate(cdt[g] + bias, slope);
       const float step = ok ? soft : 0.f, u = ok ? soft * cx[g] : 0.f;
@@ -291,6 +290,16 @@ __global__ __launch_bounds__(kThreads) void k_scan(ScanP<E> p) {
       frame(std::integral_constant<int, 3>{});
       const float y = OUT ? quad_sums(y4, odd, upper) : 0.f;
       if (OUT && ok) (yrow + (int64_t)(t0 + 4 * g) * p.y.t)[yat] = from_f32<E>(fmaf(skip, cx[g], y) * gate);
+    };
+    // a whole tile of whole channels in one piece, without a branch (but with
+    // the adjoint's sums one piece takes too many registers)
+    if (!ADJ && whole && w.live - t0 >= kTile) {
+#pragma unroll
+      for (int g = 0; g < G; ++g) group(g, std::true_type{});
+    } else {
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+        if (g < groups) group(g, std::false_type{});
     }
   }
   if (!w.on) return;
@@ -411,7 +420,7 @@ __device__ __forceinline__ void channel_sum(const float (&v)[V], float (&w)[kept
 }
 
 template <class E, int S>
-__global__ __launch_bounds__(kThreads, 2) void k_scan_bwd(ScanP<E> p) {
+__global__ __launch_bounds__(kThreads, S <= 4 ? 2 : 1) void k_scan_bwd(ScanP<E> p) {
   constexpr int NP = 4 * S, TL = bwd_tile<S>(), G = TL / 4;
   __shared__ __align__(16) float bc[2][TL * 2 * NP];
   __shared__ float red[TL][kWaves][2 * NP];

@@ -89,3 +89,34 @@ def test_fit_lowers_the_loss(gpu):
     target = (x.cumsum(1) / torch.arange(1, 61)[None, :, None])[..., :1].repeat(1, 1, 9).cuda()
     losses = fit(dec, x, target, steps=60, lr=3e-3, lengths=torch.tensor([60, 50, 7, 60], dtype=torch.int32, device="cuda"))
     assert losses[-1] < 0.2 * losses[0], (losses[0], losses[-1])
+
+
+def test_a_step_in_a_graph(gpu):
+    """A captured step (torch.cuda.graph) replays with new frames and carries
+    its state, as eager steps do, with other work between the replays."""
+    dec = small(torch.bfloat16)
+    x = torch.randn(3, 12, 2, generator=torch.Generator().manual_seed(6)).cuda()
+    state = dec.state(3)
+    eager = [dec.step(x[:, t], state) for t in range(12)]
+    held, frame = dec.state(3), x[:, 0].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            dec.step(frame, held)  # libraries set up outside the capture
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = dec.step(frame, held)
+    for c, s in held:
+        c.zero_()
+        s.zero_()
+    for t in range(12):
+        frame.copy_(x[:, t])
+        graph.replay()
+        assert torch.equal(out, eager[t]), t
+        if t % 3 == 0:
+            torch.cuda.synchronize()
+            dec.forward(x)  # eager work between replays
+    for (c, s), (ce, se) in zip(held, state):
+        assert torch.equal(c, ce) and torch.equal(s, se)
