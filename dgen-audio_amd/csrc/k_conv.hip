@@ -231,49 +231,54 @@ __global__ __launch_bounds__(kBwdGroups* kBwdTiles) void k_conv_bwd(
       for (int e = 0; e < 4; ++e) du[q][e] = 0.f;
     }
     for (int64_t t = t0; t < t1 + W - 1; t += kGroup) {
+      Four<T> cx[kGroup], cg[kGroup];
 #pragma unroll
-      for (int k = 0; k < kGroup; ++k)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool in = t + k < n;
-          win[W - 1 + k][e] = in ? to_f32(nextx[k].e[e]) : 0.f;
-          du[W - 1 + k][e] = in ? to_f32(nextg[k].e[e]) : 0.f;
-        }
+      for (int k = 0; k < kGroup; ++k) cx[k] = nextx[k], cg[k] = nextg[k];
       if (t + kGroup < t1 + W - 1) fetch(t + kGroup);
+      // INSIDE: every frame of the group lies in the tile and the sequence, and
+      // the ones that get their gradient now do too
+      auto group = [&](auto insidec) {
+        constexpr bool INSIDE = decltype(insidec)::value;
 #pragma unroll
-      for (int k = 0; k < kGroup; ++k) {
-        const bool own = t + k < t1;  // (frames past the tile only for the gradients before them)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float d = du[W - 1 + k][e];
-          if (SILU) {
-            float u = taps.bias[e];
-#pragma unroll
-            for (int q = 0; q < W; ++q) u = fmaf(taps.w[q][e], win[k + q][e], u);
-            const float sl = silu_grad(u, sigmoid(u));
-            d = t + k < n ? d * sl : 0.f;
-            du[W - 1 + k][e] = d;
-          }
-          const float mine = own ? d : 0.f;
-          dbs[e] += mine;
-#pragma unroll
-          for (int q = 0; q < W; ++q) dw[q][e] = fmaf(mine, win[k + q][e], dw[q][e]);
-        }
-        // the frame that has all of its du now
-        const int64_t to = t + k - (W - 1);
-        if (to >= t0 && to < t1) {
-          float o[4];
+        for (int k = 0; k < kGroup; ++k) {
+          const bool in = INSIDE || t + k < n;
+          const bool own = INSIDE || t + k < t1;  // (frames past the tile only for the gradients before them)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            o[e] = 0.f;
-            // dx[to] = sum_q w[q] du[to + W-1-q]
+            const float x = to_f32(cx[k].e[e]);
+            float d = to_f32(cg[k].e[e]);
+            win[W - 1 + k][e] = in ? x : 0.f;
+            if (SILU) {
+              float u = taps.bias[e];
 #pragma unroll
-            for (int q = 0; q < W; ++q) o[e] = fmaf(taps.w[q][e], du[W - 1 + k - q][e], o[e]);
-            if (to >= n) o[e] = 0.f;
+              for (int q = 0; q < W; ++q) u = fmaf(taps.w[q][e], win[k + q][e], u);
+              d *= silu_grad(u, sigmoid(u));
+            }
+            if (!in) d = 0.f;
+            du[W - 1 + k][e] = d;
+            const float mine = own ? d : 0.f;
+            dbs[e] += mine;
+#pragma unroll
+            for (int q = 0; q < W; ++q) dw[q][e] = fmaf(mine, win[k + q][e], dw[q][e]);
           }
-          put_four(op + to * dt, ch, o);
+          // the frame that has all of its du now
+          const int64_t to = t + k - (W - 1);
+          if (INSIDE || (to >= t0 && to < t1)) {
+            float o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              o[e] = 0.f;
+              // dx[to] = sum_q w[q] du[to + W-1-q]
+#pragma unroll
+              for (int q = 0; q < W; ++q) o[e] = fmaf(taps.w[q][e], du[W - 1 + k - q][e], o[e]);
+              if (!INSIDE && to >= n) o[e] = 0.f;
+            }
+            put_four(op + to * dt, ch, o);
+          }
         }
-      }
+      };
+      if (t - (W - 1) >= t0 && t + kGroup <= t1 && t + kGroup <= n) group(std::true_type{});
+      else group(std::false_type{});
 #pragma unroll
       for (int q = 0; q < W - 1; ++q)
 #pragma unroll

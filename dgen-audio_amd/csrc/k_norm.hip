@@ -183,12 +183,14 @@ void row_shape(int64_t n, int& tpr, int& it) {
 }
 
 // Workgroups of the backward pass: each walks rows and leaves one partial
-// row, so no more than fill the chip (four workgroups of four waves a CU).
+// row.  Two or more steps each, up to four workgroups a CU (32000 x 512: 48 us
+// with 1024 workgroups, 64 with 512; 4001 x 1023, 1001 steps: 19.8 us with 512,
+// 21.0 with 1001, whose partial rows take longer to add).
 int64_t norm_blocks(const dgen_hip_norm& a) {
   int tpr, it;
   row_shape(a.width, tpr, it);
-  const int64_t rpb = tpr > 256 ? 1 : 256 / tpr, groups = (a.rows + rpb - 1) / rpb;
-  return std::min<int64_t>(groups, tpr > 256 ? 512 : 1024);
+  const int64_t rpb = tpr > 256 ? 1 : 256 / tpr, steps = (a.rows + rpb - 1) / rpb;
+  return std::min<int64_t>((steps + 1) / 2, 1024);
 }
 
 template <class TX, class TS, int TPR, int IT>

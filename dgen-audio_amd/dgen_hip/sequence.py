@@ -28,6 +28,7 @@ No counterpart in the reference, whose decoder sees one frame at a time
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import NamedTuple, Optional
 
 import torch
@@ -36,47 +37,25 @@ from .runtime import HIPError, load_library
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
 _ACTS = {"silu": 0, "gelu": 1}
-_VP, _I32, _I64, _U32, _U64, _F = (ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_uint32, ctypes.c_uint64,
-                                   ctypes.c_float)
 
 
-class CSeq(ctypes.Structure):
-    _fields_ = [("data", _VP), ("stride_b", _I64), ("stride_t", _I64)]
+def _descriptor(fields: str) -> struct.Struct:
+    """A descriptor of dgen_hip.h in native layout but for its last two
+    fields, the workspace's address and size.  p: address, v: address and
+    stride of rows, s: address and two strides of a sequence tensor."""
+    return struct.Struct("@" + fields.replace("p", "Q").replace("v", "Qq").replace("s", "Qqq"))
 
 
-class CNorm(ctypes.Structure):
-    _fields_ = [("struct_size", _U32), ("x_type", _I32), ("s_type", _I32), ("eps", _F), ("rows", _I64), ("width", _I64),
-                ("weight", _VP), ("x", _VP), ("x_stride", _I64), ("residual", _VP), ("residual_stride", _I64),
-                ("y", _VP), ("y_stride", _I64), ("s", _VP), ("s_stride", _I64), ("dy", _VP), ("dy_stride", _I64),
-                ("ds", _VP), ("ds_stride", _I64), ("dx", _VP), ("dx_stride", _I64), ("dweight", _VP),
-                ("workspace", _VP), ("workspace_bytes", _U64)]
-
-
-class CConv(ctypes.Structure):
-    _fields_ = [("struct_size", _U32), ("type", _I32), ("silu", _I32), ("width", _I32), ("batch", _I64), ("T", _I64),
-                ("D", _I64), ("weight", _VP), ("bias", _VP), ("lengths", _VP), ("x", CSeq), ("y", CSeq),
-                ("state", _VP), ("state_out", _VP), ("dy", CSeq), ("dx", CSeq), ("dweight", _VP), ("dbias", _VP),
-                ("workspace", _VP), ("workspace_bytes", _U64)]
-
-
-class CScan(ctypes.Structure):
-    _fields_ = [("struct_size", _U32), ("type", _I32), ("batch", _I64), ("T", _I64), ("D", _I64), ("N", _I64),
-                ("A", _VP), ("skip", _VP), ("dt_bias", _VP), ("lengths", _VP), ("state", _VP), ("state_out", _VP),
-                ("x", CSeq), ("dt", CSeq), ("z", CSeq), ("B", CSeq), ("C", CSeq), ("y", CSeq), ("dy", CSeq),
-                ("dx", CSeq), ("ddt", CSeq), ("dz", CSeq), ("dB", CSeq), ("dC", CSeq), ("dA", _VP), ("dskip", _VP),
-                ("ddt_bias", _VP), ("workspace", _VP), ("workspace_bytes", _U64)]
-
-
-class CMlp(ctypes.Structure):
-    _fields_ = [("struct_size", _U32), ("type", _I32), ("act", _I32), ("reserved", _I32), ("rows", _I64),
-                ("width", _I64), ("hidden", _I64), ("x", _VP), ("x_stride", _I64), ("w_gate", _VP),
-                ("w_gate_stride", _I64), ("w_up", _VP), ("w_up_stride", _I64), ("h", _VP), ("h_stride", _I64),
-                ("dh", _VP), ("dh_stride", _I64), ("dx", _VP), ("dx_stride", _I64), ("dw_gate", _VP),
-                ("dw_gate_stride", _I64), ("dw_up", _VP), ("dw_up_stride", _I64), ("workspace", _VP),
-                ("workspace_bytes", _U64)]
-
-
-_NONE = (None, 0, 0)
+# (packed as bytes: a ctypes structure took 3 us more a call)
+_NORM = _descriptor("Iiif qq p v v v v v v v p")           # struct dgen_hip_norm
+_CONV = _descriptor("Iiii qqq ppp s s pp s s pp")          # struct dgen_hip_conv
+_SCAN = _descriptor("Ii qqqq pppppp ssssssssssss ppp")     # struct dgen_hip_scan
+_MLP = _descriptor("Iiii qqq vvvvvvvv")                    # struct dgen_hip_mlp
+_WORKSPACE = struct.Struct("@QQ")
+_NO_WORKSPACE = _WORKSPACE.pack(0, 0)
+# the descriptors' struct_size
+_NORM_SIZE, _CONV_SIZE, _SCAN_SIZE, _MLP_SIZE = (d.size + 16 for d in (_NORM, _CONV, _SCAN, _MLP))
+_NONE, _NO_ROWS = (0, 0, 0), (0, 0)
 
 
 def _current_stream(index: int) -> int:
@@ -96,16 +75,17 @@ class _Op:
         self.workspace = getattr(L, f"dgen_hip_{name}_workspace")
         self.error = L.dgen_hip_last_error
 
-    def __call__(self, desc, device: torch.device, backward: bool, scratch: bool) -> None:
-        ref, index = ctypes.byref(desc), device.index
+    def __call__(self, desc: bytes, device: torch.device, backward: bool, scratch: bool) -> None:
+        index, tail = device.index, _NO_WORKSPACE
         if scratch:
-            need = _U64(0)
-            self._check(self.workspace(index, ref, int(backward), ctypes.byref(need)))
+            need = ctypes.c_uint64(0)
+            self._check(self.workspace(index, desc + tail, int(backward), ctypes.byref(need)))
             if need.value:
                 ws = torch.empty(need.value, dtype=torch.uint8, device=device)
-                desc.workspace, desc.workspace_bytes = ws.data_ptr(), need.value
-        fn = self.backward if backward else self.forward
-        self._check(fn(index, ref, _raw_stream(index)))
+                tail = _WORKSPACE.pack(ws.data_ptr(), need.value)
+        rc = (self.backward if backward else self.forward)(index, desc + tail, _raw_stream(index))
+        if rc:
+            self._check(rc)
 
     def _check(self, rc: int) -> None:
         if rc:
@@ -153,9 +133,9 @@ def _seq(t, name: str, shape, dtype, device):
 
 
 def _dense(t, name: str, shape, dtype, device):
-    """Address of a contiguous tensor (None stays None)."""
+    """Address of a contiguous tensor (0 for None)."""
     if t is None:
-        return None
+        return 0
     if not _is(t, shape, dtype, device):
         raise _wrong(name, t, f"{tuple(shape)} {dtype} on {device}")
     if not t.is_contiguous():
@@ -203,7 +183,7 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-5, out=None, sum_out=None
     if out is None:
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
     yp = _rows(out, "out", shape, x.dtype, dev)
-    rp = sp = (None, 0)
+    rp = sp = _NO_ROWS
     st = ty
     if residual is not None:
         st = _type(residual, "residual")
@@ -213,7 +193,7 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-5, out=None, sum_out=None
         sp = _rows(sum_out, "sum_out", shape, residual.dtype, dev)
     elif sum_out is not None:
         raise ValueError("sum_out: only with a residual")
-    d = CNorm(ctypes.sizeof(CNorm), ty, st, float(eps), _count(shape), shape[-1], w, *xp, *rp, *yp, *sp)
+    d = _NORM.pack(_NORM_SIZE, ty, st, eps, _count(shape), shape[-1], w, *xp, *rp, *yp, *sp, 0, 0, 0, 0, 0, 0, 0)
     _op("rms_norm")(d, dev, False, False)
     return out if residual is None else (out, sum_out)
 
@@ -229,15 +209,11 @@ def rms_norm_backward(dy, s, weight, ds=None, eps: float = 1e-5, out=None):
     if out is None:
         out = torch.empty_like(s, memory_format=torch.contiguous_format)
     dw = torch.empty(shape[-1], dtype=torch.float32, device=dev)
-    d = CNorm(struct_size=ctypes.sizeof(CNorm), x_type=ty, s_type=st, eps=float(eps), rows=_count(shape),
-              width=shape[-1], weight=_dense(weight, "weight", shape[-1:], torch.float32, dev), dweight=dw.data_ptr())
-    if d.weight is None:
-        raise ValueError("weight: missing")
-    d.dy, d.dy_stride = _rows(dy, "dy", shape, dy.dtype, dev)
-    d.s, d.s_stride = _rows(s, "s", shape, s.dtype, dev)
-    d.dx, d.dx_stride = _rows(out, "out", shape, s.dtype, dev)
-    if ds is not None:
-        d.ds, d.ds_stride = _rows(ds, "ds", shape, s.dtype, dev)
+    d = _NORM.pack(_NORM_SIZE, ty, st, eps, _count(shape), shape[-1],
+                   _dense(weight, "weight", shape[-1:], torch.float32, dev), 0, 0, 0, 0, 0, 0,
+                   *_rows(s, "s", shape, s.dtype, dev), *_rows(dy, "dy", shape, dy.dtype, dev),
+                   *(_NO_ROWS if ds is None else _rows(ds, "ds", shape, s.dtype, dev)),
+                   *_rows(out, "out", shape, s.dtype, dev), dw.data_ptr())
     _op("rms_norm")(d, dev, True, True)
     return out, dw
 
@@ -266,9 +242,8 @@ def causal_conv(x, weight, bias=None, silu: bool = True, state=None, state_out=N
     W, dev, (ty, (B, T, D), w, b, n, xs, st) = _conv_parts(x, weight, bias, state, lengths)
     if out is None:
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
-    d = CConv(ctypes.sizeof(CConv), ty, 1 if silu else 0, W, B, T, D, w, b, n, xs,
-              _seq(out, "out", x.shape, x.dtype, dev), st,
-              _dense(state_out, "state_out", (B, W - 1, D), x.dtype, dev))
+    d = _CONV.pack(_CONV_SIZE, ty, 1 if silu else 0, W, B, T, D, w, b, n, *xs, *_seq(out, "out", x.shape, x.dtype, dev),
+                   st, _dense(state_out, "state_out", (B, W - 1, D), x.dtype, dev), 0, 0, 0, 0, 0, 0, 0, 0)
     _op("causal_conv")(d, dev, False, False)
     return out
 
@@ -281,9 +256,9 @@ def causal_conv_backward(dy, x, weight, bias=None, silu: bool = True, state=None
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
     dw = torch.empty((D, W), dtype=torch.float32, device=dev)
     db = None if bias is None else torch.empty(D, dtype=torch.float32, device=dev)
-    d = CConv(ctypes.sizeof(CConv), ty, 1 if silu else 0, W, B, T, D, w, b, n, xs, _NONE, st, None,
-              _seq(dy, "dy", x.shape, x.dtype, dev), _seq(out, "out", x.shape, x.dtype, dev), dw.data_ptr(),
-              None if db is None else db.data_ptr())
+    d = _CONV.pack(_CONV_SIZE, ty, 1 if silu else 0, W, B, T, D, w, b, n, *xs, 0, 0, 0, st, 0,
+                   *_seq(dy, "dy", x.shape, x.dtype, dev), *_seq(out, "out", x.shape, x.dtype, dev), dw.data_ptr(),
+                   0 if db is None else db.data_ptr())
     _op("causal_conv")(d, dev, True, True)
     return out, dw, db
 
@@ -301,7 +276,8 @@ class ScanGrads(NamedTuple):
     ddt_bias: Optional[torch.Tensor]
 
 
-def _scan_desc(x, dt, A, B, C, D, z, dt_bias, state, lengths):
+def _scan_parts(x, dt, A, B, C, D, z, dt_bias, state, lengths):
+    """(device, sizes, the descriptor's first fields, those of the inputs)."""
     ty = _type(x, "x")
     if x.dim() != 3:
         raise _wrong("x", x, "[batch][time][channel]")
@@ -310,13 +286,16 @@ def _scan_desc(x, dt, A, B, C, D, z, dt_bias, state, lengths):
     shape, dev, f32, et = x.shape, x.device, torch.float32, x.dtype
     n, T, ch = shape
     N = A.shape[1]
-    bc = torch.Size((n, T, N))
-    return CScan(ctypes.sizeof(CScan), ty, n, T, ch, N, _dense(A, "A", (ch, N), f32, dev),
-                 _dense(D, "D", (ch,), f32, dev), _dense(dt_bias, "dt_bias", (ch,), f32, dev),
-                 _dense(lengths, "lengths", (n,), torch.int32, dev), _dense(state, "state", (n, ch, N), f32, dev), None,
-                 _seq(x, "x", shape, et, dev), _seq(dt, "dt", shape, et, dev),
-                 _NONE if z is None else _seq(z, "z", shape, et, dev), _seq(B, "B", bc, et, dev),
-                 _seq(C, "C", bc, et, dev))
+    bc = (n, T, N)
+    head = (_SCAN_SIZE, ty, n, T, ch, N, _dense(A, "A", (ch, N), f32, dev), _dense(D, "D", (ch,), f32, dev),
+            _dense(dt_bias, "dt_bias", (ch,), f32, dev), _dense(lengths, "lengths", (n,), torch.int32, dev),
+            _dense(state, "state", (n, ch, N), f32, dev))
+    return dev, (n, T, ch, N), head, (*_seq(x, "x", shape, et, dev), *_seq(dt, "dt", shape, et, dev),
+                                      *(_NONE if z is None else _seq(z, "z", shape, et, dev)),
+                                      *_seq(B, "B", bc, et, dev), *_seq(C, "C", bc, et, dev))
+
+
+_NO_SCAN_GRADS = (0,) * 21
 
 
 def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, state=None, state_out=None, lengths=None, out=None):
@@ -327,43 +306,39 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, state=None, sta
     ([batch][channels][N]) are float32; D, z and dt_bias may be left out.
     Results of a sequence can differ in rounding with the number of sequences
     and channels in the call, which decide how time is cut."""
-    d = _scan_desc(x, dt, A, B, C, D, z, dt_bias, state, lengths)
-    dev = x.device
+    dev, (n, T, ch, N), head, ins = _scan_parts(x, dt, A, B, C, D, z, dt_bias, state, lengths)
     if out is None:
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
-    d.y = _seq(out, "out", x.shape, x.dtype, dev)
-    d.state_out = _dense(state_out, "state_out", (d.batch, d.D, d.N), torch.float32, dev)
+    d = _SCAN.pack(*head, _dense(state_out, "state_out", (n, ch, N), torch.float32, dev), *ins,
+                   *_seq(out, "out", x.shape, x.dtype, dev), *_NO_SCAN_GRADS)
     # (a call of few frames is one launch without scratch)
-    _op("selective_scan")(d, dev, False, d.T > 32)
+    _op("selective_scan")(d, dev, False, T > 32)
     return out
 
 
 def selective_scan_backward(dy, x, dt, A, B, C, D=None, z=None, dt_bias=None, state=None, lengths=None) -> ScanGrads:
     """Gradients of ``selective_scan``; the state counts as given."""
-    d = _scan_desc(x, dt, A, B, C, D, z, dt_bias, state, lengths)
-    dev, et, f32 = x.device, x.dtype, torch.float32
-    d.dy = _seq(dy, "dy", x.shape, et, dev)
+    dev, (n, T, ch, N), head, ins = _scan_parts(x, dt, A, B, C, D, z, dt_bias, state, lengths)
+    et, f32 = x.dtype, torch.float32
 
-    def like(shape, dtype, given=True):
+    def new(shape, dtype, given=True):
         return torch.empty(shape, dtype=dtype, device=dev) if given else None
 
-    bc = (d.batch, d.T, d.N)
-    g = ScanGrads(like(x.shape, et), like(x.shape, et), like((d.D, d.N), f32), like(bc, et), like(bc, et),
-                  like((d.D,), f32, D is not None), like(x.shape, et, z is not None),
-                  like((d.D,), f32, dt_bias is not None))
-    for name in ("dx", "ddt", "dB", "dC", "dz"):
-        t = getattr(g, name)
-        if t is not None:
-            setattr(d, name, (t.data_ptr(), t.stride(0), t.stride(1)))
-    d.dA = g.dA.data_ptr()
-    d.dskip = None if g.dD is None else g.dD.data_ptr()
-    d.ddt_bias = None if g.ddt_bias is None else g.ddt_bias.data_ptr()
+    bc = (n, T, N)
+    g = ScanGrads(new(x.shape, et), new(x.shape, et), new((ch, N), f32), new(bc, et), new(bc, et),
+                  new((ch,), f32, D is not None), new(x.shape, et, z is not None), new((ch,), f32, dt_bias is not None))
+    wide, narrow = (T * ch, ch), (T * N, N)
+    d = _SCAN.pack(*head, 0, *ins, 0, 0, 0, *_seq(dy, "dy", x.shape, et, dev), g.dx.data_ptr(), *wide,
+                   g.ddt.data_ptr(), *wide, *(_NONE if g.dz is None else (g.dz.data_ptr(), *wide)), g.dB.data_ptr(),
+                   *narrow, g.dC.data_ptr(), *narrow, g.dA.data_ptr(), 0 if g.dD is None else g.dD.data_ptr(),
+                   0 if g.ddt_bias is None else g.ddt_bias.data_ptr())
     _op("selective_scan")(d, dev, True, True)
     return g
 
 
 # ------------------------------------------------------ gated feed-forward
-def _mlp_desc(x, w_gate, w_up, activation):
+def _mlp_parts(x, w_gate, w_up, activation):
+    """(device, hidden, the descriptor's fields up to the weights)."""
     ty = _type(x, "x")
     if x.dim() < 2:
         raise _wrong("x", x, "rows ([..., width])")
@@ -375,8 +350,8 @@ def _mlp_desc(x, w_gate, w_up, activation):
     dev, shape, ws = x.device, x.shape, w_gate.shape
     if ws[0] != shape[-1]:
         raise _wrong("w_gate", w_gate, f"[{shape[-1]}][hidden]")
-    return CMlp(ctypes.sizeof(CMlp), ty, act, 0, _count(shape), ws[0], ws[1], *_rows(x, "x", shape, x.dtype, dev),
-                *_rows(w_gate, "w_gate", ws, x.dtype, dev), *_rows(w_up, "w_up", ws, x.dtype, dev))
+    return dev, ws[1], (_MLP_SIZE, ty, act, 0, _count(shape), ws[0], ws[1], *_rows(x, "x", shape, x.dtype, dev),
+                        *_rows(w_gate, "w_gate", ws, x.dtype, dev), *_rows(w_up, "w_up", ws, x.dtype, dev))
 
 
 def gated_mlp(x, w_gate, w_up, activation: str = "silu", out=None):
@@ -384,26 +359,23 @@ def gated_mlp(x, w_gate, w_up, activation: str = "silu", out=None):
     [width][hidden] of x's type; act is "silu" or "gelu" (tanh form).  Products
     of bfloat16 are accumulated in float32; float32 operands are multiplied as
     accurately as in float32."""
-    d = _mlp_desc(x, w_gate, w_up, activation)
-    shape = (*x.shape[:-1], d.hidden)
+    dev, hidden, head = _mlp_parts(x, w_gate, w_up, activation)
+    shape = (*x.shape[:-1], hidden)
     if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=x.device)
-    d.h, d.h_stride = _rows(out, "out", shape, x.dtype, x.device)
+        out = torch.empty(shape, dtype=x.dtype, device=dev)
+    d = _MLP.pack(*head, *_rows(out, "out", shape, x.dtype, dev), 0, 0, 0, 0, 0, 0, 0, 0)
     # (few rows take no scratch)
-    _op("gated_mlp")(d, x.device, False, d.rows > 16)
+    _op("gated_mlp")(d, dev, False, head[4] > 16)
     return out
 
 
 def gated_mlp_backward(dh, x, w_gate, w_up, activation: str = "silu"):
     """(dx, dw_gate, dw_up) of ``gated_mlp``; the projections are formed
     again, so nothing is kept between the passes."""
-    d = _mlp_desc(x, w_gate, w_up, activation)
-    dev = x.device
-    d.dh, d.dh_stride = _rows(dh, "dh", (*x.shape[:-1], d.hidden), x.dtype, dev)
+    dev, hidden, head = _mlp_parts(x, w_gate, w_up, activation)
     dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
     dg, du = (torch.empty(w_gate.shape, dtype=x.dtype, device=dev) for _ in range(2))
-    d.dx, d.dx_stride = dx.data_ptr(), d.width
-    d.dw_gate, d.dw_gate_stride = dg.data_ptr(), d.hidden
-    d.dw_up, d.dw_up_stride = du.data_ptr(), d.hidden
+    d = _MLP.pack(*head, 0, 0, *_rows(dh, "dh", (*x.shape[:-1], hidden), x.dtype, dev), dx.data_ptr(), x.shape[-1],
+                  dg.data_ptr(), hidden, du.data_ptr(), hidden)
     _op("gated_mlp")(d, dev, True, True)
     return dx, dg, du
