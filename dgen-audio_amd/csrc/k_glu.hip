@@ -552,7 +552,8 @@ __global__ __launch_bounds__(kDThreads, 2) void k_glu_direct(GluD p) {
   };
   // Stage s + 1 is waited for in the middle of stage s: each wave for its own
   // copies, then for the other waves; after that the buffer of stage s - 1 is
-  // free, which every wave has left.
+  // free, which every wave has left.  The copies into it go last: ahead of the
+  // products they delay the LDS reads (dW: 410 us against 380).
   if (stages > 0) {
     issue(0);
     if (stages > 1) issue(1);
@@ -569,12 +570,11 @@ __global__ __launch_bounds__(kDThreads, 2) void k_glu_direct(GluD p) {
       read(s, 1);
       __builtin_amdgcn_sched_barrier(0);  // the reads first: they land behind the products
       multiply(0);
-      __builtin_amdgcn_sched_barrier(0);
       asm volatile("s_waitcnt vmcnt(4)\n\ts_barrier" ::: "memory");
-      issue(s + 3);
       read(s + 1, 0);
       __builtin_amdgcn_sched_barrier(0);
       multiply(1);
+      issue(s + 3);
     }
     if (dh_copied && stages == 1) copy_dh();
     for (; s < stages; ++s) {
@@ -798,11 +798,23 @@ __global__ __launch_bounds__(kFewThreads) void k_glu_few(GluP<E> p) {
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 int64_t tiles(int64_t n, int64_t of) { return (n + of - 1) / of; }
 
+// Forward by k_glu_few.  It reads the weights once more for every 8 rows and
+// multiplies on the vector unit; the tiles read them once and cost the same up
+// to 64 rows, fp32's three times bfloat16's.  512 x 1408 and 1024 x 2816, us
+// of a call, few / tiles: bfloat16, 16 rows 12 / 13 and 13 / 17, 24 rows 13 /
+// 13 and 24 / 17; fp32, 32 rows 12 / 26 and 28 / 48, 64 rows 19 / 26 and 42 /
+// 49, 96 rows 28 / 26 and 69 / 49.
+bool few(const dgen_hip_mlp& a) { return a.rows <= (a.type == DGEN_HIP_BF16 ? 16 : 64); }
+
 // bfloat16: packed operands and 256 x 256 tiles where the projections' tiles
 // come near to filling the chip's 256 CUs; else small tiles on the operands as
-// they are.  (SIDES)
+// they are.  Rows x width x hidden, us forward and backward, large / small:
+// 132 tiles, 1500 x 1024 x 2816 31 / 50 and 144 / 177, 3000 x 512 x 1408 21 /
+// 29 and 105 / 111; 88 tiles, 1024 x 1024 x 2816 30 / 33 and 112 / 118, 2000 x
+// 512 x 1408 19 / 19 and 101 / 87; 72 tiles, 9000 x 256 x 256 16 / 15 and 85 /
+// 53.
 bool large(const dgen_hip_mlp& a) {
-  return a.type == DGEN_HIP_BF16 && a.rows > 2 * kFewRows && tiles(a.rows, kDT) * tiles(2 * a.hidden, kDT) >= 128;
+  return a.type == DGEN_HIP_BF16 && !few(a) && tiles(a.rows, kDT) * tiles(2 * a.hidden, kDT) >= 128;
 }
 
 // Runs of a reduction of `steps`, as many as make the rounds of `count` tiles
@@ -838,11 +850,14 @@ struct Plan {
   int64_t dw_rows;              // rows in the runs; the rest (of x as it is) is one more
   int64_t x, xtail, wg, wu, dg, du, parts, total;
 };
-// k_glu's tile: 128 x 128 for fp32 products that have tiles (with the runs that
-// their reduction can be cut into) for every CU, else 64 x 128.
+// k_glu's tile: 128 x 128 for fp32 products that have more tiles (with the runs
+// that their reduction can be cut into) than there are CUs, else 64 x 128.  Forward, us,
+// 128 x 128 / 64 x 128: 500 x 512 x 1408 (88 tiles) 39 / 29, 3000 x 256 x 700
+// (264) 33 / 28, 2000 x 512 x 1408 (352) 52 / 54; backward of the last 165 /
+// 182, of 4000 x 512 x 512 129 / 141.
 template <class E>
 bool wide_tile(int64_t rows, int64_t cols, int64_t runs) {
-  return sizeof(E) == 4 && tiles(rows, 128) * tiles(cols, 128) * runs >= 256;
+  return sizeof(E) == 4 && tiles(rows, 128) * tiles(cols, 128) * runs >= 320;
 }
 template <class E>
 int64_t runs_small(int64_t rows, int64_t cols, int64_t mats, int64_t steps) {
@@ -1007,7 +1022,7 @@ void launch_staged(const dgen_hip_mlp& a, bool backward, const Plan& p, hipStrea
   q.M = a.rows, q.N = a.hidden, q.K = a.width;
   if (!backward) {
     q.out0 = (E*)a.h, q.old0 = a.h_stride;
-    if (a.rows <= 2 * kFewRows) {
+    if (few(a)) {
       const dim3 grid((unsigned)tiles(a.hidden, kFewCols), (unsigned)tiles(a.rows, kFewRows));
       k_glu_few<E><<<grid, kFewThreads, 0, st>>>(q);
     } else {

@@ -319,23 +319,23 @@ __global__ __launch_bounds__(kThreads) void k_scan(ScanP<E> p) {
   }
 }
 
-constexpr int kMaxChunks = 512, kMaxRun = kMaxChunks / 16;
+constexpr int kMaxChunks = 512, kMaxRun = 32;  // chunks, and of a thread in the carry
 
 // States entering each chunk, in place of the chunks' end states (reverse:
-// the adjoints entering from the chunks after).  64 states a workgroup, SEGS
+// the adjoints entering from the chunks after).  COLS states a workgroup, SEGS
 // threads over the chunks: each joins its run of chunks, the runs are joined
 // in LDS, and each walks its run again.
 // The backward pass takes both directions in one launch: the second half of
 // the grid is the adjoint's.
-template <class E, int SEGS>
-__global__ __launch_bounds__(64 * SEGS) void k_scan_carry(ScanP<E> p, int np) {
-  __shared__ float rsum[SEGS][65], rend[SEGS][65];
-  const int col = threadIdx.x & 63, seg = threadIdx.x >> 6;
-  const int64_t per = (int64_t)p.D * np, blocks = (per + 63) / 64;
+template <class E, int SEGS, int COLS>
+__global__ __launch_bounds__(COLS * SEGS) void k_scan_carry(ScanP<E> p, int np) {
+  __shared__ float rsum[SEGS][COLS + 1], rend[SEGS][COLS + 1];
+  const int col = threadIdx.x % COLS, seg = threadIdx.x / COLS;
+  const int64_t per = (int64_t)p.D * np, blocks = (per + COLS - 1) / COLS;
   const int row = (int)(blockIdx.x / blocks), b = row % p.batch;
   const bool reverse = row >= p.batch;
   float* const ends = reverse ? p.gends : p.ends;
-  const int64_t j = (blockIdx.x % blocks) * 64 + col;
+  const int64_t j = (blockIdx.x % blocks) * COLS + col;
   const bool on = j < per;
   const int64_t d = on ? j / np : 0;
   const int n = on ? (int)(j % np) : 0;
@@ -665,10 +665,13 @@ struct ScanShape {
   int64_t sums, ends, ckpt, shared, parts, total;
 };
 
-// Chunks: as many as give every CU two workgroups (two waves a SIMD), none
-// shorter than 32 frames, and none where the sequences and channel blocks
-// come near that alone: a chunked pass evaluates every decay twice.
-constexpr int64_t kFill = 512, kFillAlone = 320, kMinChunk = 32;
+// Chunks: as many as give every CU four workgroups (backward, whose LDS and
+// registers take no more, two), none shorter than 32 frames, and none where
+// the sequences and channel blocks come near filling the chip alone, as a
+// chunked pass evaluates every decay twice.  Measured, T = 1000, N = 16, bf16,
+// whole / chunked: forward 128 blocks 138 / 95 us, 192 140 / 155, 256 141 /
+// 168; backward 256 blocks 531 / 476 us, 320 670 / 745.
+constexpr int64_t kFill = 1024, kFillBackward = 512, kAlone = 160, kAloneBackward = 288, kMinChunk = 32;
 
 ScanShape scan_shape(const dgen_hip_scan& a, bool backward) {
   ScanShape s{};
@@ -677,8 +680,8 @@ ScanShape scan_shape(const dgen_hip_scan& a, bool backward) {
   s.nd = (a.D + kChannels - 1) / kChannels;
   const int64_t blocks = std::max<int64_t>(1, a.batch * s.nd);
   int64_t chunks = 1;
-  if (blocks < kFillAlone)
-    chunks = std::min({(kFill + blocks - 1) / blocks, (a.T + kMinChunk - 1) / kMinChunk, (int64_t)kMaxChunks});
+  if (blocks < (backward ? kAloneBackward : kAlone))
+    chunks = std::min({((backward ? kFillBackward : kFill) + blocks - 1) / blocks, (a.T + kMinChunk - 1) / kMinChunk, (int64_t)kMaxChunks});
   s.chunk = (a.T + chunks - 1) / chunks;
   s.chunk = (s.chunk + kTile - 1) / kTile * kTile;
   s.chunks = (a.T + s.chunk - 1) / s.chunk;
@@ -714,11 +717,14 @@ void scan_launch(const dgen_hip_scan& a, bool backward, const ScanShape& s, hipS
   p.sums = ws, p.ends = p.sums + s.sums, p.gends = p.ends + s.ends;
   if (!backward) p.y = out_rows<E>(a.y), p.state_out = a.state_out;
   const dim3 grid((unsigned)(s.nd * s.chunks * a.batch));
-  // (few chunks: four threads a state, with runs of up to 16)
+  // (threads a state by the number of chunks, for runs of up to 16 or 32)
   auto carry = [&]() {
-    const dim3 states((unsigned)((a.D * s.NP + 63) / 64 * a.batch * (backward ? 2 : 1)));
-    if (s.chunks <= 64) k_scan_carry<E, 4><<<states, 256, 0, st>>>(p, (int)s.NP);
-    else k_scan_carry<E, 16><<<states, 1024, 0, st>>>(p, (int)s.NP);
+    auto states = [&](int64_t cols) {
+      return dim3((unsigned)((a.D * s.NP + cols - 1) / cols * a.batch * (backward ? 2 : 1)));
+    };
+    if (s.chunks <= 64) k_scan_carry<E, 4, 64><<<states(64), 256, 0, st>>>(p, (int)s.NP);
+    else if (s.chunks <= 256) k_scan_carry<E, 16, 64><<<states(64), 1024, 0, st>>>(p, (int)s.NP);
+    else k_scan_carry<E, 32, 32><<<states(32), 1024, 0, st>>>(p, (int)s.NP);
   };
   if (!backward) {
     if (s.chunks == 1) {
@@ -770,7 +776,7 @@ int scan_run(const dgen_hip_scan& a, bool backward, hipStream_t st, bool dry) {
   const ScanShape s = scan_shape(a, backward);
   // (a launch takes fewer than 2^32 threads)
   DGEN_REQUIRE(s.nd * s.chunks * a.batch < (int64_t(1) << 23) && a.batch * ((a.T + 3) / 4) < (int64_t(1) << 31) &&
-                   s.nd * a.batch < (int64_t(1) << 31) && (a.D * s.NP + 63) / 64 * a.batch < (int64_t(1) << 21) &&
+                   s.nd * a.batch < (int64_t(1) << 31) && (a.D * s.NP + 31) / 32 * a.batch < (int64_t(1) << 20) &&
                    (!backward || a.batch * a.T * 2 * a.N < (int64_t(1) << 31)),
                "%s: batch %lld x T %lld x D %lld x N %lld is too large for one call", what, (long long)a.batch,
                (long long)a.T, (long long)a.D, (long long)a.N);

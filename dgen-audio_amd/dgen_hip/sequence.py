@@ -364,7 +364,7 @@ def gated_mlp(x, w_gate, w_up, activation: str = "silu", out=None):
     if out is None:
         out = torch.empty(shape, dtype=x.dtype, device=dev)
     d = _MLP.pack(*head, *_rows(out, "out", shape, x.dtype, dev), 0, 0, 0, 0, 0, 0, 0, 0)
-    # (few rows take no scratch)
+    # (up to 16 rows take no scratch)
     _op("gated_mlp")(d, dev, False, head[4] > 16)
     return out
 
