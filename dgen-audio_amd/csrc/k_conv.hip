@@ -201,7 +201,8 @@ __global__ __launch_bounds__(kBwdGroups* kBwdTiles) void k_conv_bwd(
   if (t0 < s.T && g < s.G) {
     const T* xp = x + b * xb + ch.c;
     const T* gp = dy + b * gb + ch.c;
-    const T* sp = state ? state + b * (W - 1) * s.D + ch.c : nullptr;
+    // (a sequence without frames takes nothing of its state, whatever that holds)
+    const T* sp = state && n > 0 ? state + b * (W - 1) * s.D + ch.c : nullptr;
     T* op = dx + b * db + ch.c;
     Four<T> nextx[kGroup], nextg[kGroup];
     auto fetch = [&](int64_t t) {

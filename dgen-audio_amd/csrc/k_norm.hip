@@ -144,32 +144,10 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_rms_norm_bwd(
   }
 }
 
-// Columns of a 64-wide block, 16 threads each over the rows.
-__global__ __launch_bounds__(1024) void k_sum_parts(const float* __restrict__ ws, int64_t parts, SumOut o,
-                                                    int64_t width) {
-  __shared__ float red[16][65];
-  const int col = threadIdx.x & 63, sub = threadIdx.x >> 6;
-  const int64_t j = (int64_t)blockIdx.x * 64 + col;
-  float a[4] = {0.f, 0.f, 0.f, 0.f};
-  if (j < width) {
-    int64_t p = sub;
-    for (; p + 48 < parts; p += 64)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) a[q] += ws[(p + 16 * q) * width + j];
-    for (; p < parts; p += 16) a[0] += ws[p * width + j];
-  }
-  red[sub][col] = (a[0] + a[1]) + (a[2] + a[3]);
-  __syncthreads();
-  if (sub == 0 && j < width) {
-    float t = 0.f;
-#pragma unroll
-    for (int q = 0; q < 16; ++q) t += red[q][col];
-    int64_t at = j;
-    for (int k = 0; k < 3; ++k) {
-      if (at >= 0 && at < o.n[k] && o.out[k]) o.out[k][at] = t;
-      at -= o.n[k];
-    }
-  }
+__global__ __launch_bounds__(kSumThreads) void k_sum_parts(const float* __restrict__ ws, int64_t parts, SumOut o,
+                                                           int64_t width) {
+  __shared__ float red[kSumThreads / kSumCols][kSumCols + 1];
+  sum_parts_block(ws, parts, o, width, blockIdx.x, red);
 }
 
 constexpr int64_t kMaxWidth = 32768;
@@ -233,7 +211,7 @@ void norm_shape(const dgen_hip_norm& a, bool backward, hipStream_t st) {
 
 void enqueue_sum_parts(hipStream_t stream, const float* ws, int64_t parts, const SumOut& out) {
   const int64_t width = out.n[0] + out.n[1] + out.n[2];
-  k_sum_parts<<<dim3((unsigned)((width + 63) / 64)), 1024, 0, stream>>>(ws, parts, out, width);
+  k_sum_parts<<<dim3((unsigned)((width + kSumCols - 1) / kSumCols)), kSumThreads, 0, stream>>>(ws, parts, out, width);
 }
 
 int64_t norm_workspace(const dgen_hip_norm& a, bool backward) {

@@ -53,6 +53,7 @@ struct ScanP {
   const int32_t* lengths;
   float* state_out;
   int T, D, N, chunk, chunks, nd, batch;  // nd: blocks of 64 channels
+  bool walk;                              // the chunks join their entering states themselves
   float* sums;                         // [batch][chunks][D]: summed steps
   float* ends;                         // [batch][chunks][D][NP]: end states, then the states entering
   float* gends;                        // the same of the adjoint
@@ -117,6 +118,7 @@ struct Place {
   int b, c, d, lane, wave, q;
   bool on;
   int begin, end, live;  // the chunk's frames, and how far they are inside the sequence
+  int frames;            // the sequence's
 };
 template <class E>
 __device__ __forceinline__ Place place_of(const ScanP<E>& p) {
@@ -131,8 +133,8 @@ __device__ __forceinline__ Place place_of(const ScanP<E>& p) {
   w.b = i / nc;
   w.begin = w.c * p.chunk;
   w.end = w.begin + p.chunk < p.T ? w.begin + p.chunk : p.T;
-  const int n = live_of(p.lengths, w.b, p.T);
-  w.live = n < w.end ? n : w.end;
+  w.frames = live_of(p.lengths, w.b, p.T);
+  w.live = w.frames < w.end ? w.frames : w.end;
   return w;
 }
 
@@ -199,6 +201,32 @@ struct Lane {
   }
 };
 
+constexpr int kWalkStates = 4;  // of a lane, at most
+// Joins `count` chunks' end states to h, from chunk `first` on in steps of
+// `dir`: h = exp(A sum) h + end.  a2: A log2(e).  The loads of 16 chunks
+// are in flight at once.
+template <class E, int S>
+__device__ __forceinline__ void join_chunks(const ScanP<E>& p, const Place& w, const float* __restrict__ ends, int first,
+                                            int count, int dir, const float (&a2)[S], float (&h)[S]) {
+  constexpr int K = 16;
+  const int64_t row = (int64_t)w.b * p.chunks, d = w.on ? w.d : p.D - 1;
+  for (int c0 = 0; c0 < count; c0 += K) {
+    float sum[K], end[K][S];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = c0 + k < count ? c0 + k : count - 1;
+      const int64_t at = (row + first + dir * c) * p.D + d;
+      sum[k] = p.sums[at];
+      read_states<S>(ends + at * (4 * S) + w.q * S, end[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (c0 + k < count)
+#pragma unroll
+        for (int s = 0; s < S; ++s) h[s] = fmaf(__builtin_amdgcn_exp2f(sum[k] * a2[s]), h[s], end[k][s]);
+  }
+}
+
 enum Mode { kWhole, kSummary, kReplay, kSummaryBoth };
 
 // Forward: kWhole (one chunk: state to state_out), kReplay (from the state
@@ -211,7 +239,11 @@ __global__ __launch_bounds__(kThreads) void k_scan(ScanP<E> p) {
   constexpr bool OUT = MODE == kWhole || MODE == kReplay, ADJ = MODE == kSummaryBoth;
   __shared__ __align__(16) float bc[2][kTile * 2 * NP];
   const Place w = place_of(p);
-  if (!OUT && w.begin >= w.live) return;  // a chunk past the sequence: the carry leaves it out
+  // Where the chunks join their states themselves nobody needs the last one's
+  // end, and its place takes the state before the first, which the replay may
+  // overwrite (state_out) before all of its workgroups have read it.
+  const bool walk = S <= kWalkStates && p.walk, copy = MODE == kSummary && walk && w.c == p.chunks - 1;
+  if (!OUT && w.begin >= w.live && !copy) return;  // a chunk past the sequence is left out
 
   float h[S], a2[S], prod[S], adj[S];
   const float bias = p.bias && w.on ? p.bias[w.d] : 0.f, skip = p.skip && w.on ? p.skip[w.d] : 0.f;
@@ -222,11 +254,20 @@ __global__ __launch_bounds__(kThreads) void k_scan(ScanP<E> p) {
     const bool real = w.on && n < p.N;
     a2[s] = real ? p.A[(int64_t)w.d * p.N + n] * kLog2e : 0.f;
     h[s] = 0.f;
-    if (MODE == kWhole && p.state && real) h[s] = p.state[((int64_t)w.b * p.D + w.d) * p.N + n];
+    if ((MODE == kWhole || copy) && p.state && real) h[s] = p.state[((int64_t)w.b * p.D + w.d) * p.N + n];
     prod[s] = 1.f;
     adj[s] = 0.f;
   }
-  if (MODE == kReplay && w.on) read_states<S>(p.ends + at, h);
+  if (copy) {
+    if (w.on) write_states<S>(p.ends + at, h);
+    return;
+  }
+  if (MODE == kReplay && walk) {
+    if (w.on) read_states<S>(p.ends + ((int64_t)(w.b * p.chunks + p.chunks - 1) * p.D + w.d) * NP + w.q * S, h);
+    if (w.begin < w.live) join_chunks<E, S>(p, w, p.ends, 0, w.c, 1, a2, h);
+  } else if (MODE == kReplay && w.on) {
+    read_states<S>(p.ends + at, h);
+  }
 
   const bool odd = w.q & 1, upper = w.q & 2;
   float sum = 0.f;
@@ -306,7 +347,9 @@ __global__ __launch_bounds__(kThreads) void k_scan(ScanP<E> p) {
   if (OUT)
     for (int t = (w.live > w.begin ? w.live : w.begin) + w.q; t < w.end; t += 4)
       p.y.p[w.b * p.y.b + (int64_t)t * p.y.t + w.d] = from_f32<E>(0.f);
-  if (MODE == kWhole && p.state_out) {
+  // (of chunks, the one with the sequence's last frame)
+  const bool last = MODE == kWhole || (walk && w.frames <= w.end && (w.begin < w.frames || w.c == 0));
+  if (OUT && p.state_out && last) {
 #pragma unroll
     for (int s = 0; s < S; ++s)
       if (w.q * S + s < p.N) p.state_out[((int64_t)w.b * p.D + w.d) * p.N + w.q * S + s] = h[s];
@@ -321,7 +364,7 @@ __global__ __launch_bounds__(kThreads) void k_scan(ScanP<E> p) {
 
 constexpr int kMaxChunks = 512, kMaxRun = 32;  // chunks, and of a thread in the carry
 
-// States entering each chunk, in place of the chunks' end states (reverse:
+// Of many chunks: states entering each, in place of the chunks' end states (reverse:
 // the adjoints entering from the chunks after).  COLS states a workgroup, SEGS
 // threads over the chunks: each joins its run of chunks, the runs are joined
 // in LDS, and each walks its run again.
@@ -427,6 +470,7 @@ __global__ __launch_bounds__(kThreads, S <= 4 ? 2 : 1) void k_scan_bwd(ScanP<E> 
   // the tile's states before each frame, a lane's own
   __shared__ __align__(16) float hs[TL][kThreads][S];
   const Place w = place_of(p);
+  const bool walk = S <= kWalkStates && p.walk;
   const int tiles_all = (p.T + TL - 1) / TL, tile0 = w.begin / TL;
   const int tiles = w.live > w.begin ? (w.live - w.begin + TL - 1) / TL : 0;
 
@@ -438,11 +482,18 @@ __global__ __launch_bounds__(kThreads, S <= 4 ? 2 : 1) void k_scan_bwd(ScanP<E> 
     const int n = w.q * S + s;
     const bool real = w.on && n < p.N;
     a[s] = real ? p.A[(int64_t)w.d * p.N + n] : 0.f;
-    h[s] = p.chunks == 1 && p.state && real ? p.state[((int64_t)w.b * p.D + w.d) * p.N + n] : 0.f;
+    h[s] = (p.chunks == 1 || walk) && p.state && real ? p.state[((int64_t)w.b * p.D + w.d) * p.N + n] : 0.f;
     g[s] = 0.f;
     dA[s] = 0.f;
   }
-  if (p.chunks > 1 && tiles > 0 && w.on) {
+  if (walk && tiles > 0) {
+    float a2[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) a2[s] = a[s] * kLog2e;
+    const int used = (w.frames + p.chunk - 1) / p.chunk;
+    join_chunks<E, S>(p, w, p.ends, 0, w.c, 1, a2, h);
+    join_chunks<E, S>(p, w, p.gends, used - 1, used - 1 - w.c, -1, a2, g);
+  } else if (p.chunks > 1 && tiles > 0 && w.on) {
     read_states<S>(p.ends + at, h);
     read_states<S>(p.gends + at, g);
   }
@@ -643,17 +694,22 @@ __global__ __launch_bounds__(kThreads, S <= 4 ? 2 : 1) void k_scan_bwd(ScanP<E> 
   }
 }
 
-// dB and dC: the channel blocks' sums added in order.
+// The last sums of the backward pass, in order: workgroups before `first` add
+// the channel blocks' dB and dC, the others dA, dskip and ddt_bias.
 template <class E>
-__global__ __launch_bounds__(256) void k_scan_shared(const float* __restrict__ shared, const int32_t* __restrict__ lengths,
-                                                     Rows<E> dB, Rows<E> dC, int64_t nd, int64_t batch, int64_t T,
-                                                     int64_t N) {
-  const int64_t total = batch * T * 2 * N, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+__global__ __launch_bounds__(kSumThreads) void k_scan_join(ScanP<E> p, Rows<E> dB, Rows<E> dC, uint32_t first, SumOut o,
+                                                           int64_t width) {
+  __shared__ float red[kSumThreads / kSumCols][kSumCols + 1];
+  if (blockIdx.x >= first) {
+    sum_parts_block(p.parts, (int64_t)p.batch * p.chunks, o, width, blockIdx.x - first, red);
+    return;
+  }
+  const int64_t N = p.N, T = p.T, total = p.batch * T * 2 * N, i = (int64_t)blockIdx.x * kSumThreads + threadIdx.x;
   if (i >= total) return;
   const int64_t row = i / (2 * N), col = i - row * 2 * N, b = row / T, t = row - b * T;
   float v = 0.f;
-  if (t < live_of(lengths, (int)b, (int)T))
-    for (int64_t k = 0; k < nd; ++k) v += shared[k * total + i];
+  if (t < live_of(p.lengths, (int)b, p.T))
+    for (int64_t k = 0; k < p.nd; ++k) v += p.shared[k * total + i];
   const Rows<E>& m = col < N ? dB : dC;
   m.p[b * m.b + t * (int64_t)m.t + (col < N ? col : col - N)] = from_f32<E>(v);
 }
@@ -672,6 +728,12 @@ struct ScanShape {
 // whole / chunked: forward 128 blocks 138 / 95 us, 192 140 / 155, 256 141 /
 // 168; backward 256 blocks 531 / 476 us, 320 670 / 745.
 constexpr int64_t kFill = 1024, kFillBackward = 512, kAlone = 160, kAloneBackward = 288, kMinChunk = 32;
+// Chunks up to which, of up to 16 states, each joins the ones before it (and
+// after it, backward) by itself; more go through k_scan_carry.  Calls, us, joined / carried: N = 16,
+// forward 4 x 256 x 256 (8 chunks) 20 / 22, 2 x 1024 x 128 (32) 19 / 22, 4 x
+// 2048 x 64 (64) 22 / 22, 1 x 4096 x 64 (128) 28 / 21; backward 32 / 34, 33 /
+// 34, 40 / 39, 43 / 36; N = 64, 32 chunks, 41 / 33 and 90 / 86.
+constexpr int64_t kWalk = 32;
 
 ScanShape scan_shape(const dgen_hip_scan& a, bool backward) {
   ScanShape s{};
@@ -714,6 +776,7 @@ void scan_launch(const dgen_hip_scan& a, bool backward, const ScanShape& s, hipS
   p.A = a.A, p.skip = a.skip, p.bias = a.dt_bias, p.state = a.state, p.lengths = a.lengths;
   p.T = (int)a.T, p.D = (int)a.D, p.N = (int)a.N, p.chunk = (int)s.chunk, p.chunks = (int)s.chunks, p.nd = (int)s.nd;
   p.batch = (int)a.batch;
+  p.walk = S <= kWalkStates && s.chunks > 1 && s.chunks <= kWalk;
   p.sums = ws, p.ends = p.sums + s.sums, p.gends = p.ends + s.ends;
   if (!backward) p.y = out_rows<E>(a.y), p.state_out = a.state_out;
   const dim3 grid((unsigned)(s.nd * s.chunks * a.batch));
@@ -731,7 +794,7 @@ void scan_launch(const dgen_hip_scan& a, bool backward, const ScanShape& s, hipS
       k_scan<E, S, kWhole><<<grid, kThreads, 0, st>>>(p);
     } else {
       k_scan<E, S, kSummary><<<grid, kThreads, 0, st>>>(p);
-      carry();
+      if (!p.walk) carry();
       k_scan<E, S, kReplay><<<grid, kThreads, 0, st>>>(p);
     }
     return;
@@ -740,12 +803,13 @@ void scan_launch(const dgen_hip_scan& a, bool backward, const ScanShape& s, hipS
   p.ckpt = p.gends + s.ends, p.shared = p.ckpt + s.ckpt, p.parts = p.shared + s.shared;
   if (s.chunks > 1) {
     k_scan<E, S, kSummaryBoth><<<grid, kThreads, 0, st>>>(p);
-    carry();
+    if (!p.walk) carry();
   }
   k_scan_bwd<E, S><<<grid, kThreads, 0, st>>>(p);
-  k_scan_shared<E><<<dim3((unsigned)((a.batch * a.T * 2 * a.N + 255) / 256)), 256, 0, st>>>(
-      p.shared, a.lengths, out_rows<E>(a.dB), out_rows<E>(a.dC), s.nd, a.batch, a.T, a.N);
-  enqueue_sum_parts(st, p.parts, a.batch * s.chunks, {{a.dA, a.dskip, a.ddt_bias}, {a.D * a.N, a.D, a.D}});
+  const uint32_t first = (uint32_t)((a.batch * a.T * 2 * a.N + kSumThreads - 1) / kSumThreads);
+  const int64_t width = a.D * (a.N + 2);
+  k_scan_join<E><<<dim3(first + (unsigned)((width + kSumCols - 1) / kSumCols)), kSumThreads, 0, st>>>(
+      p, out_rows<E>(a.dB), out_rows<E>(a.dC), first, {{a.dA, a.dskip, a.ddt_bias}, {a.D * a.N, a.D, a.D}}, width);
 }
 
 template <class E>

@@ -95,6 +95,34 @@ struct SumOut {
   float* out[3];
   int64_t n[3];  // columns of each (0: none); a NULL output is skipped
 };
+constexpr int kSumThreads = 1024, kSumCols = 64;
+// One workgroup's share: columns from 64 `block` on, 16 threads each over the
+// rows.
+__device__ __forceinline__ void sum_parts_block(const float* __restrict__ ws, int64_t parts, const SumOut& o,
+                                                int64_t width, int64_t block, float (*red)[kSumCols + 1]) {
+  const int col = threadIdx.x % kSumCols, sub = threadIdx.x / kSumCols;
+  const int64_t j = block * kSumCols + col;
+  float a[4] = {0.f, 0.f, 0.f, 0.f};
+  if (j < width) {
+    int64_t p = sub;
+    for (; p + 48 < parts; p += 64)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) a[q] += ws[(p + 16 * q) * width + j];
+    for (; p < parts; p += 16) a[0] += ws[p * width + j];
+  }
+  red[sub][col] = (a[0] + a[1]) + (a[2] + a[3]);
+  __syncthreads();
+  if (sub == 0 && j < width) {
+    float t = 0.f;
+#pragma unroll
+    for (int q = 0; q < kSumThreads / kSumCols; ++q) t += red[q][col];
+    int64_t at = j;
+    for (int k = 0; k < 3; ++k) {
+      if (at >= 0 && at < o.n[k] && o.out[k]) o.out[k][at] = t;
+      at -= o.n[k];
+    }
+  }
+}
 void enqueue_sum_parts(hipStream_t stream, const float* ws, int64_t parts, const SumOut& out);
 
 // Device to run on, restored at the end of the scope.

@@ -160,6 +160,23 @@ def _rows(t, name: str, shape, dtype, device):
     return t.data_ptr(), rs
 
 
+def _fresh(like, out, name: str, shape):
+    """A result in rows, given or made: the tensor, its address and row stride
+    (one that is made here needs no test)."""
+    if out is None:
+        out = torch.empty_like(like, memory_format=torch.contiguous_format)
+        return out, (out.data_ptr(), shape[-1])
+    return out, _rows(out, name, shape, like.dtype, like.device)
+
+
+def _fresh_seq(like, out, shape):
+    """The same of a sequence tensor."""
+    if out is None:
+        out = torch.empty_like(like, memory_format=torch.contiguous_format)
+        return out, (out.data_ptr(), shape[1] * shape[2], shape[2])
+    return out, _seq(out, "out", shape, like.dtype, like.device)
+
+
 def _count(shape) -> int:
     n = 1
     for s in shape[:-1]:
@@ -180,17 +197,13 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-5, out=None, sum_out=None
         raise _wrong("x", x, "rows ([..., width])")
     xp = _rows(x, "x", shape, x.dtype, dev)
     w = _dense(weight, "weight", shape[-1:], torch.float32, dev)
-    if out is None:
-        out = torch.empty_like(x, memory_format=torch.contiguous_format)
-    yp = _rows(out, "out", shape, x.dtype, dev)
+    out, yp = _fresh(x, out, "out", shape)
     rp = sp = _NO_ROWS
     st = ty
     if residual is not None:
         st = _type(residual, "residual")
         rp = _rows(residual, "residual", shape, residual.dtype, dev)
-        if sum_out is None:
-            sum_out = torch.empty_like(residual, memory_format=torch.contiguous_format)
-        sp = _rows(sum_out, "sum_out", shape, residual.dtype, dev)
+        sum_out, sp = _fresh(residual, sum_out, "sum_out", shape)
     elif sum_out is not None:
         raise ValueError("sum_out: only with a residual")
     d = _NORM.pack(_NORM_SIZE, ty, st, eps, _count(shape), shape[-1], w, *xp, *rp, *yp, *sp, 0, 0, 0, 0, 0, 0, 0)
@@ -206,14 +219,13 @@ def rms_norm_backward(dy, s, weight, ds=None, eps: float = 1e-5, out=None):
     ty, st, shape, dev = _type(dy, "dy"), _type(s, "s"), s.shape, s.device
     if s.dim() < 2:
         raise _wrong("s", s, "rows ([..., width])")
-    if out is None:
-        out = torch.empty_like(s, memory_format=torch.contiguous_format)
-    dw = torch.empty(shape[-1], dtype=torch.float32, device=dev)
+    out, op = _fresh(s, out, "out", shape)
+    dw = s.new_empty(shape[-1], dtype=torch.float32)
     d = _NORM.pack(_NORM_SIZE, ty, st, eps, _count(shape), shape[-1],
                    _dense(weight, "weight", shape[-1:], torch.float32, dev), 0, 0, 0, 0, 0, 0,
                    *_rows(s, "s", shape, s.dtype, dev), *_rows(dy, "dy", shape, dy.dtype, dev),
                    *(_NO_ROWS if ds is None else _rows(ds, "ds", shape, s.dtype, dev)),
-                   *_rows(out, "out", shape, s.dtype, dev), dw.data_ptr())
+                   *op, dw.data_ptr())
     _op("rms_norm")(d, dev, True, True)
     return out, dw
 
@@ -240,10 +252,9 @@ def causal_conv(x, weight, bias=None, silu: bool = True, state=None, state_out=N
     first are ``state`` ([batch][W-1][D], x's type, oldest first) or 0;
     ``state_out`` receives the last W-1 frames of each sequence."""
     W, dev, (ty, (B, T, D), w, b, n, xs, st) = _conv_parts(x, weight, bias, state, lengths)
-    if out is None:
-        out = torch.empty_like(x, memory_format=torch.contiguous_format)
-    d = _CONV.pack(_CONV_SIZE, ty, 1 if silu else 0, W, B, T, D, w, b, n, *xs, *_seq(out, "out", x.shape, x.dtype, dev),
-                   st, _dense(state_out, "state_out", (B, W - 1, D), x.dtype, dev), 0, 0, 0, 0, 0, 0, 0, 0)
+    out, ys = _fresh_seq(x, out, x.shape)
+    d = _CONV.pack(_CONV_SIZE, ty, 1 if silu else 0, W, B, T, D, w, b, n, *xs, *ys, st,
+                   _dense(state_out, "state_out", (B, W - 1, D), x.dtype, dev), 0, 0, 0, 0, 0, 0, 0, 0)
     _op("causal_conv")(d, dev, False, False)
     return out
 
@@ -252,13 +263,11 @@ def causal_conv_backward(dy, x, weight, bias=None, silu: bool = True, state=None
     """(dx, dweight, dbias) of ``causal_conv`` (dbias None without a bias);
     the state counts as given."""
     W, dev, (ty, (B, T, D), w, b, n, xs, st) = _conv_parts(x, weight, bias, state, lengths)
-    if out is None:
-        out = torch.empty_like(x, memory_format=torch.contiguous_format)
-    dw = torch.empty((D, W), dtype=torch.float32, device=dev)
-    db = None if bias is None else torch.empty(D, dtype=torch.float32, device=dev)
+    out, ds = _fresh_seq(x, out, x.shape)
+    dw = weight.new_empty((D, W))
+    db = None if bias is None else bias.new_empty(D)
     d = _CONV.pack(_CONV_SIZE, ty, 1 if silu else 0, W, B, T, D, w, b, n, *xs, 0, 0, 0, st, 0,
-                   *_seq(dy, "dy", x.shape, x.dtype, dev), *_seq(out, "out", x.shape, x.dtype, dev), dw.data_ptr(),
-                   0 if db is None else db.data_ptr())
+                   *_seq(dy, "dy", x.shape, x.dtype, dev), *ds, dw.data_ptr(), 0 if db is None else db.data_ptr())
     _op("causal_conv")(d, dev, True, True)
     return out, dw, db
 
@@ -307,10 +316,9 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, state=None, sta
     Results of a sequence can differ in rounding with the number of sequences
     and channels in the call, which decide how time is cut."""
     dev, (n, T, ch, N), head, ins = _scan_parts(x, dt, A, B, C, D, z, dt_bias, state, lengths)
-    if out is None:
-        out = torch.empty_like(x, memory_format=torch.contiguous_format)
-    d = _SCAN.pack(*head, _dense(state_out, "state_out", (n, ch, N), torch.float32, dev), *ins,
-                   *_seq(out, "out", x.shape, x.dtype, dev), *_NO_SCAN_GRADS)
+    out, ys = _fresh_seq(x, out, x.shape)
+    d = _SCAN.pack(*head, _dense(state_out, "state_out", (n, ch, N), torch.float32, dev), *ins, *ys,
+                   *_NO_SCAN_GRADS)
     # (a call of few frames is one launch without scratch)
     _op("selective_scan")(d, dev, False, T > 32)
     return out
@@ -319,16 +327,13 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, state=None, sta
 def selective_scan_backward(dy, x, dt, A, B, C, D=None, z=None, dt_bias=None, state=None, lengths=None) -> ScanGrads:
     """Gradients of ``selective_scan``; the state counts as given."""
     dev, (n, T, ch, N), head, ins = _scan_parts(x, dt, A, B, C, D, z, dt_bias, state, lengths)
-    et, f32 = x.dtype, torch.float32
 
-    def new(shape, dtype, given=True):
-        return torch.empty(shape, dtype=dtype, device=dev) if given else None
+    def new(like):
+        return None if like is None else torch.empty_like(like, memory_format=torch.contiguous_format)
 
-    bc = (n, T, N)
-    g = ScanGrads(new(x.shape, et), new(x.shape, et), new((ch, N), f32), new(bc, et), new(bc, et),
-                  new((ch,), f32, D is not None), new(x.shape, et, z is not None), new((ch,), f32, dt_bias is not None))
+    g = ScanGrads(new(x), new(dt), new(A), new(B), new(C), new(D), new(z), new(dt_bias))
     wide, narrow = (T * ch, ch), (T * N, N)
-    d = _SCAN.pack(*head, 0, *ins, 0, 0, 0, *_seq(dy, "dy", x.shape, et, dev), g.dx.data_ptr(), *wide,
+    d = _SCAN.pack(*head, 0, *ins, 0, 0, 0, *_seq(dy, "dy", x.shape, x.dtype, dev), g.dx.data_ptr(), *wide,
                    g.ddt.data_ptr(), *wide, *(_NONE if g.dz is None else (g.dz.data_ptr(), *wide)), g.dB.data_ptr(),
                    *narrow, g.dC.data_ptr(), *narrow, g.dA.data_ptr(), 0 if g.dD is None else g.dD.data_ptr(),
                    0 if g.ddt_bias is None else g.ddt_bias.data_ptr())
@@ -362,8 +367,11 @@ def gated_mlp(x, w_gate, w_up, activation: str = "silu", out=None):
     dev, hidden, head = _mlp_parts(x, w_gate, w_up, activation)
     shape = (*x.shape[:-1], hidden)
     if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=dev)
-    d = _MLP.pack(*head, *_rows(out, "out", shape, x.dtype, dev), 0, 0, 0, 0, 0, 0, 0, 0)
+        out = x.new_empty(shape)
+        hp = out.data_ptr(), hidden
+    else:
+        hp = _rows(out, "out", shape, x.dtype, dev)
+    d = _MLP.pack(*head, *hp, 0, 0, 0, 0, 0, 0, 0, 0)
     # (up to 16 rows take no scratch)
     _op("gated_mlp")(d, dev, False, head[4] > 16)
     return out
@@ -373,8 +381,7 @@ def gated_mlp_backward(dh, x, w_gate, w_up, activation: str = "silu"):
     """(dx, dw_gate, dw_up) of ``gated_mlp``; the projections are formed
     again, so nothing is kept between the passes."""
     dev, hidden, head = _mlp_parts(x, w_gate, w_up, activation)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    dg, du = (torch.empty(w_gate.shape, dtype=x.dtype, device=dev) for _ in range(2))
+    dx, dg, du = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (x, w_gate, w_up))
     d = _MLP.pack(*head, 0, 0, *_rows(dh, "dh", (*x.shape[:-1], hidden), x.dtype, dev), dx.data_ptr(), x.shape[-1],
                   dg.data_ptr(), hidden, du.data_ptr(), hidden)
     _op("gated_mlp")(d, dev, True, True)
