@@ -10,6 +10,11 @@
 // statistics are kept); each thread adds its columns' dy s r over the rows
 // that its workgroup walks, one partial row per workgroup, summed in a fixed
 // order afterwards.
+//
+// Measured (a large copy: 4.97 TB/s): forward of 32000 x 512, x and y bf16,
+// residual and sum fp32, 42.7 us, 4.6 TB/s; backward of the same without ds
+// 47.5 us, 3.4 TB/s, and 7 us for the partial rows; backward of 4001 x 1023
+// fp32 with ds 15.7 us, 4.2 TB/s, and 5 us.
 #include "seq.h"
 
 namespace dgen {

@@ -19,10 +19,16 @@
 //
 // The backward pass first runs a chunk forward and stores the state before
 // every tile of 16 frames, then takes the tiles from the last: a tile's
-// states and decays are formed again in registers, and the adjoint steps down
-// through them.  Sums over channels (gradients of B and C) go over the wave's
+// states (kept in LDS) and decays (in registers) are formed again, and the
+// adjoint steps down through them.  Sums over channels (gradients of B and C) go over the wave's
 // 16 channels in registers, over the four waves in LDS, and over workgroups in
 // a fixed order afterwards; no atomics.
+//
+// Measured, bf16, 32 x 1000 x 1024 x 16: forward in one piece 227 us, backward
+// 680 us and 20 for the sums over workgroups (the vector unit issues in 75 to
+// 80 % of the cycles; two workgroups a CU by registers and LDS).  fp32, 1 x
+// 65536 x 64 x 16 in 512 chunks: ends 22 us, carry 10, replay 31.  fp32, one
+// frame of 32 x 1024 x 16: 8 us.
 #include "seq.h"
 
 namespace dgen {
@@ -34,7 +40,8 @@ constexpr int kTile = 32;  // frames staged at a time, forward
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Frames of a backward tile: its decays are S registers a frame, its states S
-// LDS words a lane and frame (64 KB a workgroup at S = 4, two workgroups a CU).
+// LDS words a lane and frame (64 KB a workgroup at S = 4, two workgroups a CU;
+// tiles of 8 frames, 32 x 1000 x 1024 x 16 bf16: 760 us for 712).
 template <int S>
 constexpr int bwd_tile() { return S <= 4 ? 16 : 64 / S; }
 
@@ -364,8 +371,8 @@ __global__ __launch_bounds__(kThreads) void k_scan(ScanP<E> p) {
 
 constexpr int kMaxChunks = 512, kMaxRun = 32;  // chunks, and of a thread in the carry
 
-// Of many chunks: states entering each, in place of the chunks' end states (reverse:
-// the adjoints entering from the chunks after).  COLS states a workgroup, SEGS
+// Of many chunks: states entering each, in place of the chunks' end states
+// (reverse: the adjoints entering from the chunks after).  COLS states a workgroup, SEGS
 // threads over the chunks: each joins its run of chunks, the runs are joined
 // in LDS, and each walks its run again.
 // The backward pass takes both directions in one launch: the second half of
@@ -729,10 +736,11 @@ struct ScanShape {
 // 168; backward 256 blocks 531 / 476 us, 320 670 / 745.
 constexpr int64_t kFill = 1024, kFillBackward = 512, kAlone = 160, kAloneBackward = 288, kMinChunk = 32;
 // Chunks up to which, of up to 16 states, each joins the ones before it (and
-// after it, backward) by itself; more go through k_scan_carry.  Calls, us, joined / carried: N = 16,
-// forward 4 x 256 x 256 (8 chunks) 20 / 22, 2 x 1024 x 128 (32) 19 / 22, 4 x
-// 2048 x 64 (64) 22 / 22, 1 x 4096 x 64 (128) 28 / 21; backward 32 / 34, 33 /
-// 34, 40 / 39, 43 / 36; N = 64, 32 chunks, 41 / 33 and 90 / 86.
+// after it, backward) by itself; more go through k_scan_carry.  Calls, us,
+// joined / carried: N = 16, forward 4 x 256 x 256 (8 chunks) 20 / 22, 2 x 1024
+// x 128 (32) 19 / 22, 4 x 2048 x 64 (64) 22 / 22, 1 x 4096 x 64 (128) 28 / 21;
+// backward 32 / 34, 33 / 34, 40 / 39, 43 / 36; N = 64, 32 chunks, 41 / 33 and
+// 90 / 86.
 constexpr int64_t kWalk = 32;
 
 ScanShape scan_shape(const dgen_hip_scan& a, bool backward) {

@@ -815,7 +815,8 @@ int dgen_hip_biquad_forward_noalloc(int device, const float* x, const float* mod
  * a stream (a hipStream_t, or NULL for the null stream), checks the
  * descriptor, enqueues its kernels on the stream and returns without waiting.
  * Nothing is allocated: an operator that needs scratch says how much
- * (..._workspace, which depends on the sizes and on which pointers are set)
+ * (..._workspace, for a descriptor that is complete but for the workspace: the
+ * sizes, the pointers that are set, their alignment and the strides count)
  * and takes it in `workspace`, 256-byte aligned, free again once the call's
  * work is done; two calls that can overlap need two.  Workspaces are written
  * before they are read and their contents do not matter.  The caller's
