@@ -33,9 +33,11 @@ from typing import NamedTuple, Optional
 
 import torch
 
+from ._tensor_args import dense, rows, sequence
 from .runtime import HIPError, load_library
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
+_F32, _INT32 = 0, 2  # as the native tests name them
 _ACTS = {"silu": 0, "gelu": 1}
 
 
@@ -115,6 +117,9 @@ def _type(x, name: str) -> int:
     return ty
 
 
+# Tests of an argument: dense, rows and sequence (csrc/tensor_args.cpp) give its
+# address and strides; what they turn down comes to the functions here, which
+# say what is wrong with it, or take it after all.
 def _is(t, shape, dtype, device) -> bool:
     try:
         return t.dtype is dtype and t.shape == shape and t.device == device
@@ -166,7 +171,8 @@ def _fresh(like, out, name: str, shape):
     if out is None:
         out = torch.empty_like(like, memory_format=torch.contiguous_format)
         return out, (out.data_ptr(), shape[-1])
-    return out, _rows(out, name, shape, like.dtype, like.device)
+    return out, (rows(out, shape, _TYPES[like.dtype], like.get_device())
+                 or _rows(out, name, shape, like.dtype, like.device))
 
 
 def _fresh_seq(like, out, shape):
@@ -174,7 +180,8 @@ def _fresh_seq(like, out, shape):
     if out is None:
         out = torch.empty_like(like, memory_format=torch.contiguous_format)
         return out, (out.data_ptr(), shape[1] * shape[2], shape[2])
-    return out, _seq(out, "out", shape, like.dtype, like.device)
+    return out, (sequence(out, shape, _TYPES[like.dtype], like.get_device())
+                 or _seq(out, "out", shape, like.dtype, like.device))
 
 
 def _count(shape) -> int:
@@ -195,14 +202,15 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-5, out=None, sum_out=None
         raise _wrong("x", x, "at least one axis")
     if x.dim() == 1:
         raise _wrong("x", x, "rows ([..., width])")
-    xp = _rows(x, "x", shape, x.dtype, dev)
-    w = _dense(weight, "weight", shape[-1:], torch.float32, dev)
+    i = dev.index
+    xp = rows(x, shape, ty, i) or _rows(x, "x", shape, x.dtype, dev)
+    w = dense(weight, shape[-1:], _F32, i) or _dense(weight, "weight", shape[-1:], torch.float32, dev)
     out, yp = _fresh(x, out, "out", shape)
     rp = sp = _NO_ROWS
     st = ty
     if residual is not None:
         st = _type(residual, "residual")
-        rp = _rows(residual, "residual", shape, residual.dtype, dev)
+        rp = rows(residual, shape, st, i) or _rows(residual, "residual", shape, residual.dtype, dev)
         sum_out, sp = _fresh(residual, sum_out, "sum_out", shape)
     elif sum_out is not None:
         raise ValueError("sum_out: only with a residual")
@@ -219,12 +227,14 @@ def rms_norm_backward(dy, s, weight, ds=None, eps: float = 1e-5, out=None):
     ty, st, shape, dev = _type(dy, "dy"), _type(s, "s"), s.shape, s.device
     if s.dim() < 2:
         raise _wrong("s", s, "rows ([..., width])")
+    i, width = dev.index, shape[-1:]
     out, op = _fresh(s, out, "out", shape)
     dw = s.new_empty(shape[-1], dtype=torch.float32)
     d = _NORM.pack(_NORM_SIZE, ty, st, eps, _count(shape), shape[-1],
-                   _dense(weight, "weight", shape[-1:], torch.float32, dev), 0, 0, 0, 0, 0, 0,
-                   *_rows(s, "s", shape, s.dtype, dev), *_rows(dy, "dy", shape, dy.dtype, dev),
-                   *(_NO_ROWS if ds is None else _rows(ds, "ds", shape, s.dtype, dev)),
+                   dense(weight, width, _F32, i) or _dense(weight, "weight", width, torch.float32, dev),
+                   0, 0, 0, 0, 0, 0, *(rows(s, shape, st, i) or _rows(s, "s", shape, s.dtype, dev)),
+                   *(rows(dy, shape, ty, i) or _rows(dy, "dy", shape, dy.dtype, dev)),
+                   *(_NO_ROWS if ds is None else rows(ds, shape, st, i) or _rows(ds, "ds", shape, s.dtype, dev)),
                    *op, dw.data_ptr())
     _op("rms_norm")(d, dev, True, True)
     return out, dw
@@ -238,11 +248,13 @@ def _conv_parts(x, weight, bias, state, lengths):
     B, T, D = shape = x.shape
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
         raise _wrong("weight", weight, "[channel][width]")
-    W, dev = weight.shape[1], x.device
-    f32 = torch.float32
-    head = (ty, (B, T, D), _dense(weight, "weight", (D, W), f32, dev), _dense(bias, "bias", (D,), f32, dev),
-            _dense(lengths, "lengths", (B,), torch.int32, dev), _seq(x, "x", shape, x.dtype, dev),
-            _dense(state, "state", (B, W - 1, D), x.dtype, dev))
+    W, dev, f32, before = weight.shape[1], x.device, torch.float32, (B, weight.shape[1] - 1, D)
+    i = dev.index
+    head = (ty, (B, T, D), dense(weight, (D, W), _F32, i) or _dense(weight, "weight", (D, W), f32, dev),
+            dense(bias, (D,), _F32, i) or _dense(bias, "bias", (D,), f32, dev),
+            dense(lengths, (B,), _INT32, i) or _dense(lengths, "lengths", (B,), torch.int32, dev),
+            sequence(x, shape, ty, i) or _seq(x, "x", shape, x.dtype, dev),
+            dense(state, before, ty, i) or _dense(state, "state", before, x.dtype, dev))
     return W, dev, head
 
 
@@ -253,8 +265,9 @@ def causal_conv(x, weight, bias=None, silu: bool = True, state=None, state_out=N
     ``state_out`` receives the last W-1 frames of each sequence."""
     W, dev, (ty, (B, T, D), w, b, n, xs, st) = _conv_parts(x, weight, bias, state, lengths)
     out, ys = _fresh_seq(x, out, x.shape)
-    d = _CONV.pack(_CONV_SIZE, ty, 1 if silu else 0, W, B, T, D, w, b, n, *xs, *ys, st,
-                   _dense(state_out, "state_out", (B, W - 1, D), x.dtype, dev), 0, 0, 0, 0, 0, 0, 0, 0)
+    after = (B, W - 1, D)
+    so = dense(state_out, after, ty, dev.index) or _dense(state_out, "state_out", after, x.dtype, dev)
+    d = _CONV.pack(_CONV_SIZE, ty, 1 if silu else 0, W, B, T, D, w, b, n, *xs, *ys, st, so, 0, 0, 0, 0, 0, 0, 0, 0)
     _op("causal_conv")(d, dev, False, False)
     return out
 
@@ -267,7 +280,8 @@ def causal_conv_backward(dy, x, weight, bias=None, silu: bool = True, state=None
     dw = weight.new_empty((D, W))
     db = None if bias is None else bias.new_empty(D)
     d = _CONV.pack(_CONV_SIZE, ty, 1 if silu else 0, W, B, T, D, w, b, n, *xs, 0, 0, 0, st, 0,
-                   *_seq(dy, "dy", x.shape, x.dtype, dev), *ds, dw.data_ptr(), 0 if db is None else db.data_ptr())
+                   *(sequence(dy, x.shape, ty, dev.index) or _seq(dy, "dy", x.shape, x.dtype, dev)), *ds,
+                   dw.data_ptr(), 0 if db is None else db.data_ptr())
     _op("causal_conv")(d, dev, True, True)
     return out, dw, db
 
@@ -295,13 +309,18 @@ def _scan_parts(x, dt, A, B, C, D, z, dt_bias, state, lengths):
     shape, dev, f32, et = x.shape, x.device, torch.float32, x.dtype
     n, T, ch = shape
     N = A.shape[1]
-    bc = (n, T, N)
-    head = (_SCAN_SIZE, ty, n, T, ch, N, _dense(A, "A", (ch, N), f32, dev), _dense(D, "D", (ch,), f32, dev),
-            _dense(dt_bias, "dt_bias", (ch,), f32, dev), _dense(lengths, "lengths", (n,), torch.int32, dev),
-            _dense(state, "state", (n, ch, N), f32, dev))
-    return dev, (n, T, ch, N), head, (*_seq(x, "x", shape, et, dev), *_seq(dt, "dt", shape, et, dev),
-                                      *(_NONE if z is None else _seq(z, "z", shape, et, dev)),
-                                      *_seq(B, "B", bc, et, dev), *_seq(C, "C", bc, et, dev))
+    bc, per, states, i = (n, T, N), (ch,), (n, ch, N), dev.index
+    head = (_SCAN_SIZE, ty, n, T, ch, N, dense(A, (ch, N), _F32, i) or _dense(A, "A", (ch, N), f32, dev),
+            dense(D, per, _F32, i) or _dense(D, "D", per, f32, dev),
+            dense(dt_bias, per, _F32, i) or _dense(dt_bias, "dt_bias", per, f32, dev),
+            dense(lengths, (n,), _INT32, i) or _dense(lengths, "lengths", (n,), torch.int32, dev),
+            dense(state, states, _F32, i) or _dense(state, "state", states, f32, dev))
+    return dev, (n, T, ch, N), head, (*(sequence(x, shape, ty, i) or _seq(x, "x", shape, et, dev)),
+                                      *(sequence(dt, shape, ty, i) or _seq(dt, "dt", shape, et, dev)),
+                                      *(_NONE if z is None else
+                                        sequence(z, shape, ty, i) or _seq(z, "z", shape, et, dev)),
+                                      *(sequence(B, bc, ty, i) or _seq(B, "B", bc, et, dev)),
+                                      *(sequence(C, bc, ty, i) or _seq(C, "C", bc, et, dev)))
 
 
 _NO_SCAN_GRADS = (0,) * 21
@@ -317,8 +336,9 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, state=None, sta
     and channels in the call, which decide how time is cut."""
     dev, (n, T, ch, N), head, ins = _scan_parts(x, dt, A, B, C, D, z, dt_bias, state, lengths)
     out, ys = _fresh_seq(x, out, x.shape)
-    d = _SCAN.pack(*head, _dense(state_out, "state_out", (n, ch, N), torch.float32, dev), *ins, *ys,
-                   *_NO_SCAN_GRADS)
+    after = (n, ch, N)
+    so = dense(state_out, after, _F32, dev.index) or _dense(state_out, "state_out", after, torch.float32, dev)
+    d = _SCAN.pack(*head, so, *ins, *ys, *_NO_SCAN_GRADS)
     # (a call of few frames is one launch without scratch)
     _op("selective_scan")(d, dev, False, T > 32)
     return out
@@ -333,7 +353,8 @@ def selective_scan_backward(dy, x, dt, A, B, C, D=None, z=None, dt_bias=None, st
 
     g = ScanGrads(new(x), new(dt), new(A), new(B), new(C), new(D), new(z), new(dt_bias))
     wide, narrow = (T * ch, ch), (T * N, N)
-    d = _SCAN.pack(*head, 0, *ins, 0, 0, 0, *_seq(dy, "dy", x.shape, x.dtype, dev), g.dx.data_ptr(), *wide,
+    d = _SCAN.pack(*head, 0, *ins, 0, 0, 0,
+                   *(sequence(dy, x.shape, head[1], dev.index) or _seq(dy, "dy", x.shape, x.dtype, dev)), g.dx.data_ptr(), *wide,
                    g.ddt.data_ptr(), *wide, *(_NONE if g.dz is None else (g.dz.data_ptr(), *wide)), g.dB.data_ptr(),
                    *narrow, g.dC.data_ptr(), *narrow, g.dA.data_ptr(), 0 if g.dD is None else g.dD.data_ptr(),
                    0 if g.ddt_bias is None else g.ddt_bias.data_ptr())
@@ -355,8 +376,11 @@ def _mlp_parts(x, w_gate, w_up, activation):
     dev, shape, ws = x.device, x.shape, w_gate.shape
     if ws[0] != shape[-1]:
         raise _wrong("w_gate", w_gate, f"[{shape[-1]}][hidden]")
-    return dev, ws[1], (_MLP_SIZE, ty, act, 0, _count(shape), ws[0], ws[1], *_rows(x, "x", shape, x.dtype, dev),
-                        *_rows(w_gate, "w_gate", ws, x.dtype, dev), *_rows(w_up, "w_up", ws, x.dtype, dev))
+    i, et = dev.index, x.dtype
+    return dev, ws[1], (_MLP_SIZE, ty, act, 0, _count(shape), ws[0], ws[1],
+                        *(rows(x, shape, ty, i) or _rows(x, "x", shape, et, dev)),
+                        *(rows(w_gate, ws, ty, i) or _rows(w_gate, "w_gate", ws, et, dev)),
+                        *(rows(w_up, ws, ty, i) or _rows(w_up, "w_up", ws, et, dev)))
 
 
 def gated_mlp(x, w_gate, w_up, activation: str = "silu", out=None):
@@ -370,7 +394,7 @@ def gated_mlp(x, w_gate, w_up, activation: str = "silu", out=None):
         out = x.new_empty(shape)
         hp = out.data_ptr(), hidden
     else:
-        hp = _rows(out, "out", shape, x.dtype, dev)
+        hp = rows(out, shape, head[1], dev.index) or _rows(out, "out", shape, x.dtype, dev)
     d = _MLP.pack(*head, *hp, 0, 0, 0, 0, 0, 0, 0, 0)
     # (up to 16 rows take no scratch)
     _op("gated_mlp")(d, dev, False, head[4] > 16)
@@ -382,7 +406,9 @@ def gated_mlp_backward(dh, x, w_gate, w_up, activation: str = "silu"):
     again, so nothing is kept between the passes."""
     dev, hidden, head = _mlp_parts(x, w_gate, w_up, activation)
     dx, dg, du = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (x, w_gate, w_up))
-    d = _MLP.pack(*head, 0, 0, *_rows(dh, "dh", (*x.shape[:-1], hidden), x.dtype, dev), dx.data_ptr(), x.shape[-1],
+    shape = (*x.shape[:-1], hidden)
+    dhp = rows(dh, shape, head[1], dev.index) or _rows(dh, "dh", shape, x.dtype, dev)
+    d = _MLP.pack(*head, 0, 0, *dhp, dx.data_ptr(), x.shape[-1],
                   dg.data_ptr(), hidden, du.data_ptr(), hidden)
     _op("gated_mlp")(d, dev, True, True)
     return dx, dg, du
