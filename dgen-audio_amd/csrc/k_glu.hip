@@ -33,7 +33,7 @@
 // activations in the open); 20000 rows forward 272 us, 0.85 PFLOP/s.  fp32,
 // 8003 x 512 x 1365 forward 160 us, 140 TFLOP/s; 16000 x 512 x 1408 backward
 // 390, 287 and 350 us, 118 to 161 TFLOP/s (bound by the six products and the
-// splitting).  bf16, 8 x 512 x 1408 forward: 9 us, the latency of the launch
+// splitting).  bf16, 8 x 512 x 1408 forward: 5 us, the latency of the launch
 // and of one round of loads.
 #include "seq.h"
 
@@ -724,33 +724,34 @@ __global__ __launch_bounds__(256) void k_glu_join(const float* __restrict__ part
 
 // Forward for a few rows (single frames of some voices): the weights' reading
 // is all that counts, and its latency, so the vector unit multiplies.  A
-// workgroup owns 32 columns (16 lanes x 2); the quarter-waves of 16 waves take
-// every 64th k, each with all of its 8 loads of a round of 512 k's in flight
-// at once; the 64 sums meet in registers, then in LDS.  (64 columns a workgroup
-// leave most CUs idle: 512 x 1408, 8 rows: 11.8 us against 9.8.)
-constexpr int kFewRows = 8, kFewThreads = 1024, kFewCols = 32, kFewK = 512;
-constexpr int kFewLanes = kFewCols / 2, kFewSlices = kFewThreads / kFewLanes, kFewLoads = kFewK / kFewSlices;
-template <class E>
+// workgroup owns COLS columns (two a lane) of 8 rows; the 16 waves' slices take
+// every 64th or 128th k, each with all of its loads of a round of 512 k's in
+// flight at once (the next round's behind them cost registers: 5.9 us for 5.0
+// at 8 x 512 x 1408 bf16); the slices' sums meet by exchange in registers, then
+// in LDS.
+constexpr int kFewRows = 8, kFewThreads = 1024, kFewRound = 512;
+template <class E, int COLS>
 __global__ __launch_bounds__(kFewThreads) void k_glu_few(GluP<E> p) {
-  __shared__ __align__(16) float xs[kFewK][kFewRows];
-  __shared__ float red[16][kFewCols][2][kFewRows + 1];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, slice = threadIdx.x / kFewLanes;
-  const int64_t m0 = (int64_t)blockIdx.y * kFewRows, f = (int64_t)blockIdx.x * kFewCols + (lane % kFewLanes) * 2;
+  constexpr int LANES = COLS / 2, SLICES = kFewThreads / LANES, LOADS = kFewRound / SLICES, ROUND = kFewRound;
+  constexpr int XS = ROUND * kFewRows / kFewThreads;
+  __shared__ __align__(16) float xs[ROUND][kFewRows];
+  __shared__ float red[16][COLS][2][kFewRows + 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, slice = threadIdx.x / LANES;
+  const int64_t m0 = (int64_t)blockIdx.y * kFewRows, f = (int64_t)blockIdx.x * COLS + (lane % LANES) * 2;
   const bool two = f + 1 < p.N;
   const int64_t col = two ? f : f < p.N ? f : p.N - 1;  // (columns past the end are not stored)
-  float acc[2][2][kFewRows] = {};
-  for (int64_t k0 = 0; k0 < p.K; k0 += kFewK) {
-    float xv[kFewK * kFewRows / kFewThreads];
+  const E *g = p.n0 + col, *u = p.n1 + col;
+  float acc[2][2][kFewRows] = {}, xv[XS];
+  Vec<E, 2> w[LOADS][2];
+  auto load = [&](int64_t k0) {
 #pragma unroll
-    for (int i = 0; i < kFewK * kFewRows / kFewThreads; ++i) {
-      const int id = threadIdx.x + i * kFewThreads, m = id / kFewK, k = id % kFewK;
+    for (int i = 0; i < XS; ++i) {
+      const int id = threadIdx.x + i * kFewThreads, m = id / ROUND, k = id % ROUND;
       xv[i] = k0 + k < p.K && m0 + m < p.M ? to_f32(p.m0[(m0 + m) * p.mld0 + k0 + k]) : 0.f;
     }
-    Vec<E, 2> w[kFewLoads][2];
-    const E *g = p.n0 + col, *u = p.n1 + col;
 #pragma unroll
-    for (int i = 0; i < kFewLoads; ++i) {
-      const int64_t k = k0 + slice + kFewSlices * i, kc = k < p.K ? k : p.K - 1;  // (x is 0 past the end)
+    for (int i = 0; i < LOADS; ++i) {
+      const int64_t k = k0 + slice + SLICES * i, kc = k < p.K ? k : p.K - 1;
       if (two) {
         w[i][0] = *reinterpret_cast<const Vec<E, 2>*>(g + kc * p.nld0);
         w[i][1] = *reinterpret_cast<const Vec<E, 2>*>(u + kc * p.nld1);
@@ -759,20 +760,23 @@ __global__ __launch_bounds__(kFewThreads) void k_glu_few(GluP<E> p) {
         w[i][1].e[0] = w[i][1].e[1] = u[kc * p.nld1];
       }
     }
+  };
+  for (int64_t k0 = 0; k0 < p.K; k0 += ROUND) {
+    load(k0);
     if (k0 > 0) __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kFewK * kFewRows / kFewThreads; ++i) {
+    for (int i = 0; i < XS; ++i) {
       const int id = threadIdx.x + i * kFewThreads;
-      xs[id % kFewK][id / kFewK] = xv[i];
+      xs[id % ROUND][id / ROUND] = xv[i];
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kFewLoads; ++i) {
+    for (int i = 0; i < LOADS; ++i) {
       // (past the end the weights are a row inside, which may hold anything)
-      if (k0 + slice + kFewSlices * i >= p.K) continue;
+      if (k0 + slice + SLICES * i >= p.K) continue;
 #pragma unroll
       for (int m = 0; m < kFewRows; ++m) {
-        const float x = xs[slice + kFewSlices * i][m];
+        const float x = xs[slice + SLICES * i][m];
 #pragma unroll
         for (int a = 0; a < 2; ++a)
 #pragma unroll
@@ -780,21 +784,22 @@ __global__ __launch_bounds__(kFewThreads) void k_glu_few(GluP<E> p) {
       }
     }
   }
+  // over the wave's slices: a lane keeps, of four rows, 2 (its bit 4) + (its bit 5)
 #pragma unroll
   for (int a = 0; a < 2; ++a)
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int m = 0; m < kFewRows; ++m) {
-        float t = acc[a][b][m];
-        t += __shfl_xor(t, 16, 64);
-        t += __shfl_xor(t, 32, 64);
-        if (lane < kFewLanes) red[wave][lane * 2 + b][a][m] = t;
+      for (int m = 0; m < kFewRows; m += 4) {
+        const float* v = acc[a][b] + m;
+        float t = swap_add16(swap_add32(v[0], v[1]), swap_add32(v[2], v[3]));
+        if constexpr (LANES == 8) t += dpp<0x128>(t);  // row_ror:8
+        if ((lane & 15) < LANES) red[wave][lane % LANES * 2 + b][a][m + 2 * ((lane >> 4) & 1) + (lane >> 5)] = t;
       }
   __syncthreads();
-  if (threadIdx.x >= kFewCols * kFewRows) return;
-  const int c = threadIdx.x % kFewCols, m = threadIdx.x / kFewCols;
-  const int64_t n = (int64_t)blockIdx.x * kFewCols + c;
+  if (threadIdx.x >= COLS * kFewRows) return;
+  const int c = threadIdx.x % COLS, m = threadIdx.x / COLS;
+  const int64_t n = (int64_t)blockIdx.x * COLS + c;
   float s[2] = {0.f, 0.f}, slope;
 #pragma unroll
   for (int w = 0; w < 16; ++w) {
@@ -809,12 +814,17 @@ int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 int64_t tiles(int64_t n, int64_t of) { return (n + of - 1) / of; }
 
 // Forward by k_glu_few.  It reads the weights once more for every 8 rows and
-// multiplies on the vector unit; the tiles read them once and cost the same up
-// to 64 rows, fp32's three times bfloat16's.  512 x 1408 and 1024 x 2816, us
-// of a call, few / tiles: bfloat16, 16 rows 12 / 13 and 13 / 17, 24 rows 13 /
-// 13 and 24 / 17; fp32, 32 rows 12 / 26 and 28 / 48, 64 rows 19 / 26 and 42 /
-// 49, 96 rows 28 / 26 and 69 / 49.
-bool few(const dgen_hip_mlp& a) { return a.rows <= (a.type == DGEN_HIP_BF16 ? 16 : 64); }
+// multiplies on the vector unit, so it is taken while its workgroups (of 32
+// columns and 8 rows) are one round of the 256 CUs, two for fp32, whose tiles
+// take three times as long.  Kernels, us, few / tiles (whose time does not
+// change up to 128 rows): bfloat16, 512 x 1408, 16 rows 5 / 10, 40 (220
+// workgroups) 6 / 10, 48 (264) 9.9 / 10.3, 96 (528) 14 / 10.5; 1024 x 2816, 16
+// (176) 11 / 20, 48 (528) 27 / 20; 1024 x 16384, 8 (512) 28 / 26, 16 (1024) 53
+// / 25; 2048 x 512, 128 (256) 17 / 31; fp32, 512 x 1408, 64 (352) 13 / 26; 1024
+// x 8192, 16 (512) 30 / 48, 32 (1024) 56 / 48; 1024 x 2816, 96 (1056) 55 / 49.
+bool few(const dgen_hip_mlp& a) {
+  return a.rows <= 128 && tiles(a.hidden, 32) * tiles(a.rows, kFewRows) <= (a.type == DGEN_HIP_BF16 ? 256 : 512);
+}
 
 // bfloat16: packed operands and 256 x 256 tiles where the projections' tiles
 // come near to filling the chip's 256 CUs; else small tiles on the operands as
@@ -1033,8 +1043,13 @@ void launch_staged(const dgen_hip_mlp& a, bool backward, const Plan& p, hipStrea
   if (!backward) {
     q.out0 = (E*)a.h, q.old0 = a.h_stride;
     if (few(a)) {
-      const dim3 grid((unsigned)tiles(a.hidden, kFewCols), (unsigned)tiles(a.rows, kFewRows));
-      k_glu_few<E><<<grid, kFewThreads, 0, st>>>(q);
+      // 16 columns a workgroup while there is a CU for each workgroup, else 32
+      // (bf16, 16 / 32 columns, us: 8 x 512 x 1408, 88 of 16, 5.0 / 6.3; 8 x 1024
+      // x 2816, 176, 12.1 / 12.2; 16 x 1024 x 2816, 352, 19.6 / 12.1)
+      const int64_t groups = tiles(a.rows, kFewRows), cols = tiles(a.hidden, 16) * groups <= 256 ? 16 : 32;
+      const dim3 grid((unsigned)tiles(a.hidden, cols), (unsigned)groups);
+      if (cols == 16) k_glu_few<E, 16><<<grid, kFewThreads, 0, st>>>(q);
+      else k_glu_few<E, 32><<<grid, kFewThreads, 0, st>>>(q);
     } else {
       staged<E, kForward>(q, st);
     }

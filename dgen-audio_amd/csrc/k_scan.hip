@@ -75,10 +75,6 @@ __device__ __forceinline__ int live_of(const int32_t* __restrict__ lengths, int 
   return n < 0 ? 0 : n < T ? n : T;
 }
 
-template <int CTRL>
-__device__ __forceinline__ float dpp(float v) {
-  return __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(v), CTRL, 0xf, 0xf, true));
-}
 // The value that lane J of each quad holds.
 template <int J>
 __device__ __forceinline__ float quad(float v) { return dpp<J * 0x55>(v); }
@@ -441,14 +437,6 @@ __global__ __launch_bounds__(COLS * SEGS) void k_scan_carry(ScanP<E> p, int np) 
 // exchange: after the half-wave and row swaps a lane holds a quarter of the
 // values; those are summed over lane bits 2 and 3 by row rotations.  w[k] is
 // value index 4 k + 2 (lane bit 4) + (lane bit 5) (V = 2: lane bit 5).
-__device__ __forceinline__ float swap_add32(float a, float b) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-__device__ __forceinline__ float swap_add16(float a, float b) {
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
 template <int V>
 constexpr int kept() { return V >= 4 ? V / 4 : 1; }
 template <int V>

@@ -59,6 +59,21 @@ __device__ __forceinline__ void store_four(T* __restrict__ p, int valid, const f
   }
 }
 
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
+// Sums across the wave by exchange: each lane gets a's sum over the lanes that
+// differ in bit 5 (or 4) if that bit of its own is 0, else b's.
+__device__ __forceinline__ float swap_add32(float a, float b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float swap_add16(float a, float b) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
 // sigmoid(x) = 1 / (1 + e^-x): e^-x overflows to infinity for x < -88, whose
 // reciprocal is the right 0.
 __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + hw_exp(-x)); }

@@ -396,8 +396,8 @@ def gated_mlp(x, w_gate, w_up, activation: str = "silu", out=None):
     else:
         hp = rows(out, shape, head[1], dev.index) or _rows(out, "out", shape, x.dtype, dev)
     d = _MLP.pack(*head, *hp, 0, 0, 0, 0, 0, 0, 0, 0)
-    # (up to 16 rows take no scratch)
-    _op("gated_mlp")(d, dev, False, head[4] > 16)
+    # (up to 16 rows of a block that is not very wide take no scratch)
+    _op("gated_mlp")(d, dev, False, head[4] > 16 or hidden > 8192)
     return out
 
 
