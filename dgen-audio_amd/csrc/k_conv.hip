@@ -8,12 +8,12 @@
 // x; the weight and bias gradients are summed per thread over its tile, over
 // the workgroup's tiles in LDS, and over workgroups in a fixed order.
 //
-// Measured at 32 x 1000 x 1024 bf16, W = 4 (a large copy: 4.97 TB/s): forward
-// 33 us, 4.0 TB/s; backward 54 us with the partial rows, 3.6 TB/s.
-// The loads' latency is what is left: a wave's four channels a lane are 512
-// bytes a frame and tensor, with four frames in flight (eight: 37 and 63 us, by
-// their registers), and about half of the issue slots go to the sigmoid and the
-// window.
+// Measured at 32 x 1000 x 1024 bf16, W = 4, calls in a row on two sets of
+// operands (a large copy: 4.97 TB/s): forward 33 us, 4.0 TB/s; backward 54 us
+// with the partial rows, 3.6 TB/s.  The loads' latency is what is left: a
+// wave's four channels a lane are 512 bytes a frame and tensor, with four
+// frames in flight (eight: 37 and 63 us, by their registers), and about half of
+// the issue slots go to the sigmoid and the window.
 #include "seq.h"
 
 namespace dgen {
