@@ -5,7 +5,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_gpu_gated_mlp import TYPES, check_forward  # noqa: E402
+from test_gpu_gated_mlp import TYPES, check_backward, check_forward  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -17,3 +17,9 @@ pytestmark = pytest.mark.gpu
 @pytest.mark.parametrize("act", ["silu", "gelu"])
 def test_forward(gpu, rows, width, hidden, ty, act):
     check_forward(rows, width, hidden, ty, act)
+
+
+@pytest.mark.parametrize("rows,width,hidden", [(1, 64, 16416), (3, 40, 16390), (31, 64, 16416), (33, 64, 16416)])
+@pytest.mark.parametrize("ty", TYPES)
+def test_backward_of_few_rows_of_a_wide_block(gpu, rows, width, hidden, ty):
+    check_backward(rows, width, hidden, ty, "silu")
