@@ -104,7 +104,8 @@ class RecurrentDecoder:
     def forward(self, x, lengths=None, state=None, keep: bool = False):
         """Head pre-activations [batch][frames][controls] (float32) of features
         [batch][frames][features].  ``state`` (from :meth:`state`) is read and
-        moved on; with ``keep`` the result is (Z, saved) for :meth:`backward`."""
+        moved on; with ``keep`` the result is (Z, saved) for :meth:`backward`,
+        to which the state counts as given (a copy of it is kept)."""
         c, P = self.cfg, self.params
         if x.dim() != 3 or x.shape[2] != c.features:
             raise ValueError(f"features: [batch][frames][{c.features}] expected, got {tuple(x.shape)}")
@@ -118,6 +119,9 @@ class RecurrentDecoder:
             xz = _mm(y1, P[p + "xz"])
             u, z = xz[..., :c.inner], xz[..., c.inner:]
             conv, scan = (None, None) if state is None else state[i]
+            start = (conv, scan)
+            if keep and state is not None:  # (the calls below move it on in place)
+                start = (conv.clone(), scan.clone())
             v = Q.causal_conv(u, P[p + "conv"], P[p + "conv_bias"], state=conv, state_out=conv, lengths=lengths)
             q = _mm(v, P[p + "proj"])
             low, B, C = q[..., :c.rank], q[..., c.rank:c.rank + c.states], q[..., c.rank + c.states:]
@@ -129,7 +133,7 @@ class RecurrentDecoder:
             g = Q.gated_mlp(y2, P[p + "gate"], P[p + "up"], activation=c.activation)
             h = _mm(g, P[p + "down"])
             if keep:
-                saved.append((y1, r1, xz, v, q, dt, A, s, y2, r, g))
+                saved.append((y1, r1, xz, v, q, dt, A, s, y2, r, g, start))
         y, r = Q.rms_norm(h, P["norm"], residual=r)
         Z = _mm(y, P["heads"]).float() + P["heads_bias"]
         return (Z, (x, lengths, saved, y, r)) if keep else Z
@@ -143,7 +147,7 @@ class RecurrentDecoder:
         dr, G["norm"] = Q.rms_norm_backward(dy, r, P["norm"])
         for i in reversed(range(c.blocks)):
             p = f"{i}."
-            y1, r1, xz, v, q, dt, A, s, y2, r2, g = saved[i]
+            y1, r1, xz, v, q, dt, A, s, y2, r2, g, (conv, scan) = saved[i]
             # dr: of the stream after the block, hence of its last branch too
             dg, G[p + "down"] = _mm_grads(dr.to(c.dtype), g, P[p + "down"])
             dy2, G[p + "gate"], G[p + "up"] = Q.gated_mlp_backward(dg, y2, P[p + "gate"], P[p + "up"],
@@ -152,12 +156,12 @@ class RecurrentDecoder:
             ds, G[p + "out"] = _mm_grads(dr.to(c.dtype), s, P[p + "out"])
             low, B, C = q[..., :c.rank], q[..., c.rank:c.rank + c.states], q[..., c.rank + c.states:]
             t = Q.selective_scan_backward(ds, v, dt, A, B, C, D=P[p + "D"], z=xz[..., c.inner:],
-                                          dt_bias=P[p + "dt_bias"], lengths=lengths)
+                                          dt_bias=P[p + "dt_bias"], state=scan, lengths=lengths)
             G[p + "log_A"], G[p + "D"], G[p + "dt_bias"] = t.dA * A, t.dD, t.ddt_bias
             dlow, G[p + "dt"] = _mm_grads(t.ddt, low, P[p + "dt"])
             dv, G[p + "proj"] = _mm_grads(torch.cat([dlow, t.dB, t.dC], -1), v, P[p + "proj"])
             du, G[p + "conv"], G[p + "conv_bias"] = Q.causal_conv_backward(
-                dv + t.dx, xz[..., :c.inner], P[p + "conv"], P[p + "conv_bias"], lengths=lengths)
+                dv + t.dx, xz[..., :c.inner], P[p + "conv"], P[p + "conv_bias"], state=conv, lengths=lengths)
             dy1, G[p + "xz"] = _mm_grads(torch.cat([du, t.dz], -1), y1, P[p + "xz"])
             dr, G[p + "norm1"] = Q.rms_norm_backward(dy1, r1, P[p + "norm1"], ds=dr)
         _, G["in"] = _mm_grads(dr.to(c.dtype), x, P["in"])
