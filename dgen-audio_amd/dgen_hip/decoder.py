@@ -105,7 +105,9 @@ class RecurrentDecoder:
         """Head pre-activations [batch][frames][controls] (float32) of features
         [batch][frames][features].  ``state`` (from :meth:`state`) is read and
         moved on; with ``keep`` the result is (Z, saved) for :meth:`backward`,
-        to which the state counts as given (a copy of it is kept)."""
+        to which the state counts as given (a copy of it is kept).  Frames past
+        a clip's end pass through the parts that see one frame at a time, as any
+        others: a program pads with finite features and gives them no gradient."""
         c, P = self.cfg, self.params
         if x.dim() != 3 or x.shape[2] != c.features:
             raise ValueError(f"features: [batch][frames][{c.features}] expected, got {tuple(x.shape)}")
@@ -174,21 +176,28 @@ class RecurrentDecoder:
 
 
 def fit(decoder: RecurrentDecoder, x, target, steps: int, lr: float = 1e-3, lengths=None) -> list[float]:
-    """Adam on the mean squared error of Z over the sequences' frames; the
-    losses of the steps.  Parameters are kept in 32 bits and rounded to their
-    own type for each pass."""
+    """Adam on the mean squared error of Z over the sequences' own frames
+    (``lengths``: on the host or the device; what lies past a sequence's end
+    may be anything); the losses of the steps.  Parameters are kept in 32 bits
+    and rounded to their own type for each pass."""
     master = {k: v.float().clone().requires_grad_() for k, v in decoder.params.items()}
     opt = torch.optim.Adam(master.values(), lr=lr)
-    frames = torch.arange(x.shape[1], device=decoder.device)[None, :, None]
-    n = None if lengths is None else lengths.to(decoder.device)[:, None, None]
+    inside, count = None, target.numel()
+    if lengths is not None:
+        lengths = lengths.to(device=decoder.device, dtype=torch.int32)
+        x = x.to(decoder.device)
+        inside = (torch.arange(x.shape[1], device=decoder.device) < lengths[:, None])[..., None]
+        # (padded frames pass through the frame-wise parts: with finite values and no gradient they count for nothing)
+        x = torch.where(inside, x, 0.0)
+        count = max(1, int(inside.sum())) * target.shape[2]
     losses = []
     for _ in range(steps):
         Z, kept = decoder.forward(x, lengths=lengths, keep=True)
         d = Z - target
-        if n is not None:
-            d = torch.where(frames < n, d, 0.0)
-        losses.append(float(d.square().mean()))
-        grads = decoder.backward(d * (2.0 / d.numel()), kept)
+        if inside is not None:
+            d = torch.where(inside, d, 0.0)
+        losses.append(float(d.square().sum() / count))
+        grads = decoder.backward(d * (2.0 / count), kept)
         for k, p in master.items():
             p.grad = grads[k]
         opt.step()

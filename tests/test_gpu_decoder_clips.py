@@ -1,9 +1,10 @@
 """The recurrent control decoder trained on pieces of clips, which go on from a
-state.  Needs a GPU."""
+state, and fitted to padded ones.  Needs a GPU."""
 import pytest
 
 torch = pytest.importorskip("torch")
 
+from dgen_hip.decoder import fit  # noqa: E402
 from test_gpu_decoder import F64, norm, small  # noqa: E402
 
 pytestmark = pytest.mark.gpu
@@ -59,3 +60,25 @@ def test_gradients_of_a_piece_that_goes_on_from_a_state(gpu):
     assert torch.equal(dec.forward(x, state=again), Z)
     for (c, s), (cm, sm) in zip(again, moved):
         assert torch.equal(c, cm) and torch.equal(s, sm)
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+@pytest.mark.parametrize("device", ["cpu", "cuda"])
+def test_fit_takes_the_lengths_as_a_program_has_them(gpu, dtype, device):
+    """On the host or the device, in 32 or 64 bits; the loss is the mean over
+    the clips' own frames, whatever the padding holds."""
+    losses = []
+    for pad in (0, 13):
+        dec = small()
+        g = torch.Generator().manual_seed(10)
+        x, target = torch.randn(2, 30, 2, generator=g), torch.randn(2, 30, 9, generator=g)
+        x = torch.cat([x, torch.full((2, pad, 2), float("nan"))], 1)
+        target = torch.cat([target, torch.full((2, pad, 9), float("nan"))], 1).cuda()
+        losses.append(fit(dec, x, target, steps=4, lengths=torch.tensor([30, 11], dtype=dtype, device=device)))
+    for a, b in zip(*losses):
+        assert abs(a - b) <= 1e-5 * a, losses
+    dec = small()
+    Z = dec.forward(x[:, :30], lengths=torch.tensor([30, 11], dtype=torch.int32, device="cuda"))
+    d = (Z - target[:, :30]).square()
+    mean = (d[0].sum() + d[1, :11].sum()) / (41 * 9)
+    assert abs(losses[0][0] - mean.item()) <= 1e-5 * mean.item()
