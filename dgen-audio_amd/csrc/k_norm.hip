@@ -43,8 +43,8 @@ constexpr int norm_threads() { return TPR > 256 ? TPR : 256; }
 
 template <class TX, class TS, int TPR, int IT>
 __global__ __launch_bounds__(norm_threads<TPR>()) void k_rms_norm(
-    const TX* __restrict__ x, int64_t xld, const TS* res, int64_t rld, TX* __restrict__ y, int64_t yld, TS* s,
-    int64_t sld, const float* __restrict__ w, int64_t rows, int n, float inv_n, float eps) {
+    const TX* x, int64_t xld, const TS* res, int64_t rld, TX* y, int64_t yld, TS* s, int64_t sld,
+    const float* __restrict__ w, int64_t rows, int n, float inv_n, float eps) {
   constexpr int RPB = norm_threads<TPR>() / TPR;
   __shared__ float red[16];
   const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
@@ -82,8 +82,8 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_rms_norm(
 
 template <class TX, class TS, int TPR, int IT>
 __global__ __launch_bounds__(norm_threads<TPR>()) void k_rms_norm_bwd(
-    const TX* __restrict__ dy, int64_t dyld, const TS* __restrict__ s, int64_t sld, const TS* ds, int64_t dsld, TS* dx,
-    int64_t dxld, const float* __restrict__ w, float* __restrict__ parts, int64_t rows, int n, float inv_n, float eps) {
+    const TX* dy, int64_t dyld, const TS* s, int64_t sld, const TS* ds, int64_t dsld, TS* dx, int64_t dxld,
+    const float* __restrict__ w, float* __restrict__ parts, int64_t rows, int n, float inv_n, float eps) {
   constexpr int RPB = norm_threads<TPR>() / TPR;
   __shared__ float red[2][16];
   __shared__ float acc[RPB > 1 ? RPB : 1][RPB > 1 ? TPR * 4 : 1];

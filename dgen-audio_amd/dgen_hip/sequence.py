@@ -17,6 +17,13 @@ torch's allocator on that stream.  Nothing is recorded for autograd: a program
 calls the backward functions itself.  A wrong argument raises ``ValueError``, a
 failing launch ``HIPError``.
 
+Results that the caller gives a place for (``out``, ``sum_out``, ``state_out``)
+may lie over the operands: where the operator would overwrite what it still
+reads, it writes to a tensor of its own, which is copied there afterwards.
+What may be replaced in place without one: x, residual, ds, s and dy in the
+norms, x, dt and z in the scan, the state by ``state_out``.  Two results must
+not share memory.
+
 Clips of unequal length: ``lengths`` ([batch] int32) ends each sequence; later
 frames are not read, and their outputs and gradients are 0.  Streaming: the
 state that a call leaves (``state_out``) is the next call's ``state``, the
@@ -33,7 +40,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from ._tensor_args import dense, rows, sequence
+from ._tensor_args import covers, dense, rows, sequence
 from .runtime import HIPError, load_library
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
@@ -184,6 +191,16 @@ def _fresh_seq(like, out, shape):
                  or _seq(out, "out", shape, like.dtype, like.device))
 
 
+def _given(target, written):
+    """A result in the place that the caller gave."""
+    return written if target is written else target.copy_(written)
+
+
+def _two_results(a: str, x, b: str, y) -> None:
+    if y is not None and covers(0, x, y):
+        raise ValueError(f"{a} and {b}: the two results share memory")
+
+
 def _count(shape) -> int:
     n = 1
     for s in shape[:-1]:
@@ -205,18 +222,28 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-5, out=None, sum_out=None
     i = dev.index
     xp = rows(x, shape, ty, i) or _rows(x, "x", shape, x.dtype, dev)
     w = dense(weight, shape[-1:], _F32, i) or _dense(weight, "weight", shape[-1:], torch.float32, dev)
-    out, yp = _fresh(x, out, "out", shape)
+    y, yp = _fresh(x, out, "out", shape)
     rp = sp = _NO_ROWS
     st = ty
     if residual is not None:
         st = _type(residual, "residual")
         rp = rows(residual, shape, st, i) or _rows(residual, "residual", shape, residual.dtype, dev)
-        sum_out, sp = _fresh(residual, sum_out, "sum_out", shape)
+        s, sp = _fresh(residual, sum_out, "sum_out", shape)
+        if sum_out is not None and covers(2, s, residual, x, weight):
+            s, sp = _fresh(residual, None, "sum_out", shape)
     elif sum_out is not None:
         raise ValueError("sum_out: only with a residual")
+    if out is not None:
+        _two_results("out", out, "sum_out", sum_out)
+        if covers(2, out, x, residual, weight):
+            y, yp = _fresh(x, None, "out", shape)
     d = _NORM.pack(_NORM_SIZE, ty, st, eps, _count(shape), shape[-1], w, *xp, *rp, *yp, *sp, 0, 0, 0, 0, 0, 0, 0)
     _op("rms_norm")(d, dev, False, False)
-    return out if residual is None else (out, sum_out)
+    if out is not None:
+        y = _given(out, y)
+    if residual is None:
+        return y
+    return y, s if sum_out is None else _given(sum_out, s)
 
 
 def rms_norm_backward(dy, s, weight, ds=None, eps: float = 1e-5, out=None):
@@ -228,7 +255,9 @@ def rms_norm_backward(dy, s, weight, ds=None, eps: float = 1e-5, out=None):
     if s.dim() < 2:
         raise _wrong("s", s, "rows ([..., width])")
     i, width = dev.index, shape[-1:]
-    out, op = _fresh(s, out, "out", shape)
+    dx, op = _fresh(s, out, "out", shape)
+    if out is not None and covers(3, out, s, dy, ds, weight):
+        dx, op = _fresh(s, None, "out", shape)
     dw = s.new_empty(shape[-1], dtype=torch.float32)
     d = _NORM.pack(_NORM_SIZE, ty, st, eps, _count(shape), shape[-1],
                    dense(weight, width, _F32, i) or _dense(weight, "weight", width, torch.float32, dev),
@@ -237,7 +266,7 @@ def rms_norm_backward(dy, s, weight, ds=None, eps: float = 1e-5, out=None):
                    *(_NO_ROWS if ds is None else rows(ds, shape, st, i) or _rows(ds, "ds", shape, s.dtype, dev)),
                    *op, dw.data_ptr())
     _op("rms_norm")(d, dev, True, True)
-    return out, dw
+    return (dx if out is None else _given(out, dx)), dw
 
 
 # -------------------------------------------------------------- convolution
@@ -264,26 +293,37 @@ def causal_conv(x, weight, bias=None, silu: bool = True, state=None, state_out=N
     first are ``state`` ([batch][W-1][D], x's type, oldest first) or 0;
     ``state_out`` receives the last W-1 frames of each sequence."""
     W, dev, (ty, (B, T, D), w, b, n, xs, st) = _conv_parts(x, weight, bias, state, lengths)
-    out, ys = _fresh_seq(x, out, x.shape)
-    after = (B, W - 1, D)
+    y, ys = _fresh_seq(x, out, x.shape)
+    if out is not None:
+        _two_results("out", out, "state_out", state_out)
+        if covers(0, out, x, weight, bias, state, lengths):
+            y, ys = _fresh_seq(x, None, x.shape)
+    after, left = (B, W - 1, D), state_out
     so = dense(state_out, after, ty, dev.index) or _dense(state_out, "state_out", after, x.dtype, dev)
+    if so and covers(1, state_out, state, x, weight, bias, lengths):
+        left = torch.empty_like(state_out)
+        so = left.data_ptr()
     d = _CONV.pack(_CONV_SIZE, ty, 1 if silu else 0, W, B, T, D, w, b, n, *xs, *ys, st, so, 0, 0, 0, 0, 0, 0, 0, 0)
     _op("causal_conv")(d, dev, False, False)
-    return out
+    if left is not state_out:
+        state_out.copy_(left)
+    return y if out is None else _given(out, y)
 
 
 def causal_conv_backward(dy, x, weight, bias=None, silu: bool = True, state=None, lengths=None, out=None):
     """(dx, dweight, dbias) of ``causal_conv`` (dbias None without a bias);
     the state counts as given."""
     W, dev, (ty, (B, T, D), w, b, n, xs, st) = _conv_parts(x, weight, bias, state, lengths)
-    out, ds = _fresh_seq(x, out, x.shape)
+    dx, ds = _fresh_seq(x, out, x.shape)
+    if out is not None and covers(0, out, dy, x, weight, bias, state, lengths):
+        dx, ds = _fresh_seq(x, None, x.shape)
     dw = weight.new_empty((D, W))
     db = None if bias is None else bias.new_empty(D)
     d = _CONV.pack(_CONV_SIZE, ty, 1 if silu else 0, W, B, T, D, w, b, n, *xs, 0, 0, 0, st, 0,
                    *(sequence(dy, x.shape, ty, dev.index) or _seq(dy, "dy", x.shape, x.dtype, dev)), *ds,
                    dw.data_ptr(), 0 if db is None else db.data_ptr())
     _op("causal_conv")(d, dev, True, True)
-    return out, dw, db
+    return (dx if out is None else _given(out, dx)), dw, db
 
 
 # --------------------------------------------------------------------- scan
@@ -335,13 +375,22 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, state=None, sta
     Results of a sequence can differ in rounding with the number of sequences
     and channels in the call, which decide how time is cut."""
     dev, (n, T, ch, N), head, ins = _scan_parts(x, dt, A, B, C, D, z, dt_bias, state, lengths)
-    out, ys = _fresh_seq(x, out, x.shape)
-    after = (n, ch, N)
+    y, ys = _fresh_seq(x, out, x.shape)
+    if out is not None:
+        _two_results("out", out, "state_out", state_out)
+        if covers(3, out, x, dt, z, A, B, C, D, dt_bias, state, lengths):
+            y, ys = _fresh_seq(x, None, x.shape)
+    after, left = (n, ch, N), state_out
     so = dense(state_out, after, _F32, dev.index) or _dense(state_out, "state_out", after, torch.float32, dev)
+    if so and covers(1, state_out, state, x, dt, z, A, B, C, D, dt_bias, lengths):
+        left = torch.empty_like(state_out)
+        so = left.data_ptr()
     d = _SCAN.pack(*head, so, *ins, *ys, *_NO_SCAN_GRADS)
     # (a call of few frames is one launch without scratch)
     _op("selective_scan")(d, dev, False, T > 32)
-    return out
+    if left is not state_out:
+        state_out.copy_(left)
+    return y if out is None else _given(out, y)
 
 
 def selective_scan_backward(dy, x, dt, A, B, C, D=None, z=None, dt_bias=None, state=None, lengths=None) -> ScanGrads:
@@ -390,15 +439,16 @@ def gated_mlp(x, w_gate, w_up, activation: str = "silu", out=None):
     accurately as in float32."""
     dev, hidden, head = _mlp_parts(x, w_gate, w_up, activation)
     shape = (*x.shape[:-1], hidden)
-    if out is None:
-        out = x.new_empty(shape)
-        hp = out.data_ptr(), hidden
-    else:
+    h, hp = out, None
+    if out is not None:
         hp = rows(out, shape, head[1], dev.index) or _rows(out, "out", shape, x.dtype, dev)
+    if out is None or covers(0, out, x, w_gate, w_up):
+        h = x.new_empty(shape)
+        hp = h.data_ptr(), hidden
     d = _MLP.pack(*head, *hp, 0, 0, 0, 0, 0, 0, 0, 0)
     # (up to 16 rows of a block that is not very wide take no scratch)
     _op("gated_mlp")(d, dev, False, head[4] > 16 or hidden > 8192)
-    return out
+    return h if out is None else _given(out, h)
 
 
 def gated_mlp_backward(dh, x, w_gate, w_up, activation: str = "silu"):
