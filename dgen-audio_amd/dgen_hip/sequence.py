@@ -40,8 +40,12 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from ._tensor_args import covers, dense, rows, sequence
 from .runtime import HIPError, load_library
+
+try:
+    from ._tensor_args import covers, dense, rows, sequence
+except ImportError:  # the library was built without PyTorch's headers: the same in Python
+    from ._tensor_args_python import covers, dense, rows, sequence
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
 _F32, _INT32 = 0, 2  # as the native tests name them
