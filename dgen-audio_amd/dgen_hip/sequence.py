@@ -79,11 +79,26 @@ def _current_stream(index: int) -> int:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _current_stream)
 
 
+def _hip_runtimes() -> list[str]:
+    """The HIP runtimes that this process has loaded.  PyTorch brings its own,
+    which the library uses too if that is there first; if the library comes
+    first it takes the system's, and PyTorch loads a second one."""
+    try:
+        with open("/proc/self/maps") as maps:
+            return sorted({line.split()[-1] for line in maps if "/libamdhip64.so" in line})
+    except OSError:
+        return []
+
+
 class _Op:
     """One operator's C entries."""
 
     def __init__(self, name: str):
         L = load_library()
+        runtimes = _hip_runtimes()
+        if len(runtimes) > 1:
+            raise HIPError(f"two HIP runtimes in this process ({', '.join(runtimes)}): PyTorch's streams and memory are "
+                           "unknown to the other one; import torch (or dgen_hip.sequence) before the library is loaded")
         self.forward, self.backward = getattr(L, f"dgen_hip_{name}"), getattr(L, f"dgen_hip_{name}_backward")
         self.workspace = getattr(L, f"dgen_hip_{name}_workspace")
         self.error = L.dgen_hip_last_error
