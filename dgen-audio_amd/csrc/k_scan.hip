@@ -723,6 +723,7 @@ struct ScanShape {
 // whole / chunked: forward 128 blocks 138 / 95 us, 192 140 / 155, 256 141 /
 // 168; backward 256 blocks 531 / 476 us, 320 670 / 745.
 constexpr int64_t kFill = 1024, kFillBackward = 512, kAlone = 160, kAloneBackward = 288, kMinChunk = 32;
+static_assert(2 * kAloneBackward * (kChannels * 64 / 32) * 1024 < int64_t(1) << 32, "threads of the largest carry");
 // Chunks up to which, of up to 16 states, each joins the ones before it (and
 // after it, backward) by itself; more go through k_scan_carry.  Calls, us,
 // joined / carried: N = 16, forward 4 x 256 x 256 (8 chunks) 20 / 22, 2 x 1024
@@ -834,9 +835,10 @@ int scan_run(const dgen_hip_scan& a, bool backward, hipStream_t st, bool dry) {
   DGEN_REQUIRE(a.T >= 1 && a.T <= (1 << 24), "%s: T %lld outside [1, 2^24]", what, (long long)a.T);
   DGEN_REQUIRE(a.D >= 1 && a.D <= (1 << 20), "%s: D %lld outside [1, 2^20]", what, (long long)a.D);
   const ScanShape s = scan_shape(a, backward);
-  // (a launch takes fewer than 2^32 threads)
+  // (a launch takes fewer than 2^32 threads; the carry's is far from that, as
+  // time is cut only where sequences and channel blocks are few)
   DGEN_REQUIRE(s.nd * s.chunks * a.batch < (int64_t(1) << 23) && a.batch * ((a.T + 3) / 4) < (int64_t(1) << 31) &&
-                   s.nd * a.batch < (int64_t(1) << 31) && (a.D * s.NP + 31) / 32 * a.batch < (int64_t(1) << 20) &&
+                   s.nd * a.batch < (int64_t(1) << 31) &&
                    (!backward || a.batch * a.T * 2 * a.N < (int64_t(1) << 31)),
                "%s: batch %lld x T %lld x D %lld x N %lld is too large for one call", what, (long long)a.batch,
                (long long)a.T, (long long)a.D, (long long)a.N);
