@@ -760,22 +760,25 @@ ScanShape scan_shape(const dgen_hip_scan& a, bool backward) {
   return s;
 }
 
+// (a single frame's stride says nothing)
 template <class E>
-Rows<const E> in_rows(const dgen_hip_seq& v) { return {(const E*)v.data, v.stride_b, (int)v.stride_t}; }
-template <class E>
-Rows<E> out_rows(const dgen_hip_seq& v) { return {(E*)v.data, v.stride_b, (int)v.stride_t}; }
+Rows<E> rows_of(const dgen_hip_scan& a, const dgen_hip_seq& v) {
+  return {(E*)v.data, v.stride_b, a.T > 1 ? (int)v.stride_t : 0};
+}
 
 template <class E, int S>
 void scan_launch(const dgen_hip_scan& a, bool backward, const ScanShape& s, hipStream_t st) {
   float* ws = (float*)a.workspace;
+  auto in = [&](const dgen_hip_seq& v) { return rows_of<const E>(a, v); };
+  auto out = [&](const dgen_hip_seq& v) { return rows_of<E>(a, v); };
   ScanP<E> p{};
-  p.x = in_rows<E>(a.x), p.dt = in_rows<E>(a.dt), p.z = in_rows<E>(a.z), p.B = in_rows<E>(a.B), p.C = in_rows<E>(a.C);
+  p.x = in(a.x), p.dt = in(a.dt), p.z = in(a.z), p.B = in(a.B), p.C = in(a.C);
   p.A = a.A, p.skip = a.skip, p.bias = a.dt_bias, p.state = a.state, p.lengths = a.lengths;
   p.T = (int)a.T, p.D = (int)a.D, p.N = (int)a.N, p.chunk = (int)s.chunk, p.chunks = (int)s.chunks, p.nd = (int)s.nd;
   p.batch = (int)a.batch;
   p.walk = S <= kWalkStates && s.chunks > 1 && s.chunks <= kWalk;
   p.sums = ws, p.ends = p.sums + s.sums, p.gends = p.ends + s.ends;
-  if (!backward) p.y = out_rows<E>(a.y), p.state_out = a.state_out;
+  if (!backward) p.y = out(a.y), p.state_out = a.state_out;
   const dim3 grid((unsigned)(s.nd * s.chunks * a.batch));
   // (threads a state by the number of chunks, for runs of up to 16 or 32)
   auto carry = [&]() {
@@ -796,7 +799,7 @@ void scan_launch(const dgen_hip_scan& a, bool backward, const ScanShape& s, hipS
     }
     return;
   }
-  p.dy = in_rows<E>(a.dy), p.dx = out_rows<E>(a.dx), p.ddt = out_rows<E>(a.ddt), p.dz = out_rows<E>(a.dz);
+  p.dy = in(a.dy), p.dx = out(a.dx), p.ddt = out(a.ddt), p.dz = out(a.dz);
   p.ckpt = p.gends + s.ends, p.shared = p.ckpt + s.ckpt, p.parts = p.shared + s.shared;
   if (s.chunks > 1) {
     k_scan<E, S, kSummaryBoth><<<grid, kThreads, 0, st>>>(p);
@@ -806,7 +809,7 @@ void scan_launch(const dgen_hip_scan& a, bool backward, const ScanShape& s, hipS
   const uint32_t first = (uint32_t)((a.batch * a.T * 2 * a.N + kSumThreads - 1) / kSumThreads);
   const int64_t width = a.D * (a.N + 2);
   k_scan_join<E><<<dim3(first + (unsigned)((width + kSumCols - 1) / kSumCols)), kSumThreads, 0, st>>>(
-      p, out_rows<E>(a.dB), out_rows<E>(a.dC), first, {{a.dA, a.dskip, a.ddt_bias}, {a.D * a.N, a.D, a.D}}, width);
+      p, out(a.dB), out(a.dC), first, {{a.dA, a.dskip, a.ddt_bias}, {a.D * a.N, a.D, a.D}}, width);
 }
 
 template <class E>
@@ -844,7 +847,7 @@ int scan_run(const dgen_hip_scan& a, bool backward, hipStream_t st, bool dry) {
                (long long)a.T, (long long)a.D, (long long)a.N);
   DGEN_REQUIRE(a.A, "%s: null A", what);
   for (const dgen_hip_seq* v : {&a.x, &a.dt, &a.z, &a.B, &a.C, &a.y, &a.dy, &a.dx, &a.ddt, &a.dz, &a.dB, &a.dC})
-    DGEN_REQUIRE(v->stride_t < (1 << 26), "%s: stride of %lld between frames, at most 2^26", what,
+    DGEN_REQUIRE(a.T == 1 || v->stride_t < (1 << 26), "%s: stride of %lld between frames, at most 2^26", what,
                  (long long)v->stride_t);  // (a tile's offsets are 32 bits: 32 frames)
   const bool empty = a.batch == 0;
   for (const dgen_hip_seq* v : {&a.x, &a.dt, &a.B, &a.C})

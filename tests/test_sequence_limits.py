@@ -27,6 +27,29 @@ def test_scans_past_a_launch_are_refused(batch, T, D, N):
     assert workspace("selective_scan", scan_of(batch, T, D, N), 0)[0] == -1
 
 
+@pytest.mark.parametrize("T,taken", [(1, True), (2, False)])
+def test_the_stride_of_a_single_frame_says_nothing(T, taken):
+    """One frame out of a time-major recording of many voices."""
+    d = scan(batch=4, T=T, D=8, x=(AT, 8, 1 << 27), y=(AT, 40, 8))
+    assert (workspace("selective_scan", d, 0) == (0, 0)) is taken
+
+
+@pytest.mark.gpu
+def test_a_single_frame_with_a_far_stride(gpu):
+    torch = pytest.importorskip("torch")
+    g = torch.Generator().manual_seed(2)
+    B, D, N = 3, 40, 8
+    x, dt, Bm, Cm = (torch.randn(B, n, generator=g).cuda() for n in (D, D, N, N))
+    A = -torch.rand(D, N, generator=g).cuda()
+    far = [t.as_strided((B, 1, t.shape[1]), (t.shape[1], 1 << 40, 1)) for t in (x, dt, Bm, Cm)]
+    assert torch.equal(sequence.selective_scan(far[0], far[1], A, far[2], far[3]),
+                       sequence.selective_scan(x[:, None], dt[:, None], A, Bm[:, None], Cm[:, None]))
+    got = sequence.selective_scan_backward(far[0], far[0], far[1], A, far[2], far[3])
+    want = sequence.selective_scan_backward(x[:, None], x[:, None], dt[:, None], A, Bm[:, None], Cm[:, None])
+    for a, b in zip(got, want):
+        assert a is b is None or torch.equal(a, b)
+
+
 @pytest.mark.gpu
 def test_one_frame_of_many_voices(gpu):
     """As the halves of the voices, bit for bit."""
