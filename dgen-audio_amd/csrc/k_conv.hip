@@ -267,10 +267,11 @@ __global__ __launch_bounds__(kBwdGroups* kBwdTiles) void k_conv_bwd(
             }
             if (!in) d = 0.f;
             du[W - 1 + k][e] = d;
-            const float mine = own ? d : 0.f;
-            dbs[e] += mine;
+            if (in && own) {  // (0 times a frame before the end is no 0 where that is infinite)
+              dbs[e] += d;
 #pragma unroll
-            for (int q = 0; q < W; ++q) dw[q][e] = fmaf(mine, win[k + q][e], dw[q][e]);
+              for (int q = 0; q < W; ++q) dw[q][e] = fmaf(d, win[k + q][e], dw[q][e]);
+            }
           }
           // the frame that has all of its du now
           const int64_t to = t + k - (W - 1);
