@@ -2,8 +2,8 @@
 //
 // Per sequence and channel, N states with decays that depend on the input:
 // h[t][n] = exp(step[t] A[n]) h[t-1][n] + step[t] x[t] B[t][n], y = C.h.  Four
-// neighbouring lanes share a channel and hold N/4 states each (padded: A = B =
-// C = 0), so a wave has 16 channels and a workgroup of four waves 64.  The
+// neighbouring lanes share a channel and hold N/4 states each (padded by states
+// that stay 0), so a wave has 16 channels and a workgroup of four waves 64.  The
 // four lanes take four frames at a time: each evaluates softplus, gate and
 // loads of one of the four, and the others read its step by a quad
 // permutation; y is summed over the quad the same way.  B and C, which all
@@ -232,11 +232,21 @@ __device__ __forceinline__ void join_chunks(const ScanP<E>& p, const Place& w, c
 
 enum Mode { kWhole, kSummary, kReplay, kSummaryBoth };
 
+// What a padded state is fed: 0, as B = 0 does not keep its channel's infinity
+// out.  (Its decay is that of A = -1.)  Where whole lanes are padded, that is
+// one select a frame, else one a state: 32 x 1000 x 1024 bf16 forward, N = 16,
+// 12 and 13: 210, 212 and 225 us (209 and 214 without the selects).
+enum Pad { kNoPad, kLanes, kStates };
+template <int PAD, int S>
+__device__ __forceinline__ float fed(const bool (&own)[S], int s, float v) {
+  return PAD == kNoPad || own[PAD == kLanes ? 0 : s] ? v : 0.f;
+}
+
 // Forward: kWhole (one chunk: state to state_out), kReplay (from the state
 // that enters the chunk); kSummary: end state from zero and summed steps;
 // kSummaryBoth: the adjoint's too, accumulated forwards with the running
 // product of decays.
-template <class E, int S, int MODE>
+template <class E, int S, int MODE, int PAD>
 __global__ __launch_bounds__(kThreads) void k_scan(ScanP<E> p) {
   constexpr int NP = 4 * S, G = kTile / 4;
   constexpr bool OUT = MODE == kWhole || MODE == kReplay, ADJ = MODE == kSummaryBoth;
@@ -249,13 +259,15 @@ __global__ __launch_bounds__(kThreads) void k_scan(ScanP<E> p) {
   if (!OUT && w.begin >= w.live && !copy) return;  // a chunk past the sequence is left out
 
   float h[S], a2[S], prod[S], adj[S];
+  bool own[S];  // not a padded state
   const float bias = p.bias && w.on ? p.bias[w.d] : 0.f, skip = p.skip && w.on ? p.skip[w.d] : 0.f;
   const int64_t at = ((int64_t)(w.b * p.chunks + w.c) * p.D + w.d) * NP + w.q * S;
 #pragma unroll
   for (int s = 0; s < S; ++s) {
     const int n = w.q * S + s;
-    const bool real = w.on && n < p.N;
-    a2[s] = real ? p.A[(int64_t)w.d * p.N + n] * kLog2e : 0.f;
+    own[s] = n < p.N;
+    const bool real = w.on && own[s];
+    a2[s] = real ? p.A[(int64_t)w.d * p.N + n] * kLog2e : -kLog2e;
     h[s] = 0.f;
     if ((MODE == kWhole || copy) && p.state && real) h[s] = p.state[((int64_t)w.b * p.D + w.d) * p.N + n];
     prod[s] = 1.f;
@@ -319,11 +331,11 @@ __global__ __launch_bounds__(kThreads) void k_scan(ScanP<E> p) {
 #pragma unroll
         for (int s = 0; s < S; ++s) {
           const float a = __builtin_amdgcn_exp2f(sj * a2[s]);
-          h[s] = fmaf(a, h[s], uj * bv[s]);
+          h[s] = fmaf(a, h[s], fed<PAD>(own, s, uj) * bv[s]);
           if (OUT) yj = fmaf(cv[s], h[s], yj);
           if (ADJ) {
             prod[s] *= a;
-            adj[s] = fmaf(prod[s] * cv[s], dj, adj[s]);
+            adj[s] = fmaf(prod[s] * cv[s], fed<PAD>(own, s, dj), adj[s]);
           }
         }
         y4[J] = yj;
@@ -333,7 +345,8 @@ __global__ __launch_bounds__(kThreads) void k_scan(ScanP<E> p) {
       frame(std::integral_constant<int, 2>{});
       frame(std::integral_constant<int, 3>{});
       const float y = OUT ? quad_sums(y4, odd, upper) : 0.f;
-      if (OUT && ok) (yrow + (int64_t)(t0 + 4 * g) * p.y.t)[yat] = from_f32<E>(fmaf(skip, cx[g], y) * gate);
+      const float through = p.skip ? cx[g] : 0.f;
+      if (OUT && ok) (yrow + (int64_t)(t0 + 4 * g) * p.y.t)[yat] = from_f32<E>(fmaf(skip, through, y) * gate);
     };
     // a whole tile of whole channels in one piece, without a branch (but with
     // the adjoint's sums one piece takes too many registers)
@@ -386,7 +399,7 @@ __global__ __launch_bounds__(COLS * SEGS) void k_scan_carry(ScanP<E> p, int np) 
   const int64_t d = on ? j / np : 0;
   const int n = on ? (int)(j % np) : 0;
   const bool real = on && n < p.N;
-  const float a2 = real ? p.A[d * p.N + n] * kLog2e : 0.f;
+  const float a2 = real ? p.A[d * p.N + n] * kLog2e : -kLog2e;
   const int live = live_of(p.lengths, b, p.T), used = (live + p.chunk - 1) / p.chunk;
   const int run = (p.chunks + SEGS - 1) / SEGS, lo = seg * run, hi = lo + run < used ? lo + run : used;
   float* e = ends + (int64_t)b * p.chunks * per + j;
@@ -457,7 +470,7 @@ __device__ __forceinline__ void channel_sum(const float (&v)[V], float (&w)[kept
   }
 }
 
-template <class E, int S>
+template <class E, int S, int PAD>
 __global__ __launch_bounds__(kThreads, S <= 4 ? 2 : 1) void k_scan_bwd(ScanP<E> p) {
   constexpr int NP = 4 * S, TL = bwd_tile<S>(), G = TL / 4;
   __shared__ __align__(16) float bc[2][TL * 2 * NP];
@@ -470,13 +483,15 @@ __global__ __launch_bounds__(kThreads, S <= 4 ? 2 : 1) void k_scan_bwd(ScanP<E> 
   const int tiles = w.live > w.begin ? (w.live - w.begin + TL - 1) / TL : 0;
 
   float h[S], a[S], g[S], dA[S];
+  bool own[S];
   const float bias = p.bias && w.on ? p.bias[w.d] : 0.f, skip = p.skip && w.on ? p.skip[w.d] : 0.f;
   const int64_t at = ((int64_t)(w.b * p.chunks + w.c) * p.D + w.d) * NP + w.q * S;
 #pragma unroll
   for (int s = 0; s < S; ++s) {
     const int n = w.q * S + s;
-    const bool real = w.on && n < p.N;
-    a[s] = real ? p.A[(int64_t)w.d * p.N + n] : 0.f;
+    own[s] = n < p.N;
+    const bool real = w.on && own[s];
+    a[s] = real ? p.A[(int64_t)w.d * p.N + n] : -1.f;
     h[s] = (p.chunks == 1 || walk) && p.state && real ? p.state[((int64_t)w.b * p.D + w.d) * p.N + n] : 0.f;
     g[s] = 0.f;
     dA[s] = 0.f;
@@ -488,6 +503,10 @@ __global__ __launch_bounds__(kThreads, S <= 4 ? 2 : 1) void k_scan_bwd(ScanP<E> 
     const int used = (w.frames + p.chunk - 1) / p.chunk;
     join_chunks<E, S>(p, w, p.ends, 0, w.c, 1, a2, h);
     join_chunks<E, S>(p, w, p.gends, used - 1, used - 1 - w.c, -1, a2, g);
+    if (!w.on) {
+#pragma unroll
+      for (int s = 0; s < S; ++s) h[s] = g[s] = 0.f;
+    }
   } else if (p.chunks > 1 && tiles > 0 && w.on) {
     read_states<S>(p.ends + at, h);
     read_states<S>(p.gends + at, g);
@@ -529,7 +548,8 @@ __global__ __launch_bounds__(kThreads, S <= 4 ? 2 : 1) void k_scan_bwd(ScanP<E> 
           float bv[S];
           read_states<S>(lds + (4 * k + J) * 2 * NP + w.q * S, bv);
 #pragma unroll
-          for (int s = 0; s < S; ++s) h[s] = fmaf(__builtin_amdgcn_exp2f(sj * a[s]), h[s], uj * bv[s]);
+          for (int s = 0; s < S; ++s)
+            h[s] = fmaf(__builtin_amdgcn_exp2f(sj * a[s]), h[s], fed<PAD>(own, s, uj) * bv[s]);
         };
         frame(std::integral_constant<int, 0>{});
         frame(std::integral_constant<int, 1>{});
@@ -562,7 +582,7 @@ __global__ __launch_bounds__(kThreads, S <= 4 ? 2 : 1) void k_scan_bwd(ScanP<E> 
     bcv.store(lds);
     float cx[G], cz[G], cdy[G], step[G], slope[G], u[G], up[G], y[G];
 #pragma unroll
-    for (int s = 0; s < S; ++s) h[s] = hn[s];
+    for (int s = 0; s < S; ++s) h[s] = w.on ? hn[s] : 0.f;
 #pragma unroll
     for (int k = 0; k < G; ++k) {
       const bool ok = w.on && t0 + 4 * k + w.q < w.live;
@@ -593,7 +613,7 @@ __global__ __launch_bounds__(kThreads, S <= 4 ? 2 : 1) void k_scan_bwd(ScanP<E> 
         for (int s = 0; s < S; ++s) {
           const float e = __builtin_amdgcn_exp2f(sj * a[s]);
           as[4 * k + J][s] = e;
-          h[s] = fmaf(e, h[s], uj * bv[s]);
+          h[s] = fmaf(e, h[s], fed<PAD>(own, s, uj) * bv[s]);
           yj = fmaf(cv[s], h[s], yj);
         }
         y4[J] = yj;
@@ -619,7 +639,7 @@ __global__ __launch_bounds__(kThreads, S <= 4 ? 2 : 1) void k_scan_bwd(ScanP<E> 
         read_states<S>(hs[f][threadIdx.x], hb);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-          g[s] = fmaf(cv[s], dj, g[s]);
+          g[s] = fmaf(cv[s], fed<PAD>(own, s, dj), g[s]);
           v[s] = g[s] * uj;       // dB
           v[S + s] = h[s] * dj;   // dC
           gbj = fmaf(g[s], bv[s], gbj);
@@ -651,11 +671,12 @@ __global__ __launch_bounds__(kThreads, S <= 4 ? 2 : 1) void k_scan_bwd(ScanP<E> 
         const float draw = fmaf(gb, cx[k], ga) * slope[k];
         dbias += draw;
         dskip = fmaf(up[k], cx[k], dskip);
-        (dxr + (int64_t)(t0 + 4 * k) * p.dx.t)[dxat] = from_f32<E>(fmaf(step[k], gb, skip * up[k]));
+        const float dthrough = p.skip ? skip * up[k] : 0.f, through = p.skip ? cx[k] : 0.f;
+        (dxr + (int64_t)(t0 + 4 * k) * p.dx.t)[dxat] = from_f32<E>(fmaf(step[k], gb, dthrough));
         (ddtr + (int64_t)(t0 + 4 * k) * p.ddt.t)[ddtat] = from_f32<E>(draw);
         if (p.z.p)
           (dzr + (int64_t)(t0 + 4 * k) * p.dz.t)[dzat] =
-              from_f32<E>(cdy[k] * fmaf(skip, cx[k], y[k]) * silu_grad(cz[k], sigmoid(cz[k])));
+              from_f32<E>(cdy[k] * fmaf(skip, through, y[k]) * silu_grad(cz[k], sigmoid(cz[k])));
       }
     }
     __syncthreads();
@@ -766,7 +787,7 @@ Rows<E> rows_of(const dgen_hip_scan& a, const dgen_hip_seq& v) {
   return {(E*)v.data, v.stride_b, a.T > 1 ? (int)v.stride_t : 0};
 }
 
-template <class E, int S>
+template <class E, int S, int PAD>
 void scan_launch(const dgen_hip_scan& a, bool backward, const ScanShape& s, hipStream_t st) {
   float* ws = (float*)a.workspace;
   auto in = [&](const dgen_hip_seq& v) { return rows_of<const E>(a, v); };
@@ -791,35 +812,42 @@ void scan_launch(const dgen_hip_scan& a, bool backward, const ScanShape& s, hipS
   };
   if (!backward) {
     if (s.chunks == 1) {
-      k_scan<E, S, kWhole><<<grid, kThreads, 0, st>>>(p);
+      k_scan<E, S, kWhole, PAD><<<grid, kThreads, 0, st>>>(p);
     } else {
-      k_scan<E, S, kSummary><<<grid, kThreads, 0, st>>>(p);
+      k_scan<E, S, kSummary, PAD><<<grid, kThreads, 0, st>>>(p);
       if (!p.walk) carry();
-      k_scan<E, S, kReplay><<<grid, kThreads, 0, st>>>(p);
+      k_scan<E, S, kReplay, PAD><<<grid, kThreads, 0, st>>>(p);
     }
     return;
   }
   p.dy = in(a.dy), p.dx = out(a.dx), p.ddt = out(a.ddt), p.dz = out(a.dz);
   p.ckpt = p.gends + s.ends, p.shared = p.ckpt + s.ckpt, p.parts = p.shared + s.shared;
   if (s.chunks > 1) {
-    k_scan<E, S, kSummaryBoth><<<grid, kThreads, 0, st>>>(p);
+    k_scan<E, S, kSummaryBoth, PAD><<<grid, kThreads, 0, st>>>(p);
     if (!p.walk) carry();
   }
-  k_scan_bwd<E, S><<<grid, kThreads, 0, st>>>(p);
+  k_scan_bwd<E, S, PAD><<<grid, kThreads, 0, st>>>(p);
   const uint32_t first = (uint32_t)((a.batch * a.T * 2 * a.N + kSumThreads - 1) / kSumThreads);
   const int64_t width = a.D * (a.N + 2);
   k_scan_join<E><<<dim3(first + (unsigned)((width + kSumCols - 1) / kSumCols)), kSumThreads, 0, st>>>(
       p, out(a.dB), out(a.dC), first, {{a.dA, a.dskip, a.ddt_bias}, {a.D * a.N, a.D, a.D}}, width);
 }
 
+template <class E, int S>
+void scan_padded(const dgen_hip_scan& a, bool backward, const ScanShape& s, hipStream_t st) {
+  if (a.N == 4 * S) scan_launch<E, S, kNoPad>(a, backward, s, st);
+  else if (a.N % S == 0) scan_launch<E, S, kLanes>(a, backward, s, st);
+  else if constexpr (S > 1) scan_launch<E, S, kStates>(a, backward, s, st);
+}
+
 template <class E>
 void scan_states(const dgen_hip_scan& a, bool backward, const ScanShape& s, hipStream_t st) {
   switch (s.S) {
-    case 1: return scan_launch<E, 1>(a, backward, s, st);
-    case 2: return scan_launch<E, 2>(a, backward, s, st);
-    case 4: return scan_launch<E, 4>(a, backward, s, st);
-    case 8: return scan_launch<E, 8>(a, backward, s, st);
-    default: return scan_launch<E, 16>(a, backward, s, st);
+    case 1: return scan_padded<E, 1>(a, backward, s, st);
+    case 2: return scan_padded<E, 2>(a, backward, s, st);
+    case 4: return scan_padded<E, 4>(a, backward, s, st);
+    case 8: return scan_padded<E, 8>(a, backward, s, st);
+    default: return scan_padded<E, 16>(a, backward, s, st);
   }
 }
 

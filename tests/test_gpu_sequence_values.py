@@ -39,3 +39,45 @@ def test_weight_gradients_of_a_convolution_with_an_infinite_frame(gpu, T, at, ty
     _, got, _ = Q.causal_conv_backward(dy.cuda(), x.cuda(), w.cuda(), silu=False, lengths=lengths)
     assert torch.isinf(dw).any() and not torch.isnan(dw).any()
     alike(got, dw, "dweight")
+
+
+@pytest.mark.parametrize("N", [1, 3, 5, 12, 16, 33])
+@pytest.mark.parametrize("T", [9, 100, 1100])
+@pytest.mark.parametrize("which", ["x", "dt"])
+def test_scan_with_an_infinite_value(gpu, N, T, which):
+    """An infinite input, or step, makes its channel infinite from that frame
+    on, whatever the number of states."""
+    B, D, at = 2, 5, T // 2 + 1
+    g = torch.Generator().manual_seed(N + T)
+    x, Bm, Cm = (torch.rand(B, T, n, generator=g) + 0.5 for n in (D, N, N))
+    dt, A = torch.randn(B, T, D, generator=g) - 2.0, -(torch.rand(D, N, generator=g) + 0.1)
+    (x if which == "x" else dt)[1, at, 3] = INF
+    h, ys = torch.zeros(B, D, N, dtype=F64), []
+    step = torch.nn.functional.softplus(dt.to(F64), threshold=1e9)
+    for t in range(T):
+        h = torch.exp(step[:, t, :, None] * A.to(F64)) * h + (step[:, t] * x[:, t].to(F64))[..., None] * Bm[:, t, None].to(F64)
+        ys.append((h * Cm[:, t, None].to(F64)).sum(-1))
+    want = torch.stack(ys, 1)
+    assert torch.isinf(want[1, at:, 3]).all() and not torch.isnan(want).any()
+    after = torch.empty(B, D, N, device="cuda")
+    y = Q.selective_scan(x.cuda(), dt.cuda(), A.cuda(), Bm.cuda(), Cm.cuda(), state_out=after)
+    alike(y, want, "y", rtol=1e-4)
+    alike(after, h, "state", rtol=1e-4)
+
+
+@pytest.mark.parametrize("N", [3, 12, 16])
+def test_scan_gradients_beside_an_infinite_channel(gpu, N):
+    """The last channel's states are infinite from the middle on: its gradients
+    and the shared ones are infinite as the formula's, the other channels' are
+    numbers."""
+    B, T, D, at = 1, 48, 5, 20
+    g = torch.Generator().manual_seed(N)
+    x, Bm, Cm, dy = (torch.rand(B, T, n, generator=g) + 0.5 for n in (D, N, N, D))
+    dt, A = torch.randn(B, T, D, generator=g) - 2.0, -(torch.rand(D, N, generator=g) + 0.1)
+    x[0, at, D - 1] = INF
+    got = Q.selective_scan_backward(dy.cuda(), x.cuda(), dt.cuda(), A.cuda(), Bm.cuda(), Cm.cuda())
+    # dC[t] = sum over channels of h[t] dy[t]
+    dC = got.dC[0].cpu()
+    assert torch.isfinite(dC[:at]).all() and (dC[at:] == INF).all()
+    assert torch.isfinite(got.dx[..., :D - 1]).all() and torch.isfinite(got.ddt[..., :D - 1]).all()
+    assert torch.isfinite(got.dx).all() and torch.isfinite(got.dA[:D - 1]).all()
