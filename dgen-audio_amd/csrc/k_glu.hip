@@ -75,8 +75,11 @@ __device__ __forceinline__ float act_of(int act, float v, float& slope) {
     slope = silu_grad(v, p);
     return v * p;
   }
-  const float v2 = v * v, p = sigmoid(kGeluA * v * fmaf(kGeluB, v2, 1.f));
-  slope = p * fmaf(v * (1.f - p), kGeluA * fmaf(3.f * kGeluB, v2, 1.f), 1.f);
+  // (past 16 the sigmoid is 0 or 1 to the last bit, and so is the slope: the
+  // clamp keeps the powers of v from overflowing into 0 times infinity)
+  const float c = v > 16.f ? 16.f : v < -16.f ? -16.f : v;  // (NaN stays)
+  const float c2 = c * c, p = sigmoid(kGeluA * c * fmaf(kGeluB, c2, 1.f));
+  slope = p * fmaf(c * (1.f - p), kGeluA * fmaf(3.f * kGeluB, c2, 1.f), 1.f);
   return v * p;
 }
 

@@ -55,7 +55,8 @@ def test_scan_with_an_infinite_value(gpu, N, T, which):
     h, ys = torch.zeros(B, D, N, dtype=F64), []
     step = torch.nn.functional.softplus(dt.to(F64), threshold=1e9)
     for t in range(T):
-        h = torch.exp(step[:, t, :, None] * A.to(F64)) * h + (step[:, t] * x[:, t].to(F64))[..., None] * Bm[:, t, None].to(F64)
+        u = (step[:, t] * x[:, t].to(F64))[..., None] * Bm[:, t, None].to(F64)
+        h = torch.exp(step[:, t, :, None] * A.to(F64)) * h + u
         ys.append((h * Cm[:, t, None].to(F64)).sum(-1))
     want = torch.stack(ys, 1)
     assert torch.isinf(want[1, at:, 3]).all() and not torch.isnan(want).any()
@@ -81,3 +82,38 @@ def test_scan_gradients_beside_an_infinite_channel(gpu, N):
     assert torch.isfinite(dC[:at]).all() and (dC[at:] == INF).all()
     assert torch.isfinite(got.dx[..., :D - 1]).all() and torch.isfinite(got.ddt[..., :D - 1]).all()
     assert torch.isfinite(got.dx).all() and torch.isfinite(got.dA[:D - 1]).all()
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("ty", [torch.float32, torch.bfloat16])
+def test_slopes_of_the_activations_far_out(gpu, act, ty):
+    """There the slope is 0 or 1 (powers of the argument in GELU's overflow)."""
+    x = torch.tensor([[-1e14], [-1e8], [-1e7], [1e7], [1e8], [1e14]], dtype=ty).repeat(30, 1)
+    wg, wu = torch.full((1, 5), 1e6, dtype=ty), torch.full((1, 5), 1e-14, dtype=ty)
+    dh = torch.ones(len(x), 5, dtype=ty)
+    dx, dwg, dwu = Q.gated_mlp_backward(dh.cuda(), x.cuda(), wg.cuda(), wu.cuda(), activation=act)
+    a, b, c = x.to(F64), wg.to(F64), wu.to(F64)
+    on = (a > 0).to(F64)
+    dg, du = a @ c * on, a @ b * on
+    rtol = 2.0 ** -6 if ty == torch.bfloat16 else 1e-5  # bfloat16: three roundings of 2^-8
+    alike(dx, dg @ b.T + du @ c.T, "dx", rtol, 0.0)
+    alike(dwg, a.T @ dg, "dw_gate", rtol, 0.0)
+    alike(dwu, a.T @ du, "dw_up", rtol, 0.0)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("rows", [3, 150])
+@pytest.mark.parametrize("ty", [torch.float32, torch.bfloat16])
+def test_a_value_that_is_none_stays_so(gpu, act, rows, ty):
+    """NaN in a row reaches that row's results and gradients and the weights'
+    gradients, and no other row."""
+    g = torch.Generator().manual_seed(rows)
+    x, wg, wu = (torch.randn(*s, generator=g).to(ty) for s in ((rows, 20), (20, 30), (20, 30)))
+    dh = torch.randn(rows, 30, generator=g).to(ty)
+    x[1, 4] = float("nan")
+    h = Q.gated_mlp(x.cuda(), wg.cuda(), wu.cuda(), activation=act).isnan().cpu()
+    grads = Q.gated_mlp_backward(dh.cuda(), x.cuda(), wg.cuda(), wu.cuda(), activation=act)
+    dx, dwg, dwu = (t.isnan().cpu() for t in grads)
+    for t in (h, dx):
+        assert t[1].all() and not t[0].any() and not t[2:].any()
+    assert dwg.all() and dwu.all()
