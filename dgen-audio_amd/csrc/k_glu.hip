@@ -16,7 +16,9 @@
 // rounded to bfloat16 between the products, as the operands are).  fp32
 // operands are split exactly into three bfloat16 parts on the way to LDS, and
 // the six partial products down to 2^-16 are accumulated in fp32, as accurate
-// as fp32 products (see k_gemm.hip).
+// as fp32 products (see k_gemm.hip).  An infinity, or a number past the largest
+// bfloat16, has no such parts: its products come out as NaN, and what does is
+// formed again from the operands as they are.
 //
 // Three kernels: k_glu_direct, bfloat16, 256 x 256 tiles on operands that lie
 // in whole 16-byte chunks (packed first where they do not); k_glu, operands of
@@ -257,6 +259,51 @@ __device__ __forceinline__ void finish(const GluP<E>& p, const floatx16 (&acc)[N
   }
 }
 
+// fp32 products that came out as NaN once more, on the vector unit, from the
+// operands in memory.  cols(i, k) and rows(j, k): the lane's address of the
+// elements at k of the first of fragment i's columns (consecutive ones nstep()
+// apart, `left(i)` of them in the operand) and of its row of fragment j;
+// steps(f) calls f(k from, k to, second segment) for the wave's reduction.
+// For infinities; a tile without NaN passes by.  (8003 x 512 x 1365 forward:
+// 163 us, with an infinity in a row 1.4 ms, of NaN all over 6.8.)
+template <int NF, int MF, class Cols, class Rows, class Left, class Stride, class Steps>
+__device__ __forceinline__ void again(floatx16 (&acc)[NF][MF], Cols cols, Rows rows, Left left, Stride nstep,
+                                      Steps steps) {
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < NF; ++i)
+#pragma unroll
+    for (int j = 0; j < MF; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) bad |= __builtin_isunordered(acc[i][j][r], acc[i][j][r + 1]);
+  if (!__any(bad)) return;
+#pragma unroll
+  for (int i = 0; i < NF; ++i)
+#pragma unroll
+    for (int j = 0; j < MF; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {  // (four at a time: few registers beside the accumulators)
+        const int64_t last = left(i) - 1;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        steps([&](int64_t from, int64_t to, bool second) {
+#pragma unroll 1
+          for (int64_t k = from; k < to; ++k) {
+            const float m = *rows(j, k, second), *const p = cols(i, k, second);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int64_t c = 8 * q + e;
+              sum[e] = fmaf(p[(c < last ? c : last) * nstep(second)], m, sum[e]);
+            }
+          }
+        });
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float v = acc[i][j][4 * q + e];
+          acc[i][j][4 * q + e] = v != v ? sum[e] : v;
+        }
+      }
+}
+
 // ----------------------------------------------------------------- kernel
 // Tile of this workgroup.  Consecutive workgroups go to the eight XCDs in
 // turn, so each XCD takes a run of consecutive tiles; a run goes through
@@ -278,7 +325,7 @@ __device__ __forceinline__ TileAt tile_at(const Params& p) {
 
 // BM x BN: output rows and operand columns of a tile; WM x WN: of a wave.
 template <class E, int BM, int BN, int WM, int WN, int BK, int USE>
-__global__ __launch_bounds__(kThreads) void k_glu(GluP<E> p) {
+__global__ __launch_bounds__(kThreads, sizeof(E) == 2 ? 1 : BM == 64 && USE != kDw ? 4 : 2) void k_glu(GluP<E> p) {
   constexpr int P = planes<E>(), NF = WN / 32, MF = WM / 32;
   constexpr bool PAIR = USE == kForward || USE == kProject;
   constexpr bool NKC = USE == kDx, MKC = USE != kDw;
@@ -380,7 +427,33 @@ __global__ __launch_bounds__(kThreads) void k_glu(GluP<E> p) {
     compute(lds);
   }
 
-  finish<E, USE, NF, MF>(p, acc, m0 + wm * WM, n0 + (PAIR ? wn * (WN / 2) : wn * WN), split, mat);
+  const int64_t mb = m0 + wm * WM, nb = n0 + (PAIR ? wn * (WN / 2) : wn * WN);
+  if constexpr (P == 3) {
+    // the first column of fragment i for this lane (register 4 q + e: column 8 q + e from there)
+    auto column = [&](int i) { return nb + (PAIR ? i % (NF / 2) : i) * 32 + 4 * (lane >> 5); };
+    auto from = [&](int i) { return column(i) < p.N ? column(i) : p.N - 1; };
+    again<NF, MF>(
+        acc,
+        [&](int i, int64_t k, bool second) {
+          const bool up = second || (PAIR ? i >= NF / 2 : USE == kDw && mat);
+          const int64_t ld = up ? p.nld1 : p.nld0;
+          return (up ? p.n1 : p.n0) + (NKC ? from(i) * ld + k : k * ld + from(i));
+        },
+        [&](int j, int64_t k, bool second) {
+          const int64_t r = mb + j * 32 + (lane & 31), m = r < p.M ? r : p.M - 1, ld = second ? p.mld1 : p.mld0;
+          return (second ? p.m1 : p.m0) + (MKC ? m * ld + k : k * ld + m);
+        },
+        [&](int i) { return p.N - from(i); },
+        [&](bool second) { return NKC ? (second ? p.nld1 : p.nld0) : 1; },
+        [&](auto f) {
+          for (int64_t s = first; s < steps; ++s) {
+            const bool second = USE == kDx && s >= kblocks;
+            const int64_t k = kfrom + (second ? s - kblocks : s) * BK;
+            f(k, k + BK < kend ? k + BK : kend, second);
+          }
+        });
+  }
+  finish<E, USE, NF, MF>(p, acc, mb, nb, split, mat);
 }
 
 // ------------------------------------------------------- packed operands

@@ -117,3 +117,54 @@ def test_a_value_that_is_none_stays_so(gpu, act, rows, ty):
     for t in (h, dx):
         assert t[1].all() and not t[0].any() and not t[2:].any()
     assert dwg.all() and dwu.all()
+
+
+def form(x, wg, wu):
+    """Projections in 64 bits rounded to 32 (a sum that overflows there is an
+    infinity), and the activation and its slope."""
+    g, u = ((x.to(F64) @ w.to(F64)).float().to(F64) for w in (wg, wu))
+    p = torch.sigmoid(g)
+    return g, u, (g * p).float().to(F64), p * (1 + g * (1 - p))
+
+
+# rows of the kernel for a few, of the tiles; a reduction in one and in several pieces
+@pytest.mark.parametrize("rows,width,hidden", [(3, 40, 70), (200, 40, 70), (300, 65, 1000), (2000, 96, 1408)])
+@pytest.mark.parametrize("value", [INF, -INF, 3.4e38, -3.4e38])
+@pytest.mark.parametrize("where", ["x", "w"])
+def test_gated_block_of_32_bits_with_a_value_past_bfloat16(gpu, rows, width, hidden, value, where):
+    """The products take their operands in bfloat16 parts, whose largest is
+    3.39e38: what lies above, and an infinity, gives what it gives in 32 bits,
+    however many rows there are.  Numbers are within the bound of sums of
+    `width` products in 32 bits, passed on by the activation and the product."""
+    g = torch.Generator().manual_seed(rows)
+    x, wg, wu = (torch.randn(*s, generator=g) * 0.1 for s in ((rows, width), (width, hidden), (width, hidden)))
+    if where == "x":
+        x[2, 7] = value
+    else:
+        wu[7, 3] = value
+    _, u, f, _ = form(x, wg, wu)
+    want = f * u
+    of_gate, of_up = (x.abs().to(F64) @ w.abs().to(F64) for w in (wg, wu))
+    bound = (width + 32) * 2.0 ** -24 * (of_gate * u.abs() * 1.2 + f.abs() * of_up + want.abs()) + 1e-30
+    got = Q.gated_mlp(x.cuda(), wg.cuda(), wu.cuda()).cpu()
+    same = (got == want.float()) | (got.isnan() & want.isnan())
+    ok = same | (torch.isfinite(got) & torch.isfinite(want) & ((got.to(F64) - want).abs() <= bound))
+    assert torch.isinf(want.float()).any() or abs(value) < INF
+    assert ok.all(), (got[~ok][:4], want[~ok][:4])
+
+
+@pytest.mark.parametrize("rows,width,hidden", [(3, 40, 70), (200, 40, 70), (300, 65, 1000), (2000, 96, 1408)])
+@pytest.mark.parametrize("value", [INF, 3.4e38])
+def test_gradients_of_the_gated_block_of_32_bits_with_a_value_past_bfloat16(gpu, rows, width, hidden, value):
+    g = torch.Generator().manual_seed(rows + 1)
+    x, wg, wu = (torch.rand(*s, generator=g) * 0.1 + 0.01 for s in ((rows, width), (width, hidden), (width, hidden)))
+    dh = torch.rand(rows, hidden, generator=g) + 0.1
+    dh[1, 5] = value
+    dx, dwg, dwu = Q.gated_mlp_backward(dh.cuda(), x.cuda(), wg.cuda(), wu.cuda())
+    _, u, f, slope = form(x, wg, wu)
+    dg, du = (dh.to(F64) * u * slope).float().to(F64), (dh.to(F64) * f).float().to(F64)
+    # (everything is positive: no infinity meets its opposite, and a sum of K
+    # products is within about K 2^-24 of itself, 2000 at most here)
+    alike(dx, dg @ wg.to(F64).T + du @ wu.to(F64).T, "dx", 1.2e-4)
+    alike(dwg, x.to(F64).T @ dg, "dw_gate", 1.2e-4)
+    alike(dwu, x.to(F64).T @ du, "dw_up", 1.2e-4)
