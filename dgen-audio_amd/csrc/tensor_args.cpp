@@ -5,6 +5,7 @@
 // kInt32), and returns None for what it turns down; the caller looks at that
 // again and says why.  `covers` tells whether
 // tensors share memory.
+#include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 namespace {
@@ -25,6 +26,7 @@ const at::Tensor* tensor_of(PyObject* const* args, Py_ssize_t n) {
   if (t.dim() != PyTuple_GET_SIZE(args[1])) return nullptr;
   for (int64_t d = 0; d < t.dim(); ++d)
     if (t.size(d) != PyLong_AsLongLong(PyTuple_GET_ITEM(args[1], d))) return nullptr;
+  if (t.requires_grad() && c10::GradMode::is_enabled()) return nullptr;  // (the caller warns)
   return &t;
 }
 

@@ -14,7 +14,8 @@ first three float32), possibly views of wider ones: the last axis is
 contiguous, the others have any stride.  Work is enqueued on torch's current
 stream and the calls return without waiting; results and scratch come from
 torch's allocator on that stream.  Nothing is recorded for autograd: a program
-calls the backward functions itself.  A wrong argument raises ``ValueError``, a
+calls the backward functions itself, and an operand that requires a gradient
+brings a warning unless gradients are switched off.  A wrong argument raises ``ValueError``, a
 failing launch ``HIPError``.
 
 Results that the caller gives a place for (``out``, ``sum_out``, ``state_out``)
@@ -36,6 +37,8 @@ from __future__ import annotations
 
 import ctypes
 import struct
+import sys
+import warnings
 from typing import NamedTuple, Optional
 
 import torch
@@ -146,16 +149,24 @@ def _type(x, name: str) -> int:
 # Tests of an argument: dense, rows and sequence (csrc/tensor_args.cpp) give its
 # address and strides; what they turn down comes to the functions here, which
 # say what is wrong with it, or take it after all.
-def _is(t, shape, dtype, device) -> bool:
+def _is(t, name: str, shape, dtype, device) -> bool:
     try:
-        return t.dtype is dtype and t.shape == shape and t.device == device
+        if not (t.dtype is dtype and t.shape == shape and t.device == device):
+            return False
     except AttributeError:  # not a tensor
         return False
+    if t.requires_grad and torch.is_grad_enabled():
+        caller, up = sys._getframe(1), 2
+        while caller.f_back and caller.f_code.co_filename == __file__:
+            caller, up = caller.f_back, up + 1
+        warnings.warn(f"{name} requires a gradient, which the sequence operators do not record: call them under "
+                      "torch.no_grad() and their backward functions, or give them detached tensors", stacklevel=up)
+    return True
 
 
 def _seq(t, name: str, shape, dtype, device):
     """(address, batch stride, time stride) of a [batch][time][channel] tensor."""
-    if not _is(t, shape, dtype, device):
+    if not _is(t, name, shape, dtype, device):
         raise _wrong(name, t, f"{tuple(shape)} {dtype} on {device}")
     sb, st, sc = t.stride()
     if sc != 1 and shape[2] != 1:
@@ -167,7 +178,7 @@ def _dense(t, name: str, shape, dtype, device):
     """Address of a contiguous tensor (0 for None)."""
     if t is None:
         return 0
-    if not _is(t, shape, dtype, device):
+    if not _is(t, name, shape, dtype, device):
         raise _wrong(name, t, f"{tuple(shape)} {dtype} on {device}")
     if not t.is_contiguous():
         raise ValueError(f"{name}: must be contiguous")
@@ -176,7 +187,7 @@ def _dense(t, name: str, shape, dtype, device):
 
 def _rows(t, name: str, shape, dtype, device):
     """(address, row stride) of a tensor whose leading axes are rows."""
-    if not _is(t, shape, dtype, device):
+    if not _is(t, name, shape, dtype, device):
         raise _wrong(name, t, f"{tuple(shape)} {dtype} on {device}")
     if len(shape) != 2:
         if t.is_contiguous():
