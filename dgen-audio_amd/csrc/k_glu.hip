@@ -1008,6 +1008,16 @@ Plan plan_of(const dgen_hip_mlp& a, bool backward) {
   return p;
 }
 
+// Whether the packs and joins, a thread for 8 and 4 elements, stay below the
+// 2^32 threads of a launch (the products' tiles are limited in mlp_run).
+bool fits(const dgen_hip_mlp& a, const Plan& p, bool backward) {
+  constexpr int64_t kMost = (int64_t(1) << 32) - 256;
+  if (p.pack_x && p.width / 8 * p.rows > kMost) return false;
+  if (!backward) return true;
+  return (p.dx.runs == 1 || a.rows * tiles(a.width, 4) <= kMost) &&
+         ((!p.large && p.dw.runs == 1) || 2 * a.width * tiles(a.hidden, 4) <= kMost);
+}
+
 // ----------------------------------------------------------------- launches
 template <class E, int USE>
 void staged(GluP<E> p, hipStream_t st) {
@@ -1165,9 +1175,13 @@ void mlp_launch(const dgen_hip_mlp& a, bool backward, hipStream_t st) {
 
 }  // namespace
 
-int64_t mlp_workspace(const dgen_hip_mlp& a, bool backward) {
-  return a.type == DGEN_HIP_BF16 ? plan_of<bf16>(a, backward).total : plan_of<float>(a, backward).total;
+namespace {
+Plan plan_for(const dgen_hip_mlp& a, bool backward) {
+  return a.type == DGEN_HIP_BF16 ? plan_of<bf16>(a, backward) : plan_of<float>(a, backward);
 }
+}  // namespace
+
+int64_t mlp_workspace(const dgen_hip_mlp& a, bool backward) { return plan_for(a, backward).total; }
 
 int mlp_run(const dgen_hip_mlp& a, bool backward, hipStream_t st, bool dry) {
   const char* what = backward ? "gated_mlp_backward" : "gated_mlp";
@@ -1192,7 +1206,10 @@ int mlp_run(const dgen_hip_mlp& a, bool backward, hipStream_t st, bool dry) {
     DGEN_REQUIRE(a.dw_gate && a.dw_up && (a.width <= 1 || (a.dw_gate_stride >= a.hidden && a.dw_up_stride >= a.hidden)),
                  "%s: dw_gate or dw_up missing or overlapping itself", what);
   }
-  const int64_t need = mlp_workspace(a, backward);
+  const Plan plan = plan_for(a, backward);
+  DGEN_REQUIRE(fits(a, plan, backward), "%s: rows %lld x width %lld x hidden %lld is too large for one call", what,
+               (long long)a.rows, (long long)a.width, (long long)a.hidden);
+  const int64_t need = plan.total;
   DGEN_REQUIRE(need == 0 || (a.workspace && a.workspace_bytes >= (uint64_t)need && (uintptr_t)a.workspace % 256 == 0),
                "%s: workspace of %llu bytes, %lld needed (256-byte aligned)", what, (unsigned long long)a.workspace_bytes,
                (long long)need);

@@ -2,7 +2,7 @@
 (no device), and calls near them."""
 import pytest
 
-from test_sequence_abi import AT, scan, sequence, workspace
+from test_sequence_abi import AT, message, scan, sequence, workspace
 
 
 def scan_of(batch, T, D, N):
@@ -32,6 +32,26 @@ def test_the_stride_of_a_single_frame_says_nothing(T, taken):
     """One frame out of a time-major recording of many voices."""
     d = scan(batch=4, T=T, D=8, x=(AT, 8, 1 << 27), y=(AT, 40, 8))
     assert (workspace("selective_scan", d, 0) == (0, 0)) is taken
+
+
+def mlp_of(rows, width, hidden, type, backward, x=AT):
+    grads = (AT, hidden, AT, width, AT, hidden, AT, hidden) if backward else (0,) * 8
+    return sequence._MLP.pack(sequence._MLP_SIZE, type, 0, 0, rows, width, hidden, x, width, AT, hidden, AT, hidden,
+                              *((0, 0) if backward else (AT, hidden)), *grads)
+
+
+@pytest.mark.parametrize("rows,width,hidden,type,backward,x,taken", [
+    (300, 1 << 16, (1 << 17) - 32, 1, 1, AT, True),    # weight gradients joined by just under 2^32 threads
+    (300, 1 << 16, 1 << 17, 1, 1, AT, False),
+    (1 << 21, 1 << 13, 1 << 13, 1, 0, AT + 2, True),   # x packed by 2^31 threads
+    (1 << 22, 1 << 13, 64, 1, 0, AT + 2, False),
+    (1 << 22, 1 << 13, 64, 1, 0, AT, True),            # (aligned: not packed)
+    (64, 64, 128, 0, 1, AT, True),
+])
+def test_gated_blocks_past_a_launch_are_refused(rows, width, hidden, type, backward, x, taken):
+    rc, _ = workspace("gated_mlp", mlp_of(rows, width, hidden, type, backward, x), backward)
+    assert (rc == 0) is taken
+    assert taken or "too large" in message()
 
 
 @pytest.mark.gpu
