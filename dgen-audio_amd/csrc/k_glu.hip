@@ -492,14 +492,18 @@ typedef __attribute__((address_space(3))) short4v lds_short4;
 
 // 16 bytes a lane from `g` to LDS byte `at` + 16 lane (at: uniform).  In
 // assembly, since the compiler would wait for every copy in flight before any
-// transposing LDS read; the kernel waits for its copies itself.  (M0 has no
-// other use in it.)
+// transposing LDS read; the kernel waits for its copies itself.  (M0 is no
+// register that the compiler allocates, of which it warns, but one that it
+// writes for its own instructions: naming it keeps them apart from these.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void copy_to_lds(const bf16* g, uint32_t at) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(
                    __builtin_amdgcn_readfirstlane(at)),
                "v"(g)
-               : "memory");
+               : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 template <bool KC>
 __device__ __forceinline__ int chunk_swizzle(int row) { return KC ? (row >> 1) & 3 : (row & 3) << 1; }
