@@ -378,7 +378,7 @@ __global__ __launch_bounds__(kThreads) void k_scan(ScanP<E> p) {
   }
 }
 
-constexpr int kMaxChunks = 512, kMaxRun = 32;  // chunks, and of a thread in the carry
+constexpr int kMaxChunks = 512, kMaxRun = 16;  // chunks, and of a thread in the carry
 
 // Of many chunks: states entering each, in place of the chunks' end states
 // (reverse: the adjoints entering from the chunks after).  COLS states a workgroup, SEGS
@@ -801,7 +801,8 @@ void scan_launch(const dgen_hip_scan& a, bool backward, const ScanShape& s, hipS
   p.sums = ws, p.ends = p.sums + s.sums, p.gends = p.ends + s.ends;
   if (!backward) p.y = out(a.y), p.state_out = a.state_out;
   const dim3 grid((unsigned)(s.nd * s.chunks * a.batch));
-  // (threads a state by the number of chunks, for runs of up to 16 or 32)
+  // (threads a state by the number of chunks, for runs of up to 16)
+  static_assert(64 / 4 <= kMaxRun && 256 / 16 <= kMaxRun && kMaxChunks / 32 <= kMaxRun, "runs of the carry");
   auto carry = [&]() {
     auto states = [&](int64_t cols) {
       return dim3((unsigned)((a.D * s.NP + cols - 1) / cols * a.batch * (backward ? 2 : 1)));
