@@ -54,6 +54,23 @@ def test_gated_blocks_past_a_launch_are_refused(rows, width, hidden, type, backw
     assert taken or "too large" in message()
 
 
+@pytest.mark.parametrize("type", [0, 1])
+def test_calls_that_the_binding_gives_no_scratch_need_none(type):
+    """sequence.py asks for no scratch for scans of up to 32 frames and gated
+    blocks of up to 16 rows and 8192 columns."""
+    for T in (1, 2, 31, 32):
+        for batch in (1, 3, 64, 5000):
+            for D in (1, 64, 65, 1024):
+                for N in (1, 16, 17, 64):
+                    d = scan(type=type, batch=batch, T=T, D=D, N=N, x=(AT, T * D, D), y=(AT, T * D, D))
+                    assert workspace("selective_scan", d, 0) == (0, 0), (batch, T, D, N)
+    for rows in (1, 2, 8, 9, 15, 16):
+        for width in (1, 33, 512, 4096):
+            for hidden in (1, 16, 1408, 4096, 4097, 8191, 8192):
+                for x in (AT, AT + 4):
+                    assert workspace("gated_mlp", mlp_of(rows, width, hidden, type, 0, x), 0) == (0, 0), (rows, width, hidden)
+
+
 @pytest.mark.gpu
 def test_a_single_frame_with_a_far_stride(gpu):
     torch = pytest.importorskip("torch")
