@@ -38,6 +38,13 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
   return v;
 }
 
+// 1 / sqrt(v); the instruction takes numbers below 2^-126 (small rows without
+// an eps) for 0.
+__device__ __forceinline__ float root_of(float v) {
+  const bool low = v < 0x1p-100f;
+  return __builtin_amdgcn_rsqf(low ? v * 0x1p100f : v) * (low ? 0x1p50f : 1.f);
+}
+
 template <int TPR>
 constexpr int norm_threads() { return TPR > 256 ? TPR : 256; }
 
@@ -67,7 +74,7 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_rms_norm(
   }
   ss = row_sum<TPR>(ss, red);
   if (!live) return;
-  const float r = __builtin_amdgcn_rsqf(fmaf(ss, inv_n, eps));
+  const float r = root_of(fmaf(ss, inv_n, eps));
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
     const int c = c0 + i * TPR * 4;
@@ -108,7 +115,7 @@ __global__ __launch_bounds__(norm_threads<TPR>()) void k_rms_norm_bwd(
     }
     ss = row_sum<TPR>(ss, red[0]);
     dot = row_sum<TPR>(dot, red[1]);
-    const float r = __builtin_amdgcn_rsqf(fmaf(ss, inv_n, eps));
+    const float r = root_of(fmaf(ss, inv_n, eps));
     const float k = dot * inv_n * r * r;
 #pragma unroll
     for (int i = 0; i < IT; ++i) {

@@ -168,3 +168,14 @@ def test_gradients_of_the_gated_block_of_32_bits_with_a_value_past_bfloat16(gpu,
     alike(dx, dg @ wg.to(F64).T + du @ wu.to(F64).T, "dx", 1.2e-4)
     alike(dwg, x.to(F64).T @ dg, "dw_gate", 1.2e-4)
     alike(dwu, x.to(F64).T @ du, "dw_up", 1.2e-4)
+
+
+def test_norm_of_small_rows_without_eps(gpu):
+    """A mean square below the smallest normal number, 2^-126."""
+    w = torch.ones(8, device="cuda")
+    for e in (0, -60, -62, -64, -66):
+        x = torch.full((3, 8), 2.0 ** e, device="cuda")
+        y = Q.rms_norm(x, w, eps=0.0)
+        assert ((y - 1).abs() <= 1e-6).all(), (e, y[0, 0].item())
+        dx, dw = Q.rms_norm_backward(torch.ones_like(x), x, w, eps=0.0)
+        assert torch.isfinite(dx).all() and ((dw - 3).abs() <= 1e-5).all()
