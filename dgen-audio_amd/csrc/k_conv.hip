@@ -8,12 +8,15 @@
 // x; the weight and bias gradients are summed per thread over its tile, over
 // the workgroup's tiles in LDS, and over workgroups in a fixed order.
 //
-// Measured at 32 x 1000 x 1024 bf16, W = 4, calls in a row on two sets of
-// operands (a large copy: 4.97 TB/s): forward 33 us, 4.0 TB/s; backward 54 us
-// with the partial rows, 3.6 TB/s.  The loads' latency is what is left: a
-// wave's four channels a lane are 512 bytes a frame and tensor, with four
-// frames in flight (eight: 37 and 63 us, by their registers), and about half of
-// the issue slots go to the sigmoid and the window.
+// Measured at 32 x 1000 x 1024, W = 4, on operands that the caches do not hold
+// (a large copy: 4.97 TB/s): forward bf16 44 us, 3.0 TB/s, fp32 57 us, 4.6 TB/s;
+// backward bf16 53 us, 3.7 TB/s, fp32 91 us, 4.3 TB/s, and 5 us for the partial
+// rows of either.  (Calls in a row on two sets of operands, which lie in the
+// last cache in part: bf16 30 and 50 us.)  The loads' latency is what is left,
+// in bf16 above all: a wave's four channels a lane are 512 bytes a frame and
+// tensor, with four frames in flight (eight: 12 and 17 % more time, by their
+// registers), and about half of the issue slots go to the sigmoid and the
+// window.
 #include "seq.h"
 
 namespace dgen {
@@ -32,9 +35,9 @@ struct ConvShape {
 // Frames of a tile: long enough that the frames before it, read again, cost
 // little, short enough that the threads fill the chip (eight waves a CU);
 // 8 covers every window's past, so only the first tile reads the state.  At 32
-// x 1000 x 1024 bf16, calls of tiles of 16, 32 and 64 frames: forward 36, 33
-// and 41 us (64 leaves one round of workgroups, half of it idle at the end),
-// backward 73, 59 and 55.
+// x 1000 x 1024 bf16, calls on two sets of operands, tiles of 16, 32 and 64
+// frames: forward 36, 33 and 41 us (64 leaves one round of workgroups, half of
+// it idle at the end), backward 73, 59 and 55.
 ConvShape conv_shape(const dgen_hip_conv& c, bool backward) {
   ConvShape s{c.batch, c.T, c.D, (c.D + 3) / 4, 0, backward ? 64 : 32};
   const int64_t want = 256 * 8 * 64;

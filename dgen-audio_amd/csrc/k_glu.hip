@@ -12,8 +12,11 @@
 // Where tiles alone do not fill the chip, the reductions of dx and dW are cut
 // into runs whose parts are added in order.
 //
-// bfloat16 operands multiply as they are, accumulated in fp32 (dg and du are
-// rounded to bfloat16 between the products, as the operands are).  fp32
+// bfloat16 operands multiply as they are, accumulated in fp32.  dg and du are
+// rounded to bfloat16 between the products: gradients of 32000 x 1024 x 2816 are
+// then off by 0.0023 of their norm, for 0.0017 by the rounding of the results
+// alone.  In two bfloat16 parts each, which would leave that, the products of dx
+// and dW would be twice as many (690 us more of 1200).  fp32
 // operands are split exactly into three bfloat16 parts on the way to LDS, and
 // the six partial products down to 2^-16 are accumulated in fp32, as accurate
 // as fp32 products (see k_gemm.hip).  An infinity, or a number past the largest
@@ -28,15 +31,21 @@
 // The matrix instruction's row index is the output's column, so a lane ends
 // with four consecutive columns of one output row.
 //
-// Measured (large library products: 1227 TFLOP/s of bf16, 154 of fp32): bf16,
-// 32000 x 1024 x 2816 backward: projections with their gradients 547 us, dx
-// 358, dW 377, its parts 21 (369 GFLOP each, 0.67, 1.03 and 0.98 PFLOP/s; the
-// projections' 32 stages a tile leave its 192 KB of dh, dg and du and their
-// activations in the open); 20000 rows forward 272 us, 0.85 PFLOP/s.  fp32,
-// 8003 x 512 x 1365 forward 160 us, 140 TFLOP/s; 16000 x 512 x 1408 backward
-// 390, 287 and 350 us, 118 to 161 TFLOP/s (bound by the six products and the
-// splitting).  bf16, 8 x 512 x 1408 forward: 5 us, the latency of the launch
-// and of one round of loads.
+// Measured on operands that the caches do not hold (large library products:
+// 1227 TFLOP/s of bf16, 154 of fp32): bf16, 32000 x 1024 x 2816 backward:
+// projections with their gradients 506 us, dx 342, dW 346, its parts 22 (369
+// GFLOP each, 0.73, 1.08 and 1.07 PFLOP/s; the projections' 32 stages a tile
+// leave its 192 KB of dh, dg and du and their activations in the open); 20000
+// rows forward 257 us, 0.90 PFLOP/s.  fp32, 8003 x 512 x 1365 forward 180 us,
+// 124 TFLOP/s (calls in a row: 164, 136); 16000 x 512 x 1408 backward 359, 266
+// and 312 us, 128 to 173 TFLOP/s (bound by the six products and the splitting).
+// bf16, 8 x 512 x 1408 forward: 7 us (weights in the caches: 5), the latency of
+// the launch and of one round of loads.  Between these sizes k_glu's loop, one
+// LDS buffer and two barriers a step, and grids of fewer tiles than CUs are
+// what bounds: bf16, 2000 x 512 x 1408 forward 20 us, 5 by its products,
+// backward 23, 18 and 36 us and 10 of joins, 14 by its products; 61 x 256 x 1792
+// backward four launches of 4 to 11 us; fp32, 500 x 512 x 1408 forward 28 us, 7
+// by its products, the 16 steps of one tile.
 #include "seq.h"
 
 namespace dgen {
@@ -264,8 +273,8 @@ __device__ __forceinline__ void finish(const GluP<E>& p, const floatx16 (&acc)[N
 // elements at k of the first of fragment i's columns (consecutive ones nstep()
 // apart, `left(i)` of them in the operand) and of its row of fragment j;
 // steps(f) calls f(k from, k to, second segment) for the wave's reduction.
-// For infinities; a tile without NaN passes by.  (8003 x 512 x 1365 forward:
-// 163 us, with an infinity in a row 1.4 ms, of NaN all over 6.8.)
+// For infinities; a tile without NaN passes by.  (Calls of 8003 x 512 x 1365
+// forward: 164 us, with an infinity in a row 1.4 ms, of NaN all over 6.8.)
 template <int NF, int MF, class Cols, class Rows, class Left, class Stride, class Steps>
 __device__ __forceinline__ void again(floatx16 (&acc)[NF][MF], Cols cols, Rows rows, Left left, Stride nstep,
                                       Steps steps) {
@@ -324,6 +333,7 @@ __device__ __forceinline__ TileAt tile_at(const Params& p) {
 }
 
 // BM x BN: output rows and operand columns of a tile; WM x WN: of a wave.
+// (fp32 tiles of 64 rows fit four waves a SIMD but for again's registers.)
 template <class E, int BM, int BN, int WM, int WN, int BK, int USE>
 __global__ __launch_bounds__(kThreads, sizeof(E) == 2 ? 1 : BM == 64 && USE != kDw ? 4 : 2) void k_glu(GluP<E> p) {
   constexpr int P = planes<E>(), NF = WN / 32, MF = WM / 32;
@@ -896,8 +906,8 @@ int64_t tiles(int64_t n, int64_t of) { return (n + of - 1) / of; }
 // Forward by k_glu_few.  It reads the weights once more for every 8 rows and
 // multiplies on the vector unit, so it is taken while its workgroups (of 32
 // columns and 8 rows) are one round of the 256 CUs, two for fp32, whose tiles
-// take three times as long.  Kernels, us, few / tiles (whose time does not
-// change up to 128 rows): bfloat16, 512 x 1408, 16 rows 5 / 10, 40 (220
+// take three times as long.  Kernels, us, weights in the caches, few /
+// tiles (whose time does not change up to 128 rows): bfloat16, 512 x 1408, 16 rows 5 / 10, 40 (220
 // workgroups) 6 / 10, 48 (264) 9.9 / 10.3, 96 (528) 14 / 10.5; 1024 x 2816, 16
 // (176) 11 / 20, 48 (528) 27 / 20; 1024 x 16384, 8 (512) 28 / 26, 16 (1024) 53
 // / 25; 2048 x 512, 128 (256) 17 / 31; fp32, 512 x 1408, 64 (352) 13 / 26; 1024

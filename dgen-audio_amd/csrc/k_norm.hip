@@ -11,10 +11,11 @@
 // that its workgroup walks, one partial row per workgroup, summed in a fixed
 // order afterwards.
 //
-// Measured (a large copy: 4.97 TB/s): forward of 32000 x 512, x and y bf16,
-// residual and sum fp32, 42.7 us, 4.6 TB/s; backward of the same without ds
-// 47.5 us, 3.4 TB/s, and 7 us for the partial rows; backward of 4001 x 1023
-// fp32 with ds 15.7 us, 4.2 TB/s, and 5 us.
+// Measured on operands that the caches do not hold (a large copy: 4.97 TB/s):
+// forward of 32000 x 512, x and y bf16, residual and sum fp32, 40 us, 4.9 TB/s,
+// all fp32 48 us, 5.5 TB/s; backward with ds, dy bf16 and the rest fp32, 44 us,
+// 5.2 TB/s, and 7 us for the partial rows; backward of 4001 x 1023 fp32 with ds
+// 18 us, 3.6 TB/s, and 5 us.
 #include "seq.h"
 
 namespace dgen {
@@ -173,9 +174,9 @@ void row_shape(int64_t n, int& tpr, int& it) {
 }
 
 // Workgroups of the backward pass: each walks rows and leaves one partial
-// row.  Two or more steps each, up to four workgroups a CU (32000 x 512: 48 us
-// with 1024 workgroups, 64 with 512; 4001 x 1023, 1001 steps: 19.8 us with 512,
-// 21.0 with 1001, whose partial rows take longer to add).
+// row.  Two or more steps each, up to four workgroups a CU (calls, 32000 x 512:
+// 48 us with 1024 workgroups, 64 with 512; 4001 x 1023, 1001 steps: 19.8 us with
+// 512, 21.0 with 1001, whose partial rows take longer to add).
 int64_t norm_blocks(const dgen_hip_norm& a) {
   int tpr, it;
   row_shape(a.width, tpr, it);

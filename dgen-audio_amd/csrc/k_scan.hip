@@ -24,11 +24,12 @@
 // 16 channels in registers, over the four waves in LDS, and over workgroups in
 // a fixed order afterwards; no atomics.
 //
-// Measured, bf16, 32 x 1000 x 1024 x 16: forward in one piece 227 us, backward
-// 680 us and 20 for the sums over workgroups (the vector unit issues in 75 to
-// 80 % of the cycles; two workgroups a CU by registers and LDS).  fp32, 1 x
-// 65536 x 64 x 16 in 512 chunks: ends 22 us, carry 10, replay 31.  fp32, one
-// frame of 32 x 1024 x 16: 8 us.
+// Measured, bf16, 32 x 1000 x 1024 x 16: forward in one piece 214 us, backward
+// 672 us and 21 for the sums over workgroups (the vector unit issues in 75 to
+// 80 % of the cycles; two workgroups a CU by registers and LDS); with 12 states
+// 215, 673 and 18, as the padded ones are computed too.  fp32, 1 x 65536 x 64 x
+// 16 in 512 chunks: ends 22 us, carry 10, replay 31.  fp32, one frame of 32 x
+// 1024 x 16: 8 us, for which the tile's loads are issued as for 32 frames.
 #include "seq.h"
 
 namespace dgen {
@@ -234,8 +235,8 @@ enum Mode { kWhole, kSummary, kReplay, kSummaryBoth };
 
 // What a padded state is fed: 0, as B = 0 does not keep its channel's infinity
 // out.  (Its decay is that of A = -1.)  Where whole lanes are padded, that is
-// one select a frame, else one a state: 32 x 1000 x 1024 bf16 forward, N = 16,
-// 12 and 13: 210, 212 and 225 us (209 and 214 without the selects).
+// one select a frame, else one a state: calls of 32 x 1000 x 1024 bf16 forward,
+// N = 16, 12 and 13: 210, 212 and 225 us (12 and 13 without: 209 and 214).
 enum Pad { kNoPad, kLanes, kStates };
 template <int PAD, int S>
 __device__ __forceinline__ float fed(const bool (&own)[S], int s, float v) {

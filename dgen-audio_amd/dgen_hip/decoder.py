@@ -9,7 +9,9 @@ Each block adds two branches to a residual stream kept in 32 bits:
     norm -> gated feed-forward block -> projection back
 
 and a last norm and projection give the head pre-activations (the Z of the
-harmonic synth's heads: amplitudes, gains, taps).  The parts are the operators
+harmonic synth's heads: amplitudes, gains, taps; the synth's own training
+session makes its Z with its own decoder, and what fits this one here is a loss
+on control tracks).  The parts are the operators
 of :mod:`dgen_hip.sequence`; plain projections are library products.
 
     python -m dgen_hip.decoder          # fits control tracks, then streams them

@@ -11,7 +11,8 @@ decoder (include/dgen_hip.h, "sequence operators on device tensors").
 
 Tensors are torch tensors on one GPU (float32 or bfloat16; parameters of the
 first three float32), possibly views of wider ones: the last axis is
-contiguous, the others have any stride.  Work is enqueued on torch's current
+contiguous, and batch and time have any stride, as rows have (leading axes of
+the norms and the gated block that are one axis of rows).  Work is enqueued on torch's current
 stream and the calls return without waiting; results and scratch come from
 torch's allocator on that stream.  Nothing is recorded for autograd: a program
 calls the backward functions itself, and an operand that requires a gradient
@@ -321,7 +322,8 @@ def causal_conv(x, weight, bias=None, silu: bool = True, state=None, state_out=N
     """y[t] = silu(bias + sum_i weight[:, i] x[t - W + 1 + i]) per channel of
     x [batch][time][D], weight [D][W] (W up to 8).  The frames before the
     first are ``state`` ([batch][W-1][D], x's type, oldest first) or 0;
-    ``state_out`` receives the last W-1 frames of each sequence."""
+    ``state_out`` receives the last W-1 frames of each sequence.  A call takes
+    up to 65535 sequences."""
     W, dev, (ty, (B, T, D), w, b, n, xs, st) = _conv_parts(x, weight, bias, state, lengths)
     y, ys = _fresh_seq(x, out, x.shape)
     if out is not None:
@@ -466,7 +468,8 @@ def gated_mlp(x, w_gate, w_up, activation: str = "silu", out=None):
     """act(x w_gate) * (x w_up) for x [..., width] and weights
     [width][hidden] of x's type; act is "silu" or "gelu" (tanh form).  Products
     of bfloat16 are accumulated in float32; float32 operands are multiplied as
-    accurately as in float32."""
+    accurately as in float32 (infinities and numbers past bfloat16's largest
+    take a slower way there)."""
     dev, hidden, head = _mlp_parts(x, w_gate, w_up, activation)
     shape = (*x.shape[:-1], hidden)
     h, hp = out, None
@@ -483,7 +486,8 @@ def gated_mlp(x, w_gate, w_up, activation: str = "silu", out=None):
 
 def gated_mlp_backward(dh, x, w_gate, w_up, activation: str = "silu"):
     """(dx, dw_gate, dw_up) of ``gated_mlp``; the projections are formed
-    again, so nothing is kept between the passes."""
+    again, so nothing is kept between the passes.  The gradients of the
+    projections, between the products, have the operands' type."""
     dev, hidden, head = _mlp_parts(x, w_gate, w_up, activation)
     dx, dg, du = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (x, w_gate, w_up))
     shape = (*x.shape[:-1], hidden)

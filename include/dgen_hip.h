@@ -883,7 +883,7 @@ typedef struct dgen_hip_conv {
   int32_t type;    /* x, y, dy, dx and the states */
   int32_t silu;    /* 0: y = u */
   int32_t width;   /* W, 1 .. 8 */
-  int64_t batch, T, D;
+  int64_t batch, T, D;    /* batch up to 65535 */
   const float* weight;    /* [D][W] */
   const float* bias;      /* [D], optional */
   const int32_t* lengths; /* optional */
@@ -940,7 +940,8 @@ int dgen_hip_selective_scan_workspace(int device, const dgen_hip_scan* s, int ba
  * the weights [width][hidden] (rows contiguous, row strides given), h
  * [rows][hidden]; act is SiLU or GELU (tanh form).
  * Backward (dh, x -> dx, dw_gate, dw_up) forms the projections again instead
- * of reading them: no tensor is kept between the passes. */
+ * of reading them: no tensor is kept between the passes.  Between the products
+ * the gradients of the projections are held in `type`. */
 enum dgen_hip_act { DGEN_HIP_SILU = 0, DGEN_HIP_GELU = 1 };
 typedef struct dgen_hip_mlp {
   uint32_t struct_size;
