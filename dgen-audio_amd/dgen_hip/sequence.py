@@ -37,6 +37,7 @@ No counterpart in the reference, whose decoder sees one frame at a time
 from __future__ import annotations
 
 import ctypes
+import os
 import struct
 import sys
 import warnings
@@ -83,15 +84,16 @@ def _current_stream(index: int) -> int:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _current_stream)
 
 
-def _hip_runtimes() -> list[str]:
-    """The HIP runtimes that this process has loaded.  PyTorch brings its own,
-    which the library uses too if that is there first; if the library comes
-    first it takes the system's, and PyTorch loads a second one."""
+def _one_runtime(L: ctypes.CDLL) -> bool:
+    """Whether the library and PyTorch call the same HIP runtime.  PyTorch
+    brings its own, which the library uses too if that is there first; if the
+    library comes first it takes the system's, and PyTorch loads a second one."""
     try:
-        with open("/proc/self/maps") as maps:
-            return sorted({line.split()[-1] for line in maps if "/libamdhip64.so" in line})
-    except OSError:
-        return []
+        theirs = ctypes.CDLL("libc10_hip.so", mode=os.RTLD_NOW | os.RTLD_NOLOAD)
+        a, b = (ctypes.cast(lib.hipGetDevice, ctypes.c_void_p).value for lib in (L, theirs))
+    except (OSError, AttributeError):  # a PyTorch without HIP has no tensors to pass
+        return True
+    return a == b
 
 
 class _Op:
@@ -99,10 +101,9 @@ class _Op:
 
     def __init__(self, name: str):
         L = load_library()
-        runtimes = _hip_runtimes()
-        if len(runtimes) > 1:
-            raise HIPError(f"two HIP runtimes in this process ({', '.join(runtimes)}): PyTorch's streams and memory are "
-                           "unknown to the other one; import torch (or dgen_hip.sequence) before the library is loaded")
+        if not _one_runtime(L):
+            raise HIPError("two HIP runtimes in this process: PyTorch's streams and memory are unknown to the one that the "
+                           "library uses; import torch (or dgen_hip.sequence) before the library is loaded")
         self.forward, self.backward = getattr(L, f"dgen_hip_{name}"), getattr(L, f"dgen_hip_{name}_backward")
         self.workspace = getattr(L, f"dgen_hip_{name}_workspace")
         self.error = L.dgen_hip_last_error
