@@ -12,12 +12,12 @@ decoder (include/dgen_hip.h, "sequence operators on device tensors").
 Tensors are torch tensors on one GPU (float32 or bfloat16; parameters of the
 first three float32), possibly views of wider ones: the last axis is
 contiguous, and batch and time have any stride, as rows have (leading axes of
-the norms and the gated block that are one axis of rows).  Work is enqueued on torch's current
-stream and the calls return without waiting; results and scratch come from
-torch's allocator on that stream.  Nothing is recorded for autograd: a program
-calls the backward functions itself, and an operand that requires a gradient
-brings a warning unless gradients are switched off.  A wrong argument raises ``ValueError``, a
-failing launch ``HIPError``.
+the norms and the gated block that are one axis of rows).  Work is enqueued on
+torch's current stream and the calls return without waiting; results and
+scratch come from torch's allocator on that stream.  Nothing is recorded for
+autograd: a program calls the backward functions itself, and an operand that
+requires a gradient brings a warning unless gradients are switched off.  A
+wrong argument raises ``ValueError``, a failing launch ``HIPError``.
 
 Results that the caller gives a place for (``out``, ``sum_out``, ``state_out``)
 may lie over the operands: where the operator would overwrite what it still
