@@ -23,30 +23,6 @@ namespace dgen {
 namespace {
 
 template <int TPR>
-__device__ __forceinline__ float row_sum(float v, float* red) {
-  // butterfly within the wave (every lane gets the sum)
-#pragma unroll
-  for (int off = (TPR < 64 ? TPR : 64) / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-  if constexpr (TPR > 64) {
-    constexpr int W = TPR / 64;
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = 0.f;
-#pragma unroll
-    for (int i = 0; i < W; ++i) v += red[i];
-  }
-  return v;
-}
-
-// 1 / sqrt(v); the instruction takes numbers below 2^-126 (small rows without
-// an eps) for 0.
-__device__ __forceinline__ float root_of(float v) {
-  const bool low = v < 0x1p-100f;
-  return __builtin_amdgcn_rsqf(low ? v * 0x1p100f : v) * (low ? 0x1p50f : 1.f);
-}
-
-template <int TPR>
 constexpr int norm_threads() { return TPR > 256 ? TPR : 256; }
 
 template <class TX, class TS, int TPR, int IT>

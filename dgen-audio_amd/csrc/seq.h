@@ -104,6 +104,32 @@ __device__ __forceinline__ float softplus_accurate(float x, float& slope) {
   return fmaxf(x, 0.f) + l;
 }
 
+// Sum over a row's TPR threads, in every one of them; `red`: LDS of a row of
+// more than a wave (16 floats).
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float* red) {
+  // butterfly within the wave (every lane gets the sum)
+#pragma unroll
+  for (int off = (TPR < 64 ? TPR : 64) / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  if constexpr (TPR > 64) {
+    constexpr int W = TPR / 64;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < W; ++i) v += red[i];
+  }
+  return v;
+}
+
+// 1 / sqrt(v); the instruction takes numbers below 2^-126 (small rows without
+// an eps) for 0.
+__device__ __forceinline__ float root_of(float v) {
+  const bool low = v < 0x1p-100f;
+  return __builtin_amdgcn_rsqf(low ? v * 0x1p100f : v) * (low ? 0x1p50f : 1.f);
+}
+
 // out[j] = sum over p < parts of ws[p][j] for the columns of up to three
 // outputs that lie side by side in a row of `ws`; fixed order.
 struct SumOut {
@@ -188,5 +214,11 @@ int64_t scan_workspace(const dgen_hip_scan&, bool backward);
 int scan_run(const dgen_hip_scan&, bool backward, hipStream_t, bool dry);
 int64_t mlp_workspace(const dgen_hip_mlp&, bool backward);
 int mlp_run(const dgen_hip_mlp&, bool backward, hipStream_t, bool dry);
+int64_t block_workspace(const dgen_hip_block_norms&, bool backward);
+int block_run(const dgen_hip_block_norms&, bool backward, hipStream_t, bool dry);
+int64_t delta_workspace(const dgen_hip_delta&, bool backward);
+int delta_run(const dgen_hip_delta&, bool backward, hipStream_t, bool dry);
+int64_t adamw_workspace(const dgen_hip_adamw&);
+int adamw_run(const dgen_hip_adamw&, hipStream_t, bool dry);
 
 }  // namespace dgen

@@ -34,3 +34,24 @@ DGEN_SEQ(rms_norm, dgen_hip_norm, norm_run, norm_workspace)
 DGEN_SEQ(causal_conv, dgen_hip_conv, conv_run, conv_workspace)
 DGEN_SEQ(selective_scan, dgen_hip_scan, scan_run, scan_workspace)
 DGEN_SEQ(gated_mlp, dgen_hip_mlp, mlp_run, mlp_workspace)
+DGEN_SEQ(block_norm, dgen_hip_block_norms, block_run, block_workspace)
+DGEN_SEQ(gated_delta_rule, dgen_hip_delta, delta_run, delta_workspace)
+
+extern "C" int dgen_hip_adamw_step(int device, const dgen_hip_adamw* d, void* stream) {
+  if (!d) return fail(DGEN_HIP_E_INVALID, "adamw: null descriptor");
+  if (int rc = adamw_run(*d, nullptr, true)) return rc;
+  DeviceScope on(device);
+  if (!on.ok()) return fail(DGEN_HIP_E_DEVICE, "adamw: device %d", device);
+  return adamw_run(*d, static_cast<hipStream_t>(stream), false);
+}
+extern "C" int dgen_hip_adamw_workspace(int device, const dgen_hip_adamw* d, uint64_t* bytes) {
+  (void)device;
+  if (!d || !bytes) return fail(DGEN_HIP_E_INVALID, "adamw_workspace: null argument");
+  if (d->struct_size != sizeof(*d)) return fail(DGEN_HIP_E_INVALID, "adamw_workspace: struct_size");
+  dgen_hip_adamw t = *d;
+  t.workspace = reinterpret_cast<void*>(256);
+  t.workspace_bytes = ~0ull;
+  if (int rc = adamw_run(t, nullptr, true)) return rc;
+  *bytes = (uint64_t)adamw_workspace(*d);
+  return 0;
+}

@@ -3,10 +3,12 @@
 // bound by them: about 0.75 us a tensor in Python, 0.15 here.  Each function
 // takes (tensor, shape, type, device index), type as in dgen_hip.h (or
 // kInt32), and returns None for what it turns down; the caller looks at that
-// again and says why.  `covers` tells whether
-// tensors share memory.
+// again and says why.  `table` does so for lists of tensors, `covers` tells
+// whether tensors share memory.
 #include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/python_variable.h>
+
+#include <vector>
 
 namespace {
 
@@ -62,6 +64,53 @@ PyObject* sequence(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Tensor* t = tensor_of(args, n);
     if (!t || t->dim() != 3 || (t->stride(2) != 1 && t->size(2) != 1)) return none_if_wrong();
     return Py_BuildValue("(KLL)", address(*t), (long long)t->stride(0), (long long)t->stride(1));
+  });
+}
+
+// (address, batch, time and head stride) of a [batch][time][head][channel] tensor.
+PyObject* heads(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    const at::Tensor* t = tensor_of(args, n);
+    if (!t || t->dim() != 4 || (t->stride(3) != 1 && t->size(3) != 1)) return none_if_wrong();
+    return Py_BuildValue("(KLLL)", address(*t), (long long)t->stride(0), (long long)t->stride(1), (long long)t->stride(2));
+  });
+}
+
+// table(lists, types, device index): rows of the addresses of each list's i-th
+// tensor (0 for a list that is None) and their number of elements, as bytes; all
+// contiguous, and those of a row of one shape.
+PyObject* table(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 3 || !PyTuple_Check(args[0]) || !PyTuple_Check(args[1])) return none_if_wrong();
+    const Py_ssize_t columns = PyTuple_GET_SIZE(args[0]);
+    const long index = PyLong_AsLong(args[2]);
+    if (columns < 1 || columns != PyTuple_GET_SIZE(args[1]) || PyErr_Occurred()) return none_if_wrong();
+    Py_ssize_t rows = -1;
+    for (Py_ssize_t c = 0; c < columns; ++c) {
+      PyObject* list = PyTuple_GET_ITEM(args[0], c);
+      if (list == Py_None && c > 0) continue;
+      if (!PyList_Check(list) || (rows >= 0 && PyList_GET_SIZE(list) != rows)) return none_if_wrong();
+      rows = PyList_GET_SIZE(list);
+    }
+    std::vector<int64_t> out((size_t)(rows * (columns + 1)), 0);
+    for (Py_ssize_t c = 0; c < columns; ++c) {
+      PyObject *list = PyTuple_GET_ITEM(args[0], c), *first = PyTuple_GET_ITEM(args[0], 0);
+      if (list == Py_None) continue;
+      const long type = PyLong_AsLong(PyTuple_GET_ITEM(args[1], c));
+      const at::ScalarType want = type == kF32 ? at::kFloat : type == kBf16 ? at::kBFloat16 : at::ScalarType::Undefined;
+      for (Py_ssize_t r = 0; r < rows; ++r) {
+        PyObject *o = PyList_GET_ITEM(list, r), *like = PyList_GET_ITEM(first, r);
+        if (!THPVariable_Check(o)) return none_if_wrong();
+        const at::Tensor &t = THPVariable_Unpack(o), &u = THPVariable_Unpack(like);
+        if (!t.defined() || t.scalar_type() != want || t.layout() != at::kStrided || !t.is_cuda() ||
+            t.get_device() != index || t.sizes() != u.sizes() || !t.is_contiguous() ||
+            (t.requires_grad() && c10::GradMode::is_enabled()))
+          return none_if_wrong();
+        out[(size_t)(r * (columns + 1) + c)] = (int64_t)address(t);
+        out[(size_t)(r * (columns + 1) + columns)] = t.numel();
+      }
+    }
+    return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(out.data()), (Py_ssize_t)(out.size() * sizeof(int64_t)));
   });
 }
 
@@ -130,6 +179,8 @@ PyMethodDef methods[] = {
     {"dense", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(dense)), METH_FASTCALL, nullptr},
     {"sequence", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(sequence)), METH_FASTCALL, nullptr},
     {"rows", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rows)), METH_FASTCALL, nullptr},
+    {"heads", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(heads)), METH_FASTCALL, nullptr},
+    {"table", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(table)), METH_FASTCALL, nullptr},
     {"covers", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(covers)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_args", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -1,4 +1,4 @@
-"""What sequence.py takes from the native module ``_tensor_args``
+"""What sequence.py and optim.py take from the native module ``_tensor_args``
 (csrc/tensor_args.cpp), for hosts where that was not built."""
 from __future__ import annotations
 
@@ -6,11 +6,11 @@ import torch
 
 
 def _turned_down(t, *_):
-    """Leaves the test of an argument to sequence.py's own."""
+    """Leaves the test of an argument to sequence.py's (and optim.py's) own."""
     return None
 
 
-dense = rows = sequence = _turned_down
+dense = rows = sequence = heads = table = _turned_down
 
 
 def _extent(t: torch.Tensor, pitch: int = 0) -> int:

@@ -71,7 +71,7 @@ EPI_NONE, EPI_BIAS, EPI_BIAS_TANH, EPI_TANH_GRAD = 0, 1, 2, 3
 OP_STATIC, OP_SIDE, OP_JOIN, OP_FORK = 1, 2, 4, 8
 
 # the operators on device tensors (sequence.py)
-SEQUENCE_OPS = ("rms_norm", "causal_conv", "selective_scan", "gated_mlp")
+SEQUENCE_OPS = ("rms_norm", "causal_conv", "selective_scan", "gated_mlp", "block_norm", "gated_delta_rule")
 
 EXPORTED_SYMBOLS = (
     "dgen_hip_abi_version", "dgen_hip_device_count", "dgen_hip_create", "dgen_hip_destroy",
@@ -82,6 +82,7 @@ EXPORTED_SYMBOLS = (
     "dgen_hip_host_outputs", "dgen_hip_set_sample_rate", "dgen_hip_biquad_forward_noalloc",
     "dgen_hip_set_process_ports", "dgen_hip_process_v1", "dgen_hip_process_bind", "dgen_hip_process_memory_size",
     "dgen_hip_set_blocks", "dgen_hip_render_blocks",
+    "dgen_hip_adamw_step", "dgen_hip_adamw_workspace",
 ) + tuple(f"dgen_hip_{op}{entry}" for op in SEQUENCE_OPS for entry in ("", "_backward", "_workspace"))
 # the reference-named process-function exports (include/dgen_process_v1.h)
 PROCESS_V1_SYMBOLS = ("dgen_process_v1", "dgen_set_param_value_v1")
@@ -169,6 +170,8 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
     for op in SEQUENCE_OPS:
         sig[f"dgen_hip_{op}"] = sig[f"dgen_hip_{op}_backward"] = ([i32, vp, vp], i32)
         sig[f"dgen_hip_{op}_workspace"] = ([i32, vp, i32, ctypes.POINTER(u64)], i32)
+    sig["dgen_hip_adamw_step"] = ([i32, vp, vp], i32)
+    sig["dgen_hip_adamw_workspace"] = ([i32, vp, ctypes.POINTER(u64)], i32)
     for name, (args, res) in sig.items():
         fn = getattr(L, name)
         fn.argtypes = args

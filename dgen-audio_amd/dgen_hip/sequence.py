@@ -7,12 +7,17 @@ decoder (include/dgen_hip.h, "sequence operators on device tensors").
   convolution with SiLU;
 - ``selective_scan`` / ``selective_scan_backward``: selective state space scan
   with skip and gate;
-- ``gated_mlp`` / ``gated_mlp_backward``: gated feed-forward block.
+- ``gated_mlp`` / ``gated_mlp_backward``: gated feed-forward block;
+- ``gated_delta_rule`` / ``gated_delta_rule_backward``: a matrix-valued memory
+  per head, which decays and is overwritten key by key;
+- ``block_norm`` / ``block_norm_backward``: the norm after a block, its gate,
+  the residual's scale and addition and the norm before the next block.
 
-Tensors are torch tensors on one GPU (float32 or bfloat16; parameters of the
-first three float32), possibly views of wider ones: the last axis is
-contiguous, and batch and time have any stride, as rows have (leading axes of
-the norms and the gated block that are one axis of rows).  Work is enqueued on
+Tensors are torch tensors on one GPU (float32 or bfloat16; parameters of all
+but the gated block, and the delta rule's decays and strengths, float32),
+possibly views of wider ones: the last axis is contiguous, and batch, time and
+heads have any stride, as rows have (leading axes of the norms and the gated
+block that are one axis of rows).  Work is enqueued on
 torch's current stream and the calls return without waiting; results and
 scratch come from torch's allocator on that stream.  Nothing is recorded for
 autograd: a program calls the backward functions itself, and an operand that
@@ -23,7 +28,8 @@ Results that the caller gives a place for (``out``, ``sum_out``, ``state_out``)
 may lie over the operands: where the operator would overwrite what it still
 reads, it writes to a tensor of its own, which is copied there afterwards.
 What may be replaced in place without one: x, residual, ds, s and dy in the
-norms, x, dt and z in the scan, the state by ``state_out``.  Two results must
+norms (and the gate of each row), x, dt and z in the scan, v in the delta rule,
+the state by ``state_out``.  Two results must
 not share memory.
 
 Clips of unequal length: ``lengths`` ([batch] int32) ends each sequence; later
@@ -48,20 +54,22 @@ import torch
 from .runtime import HIPError, load_library
 
 try:
-    from ._tensor_args import covers, dense, rows, sequence
+    from ._tensor_args import covers, dense, heads, rows, sequence
 except ImportError:  # the library was built without PyTorch's headers: the same in Python
-    from ._tensor_args_python import covers, dense, rows, sequence
+    from ._tensor_args_python import covers, dense, heads, rows, sequence
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
 _F32, _INT32 = 0, 2  # as the native tests name them
 _ACTS = {"silu": 0, "gelu": 1}
+_GATES = {"none": 0, "sigmoid": 1}
 
 
 def _descriptor(fields: str) -> struct.Struct:
     """A descriptor of dgen_hip.h in native layout but for its last two
     fields, the workspace's address and size.  p: address, v: address and
-    stride of rows, s: address and two strides of a sequence tensor."""
-    return struct.Struct("@" + fields.replace("p", "Q").replace("v", "Qq").replace("s", "Qqq"))
+    stride of rows, s: address and two strides of a sequence tensor, h: address
+    and three of one with heads."""
+    return struct.Struct("@" + fields.replace("p", "Q").replace("v", "Qq").replace("s", "Qqq").replace("h", "Qqqq"))
 
 
 # (packed as bytes: a ctypes structure took 3 us more a call)
@@ -69,11 +77,14 @@ _NORM = _descriptor("Iiif qq p v v v v v v v p")           # struct dgen_hip_nor
 _CONV = _descriptor("Iiii qqq ppp s s pp s s pp")          # struct dgen_hip_conv
 _SCAN = _descriptor("Ii qqqq pppppp ssssssssssss ppp")     # struct dgen_hip_scan
 _MLP = _descriptor("Iiii qqq vvvvvvvv")                    # struct dgen_hip_mlp
+_DELTA = _descriptor("Iiif qqqqqq ppp hhh ss h hhhh ss")    # struct dgen_hip_delta
+_BLOCK = _descriptor("Iiii qqq d ppp vvvvvvvvvv ppp")       # struct dgen_hip_block_norms
 _WORKSPACE = struct.Struct("@QQ")
 _NO_WORKSPACE = _WORKSPACE.pack(0, 0)
 # the descriptors' struct_size
 _NORM_SIZE, _CONV_SIZE, _SCAN_SIZE, _MLP_SIZE = (d.size + 16 for d in (_NORM, _CONV, _SCAN, _MLP))
-_NONE, _NO_ROWS = (0, 0, 0), (0, 0)
+_DELTA_SIZE, _BLOCK_SIZE = (d.size + 16 for d in (_DELTA, _BLOCK))
+_NONE, _NO_ROWS, _NO_HEADS = (0, 0, 0), (0, 0), (0, 0, 0, 0)
 
 
 def _current_stream(index: int) -> int:
@@ -148,7 +159,7 @@ def _type(x, name: str) -> int:
     return ty
 
 
-# Tests of an argument: dense, rows and sequence (csrc/tensor_args.cpp) give its
+# Tests of an argument: dense, rows, sequence and heads (csrc/tensor_args.cpp) give its
 # address and strides; what they turn down comes to the functions here, which
 # say what is wrong with it, or take it after all.
 def _is(t, name: str, shape, dtype, device) -> bool:
@@ -174,6 +185,16 @@ def _seq(t, name: str, shape, dtype, device):
     if sc != 1 and shape[2] != 1:
         raise ValueError(f"{name}: the last axis must be contiguous")
     return t.data_ptr(), sb, st
+
+
+def _heads(t, name: str, shape, dtype, device):
+    """(address, three strides) of a [batch][time][head][channel] tensor."""
+    if not _is(t, name, shape, dtype, device):
+        raise _wrong(name, t, f"{tuple(shape)} {dtype} on {device}")
+    sb, st, sh, sc = t.stride()
+    if sc != 1 and shape[3] != 1:
+        raise ValueError(f"{name}: the last axis must be contiguous")
+    return t.data_ptr(), sb, st, sh
 
 
 def _dense(t, name: str, shape, dtype, device):
@@ -497,3 +518,187 @@ def gated_mlp_backward(dh, x, w_gate, w_up, activation: str = "silu"):
                   dg.data_ptr(), hidden, du.data_ptr(), hidden)
     _op("gated_mlp")(d, dev, True, True)
     return dx, dg, du
+
+
+# -------------------------------------------------------------- delta rule
+class DeltaGrads(NamedTuple):
+    """Gradients of ``gated_delta_rule``."""
+    dq: torch.Tensor
+    dk: torch.Tensor
+    dv: torch.Tensor
+    dg: torch.Tensor
+    dbeta: torch.Tensor
+
+
+def _delta_parts(q, k, v, g, beta, scale, normalize, state, lengths):
+    """(device, type, key heads' shape, state's shape, the descriptor's fields
+    up to the state, those of the inputs)."""
+    ty = _type(v, "v")
+    if v.dim() != 4:
+        raise _wrong("v", v, "[batch][time][head][channel]")
+    if not isinstance(q, torch.Tensor) or q.dim() != 4:
+        raise _wrong("q", q, "[batch][time][key head][channel]")
+    shape, keys, dev, et, f32 = v.shape, q.shape, v.device, v.dtype, torch.float32
+    B, T, H, V = shape
+    G, K = keys[2:]
+    if keys[:2] != shape[:2]:
+        raise _wrong("q", q, f"[{B}][{T}][key head][channel]")
+    i, each, states = dev.index, shape[:3], (B, H, K, V)
+    head = (_DELTA_SIZE, ty, 1 if normalize else 0, float(K ** -0.5 if scale is None else scale) if K else 1.0, B, T, G, H, K, V,
+            dense(lengths, (B,), _INT32, i) or _dense(lengths, "lengths", (B,), torch.int32, dev),
+            dense(state, states, _F32, i) or _dense(state, "state", states, f32, dev))
+    return dev, states, head, (*(heads(q, keys, ty, i) or _heads(q, "q", keys, et, dev)),
+                               *(heads(k, keys, ty, i) or _heads(k, "k", keys, et, dev)),
+                               *(heads(v, shape, ty, i) or _heads(v, "v", shape, et, dev)),
+                               *(sequence(g, each, _F32, i) or _seq(g, "g", each, f32, dev)),
+                               *(sequence(beta, each, _F32, i) or _seq(beta, "beta", each, f32, dev)))
+
+
+_NO_DELTA_GRADS = (0,) * 22
+_DELTA_FRAMES = 16  # longer calls take scratch
+
+
+def gated_delta_rule(q, k, v, g, beta, scale: Optional[float] = None, normalize: bool = True, state=None, state_out=None,
+                     lengths=None, out=None):
+    """A memory S [K][V] per head of v [batch][time][heads][V], read and
+    written with queries and keys [batch][time][key heads][K] (each shared by
+    heads / key heads consecutive heads of v), K up to 128 and V up to 1024:
+
+        S' = exp(g[t]) S[t-1];  S[t] = S' + k^[t] (beta[t] (v[t] - S'^T k^[t]))^T;  y[t] = scale S[t]^T q^[t]
+
+    with k^ = k / sqrt(|k|^2 + 1e-6), q^ alike (``normalize`` false: k and q as
+    they are, which keeps S bounded only if the keys' lengths do).  g, the
+    decays' logarithms (at most 0; -inf forgets, and below -128 counts as
+    that), and beta (between 0 and 2) are float32 [batch][time][heads]; scale
+    is K^-1/2 unless given.  The states ([batch][heads][K][V]) are float32.
+    Products are formed in float32's accuracy for float32, and in that of
+    bfloat16's exact values and float32 sums for bfloat16, states as accurate
+    as float32 ones.  A value that is not finite spoils its head's results from
+    up to 63 frames before it on; calls of up to 16 frames go frame by frame."""
+    dev, states, head, ins = _delta_parts(q, k, v, g, beta, scale, normalize, state, lengths)
+    B, T, H, V = shape = v.shape
+    if out is None:
+        y = torch.empty_like(v, memory_format=torch.contiguous_format)
+        yp = (y.data_ptr(), T * H * V, H * V, V)
+    else:
+        y, yp = out, heads(out, shape, head[1], dev.index) or _heads(out, "out", shape, v.dtype, dev)
+        _two_results("out", out, "state_out", state_out)
+        if covers(1, out, v, q, k, g, beta, state, lengths):
+            y = torch.empty_like(v, memory_format=torch.contiguous_format)
+            yp = (y.data_ptr(), T * H * V, H * V, V)
+    left = state_out
+    so = dense(state_out, states, _F32, dev.index) or _dense(state_out, "state_out", states, torch.float32, dev)
+    if so and covers(1, state_out, state, q, k, v, g, beta, lengths):
+        left = torch.empty_like(state_out)
+        so = left.data_ptr()
+    d = _DELTA.pack(*head, so, *ins, *yp, *_NO_DELTA_GRADS)
+    _op("gated_delta_rule")(d, dev, False, T > _DELTA_FRAMES)
+    if left is not state_out:
+        state_out.copy_(left)
+    return y if out is None else _given(out, y)
+
+
+def gated_delta_rule_backward(dy, q, k, v, g, beta, scale: Optional[float] = None, normalize: bool = True, state=None,
+                              lengths=None) -> DeltaGrads:
+    """Gradients of ``gated_delta_rule``; the state counts as given.  Those of
+    shared queries and keys are the sums over the heads that share them."""
+    dev, _, head, ins = _delta_parts(q, k, v, g, beta, scale, normalize, state, lengths)
+    r = DeltaGrads(*(torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v, g, beta)))
+    B, T, H, V = shape = v.shape
+    G, K = q.shape[2:]
+    keys, each = (T * G * K, G * K, K), (T * H, H)
+    d = _DELTA.pack(*head, 0, *ins, *_NO_HEADS,
+                    *(heads(dy, shape, head[1], dev.index) or _heads(dy, "dy", shape, v.dtype, dev)),
+                    r.dq.data_ptr(), *keys, r.dk.data_ptr(), *keys, r.dv.data_ptr(), T * H * V, H * V, V,
+                    r.dg.data_ptr(), *each, r.dbeta.data_ptr(), *each)
+    _op("gated_delta_rule")(d, dev, True, True)
+    return r
+
+
+# ------------------------------------------------------ norms around a block
+class BlockNormGrads(NamedTuple):
+    """Gradients of ``block_norm``; None for what was not given."""
+    dx: torch.Tensor
+    dresidual: torch.Tensor
+    dgate: Optional[torch.Tensor]
+    dpost: torch.Tensor
+    dpre: torch.Tensor
+    dresidual_scale: Optional[torch.Tensor]
+
+
+def _block_parts(x, post_weight, pre_weight, gate, gate_activation, residual_scale, eps, st):
+    """(the descriptor's fields up to the weights, those of x and of the gate)"""
+    ty, shape, dev, f32, et = _type(x, "x"), x.shape, x.device, torch.float32, x.dtype
+    if x.dim() < 2:
+        raise _wrong("x", x, "rows ([..., width])")
+    act = _GATES.get(gate_activation)
+    if act is None:
+        raise ValueError(f"gate_activation {gate_activation!r}: one of {sorted(_GATES)}")
+    i, width, count, each, gp = dev.index, shape[-1:], _count(shape), 1, _NO_ROWS
+    if gate is not None:
+        its = shape
+        if isinstance(gate, torch.Tensor) and gate.dim() == x.dim() and gate.shape[-2] == 1 and count:
+            # one gate for all the rows of an axis
+            each, its = shape[-2], (*shape[:-2], 1, shape[-1])
+        gp = rows(gate, its, ty, i) or _rows(gate, "gate", its, et, dev)
+    return (_BLOCK_SIZE, ty, st, act, count, shape[-1], each, eps,
+            dense(post_weight, width, _F32, i) or _dense(post_weight, "post_weight", width, f32, dev),
+            dense(pre_weight, width, _F32, i) or _dense(pre_weight, "pre_weight", width, f32, dev),
+            dense(residual_scale, width, _F32, i) or _dense(residual_scale, "residual_scale", width, f32, dev),
+            *(rows(x, shape, ty, i) or _rows(x, "x", shape, et, dev))), gp
+
+
+def block_norm(x, post_weight, residual, pre_weight, gate=None, gate_activation: str = "sigmoid", residual_scale=None,
+               eps: float = 1e-5, out=None, sum_out=None):
+    """(y, s) of a block's output x [..., width] (width up to 8192) and the
+    residual (of x's type or float32), over the last axis:
+
+        p = x / sqrt(mean(x^2) + eps) post_weight
+        s = residual_scale residual + activation(gate) p       the next residual
+        y = s / sqrt(mean(s^2) + eps) pre_weight               the next block's input
+
+    gate has x's type and shape, or 1 in the axis before the last (a clip's
+    gate for all its frames); its activation is "sigmoid" or "none".  gate and
+    residual_scale [width] may be left out; eps is at least 1e-30.  ``out`` may
+    be x or the gate itself, ``sum_out`` the residual."""
+    st = _type(residual, "residual")
+    head, gp = _block_parts(x, post_weight, pre_weight, gate, gate_activation, residual_scale, eps, st)
+    shape, dev = x.shape, x.device
+    rp = rows(residual, shape, st, dev.index) or _rows(residual, "residual", shape, residual.dtype, dev)
+    y, yp = _fresh(x, out, "out", shape)
+    s, sp = _fresh(residual, sum_out, "sum_out", shape)
+    if out is not None or sum_out is not None:
+        _two_results("out", y, "sum_out", s)
+        small = post_weight, pre_weight, residual_scale
+        if out is not None and covers(3, out, x, residual, gate, *small):
+            y, yp = _fresh(x, None, "out", shape)
+        if sum_out is not None and covers(3, sum_out, x, residual, gate, *small):
+            s, sp = _fresh(residual, None, "sum_out", shape)
+    d = _BLOCK.pack(*head, *rp, *gp, *yp, *sp, *(0,) * 13)
+    _op("block_norm")(d, dev, False, False)
+    return y if out is None else _given(out, y), s if sum_out is None else _given(sum_out, s)
+
+
+def block_norm_backward(dy, x, residual, s, post_weight, pre_weight, gate=None, gate_activation: str = "sigmoid",
+                        residual_scale=None, ds=None, eps: float = 1e-5) -> BlockNormGrads:
+    """Gradients of ``block_norm`` from that of y and the stored sum s; ``ds``
+    is the gradient that reaches the stored sum from elsewhere.  The residual
+    is read for the gradient of its scale (None will do where there is none).
+    A gate that many rows share has the sum of their gradients."""
+    st = _type(s, "s")
+    head, gp = _block_parts(x, post_weight, pre_weight, gate, gate_activation, residual_scale, eps, st)
+    ty, shape, dev = head[1], x.shape, x.device
+    i = dev.index
+    rp = _NO_ROWS
+    if residual_scale is not None:
+        rp = rows(residual, shape, st, i) or _rows(residual, "residual", shape, s.dtype, dev)
+    (dx, dxp), (dr, drp) = _fresh(x, None, "dx", shape), _fresh(s, None, "dresidual", shape)
+    dgate, dgp = (None, _NO_ROWS) if gate is None else _fresh(gate, None, "dgate", gate.shape)
+    dpost, dpre = torch.empty_like(post_weight), torch.empty_like(pre_weight)
+    dscale = None if residual_scale is None else torch.empty_like(residual_scale)
+    d = _BLOCK.pack(*head, *rp, *gp, 0, 0, *(rows(s, shape, st, i) or _rows(s, "s", shape, s.dtype, dev)),
+                    *(rows(dy, shape, ty, i) or _rows(dy, "dy", shape, x.dtype, dev)),
+                    *(_NO_ROWS if ds is None else rows(ds, shape, st, i) or _rows(ds, "ds", shape, s.dtype, dev)),
+                    *dxp, *drp, *dgp, dpost.data_ptr(), dpre.data_ptr(), 0 if dscale is None else dscale.data_ptr())
+    _op("block_norm")(d, dev, True, True)
+    return BlockNormGrads(dx, dr, dgate, dpost, dpre, dscale)

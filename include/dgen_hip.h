@@ -964,6 +964,131 @@ int dgen_hip_gated_mlp(int device, const dgen_hip_mlp* m, void* stream);
 int dgen_hip_gated_mlp_backward(int device, const dgen_hip_mlp* m, void* stream);
 int dgen_hip_gated_mlp_workspace(int device, const dgen_hip_mlp* m, int backward, uint64_t* bytes);
 
+/* The norm after a block, its gate, the residual's scale and addition, and the
+ * norm before the next block, over the `width` columns of each of `rows` rows:
+ *   p = x / sqrt(mean(x^2) + eps) * post
+ *   s = scale * residual + act(gate) * p
+ *   y = s / sqrt(mean(s^2) + eps) * pre
+ * gate is a row for each of the rows, or one for every `gate_rows` of them
+ * (a clip's gate for all its frames); act is the logistic function or nothing.
+ * gate and scale are optional (left out: 1).  s is stored, rounded to its type,
+ * and y is formed from the sum before that rounding.
+ * Backward (dy, ds, x, residual, s, gate -> dx, dresidual, dgate, dpost, dpre,
+ * dscale): from the stored s; ds (optional) is the gradient that reaches it from
+ * elsewhere. */
+enum dgen_hip_gate { DGEN_HIP_GATE_PLAIN = 0, DGEN_HIP_GATE_SIGMOID = 1 };
+typedef struct dgen_hip_block_norms {
+  uint32_t struct_size;
+  int32_t x_type;    /* x, y, gate, dy, dx, dgate */
+  int32_t s_type;    /* residual, s, ds, dresidual */
+  int32_t act;       /* enum dgen_hip_gate */
+  int64_t rows;
+  int64_t width;     /* 1 .. 8192 */
+  int64_t gate_rows; /* rows that share a gate's row, 1 .. rows; divides rows */
+  double eps;        /* 1e-30 .. 1e30 */
+  const float* post;
+  const float* pre;
+  const float* scale;                            /* optional */
+  const void* x;        int64_t x_stride;        /* elements between rows */
+  const void* residual; int64_t residual_stride; /* backward: with a scale */
+  const void* gate;     int64_t gate_stride;     /* optional */
+  void* y;              int64_t y_stride;        /* forward (may be x or the gate itself) */
+  void* s;              int64_t s_stride;        /* forward: out (may be the residual itself); backward: in */
+  const void* dy;       int64_t dy_stride;       /* backward */
+  const void* ds;       int64_t ds_stride;       /* backward, optional */
+  void* dx;             int64_t dx_stride;       /* backward */
+  void* dresidual;      int64_t dresidual_stride; /* backward */
+  void* dgate;          int64_t dgate_stride;    /* backward; with a gate */
+  float* dpost;                                  /* backward, [width] */
+  float* dpre;                                   /* backward, [width] */
+  float* dscale;                                 /* backward, [width]; with a scale */
+  void* workspace;
+  uint64_t workspace_bytes;
+} dgen_hip_block_norms;
+int dgen_hip_block_norm(int device, const dgen_hip_block_norms* n, void* stream);
+int dgen_hip_block_norm_backward(int device, const dgen_hip_block_norms* n, void* stream);
+int dgen_hip_block_norm_workspace(int device, const dgen_hip_block_norms* n, int backward, uint64_t* bytes);
+
+/* Gated delta rule: a memory S [K][V] per sequence and head that decays, is read
+ * with the key, written with what the value differs from that, and read with the
+ * query.  With k^ = k / sqrt(|k|^2 + 1e-6), q^ likewise (normalize; else as
+ * given):
+ *   S'   = exp(g[t]) S[t-1]
+ *   u    = beta[t] (v[t] - S'^T k^[t])
+ *   S[t] = S' + k^[t] u^T
+ *   y[t] = scale S[t]^T q^[t]
+ * q and k have `key_heads` heads, each shared by heads / key_heads consecutive
+ * heads of v.  g is at most 0 (-infinity forgets everything; below -128 counts as
+ * that), beta between 0 and 2.  S[-1] is `state` ([batch][heads][K][V] fp32) or
+ * 0; `state_out` receives the last S (it may be `state` itself).
+ * A value that is not finite spoils its head's results from up to 63 frames
+ * before it on.
+ * Backward: the state counts as given, no gradient reaches it, and no gradient
+ * enters through state_out. */
+typedef struct dgen_hip_heads { /* [batch][T][heads][channels], contiguous channels */
+  void* data;
+  int64_t stride_b, stride_t, stride_h; /* in elements */
+} dgen_hip_heads;
+typedef struct dgen_hip_delta {
+  uint32_t struct_size;
+  int32_t type;           /* q, k, v, y and the gradients of these; g, beta and theirs are fp32 */
+  int32_t normalize;
+  float scale;
+  int64_t batch, T, key_heads, heads;
+  int64_t K;              /* 1 .. 128 */
+  int64_t V;              /* 1 .. 1024 */
+  const int32_t* lengths; /* optional */
+  const float* state;     /* optional */
+  float* state_out;       /* forward, optional */
+  dgen_hip_heads q, k, v;
+  dgen_hip_seq g, beta;   /* [batch][T][heads] */
+  dgen_hip_heads y;       /* forward */
+  dgen_hip_heads dy, dq, dk, dv; /* backward */
+  dgen_hip_seq dg, dbeta; /* backward */
+  void* workspace;
+  uint64_t workspace_bytes;
+} dgen_hip_delta;
+int dgen_hip_gated_delta_rule(int device, const dgen_hip_delta* d, void* stream);
+int dgen_hip_gated_delta_rule_backward(int device, const dgen_hip_delta* d, void* stream);
+int dgen_hip_gated_delta_rule_workspace(int device, const dgen_hip_delta* d, int backward, uint64_t* bytes);
+
+/* ---- optimiser step on device tensors ---------------------------------------
+ * One AdamW step over `count` tensors (the reference's Adam,
+ * Sources/DGenLazy/Optimizers.swift:164-204, has no weight decay and no bound on the
+ * gradients): with g the gradient times min(1, max_norm / (|all gradients| +
+ * 1e-6)) (max_norm 0: the gradient),
+ *   m' = beta1 m + (1 - beta1) g      v' = beta2 v + (1 - beta2) g^2
+ *   p' = (1 - lr weight_decay) p - lr m' / (1 - beta1^t) / (sqrt(v' / (1 - beta2^t)) + eps)
+ * t = step, or *step_at where that is given (device memory, read when the work
+ * runs: a captured step counts on).  Parameters and moments are fp32, results may
+ * replace them in place; `copy` receives p' rounded to bf16.  Tensors are
+ * contiguous.  `tensors` is host memory, read during the call. */
+typedef struct dgen_hip_adamw_tensor {
+  const float* param;
+  const void* grad;
+  const float* m;
+  const float* v;
+  float* param_out;
+  float* m_out;
+  float* v_out;
+  void* copy; /* optional */
+  int64_t n;
+} dgen_hip_adamw_tensor;
+typedef struct dgen_hip_adamw {
+  uint32_t struct_size;
+  int32_t grad_type;
+  int64_t count;
+  const dgen_hip_adamw_tensor* tensors;
+  double lr, beta1, beta2, eps, weight_decay, max_norm;
+  int64_t step;           /* from 1 */
+  const int64_t* step_at; /* optional */
+  float* norm;            /* with max_norm: receives the gradients' norm */
+  void* workspace;
+  uint64_t workspace_bytes;
+} dgen_hip_adamw;
+int dgen_hip_adamw_step(int device, const dgen_hip_adamw* a, void* stream);
+int dgen_hip_adamw_workspace(int device, const dgen_hip_adamw* a, uint64_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif
