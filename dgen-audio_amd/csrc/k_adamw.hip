@@ -82,7 +82,15 @@ __global__ __launch_bounds__(kThreads) void k_squares(SquaresP a) {
 __global__ __launch_bounds__(1024) void k_norm_of_squares(const float* __restrict__ parts, int64_t n,
                                                           float* __restrict__ norm) {
   double s = 0.0;
-  for (int64_t i = threadIdx.x; i < n; i += 1024) s += (double)parts[i];
+  int64_t i = threadIdx.x;
+  for (; i + 7 * 1024 < n; i += 8 * 1024) {  // (eight loads in flight)
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = parts[i + k * 1024];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += (double)x[k];
+  }
+  for (; i < n; i += 1024) s += (double)parts[i];
   __shared__ double red[1024];
   red[threadIdx.x] = s;
   __syncthreads();

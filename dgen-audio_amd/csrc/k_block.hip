@@ -108,7 +108,7 @@ struct Cut {
 };
 
 template <class TX, class TS, int TPR, int IT>
-__global__ __launch_bounds__(block_threads<TPR>()) void k_block_norm_bwd(dgen_hip_block_norms a, float inv_n, Cut cut,
+__global__ __launch_bounds__(block_threads<TPR>(), TPR <= 256 ? 4 : 2) void k_block_norm_bwd(dgen_hip_block_norms a, float inv_n, Cut cut,
                                                                         float* __restrict__ parts,
                                                                         float* __restrict__ gate_parts) {
   constexpr int RPB = block_threads<TPR>() / TPR;
@@ -241,17 +241,26 @@ __global__ __launch_bounds__(block_threads<TPR>()) void k_block_norm_bwd(dgen_hi
   }
 }
 
-// A gate's gradient from those of its rows' splits.
+// The last sums: gates' gradients from those of their rows' splits in the first
+// workgroups, the partial rows in the others.
 template <class TX>
-__global__ __launch_bounds__(256) void k_gate_sums(const float* __restrict__ parts, int64_t gates, int64_t splits, int n,
-                                                   TX* __restrict__ out, int64_t stride) {
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+__global__ __launch_bounds__(kSumThreads) void k_block_sums(const float* __restrict__ gate_parts, int64_t gates, int64_t splits,
+                                                            int n, TX* __restrict__ out, int64_t stride, int64_t gate_blocks,
+                                                            const float* __restrict__ parts, int64_t rows, SumOut sums,
+                                                            int64_t width) {
+  __shared__ float red[kSumThreads / kSumCols][kSumCols + 1];
+  if (blockIdx.x >= gate_blocks) return sum_parts_block(parts, rows, sums, width, blockIdx.x - gate_blocks, red);
+  const int64_t at = (int64_t)blockIdx.x * kSumThreads + threadIdx.x;
   if (at >= gates * n) return;
   const int64_t gate = at / n, c = at % n;
-  const float* p = parts + gate * splits * n + c;
-  float t = 0.f;
-  for (int64_t k = 0; k < splits; ++k) t += p[k * n];
-  out[gate * stride + c] = from_f32<TX>(t);
+  const float* p = gate_parts + gate * splits * n + c;
+  float t[4] = {0.f, 0.f, 0.f, 0.f};
+  int64_t k = 0;
+  for (; k + 3 < splits; k += 4)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) t[q] += p[(k + q) * n];
+  for (; k < splits; ++k) t[0] += p[k * n];
+  out[gate * stride + c] = from_f32<TX>((t[0] + t[1]) + (t[2] + t[3]));
 }
 
 // Two or more steps a workgroup, up to four workgroups a CU, as in the norm.
@@ -285,10 +294,11 @@ void block_launch(const dgen_hip_block_norms& a, bool backward, hipStream_t st) 
   float *parts = (float*)a.workspace, *gate_parts = (float*)((char*)a.workspace + parts_bytes(a, c));
   const int64_t groups = c.blocks * c.splits;
   k_block_norm_bwd<TX, TS, TPR, IT><<<dim3((unsigned)groups), T, 0, st>>>(a, inv, c, parts, gate_parts);
-  if (c.shared && c.splits > 1)
-    k_gate_sums<TX><<<dim3((unsigned)((c.gates * a.width + 255) / 256)), 256, 0, st>>>(
-        gate_parts, c.gates, c.splits, (int)a.width, (TX*)a.dgate, a.dgate_stride);
-  enqueue_sum_parts(st, parts, groups, {{a.dpost, a.dpre, a.dscale}, {a.width, a.width, a.scale ? a.width : 0}});
+  const SumOut sums = {{a.dpost, a.dpre, a.dscale}, {a.width, a.width, a.scale ? a.width : 0}};
+  const int64_t width = a.width * (a.scale ? 3 : 2);
+  const int64_t gates = c.shared && c.splits > 1 ? (c.gates * a.width + kSumThreads - 1) / kSumThreads : 0;
+  k_block_sums<TX><<<dim3((unsigned)(gates + (width + kSumCols - 1) / kSumCols)), kSumThreads, 0, st>>>(
+      gate_parts, c.gates, c.splits, (int)a.width, (TX*)a.dgate, a.dgate_stride, gates, parts, groups, sums, width);
 }
 
 template <class TX, class TS>

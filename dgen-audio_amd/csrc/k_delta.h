@@ -130,15 +130,6 @@ struct Tile {
     const int by = kPieces == 4 ? (0x78 >> (row >> 2 & 3) * 2) & 3 : kPieces == 8 ? ((row >> 1) + 6) & 7 : row & 15;
     return row * COLS + ((col / kPiece) ^ by) * kPiece + col % kPiece;
   }
-  __device__ __forceinline__ void put(int row, int col, float x) {
-    const int i = at(row, col);
-#pragma unroll
-    for (int q = 0; q < kParts; ++q) {
-      const T h = (T)x;
-      d[q][i] = h;
-      x -= (float)h;
-    }
-  }
   // Four consecutive columns, from a multiple of four on.
   __device__ __forceinline__ void put4(int row, int col, floatx4 x) {
     const int i = at(row, col);
@@ -499,7 +490,8 @@ struct Split {
   int lane, w, l16, g4, v;  // v: first value of the two tiles
   int wave;
   __device__ __forceinline__ Split() {
-    lane = threadIdx.x & 63, wave = wave_index(), w = wave & 3, l16 = lane & 15, g4 = lane >> 4;
+    // (later rows have more products: a SIMD's two waves take early and late ones)
+    lane = threadIdx.x & 63, wave = wave_index(), w = wave & 4 ? 7 - wave : wave, l16 = lane & 15, g4 = lane >> 4;
     v = (wave >> 2) * 32;
   }
   // the memory's tiles: first channel and value
@@ -1048,7 +1040,8 @@ struct GradLds {
     Tile<E, kGradParts, kC, kC> m[2];
   };
   Tile<E, 1, KP, kC> kt, qt;
-  float gh[kC], gl[kC], rk[kC], db[kC], dots[2][3][kC], over[8];
+  alignas(16) float vec[kVecs * kC], dots[2][3][kC];
+  float db[kC], over[8];
 };
 
 // Eight waves: 16 rows (frames) and half the keys' channels each.
@@ -1058,7 +1051,7 @@ __global__ __launch_bounds__(kGradThreads) void k_delta_grads(DeltaP<E> p) {
   __shared__ GradLds<E, KP> L;
   const int G = p.H / p.shared, c = blockIdx.x % (uint32_t)p.chunks, bg = blockIdx.x / (uint32_t)p.chunks;
   const int b = bg / G, hk = bg % G, t0 = c * kC, live = live_of(p.lengths, b, p.T) - t0;
-  const int lane = threadIdx.x & 63, wave = wave_index(), w = wave & 3, half = wave >> 2, l16 = lane & 15, g4 = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = wave_index(), half = wave >> 2, w = half ? 7 - wave : wave, l16 = lane & 15, g4 = lane >> 4;
   const int row = 16 * w + l16, rows = 16 * w + 4 * g4, k0 = half * (KP / 2) + l16;
   if (live <= 0) {
     for (int i = threadIdx.x; i < kC * p.K; i += kGradThreads) {
@@ -1086,72 +1079,74 @@ __global__ __launch_bounds__(kGradThreads) void k_delta_grads(DeltaP<E> p) {
   // Sum over the 16 lanes of a row.
   auto row_total = [](floatx4 v) {
 #pragma unroll
-    for (int k = 1; k < 16; k *= 2)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] += __shfl_xor(v[e], k, 64);
+    for (int e = 0; e < 4; ++e) {
+      v[e] += dpp<0xB1>(v[e]);
+      v[e] += dpp<0x4E>(v[e]);
+      v[e] += dpp<0x141>(v[e]);  // (the other four of eight, whose sums are alike)
+      v[e] += dpp<0x140>(v[e]);  // (the other eight)
+    }
     return v;
   };
   floatx4 DQ[SHARED ? NK : 1] = {}, DK[NK] = {}, dqz[2][NK], qdq = {0, 0, 0, 0}, kdk = {0, 0, 0, 0}, rootk, rootq;
   for (int n = 0; n < (SHARED ? p.shared : 1); ++n) {
     const int h = hk * p.shared + n;
     const int64_t ci = ((int64_t)b * p.H + h) * p.chunks + c;
-    const float* vec = p.vec + ci * kVecs * kC;
+    const float* const vec = L.vec;
+    floatx4 vx4 = {0, 0, 0, 0};
+    if (threadIdx.x < kVecs * kC / 4) vx4 = load_vec(p.vec + ci * kVecs * kC + threadIdx.x * 4);
     const float *Sp = p.S + ci * KP * p.Vp, *Dp = p.dS + ci * KP * p.Vp;
     const float *Up = p.U + ci * kC * p.Vp, *Rp = p.dR + ci * kC * p.Vp;
-    // A block of 32 values to LDS: four rows of four values a thread, of the states
-    // and their adjoints in the first half, of U and dR in the second.
-    const int it = threadIdx.x & 255, quad = it >> 3, tv = (it & 7) * 4;
-    const bool first_half = threadIdx.x < 256, stages = first_half ? quad < KP / 4 : true;
-    floatx4 ax[4], bx[4];
-    Raw<E> dof, vf;
+    // A block of 32 values to LDS: a thread reads four rows of one value, four times,
+    // the first half of the states and their adjoints, the second of U and of dR.
+    const bool first_half = wave < 4;
+    const int tv = threadIdx.x & 31, each = first_half ? 8 : 4, quad = (threadIdx.x >> 5) & (each - 1);
+    const int quads = first_half ? KP / 4 : kC / 4;
+    const float *const from = first_half ? Sp : wave < 6 ? Up : Rp, *const also = first_half ? Dp : from;
+    struct Ahead {
+      floatx4 a[4], b[4];
+      Raw<E> dof, vf;
+    } ahead;
     auto load = [&](int v0) {
-      if (first_half) {
-        const uint32_t at = (uint32_t)(min(quad, KP / 4 - 1) * p.Vp + v0 + tv) * 4;
+      Ahead& x = ahead;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) ax[e] = load_vec(Sp + at + 4 * e), bx[e] = load_vec(Dp + at + 4 * e);
-      } else {
-        const float* x = quad < 16 ? Up : Rp;
-        const uint32_t at = (uint32_t)((quad & 15) * p.Vp + v0 + tv) * 4;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) ax[e] = load_vec(x + at + 4 * e);
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t at = (uint32_t)(min(quad + each * e, quads - 1) * p.Vp + v0 + tv) * 4;
+        x.a[e] = load_vec(from + at), x.b[e] = load_vec(also + at);
       }
       const int v = v0 + g4 * 8;
-      load_raw<WHOLE>(dof, p.dy.row(b, tc, h), v, p.V);
-      load_raw<WHOLE>(vf, p.v.row(b, tc, h), v, p.V);
+      load_raw<WHOLE>(x.dof, p.dy.row(b, tc, h), v, p.V);
+      load_raw<WHOLE>(x.vf, p.v.row(b, tc, h), v, p.V);
     };
+    const int last = p.Vp - 32;  // (no branches: the last block again where there is none)
     load(0);
-    __syncthreads();
-    if (threadIdx.x < kC) {
-      L.gh[threadIdx.x] = vec[kGHigh * kC + threadIdx.x], L.gl[threadIdx.x] = vec[kGLow * kC + threadIdx.x];
-      L.rk[threadIdx.x] = vec[kRootK * kC + threadIdx.x];
-    }
+    lds_barrier();
+    if (threadIdx.x < kVecs * kC / 4) *reinterpret_cast<floatx4*>(&L.vec[threadIdx.x * 4]) = vx4;
     // (dqz: gradients of the queries, and what the keys read; wr: what they
     // wrote; m: of the first half dy U^T, of the second dR U^T)
-    floatx4 wr[1][NK] = {}, m[4] = {};
+    floatx4 wr[1][NK] = {}, m[1][4] = {};
 #pragma unroll
     for (int k = 0; k < NK; ++k) dqz[0][k] = dqz[1][k] = floatx4{0, 0, 0, 0};
     float sd = 0.f, rv = 0.f;
     for (int v0 = 0; v0 < p.V; v0 += 32) {
       if (v0) lds_barrier();
+      const int tcol = tv & ~3;
       if (first_half) {
-        if (KP == 128 || stages) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const floatx4 x = {ax[0][e], ax[1][e], ax[2][e], ax[3][e]}, y = {bx[0][e], bx[1][e], bx[2][e], bx[3][e]};
-            const floatx4 xy = x * y;
-            sd += (xy[0] + xy[1]) + (xy[2] + xy[3]);
-            L.a.s.put4(4 * quad + e, tv, x);
-            L.a.d.put4(4 * quad + e, tv, y);
-          }
+        for (int e = 0; e < KP / 32; ++e) {
+          const floatx4 xy = ahead.a[e] * ahead.b[e];
+          sd += (xy[0] + xy[1]) + (xy[2] + xy[3]);
+          const int r = 4 * (quad + 8 * e) + (tv & 3);
+          L.a.s.put4(r, tcol, turn(ahead.a[e], lane));
+          L.a.d.put4(r, tcol, turn(ahead.b[e], lane));
         }
       } else {
-        auto& to = quad < 16 ? L.a.u : L.a.r;
+        auto& to = wave < 6 ? L.a.u : L.a.r;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) to.put4(4 * (quad & 15) + e, tv, floatx4{ax[0][e], ax[1][e], ax[2][e], ax[3][e]});
+        for (int e = 0; e < 4; ++e) to.put4(4 * (quad + 4 * e) + (tv & 3), tcol, turn(ahead.a[e], lane));
       }
-      const Wide<E, 1> of[1] = {exact_of<WHOLE>(dof, v0 + g4 * 8, p.V, on)};
-      const floatx8 vx = floats(exact_of<WHOLE>(vf, v0 + g4 * 8, p.V, on));
-      if (v0 + 32 < p.V) load(v0 + 32);  // (in flight through this block's products)
+      const Wide<E, 1> of[1] = {exact_of<WHOLE>(ahead.dof, v0 + g4 * 8, p.V, on)};
+      const floatx8 vx = floats(exact_of<WHOLE>(ahead.vf, v0 + g4 * 8, p.V, on));
+      load(min(v0 + 32, last));  // (in flight through this block's products)
       lds_barrier();
       const Wide<E, kGradParts> rf[1] = {L.a.r.frag(row, g4 * 8)}, uf[1] = {L.a.u.frag(row, g4 * 8)};
       const floatx8 rx = whole_of(rf[0]);
@@ -1168,15 +1163,12 @@ __global__ __launch_bounds__(kGradThreads) void k_delta_grads(DeltaP<E> p) {
         mma(t[0], of, o);
         dqz[0][k] = t[0][0][0], dqz[1][k] = t[1][0][0], wr[0][k] = t[2][0][0];
       }
+      Wide<E, kGradParts> x[4];
 #pragma unroll
-      for (int tj = 0; tj < 4; ++tj)
-        if (tj <= w) {
-          const Wide<E, kGradParts> o[1] = {L.a.u.frag(16 * tj + l16, g4 * 8)};
-          floatx4 t[1][1] = {{m[tj]}};
-          if (half) mma(t, rf, o);
-          else mma(t, of, o);
-          m[tj] = t[0][0];
-        }
+      for (int tj = 0; tj < 4; ++tj) x[tj] = L.a.u.frag(16 * tj + l16, g4 * 8);
+      loads_first();
+      if (half) mma(m, rf, x);
+      else mma(m, of, x);
     }
     const floatx4 beta = load_vec(vec + kBeta * kC + rows), into = load_vec(vec + kInto * kC + rows);
     const floatx4 rest = load_vec(vec + kRest * kC + rows);
@@ -1201,22 +1193,21 @@ __global__ __launch_bounds__(kGradThreads) void k_delta_grads(DeltaP<E> p) {
     // the two triangular matrices by rows, then by columns
 #pragma unroll
     for (int tj = 0; tj < 4; ++tj) {
-      if (tj > w) continue;
+      if (tj > w + 1) continue;  // (neither is read further above the diagonal)
       const int j = 16 * tj + l16;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int i = rows + e;
-        const float d = (half ? j < i : j <= i) ? exp_accurate((L.gh[i] - L.gh[j]) + (L.gl[i] - L.gl[j])) : 0.f;
-        m[tj][e] *= half ? -d : d;
+        const float d = exp_accurate((vec[kGHigh * kC + i] - vec[kGHigh * kC + j]) + (vec[kGLow * kC + i] - vec[kGLow * kC + j]));
+        m[0][tj][e] = (half ? j < i : j <= i) ? m[0][tj][e] * (half ? -d : d) : 0.f;
       }
     }
     lds_barrier();
 #pragma unroll
     for (int tj = 0; tj < 4; ++tj) {
-      if (tj > w + 1 || (tj == w + 1 && (w & 1))) continue;  // (m is 0 above the diagonal)
-      const float root = L.rk[16 * tj + l16];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) L.m[half].put(rows + e, 16 * tj + l16, m[tj][e] * root);
+      if (tj > w + 1 || (tj == w + 1 && (w & 1))) continue;
+      const float root = vec[kRootK * kC + 16 * tj + l16];
+      L.m[half].put4(rows + (l16 & 3), 16 * tj + (l16 & ~3), turn(m[0][tj] * root, l16));
     }
     lds_barrier();
 #pragma unroll
@@ -1234,7 +1225,7 @@ __global__ __launch_bounds__(kGradThreads) void k_delta_grads(DeltaP<E> p) {
 #pragma unroll
     for (int tj = 0; tj < 4; ++tj) {
       if (tj > w + 1 || (tj == w + 1 && (w & 1))) continue;
-      L.m[half].put4(16 * tj + l16, rows, m[tj] * (half ? beta * rootk : rootq));
+      L.m[half].put4(16 * tj + l16, rows, m[0][tj] * (half ? beta * rootk : rootq));
     }
     lds_barrier();
 #pragma unroll
@@ -1273,7 +1264,7 @@ __global__ __launch_bounds__(kGradThreads) void k_delta_grads(DeltaP<E> p) {
     kw = (load_vec(&L.dots[0][2][rows]) + load_vec(&L.dots[1][2][rows])) * rootk;
     qdq += q, kdk += beta * kr + kw;
     if (wave == 0) {
-      const float rk = L.rk[lane], bt = vec[kBeta * kC + lane], rq = vec[kRootQ * kC + lane] * p.scale;
+      const float rk = vec[kRootK * kC + lane], bt = vec[kBeta * kC + lane], rq = vec[kRootQ * kC + lane] * p.scale;
       const float read = (L.dots[0][1][lane] + L.dots[1][1][lane]) * rk;
       float a = (L.dots[0][0][lane] + L.dots[1][0][lane]) * rq + bt * read - (L.dots[0][2][lane] + L.dots[1][2][lane]) * rk;
 #pragma unroll
@@ -1296,18 +1287,18 @@ __global__ __launch_bounds__(kGradThreads) void k_delta_grads(DeltaP<E> p) {
     const floatx4 r = rootq * (1.f / p.scale);
     backq = qdq * r * r, backk = kdk * rootk * rootk;
   }
+  const int trow = rows + (l16 & 3);
+  E *oq = p.dq.row(b, t0 + trow, hk), *ok = p.dk.row(b, t0 + trow, hk);
 #pragma unroll
   for (int k = 0; k < NK; ++k) {
-    const int col = k0 + 16 * k;
-    if (col >= p.K) continue;
-    const floatx4 x = rootq * (SHARED ? DQ[SHARED ? k : 0] : dqz[0][k]) - L.qt.first4(col, rows) * backq, y = rootk * DK[k] - L.kt.first4(col, rows) * backk;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int i = rows + e;
-      if (t0 + i >= p.T) continue;
-      p.dq.row(b, t0 + i, hk)[col] = from_f32<E>(i < live ? x[e] : 0.f);
-      p.dk.row(b, t0 + i, hk)[col] = from_f32<E>(i < live ? y[e] : 0.f);
-    }
+    const int col = k0 + 16 * k, at = (col & ~15) + (l16 & ~3);
+    floatx4 x = turn(rootq * (SHARED ? DQ[SHARED ? k : 0] : dqz[0][k]) - L.qt.first4(col, rows) * backq, l16);
+    floatx4 y = turn(rootk * DK[k] - L.kt.first4(col, rows) * backk, l16);
+    if (trow >= live) x = y = floatx4{0.f, 0.f, 0.f, 0.f};
+    const float xs[4] = {x[0], x[1], x[2], x[3]}, ys[4] = {y[0], y[1], y[2], y[3]};
+    if (t0 + trow >= p.T) continue;
+    store_four(oq + at, p.K - at, xs);
+    store_four(ok + at, p.K - at, ys);
   }
 }
 
@@ -1359,8 +1350,8 @@ __global__ __launch_bounds__(kThreads) void k_delta_step(DeltaP<E> p) {
     }
 #pragma unroll
     for (int e = 0; e < 11; ++e) {
-#pragma unroll
-      for (int k = 8; k < 64; k *= 2) o[e] += __shfl_xor(o[e], k, 64);
+      o[e] += dpp<0x128>(o[e]);  // (lanes 8 apart)
+      o[e] = swap_add32(swap_add16(o[e], o[e]), swap_add16(o[e], o[e]));
       if (lane < 8) red[at][w][l8][e] = o[e];
     }
     __syncthreads();

@@ -105,12 +105,16 @@ __device__ __forceinline__ float softplus_accurate(float x, float& slope) {
 }
 
 // Sum over a row's TPR threads, in every one of them; `red`: LDS of a row of
-// more than a wave (16 floats).
+// more than a wave (16 floats).  Lanes 32, 16, 8, 4, 2 and 1 apart: once those 8
+// apart are added, 4 lanes on within the 16 is as good as 4 apart.
 template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float* red) {
-  // butterfly within the wave (every lane gets the sum)
-#pragma unroll
-  for (int off = (TPR < 64 ? TPR : 64) / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  if constexpr (TPR >= 64) v = swap_add32(v, v);
+  if constexpr (TPR >= 32) v = swap_add16(v, v);
+  v += dpp<0x128>(v);
+  v += dpp<0x124>(v);
+  v += dpp<0x4E>(v);
+  v += dpp<0xB1>(v);
   if constexpr (TPR > 64) {
     constexpr int W = TPR / 64;
     __syncthreads();
