@@ -77,8 +77,8 @@ PyObject* heads(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 // table(lists, types, device index): rows of the addresses of each list's i-th
-// tensor (0 for a list that is None) and their number of elements, as bytes; all
-// contiguous, and those of a row of one shape.
+// tensor (0 for None, in place of a tensor or a list, but for the first) and their
+// number of elements, as bytes; all contiguous, and those of a row of one shape.
 PyObject* table(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     if (n != 3 || !PyTuple_Check(args[0]) || !PyTuple_Check(args[1])) return none_if_wrong();
@@ -100,6 +100,7 @@ PyObject* table(PyObject*, PyObject* const* args, Py_ssize_t n) {
       const at::ScalarType want = type == kF32 ? at::kFloat : type == kBf16 ? at::kBFloat16 : at::ScalarType::Undefined;
       for (Py_ssize_t r = 0; r < rows; ++r) {
         PyObject *o = PyList_GET_ITEM(list, r), *like = PyList_GET_ITEM(first, r);
+        if (o == Py_None && c > 0) continue;
         if (!THPVariable_Check(o)) return none_if_wrong();
         const at::Tensor &t = THPVariable_Unpack(o), &u = THPVariable_Unpack(like);
         if (!t.defined() || t.scalar_type() != want || t.layout() != at::kStrided || !t.is_cuda() ||

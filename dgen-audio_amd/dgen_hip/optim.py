@@ -47,6 +47,9 @@ def _table(lists, types, device) -> bytes:
                 row.append(0)
                 continue
             t = tensors[k]
+            if t is None and name == "copies":
+                row.append(0)
+                continue
             Q._dense(t, f"{name}[{k}]", like.shape, want, device)
             row.append(t.data_ptr())
         rows.append(struct.pack(f"@{len(row)}Qq", *row, like.numel()))
@@ -66,8 +69,8 @@ def adamw(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avg
         p = (1 - lr weight_decay) p - lr (m / (1 - beta1^step)) / (sqrt(v / (1 - beta2^step)) + eps)
 
     Results replace params and moments, or go to ``out`` (three lists: params,
-    exp_avg, exp_avg_sq).  ``copies`` (bfloat16) receive the new params rounded,
-    for the next pass.  With ``max_norm`` the gradients are scaled by min(1,
+    exp_avg, exp_avg_sq).  ``copies`` (bfloat16, or None for a tensor without
+    one) receive the new params rounded, for the next pass.  With ``max_norm`` the gradients are scaled by min(1,
     max_norm / (norm + 1e-6)), and the result is their norm before that, on the
     device; else None."""
     lists = [None if x is None else list(x) for x in (params, grads, exp_avg, exp_avg_sq, *(out or (params, exp_avg, exp_avg_sq)),
@@ -121,7 +124,7 @@ def _library() -> ctypes.CDLL:
 
 class AdamW:
     """AdamW over a model's float32 tensors, in place: their moments, the count
-    of steps, and ``copies`` (bfloat16, one for each tensor, or None) that are
+    of steps, and ``copies`` (bfloat16, one for each tensor or None) that are
     kept equal to the rounded parameters.  The count lies on the device, so a
     captured step counts on when it is replayed."""
 
