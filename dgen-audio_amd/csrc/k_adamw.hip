@@ -154,48 +154,47 @@ int64_t total_groups(const dgen_hip_adamw& a) {
   return s;
 }
 
-// Memory that a step reads or writes.
+// Memory that a step reads or writes: `what` counts a tensor's addresses in their
+// order (0 .. 3 read, 4 .. 7 written).
 struct Range {
   uintptr_t begin, end;
-  int64_t tensor;
-  int role;  // 0 .. 2: parameter and moments, in or out; 3: other inputs; 4: other outputs
-  bool out;
+  int32_t tensor, what;
+  bool out() const { return what >= 4; }
 };
 
 // Whether a result lies where something else does, but for a tensor's own
 // parameter or moment that it replaces.
-int check_apart(const dgen_hip_adamw& a, const char* what) try {
+int check_apart(const dgen_hip_adamw& a, const char* name) try {
   thread_local std::vector<Range> all;
   all.clear();
-  auto add = [&](const void* p, int64_t bytes, int64_t t, int role, bool out) {
-    if (p && bytes > 0) all.push_back({(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes, t, role, out});
+  auto add = [&](const void* p, int64_t bytes, int64_t t, int what) {
+    if (p && bytes > 0) all.push_back({(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes, (int32_t)t, what});
   };
+  const int64_t g = a.grad_type == DGEN_HIP_BF16 ? 2 : 4;
   for (int64_t i = 0; i < a.count; ++i) {
     const dgen_hip_adamw_tensor& t = a.tensors[i];
-    const int64_t n = t.n * 4;
-    add(t.param, n, i, 0, false), add(t.m, n, i, 1, false), add(t.v, n, i, 2, false);
-    add(t.param_out, n, i, 0, true), add(t.m_out, n, i, 1, true), add(t.v_out, n, i, 2, true);
-    add(t.grad, a.grad_type == DGEN_HIP_BF16 ? t.n * 2 : n, i, 3, false);
-    add(t.copy, t.n * 2, i, 4, true);
+    // (what is replaced in place is there once, as a result)
+    if (t.param != t.param_out) add(t.param, t.n * 4, i, 0);
+    add(t.grad, t.n * g, i, 1);
+    if (t.m != t.m_out) add(t.m, t.n * 4, i, 2);
+    if (t.v != t.v_out) add(t.v, t.n * 4, i, 3);
+    add(t.param_out, t.n * 4, i, 4), add(t.m_out, t.n * 4, i, 5), add(t.v_out, t.n * 4, i, 6), add(t.copy, t.n * 2, i, 7);
   }
-  if (a.max_norm > 0) add(a.norm, 4, -1, 4, true);
-  if (a.step_at) add(a.step_at, 8, -1, 3, false);
+  if (a.max_norm > 0) add(a.norm, 4, -1, 4);
+  if (a.step_at) add(a.step_at, 8, -1, 0);
   std::sort(all.begin(), all.end(), [](const Range& x, const Range& y) { return x.begin < y.begin; });
   // against the range so far that reaches furthest, and the result that does
   const Range *far = nullptr, *out = nullptr;
   for (const Range& r : all) {
-    for (const Range* q : {far, out}) {
-      if (!q || q->end <= r.begin || !(q->out || r.out)) continue;
-      const bool own = q->tensor == r.tensor && q->role == r.role && q->role < 3 && q->out != r.out && q->begin == r.begin;
-      DGEN_REQUIRE(own, "%s: a result of tensor %lld shares memory with tensor %lld", what,
-                   (long long)(r.out ? r.tensor : q->tensor), (long long)(r.out ? q->tensor : r.tensor));
-    }
+    for (const Range* q : {far, out})
+      DGEN_REQUIRE(!q || q->end <= r.begin || !(q->out() || r.out()), "%s: a result of tensor %d shares memory with tensor %d", name,
+                   r.out() ? r.tensor : q->tensor, r.out() ? q->tensor : r.tensor);
     if (!far || r.end > far->end) far = &r;
-    if (r.out && (!out || r.end > out->end)) out = &r;
+    if (r.out() && (!out || r.end > out->end)) out = &r;
   }
   return 0;
 } catch (...) {
-  return fail(DGEN_HIP_E_DEVICE, "%s: out of host memory", what);
+  return fail(DGEN_HIP_E_DEVICE, "%s: out of host memory", name);
 }
 
 }  // namespace
@@ -226,7 +225,9 @@ int adamw_run(const dgen_hip_adamw& a, hipStream_t st, bool dry) {
                    "%s: tensor %lld: null address", what, (long long)i);
     }
     DGEN_REQUIRE(total_groups(a) < int64_t(1) << 31, "%s: too many elements", what);
-    if (int rc = check_apart(a, what)) return rc;
+    // (the workspace's size does not go by the places)
+    if (a.workspace_bytes != ~0ull)
+      if (int rc = check_apart(a, what)) return rc;
     const int64_t need = adamw_workspace(a);
     DGEN_REQUIRE(need == 0 || (a.workspace && a.workspace_bytes >= (uint64_t)need),
                  "%s: workspace of %llu bytes, %lld needed", what, (unsigned long long)a.workspace_bytes, (long long)need);

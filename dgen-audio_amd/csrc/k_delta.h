@@ -391,6 +391,8 @@ __global__ __launch_bounds__(kThreads) void k_delta_prepare(DeltaP<E> p) {
       A[i][j] = j < i ? kk[r] * (rk[i] * rk[j]) * d * bt[i] : 0.f;
       qk[r] = j <= i ? qk[r] * (rq[i] * rk[j] * p.scale) * d : 0.f;
     }
+    // (the quarter above the diagonal, whose products are left out, is not stored)
+    if (w < 2 && tj >= 2) continue;
     if (p.XT) {
       *reinterpret_cast<floatx4*>(Mp + j * kC + 16 * w + 4 * g4) = qk;
     } else {
@@ -440,8 +442,8 @@ __global__ __launch_bounds__(kThreads) void k_delta_prepare(DeltaP<E> p) {
   for (int i = 0; i < kC * kC / 4 / kThreads; ++i) {
     const int r = threadIdx.x / 16 + 16 * i, col = threadIdx.x % 16 * 4;
     const floatx4 x = *reinterpret_cast<const floatx4*>(&X[r][col]);
-    *reinterpret_cast<floatx4*>(Xp + r * kC + col) = col / 16 <= r / 16 ? x : floatx4{0, 0, 0, 0};
-    if (p.XT) {
+    if (col < 32 || r >= 32) *reinterpret_cast<floatx4*>(Xp + r * kC + col) = col / 16 <= r / 16 ? x : floatx4{0, 0, 0, 0};
+    if (p.XT && (col >= 32 || r < 32)) {
       const floatx4 y = {X[col][r], X[col + 1][r], X[col + 2][r], X[col + 3][r]};
       *reinterpret_cast<floatx4*>(p.XT + ci * kC * kC + r * kC + col) = col / 16 >= r / 16 ? y : floatx4{0, 0, 0, 0};
     }
@@ -1118,7 +1120,7 @@ __global__ __launch_bounds__(kGradThreads) void k_delta_grads(DeltaP<E> p) {
       load_raw<WHOLE>(x.vf, p.v.row(b, tc, h), v, p.V);
     };
     const int last = p.Vp - 32;  // (no branches: the last block again where there is none)
-    load(0);
+    if constexpr (!SHARED) load(0);
     lds_barrier();
     if (threadIdx.x < kVecs * kC / 4) *reinterpret_cast<floatx4*>(&L.vec[threadIdx.x * 4]) = vx4;
     // (dqz: gradients of the queries, and what the keys read; wr: what they
@@ -1128,6 +1130,7 @@ __global__ __launch_bounds__(kGradThreads) void k_delta_grads(DeltaP<E> p) {
     for (int k = 0; k < NK; ++k) dqz[0][k] = dqz[1][k] = floatx4{0, 0, 0, 0};
     float sd = 0.f, rv = 0.f;
     for (int v0 = 0; v0 < p.V; v0 += 32) {
+      if constexpr (SHARED) load(v0);  // (its registers hold the sums over heads)
       if (v0) lds_barrier();
       const int tcol = tv & ~3;
       if (first_half) {
@@ -1146,7 +1149,7 @@ __global__ __launch_bounds__(kGradThreads) void k_delta_grads(DeltaP<E> p) {
       }
       const Wide<E, 1> of[1] = {exact_of<WHOLE>(ahead.dof, v0 + g4 * 8, p.V, on)};
       const floatx8 vx = floats(exact_of<WHOLE>(ahead.vf, v0 + g4 * 8, p.V, on));
-      load(min(v0 + 32, last));  // (in flight through this block's products)
+      if constexpr (!SHARED) load(min(v0 + 32, last));  // (in flight through this block's products)
       lds_barrier();
       const Wide<E, kGradParts> rf[1] = {L.a.r.frag(row, g4 * 8)}, uf[1] = {L.a.u.frag(row, g4 * 8)};
       const floatx8 rx = whole_of(rf[0]);
@@ -1284,7 +1287,7 @@ __global__ __launch_bounds__(kGradThreads) void k_delta_grads(DeltaP<E> p) {
   // through the scales and the norms: x^ = x r, r = 1 / sqrt(|x|^2 + eps)
   floatx4 backq = {0, 0, 0, 0}, backk = {0, 0, 0, 0};
   if (p.normalize) {
-    const floatx4 r = rootq * (1.f / p.scale);
+    const floatx4 r = load_vec(&L.vec[kRootQ * kC + rows]);
     backq = qdq * r * r, backk = kdk * rootk * rootk;
   }
   const int trow = rows + (l16 & 3);

@@ -93,13 +93,13 @@ int delta_run(const dgen_hip_delta& a, bool backward, hipStream_t st, bool dry) 
     return (h.data || empty) && h.stride_b >= 0 && near(h.stride_t) && h.stride_h >= 0 &&
            heads_writable(h.stride_b, h.stride_t, h.stride_h, a.batch, a.T, heads, n);
   };
-  DGEN_REQUIRE(readable(a.q) && readable(a.k) && readable(a.v), "%s: q, k or v: null, or a stride below 0 or of more than 2^23 between frames", what);
-  DGEN_REQUIRE(((a.g.data && a.beta.data) || empty) && seq_readable(a.g) && seq_readable(a.beta), "%s: g or beta: null, or a stride below 0 or of more than 2^23 between frames",
+  DGEN_REQUIRE(readable(a.q) && readable(a.k) && readable(a.v), "%s: q, k or v: null, or a negative stride, or more than 2^23 between frames", what);
+  DGEN_REQUIRE(((a.g.data && a.beta.data) || empty) && seq_readable(a.g) && seq_readable(a.beta), "%s: g or beta: null, or a negative stride, or more than 2^23 between frames",
                what);
   if (!backward) {
     DGEN_REQUIRE(writable(a.y, a.heads, a.V), "%s: y: null, overlapping, or frames too far apart", what);
   } else {
-    DGEN_REQUIRE(readable(a.dy), "%s: dy: null, or a stride below 0 or of more than 2^23 between frames", what);
+    DGEN_REQUIRE(readable(a.dy), "%s: dy: null, or a negative stride, or more than 2^23 between frames", what);
     DGEN_REQUIRE(writable(a.dq, a.key_heads, a.K) && writable(a.dk, a.key_heads, a.K) && writable(a.dv, a.heads, a.V),
                  "%s: dq, dk or dv: null, overlapping, or frames too far apart", what);
     DGEN_REQUIRE(((a.dg.data && a.dbeta.data) || empty) && seq_writable(a.dg, a.batch, a.T, a.heads) &&

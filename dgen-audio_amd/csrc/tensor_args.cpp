@@ -104,8 +104,7 @@ PyObject* table(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (!THPVariable_Check(o)) return none_if_wrong();
         const at::Tensor &t = THPVariable_Unpack(o), &u = THPVariable_Unpack(like);
         if (!t.defined() || t.scalar_type() != want || t.layout() != at::kStrided || !t.is_cuda() ||
-            t.get_device() != index || t.sizes() != u.sizes() || !t.is_contiguous() ||
-            (t.requires_grad() && c10::GradMode::is_enabled()))
+            t.get_device() != index || t.sizes() != u.sizes() || !t.is_contiguous())
           return none_if_wrong();
         out[(size_t)(r * (columns + 1) + c)] = (int64_t)address(t);
         out[(size_t)(r * (columns + 1) + columns)] = t.numel();

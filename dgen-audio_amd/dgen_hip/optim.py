@@ -41,6 +41,8 @@ def _table(lists, types, device) -> bytes:
             raise ValueError(f"{name}: {len(lists[0])} tensors expected, got {len(tensors)}")
     for k, like in enumerate(lists[0]):
         row = []
+        if not isinstance(like, torch.Tensor):
+            raise Q._wrong(f"params[{k}]", like, "a float32 tensor")
         for name, ty, tensors in zip(_NAMES, types, lists):
             want = torch.bfloat16 if ty == _BF16 else torch.float32
             if tensors is None:
@@ -50,7 +52,10 @@ def _table(lists, types, device) -> bytes:
             if t is None and name == "copies":
                 row.append(0)
                 continue
-            Q._dense(t, f"{name}[{k}]", like.shape, want, device)
+            if not isinstance(t, torch.Tensor) or t.dtype is not want or t.shape != like.shape or t.device != device:
+                raise Q._wrong(f"{name}[{k}]", t, f"{tuple(like.shape)} {want} on {device}")
+            if not t.is_contiguous():
+                raise ValueError(f"{name}[{k}]: must be contiguous")
             row.append(t.data_ptr())
         rows.append(struct.pack(f"@{len(row)}Qq", *row, like.numel()))
     return b"".join(rows)

@@ -637,9 +637,9 @@ def _block_parts(x, post_weight, pre_weight, gate, gate_activation, residual_sca
     i, width, count, each, gp = dev.index, shape[-1:], _count(shape), 1, _NO_ROWS
     if gate is not None:
         its = shape
-        if isinstance(gate, torch.Tensor) and gate.dim() == x.dim() and gate.shape[-2] == 1 and count:
+        if isinstance(gate, torch.Tensor) and gate.dim() == x.dim() and gate.shape[-2] == 1:
             # one gate for all the rows of an axis
-            each, its = shape[-2], (*shape[:-2], 1, shape[-1])
+            each, its = max(1, shape[-2]), (*shape[:-2], 1, shape[-1])
         gp = rows(gate, its, ty, i) or _rows(gate, "gate", its, et, dev)
     return (_BLOCK_SIZE, ty, st, act, count, shape[-1], each, eps,
             dense(post_weight, width, _F32, i) or _dense(post_weight, "post_weight", width, f32, dev),
@@ -701,4 +701,6 @@ def block_norm_backward(dy, x, residual, s, post_weight, pre_weight, gate=None, 
                     *(_NO_ROWS if ds is None else rows(ds, shape, st, i) or _rows(ds, "ds", shape, s.dtype, dev)),
                     *dxp, *drp, *dgp, dpost.data_ptr(), dpre.data_ptr(), 0 if dscale is None else dscale.data_ptr())
     _op("block_norm")(d, dev, True, True)
+    if dgate is not None and not head[4]:
+        dgate.zero_()  # (gates of no rows)
     return BlockNormGrads(dx, dr, dgate, dpost, dpre, dscale)
