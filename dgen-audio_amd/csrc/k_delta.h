@@ -473,9 +473,9 @@ struct Place {
   int b, h, hk, bh, vb, seg;
 };
 template <class E>
-__device__ __forceinline__ Place place_of(const DeltaP<E>& p, int blocks) {
+__device__ __forceinline__ Place place_of(const DeltaP<E>& p, int blocks, uint32_t block, uint32_t of) {
   Place o;
-  uint32_t i = xcd_order(blockIdx.x, gridDim.x);
+  uint32_t i = xcd_order(block, of);
   o.vb = i % (uint32_t)blocks, i /= (uint32_t)blocks;
   o.seg = i % (uint32_t)p.segs, i /= (uint32_t)p.segs;
   o.bh = i;
@@ -603,19 +603,26 @@ __device__ __forceinline__ void store_zeros(const Heads<E>& a, const Place& at, 
     if (v0 + i % VB < V) a.row(at.b, t0 + i / VB, at.h)[v0 + i % VB] = from_f32<E>(0.f);
 }
 
+template <class E, int KP, int VB, Mode MODE>
+struct ChainLds {
+  Tile<E, kState, VB, KP> s;
+  Tile<E, kState, VB, kC> r, wr;
+  Tile<E, kResult, MODE == kOut ? VB : 1, kC> u;
+  Tile<E, 1, KP, kC> kt;
+};
 // The memory's states along a segment's chunks.
 template <class E, int KP, int VB, Mode MODE, bool WHOLE>
-__global__ __launch_bounds__(VB * 8) void k_delta_chain(DeltaP<E> p) {
+__device__ __forceinline__ void delta_chain(const DeltaP<E>& p, ChainLds<E, KP, VB, MODE>& L, uint32_t block, uint32_t blocks) {
   using W = Split<KP, VB>;
   constexpr int NF = W::NF, NV = W::NV, NKT = W::NKT, NVT = W::NVT;
-  __shared__ Tile<E, kState, VB, KP> s;
-  __shared__ Tile<E, kState, VB, kC> r, wr;
-  __shared__ Tile<E, kResult, MODE == kOut ? VB : 1, kC> u;
-  __shared__ Tile<E, 1, KP, kC> kt;
+  auto &s = L.s;
+  auto &r = L.r, &wr = L.wr;
+  auto& u = L.u;
+  auto& kt = L.kt;
   const W me;
   const int l16 = me.l16, g4 = me.g4;
   const int nvb = MODE == kEnds ? p.nvb + (KP + VB - 1) / VB : p.nvb;
-  const Place at = place_of(p, nvb);
+  const Place at = place_of(p, nvb, block, blocks);
   const int live = live_of(p.lengths, at.b, p.T);
   // (ends: the transition is the state's own columns, from the identity on and
   // with nothing written)
@@ -781,13 +788,18 @@ __global__ __launch_bounds__(VB * 8) void k_delta_chain(DeltaP<E> p) {
   }
 }
 
+template <class E, int KP, int VB, bool WHOLE>
+__global__ __launch_bounds__(VB * 8) void k_delta_forward(DeltaP<E> p) {
+  __shared__ ChainLds<E, KP, VB, kOut> lds;
+  delta_chain<E, KP, VB, kOut, WHOLE>(p, lds, blockIdx.x, gridDim.x);
+}
+
 // The states that enter the segments (BACK: the adjoints after them) from the
 // segments' ends from zero and their transitions, in the ends' place.
 template <class E, int KP, bool BACK>
-__global__ __launch_bounds__(kThreads) void k_delta_carry(DeltaP<E> p) {
+__device__ __forceinline__ void delta_carry(const DeltaP<E>& p, int block, Tile<float, 1, 16, KP> (&s)[2]) {
   constexpr int VB = 16, NF = KP / 32, NT = KP / 64 > 0 ? KP / 64 : 1;  // (16 values a workgroup, tiles of a wave)
-  __shared__ Tile<float, 1, VB, KP> s[2];
-  const int nvb = p.Vp / VB, vb = blockIdx.x % (uint32_t)nvb, bh = blockIdx.x / (uint32_t)nvb;
+  const int nvb = p.Vp / VB, vb = block % nvb, bh = block / nvb;
   const int lane = threadIdx.x & 63, w = wave_index(), l16 = lane & 15, g4 = lane >> 4, ld = p.Vp + KP;
   const int v = vb * VB + l16;
   const bool on = w * 16 < KP;  // (32 channels: two waves)
@@ -854,25 +866,41 @@ __global__ __launch_bounds__(kThreads) void k_delta_carry(DeltaP<E> p) {
   }
 }
 
-// The adjoints of the memory's states, against time.  Leaves dv, and dR.
-template <class E, int KP, int VB, Mode MODE, bool WHOLE>
-__global__ __launch_bounds__(VB * 8) void k_delta_back(DeltaP<E> p) {
-  using W = Split<KP, VB>;
-  constexpr int NF = W::NF, NV = W::NV, NKT = W::NKT, NVT = W::NVT;
+// (`both`: the first half of the workgroups one way, the second the other)
+template <class E, int KP>
+__global__ __launch_bounds__(kThreads) void k_delta_carry(DeltaP<E> p, bool both) {
+  __shared__ Tile<float, 1, 16, KP> s[2];
+  const int n = both ? gridDim.x / 2 : gridDim.x;
+  if ((int)blockIdx.x < n) delta_carry<E, KP, false>(p, blockIdx.x, s);
+  else delta_carry<E, KP, true>(p, blockIdx.x - n, s);
+}
+
+template <class E, int KP, int VB>
+struct BackLds {
   // (the adjoints' parts are read in a chunk's first products alone: what the
   // later ones take lies in their place)
-  __shared__ union {
+  union {
     Tile<E, kState, VB, KP> s;
     Tile<E, kState, VB, kC> d[2];
   } x;
-  __shared__ Tile<E, 1, VB, kC> dyt;
-  __shared__ Tile<E, kState, VB, kC> qdy;
-  __shared__ Tile<E, 1, KP, kC> kt, qt;
+  Tile<E, 1, VB, kC> dyt;
+  Tile<E, kState, VB, kC> qdy;
+  Tile<E, 1, KP, kC> kt, qt;
+};
+// The adjoints of the memory's states, against time.  Leaves dv, and dR.
+template <class E, int KP, int VB, Mode MODE, bool WHOLE>
+__device__ __forceinline__ void delta_back(const DeltaP<E>& p, BackLds<E, KP, VB>& L, uint32_t block, uint32_t blocks) {
+  using W = Split<KP, VB>;
+  constexpr int NF = W::NF, NV = W::NV, NKT = W::NKT, NVT = W::NVT;
+  auto& x = L.x;
+  auto& dyt = L.dyt;
+  auto& qdy = L.qdy;
+  auto &kt = L.kt, &qt = L.qt;
   Tile<E, kState, VB, KP>& s = x.s;
   Tile<E, kState, VB, kC>&du = x.d[0], &dr = x.d[1];
   const W me;
   const int l16 = me.l16, g4 = me.g4;
-  const Place at = place_of(p, p.nvb);
+  const Place at = place_of(p, p.nvb, block, blocks);
   const int live = live_of(p.lengths, at.b, p.T);
   const int v0 = at.vb * VB;
   const int64_t end = ((int64_t)at.bh * p.segs + at.seg) * KP;
@@ -1026,6 +1054,19 @@ __global__ __launch_bounds__(VB * 8) void k_delta_back(DeltaP<E> p) {
   if constexpr (MODE == kEnds) {
     DGEN_TILES(p.gends[(end + k + e) * p.Vp + v] = S[i][j][e];)
   }
+}
+
+// Both ways at once, as neither waits for the other: the first `forward`
+// workgroups with time, the others against it.  kEnds: the segments' ends (those
+// with time alone in a call that is not backward).
+template <class E, int KP, int VB, Mode MODE, bool WHOLE>
+__global__ __launch_bounds__(VB * 8) void k_delta_both(DeltaP<E> p, uint32_t forward) {
+  __shared__ union {
+    ChainLds<E, KP, VB, MODE> chain;
+    BackLds<E, KP, VB> back;
+  } lds;
+  if (blockIdx.x < forward) delta_chain<E, KP, VB, MODE, WHOLE>(p, lds.chain, blockIdx.x, forward);
+  else delta_back<E, KP, VB, MODE, WHOLE>(p, lds.back, blockIdx.x - forward, gridDim.x - forward);
 }
 
 // -------------------------------------------------------------------- grads
@@ -1394,19 +1435,12 @@ void delta_chains(const DeltaP<E>& p, const DeltaPlan& o, int64_t bh, bool backw
   constexpr int n = VB * 8;
   const int64_t blocks = bh * o.nvb * o.segs, carry = bh * (p.Vp / 16);
   if (o.segs > 1) {
-    k_delta_chain<E, KP, VB, kEnds, WHOLE><<<grid(bh * o.segs * (o.nvb + (KP + VB - 1) / VB)), n, 0, st>>>(p);
-    k_delta_carry<E, KP, false><<<grid(carry), kThreads, 0, st>>>(p);
+    const int64_t ends = bh * o.segs * (o.nvb + (KP + VB - 1) / VB);
+    k_delta_both<E, KP, VB, kEnds, WHOLE><<<grid(ends + (backward ? blocks : 0)), n, 0, st>>>(p, (uint32_t)ends);
+    k_delta_carry<E, KP><<<grid(backward ? 2 * carry : carry), kThreads, 0, st>>>(p, backward);
   }
-  if (!backward) {
-    k_delta_chain<E, KP, VB, kOut, WHOLE><<<grid(blocks), n, 0, st>>>(p);
-    return;
-  }
-  k_delta_chain<E, KP, VB, kKeep, WHOLE><<<grid(blocks), n, 0, st>>>(p);
-  if (o.segs > 1) {
-    k_delta_back<E, KP, VB, kEnds, WHOLE><<<grid(blocks), n, 0, st>>>(p);
-    k_delta_carry<E, KP, true><<<grid(carry), kThreads, 0, st>>>(p);
-  }
-  k_delta_back<E, KP, VB, kKeep, WHOLE><<<grid(blocks), n, 0, st>>>(p);
+  if (backward) k_delta_both<E, KP, VB, kKeep, WHOLE><<<grid(2 * blocks), n, 0, st>>>(p, (uint32_t)blocks);
+  else k_delta_forward<E, KP, VB, WHOLE><<<grid(blocks), n, 0, st>>>(p);
 }
 
 template <class E, int KP, bool WHOLE>
