@@ -1,4 +1,62 @@
-// Gated delta rule, forward and backward.
+// Gated delta rule, forward and backward.  Per sequence and head a memory S of
+// K x V numbers, frame by frame
+//   S' = e^g S,  u = beta (v - S'^T k^),  S = S' + k^ u^T,  y = scale S^T q^
+// with q^ and k^ the queries and keys, or these over their norms.
+//
+// A memory that is rewritten each frame is a chain of outer products; matrix
+// instructions need it by chunks.  With G(i) the sum of a chunk's gates up to
+// frame i, d(i, j) = e^(G(i) - G(j)) for j <= i and S the memory that enters,
+// the u of a chunk's frames solve
+//   (I + A) U = r,  A(i, j) = beta(i) d(i, j) k^(i).k^(j) for j < i,
+//   r(i) = beta(i) (v(i) - e^G(i) S^T k^(i)),
+// so that with X = (I + A)^-1, which does not depend on S,
+//   U = X r,  y = scale (e^G S^T q^ + (d q^.k^) U),  S <- e^G(end) S + k^T (d(end, .) U).
+// A sum of gates is held in two floats (from a sum in 64 bits): a difference of
+// two far sums is then right to the last bits.
+//
+// Launches: prepare (a workgroup per chunk and head: X, the queries' products
+// with the keys, decays, norms), then the chain (a workgroup per head and block
+// of values walks the chunks: three products and two of a triangle a chunk, the
+// memory in registers, its parts in LDS).  Backward the chain keeps the memory
+// that enters each chunk and U; the adjoints' chain, which needs neither, walks
+// the other way in the same launch and keeps the adjoint D of the memory after
+// each chunk and dR of r; the gradients of q, k, g and beta are then a launch
+// with a workgroup per chunk, from products over the values:
+//   dq^ = e^G dy S^T + (d dy U^T) k^,  dk^ = -beta (e^G dR S^T + (d dR U^T) k^)
+//   + e^(G(end) - G) U D^T + the transposes of these,
+//   dg(i) = sum over j >= i of q^.dq^ + k^.(dk^ as read) - k^.(dk^ as written), with
+//   <S, D> and the writes over the chunk's end,  dbeta = dR.(v - S'^T k^).
+// Few heads and a long axis: the chunks are cut into segments.  A segment is an
+// affine map of the memory, so each is run from zero and, with the identity as
+// its memory and nothing written, as a transition; a short chain over the
+// segments' ends gives the memories that enter them (k_delta.hip has when).
+//
+// Chunks of 64 frames: a chunk costs 4 K V 64 operations for the memory, a share
+// that does not depend on its length, and 64 (K + V) a frame within it, which does;
+// at K = V = 128 the two are alike, and its triangles fit next to the memory.  Blocks
+// of 64 values and eight waves where that fills the card, else of 32 and four:
+// a chunk's keys are read and turned once for twice the values (chain of 32 x
+// 1000 x 8 heads of 128, forward: 225 us, 212 in blocks of 32; adjoints: 345 and
+// 386; both in one launch 503).
+//
+// Precision: operands that are bf16 go to the bf16 instructions as they are.
+// Numbers held in 32 bits (memories, adjoints, U, dR, X) are split into three
+// bf16 parts, whose products of up to 2^-16 are kept: 24 bits, as fp32 products
+// have, at a sixth to a third of the bf16 rate, still above the fp32 instructions'.
+// Where only y, rounded to bf16, is left of a product two parts are taken
+// (2^-17 against 2^-9).  fp32 operands go to the fp32 instructions.
+//
+// What bounds it: 32 x 1000 x 8 heads of K = V = 128 in bf16 read and write 281 MB
+// (55 us at 5.1 TB/s) in 0.26 ms; prepare has 67 and the chain 222 us when profiled.
+// The matrix instructions are busy for a fifth of it, vector instructions (parts,
+// turning) for 45 %; the rest is waits at three barriers a chunk with one
+// workgroup of eight waves a CU (130 KB of LDS).  Backward 463 MB (91 us) take
+// 0.94 ms: prepare 76, the two chains 503, gradients 500 us.  The kept memories
+// and adjoints are 0.8 GB more, written and read again; a chain that took the
+// gradients as it goes would need all of V in one workgroup, 256 of them here,
+// and the sums over V in its registers.  A call of few frames goes frame by frame
+// with the memory in registers: 32 sequences of 8 heads, fp32, take 10 us for one
+// frame (34 MB: 6.7 us).
 #pragma once
 
 #include "seq.h"
@@ -13,6 +71,11 @@ struct DeltaPlan {
   int64_t chunks, vb, nvb, segs, per;  // vb: values of a workgroup, per: chunks of a segment
   int64_t X, M, XT, vec, S, dS, U, dR, ends, gends, bytes;
 };
+// Whether a call goes frame by frame: a chunk costs its 64 frames (32 sequences of 8
+// heads of 128: 30 us in bf16, 55 in fp32), a frame 2 us.
+inline bool delta_steps(const dgen_hip_delta& a, bool backward) {
+  return !backward && a.T <= (a.type == DGEN_HIP_BF16 ? 12 : 16);
+}
 DeltaPlan delta_plan(const dgen_hip_delta&, bool backward);
 void delta_enqueue_f32(const dgen_hip_delta&, bool backward, hipStream_t);
 void delta_enqueue_bf16(const dgen_hip_delta&, bool backward, hipStream_t);
@@ -25,7 +88,6 @@ typedef float floatx8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256;
-constexpr int kStepFrames = 16;  // calls of so few go frame by frame
 constexpr float kUnitEps = 1e-6f;
 
 // Parts of fp32 numbers in bf16 products: of what goes into the memory, and of
@@ -292,7 +354,7 @@ struct DeltaP {
   float* state_out;
   float scale;
   int normalize;
-  int B, T, H, shared, K, V;
+  int T, H, shared, K, V;
   int chunks, nvb, segs, per;  // chunks a segment
   // The workspace, with KP for K and Vp, whole blocks of values, for V (0 in
   // what is between).
@@ -1468,14 +1530,14 @@ void delta_launch(const dgen_hip_delta& a, bool backward, hipStream_t st) {
   p.g = gates(a.g), p.beta = gates(a.beta), p.dg = gates(a.dg), p.dbeta = gates(a.dbeta);
   p.lengths = a.lengths, p.state = a.state, p.state_out = a.state_out;
   p.scale = a.scale, p.normalize = a.normalize;
-  p.B = (int)a.batch, p.T = (int)a.T, p.H = (int)a.heads, p.shared = (int)(a.heads / a.key_heads), p.K = (int)a.K, p.V = (int)a.V;
+  p.T = (int)a.T, p.H = (int)a.heads, p.shared = (int)(a.heads / a.key_heads), p.K = (int)a.K, p.V = (int)a.V;
   p.Vp = (int)(o.nvb * o.vb);
   p.chunks = (int)o.chunks, p.nvb = (int)o.nvb, p.segs = (int)o.segs, p.per = (int)o.per;
   auto at = [&](int64_t off) { return (float*)((char*)a.workspace + off); };
   p.X = at(o.X), p.M = at(o.M), p.XT = backward ? at(o.XT) : nullptr, p.vec = at(o.vec), p.S = at(o.S), p.dS = at(o.dS), p.U = at(o.U), p.dR = at(o.dR);
   p.ends = at(o.ends), p.gends = at(o.gends);
   const int64_t bh = a.batch * a.heads;
-  if (!backward && a.T <= kStepFrames)
+  if (delta_steps(a, backward))
     k_delta_step<E, KP><<<dim3((unsigned)(bh * ((a.V + 31) / 32))), kThreads, 0, st>>>(p);
   else if (a.K % 8 == 0 && a.V % 8 == 0) delta_kernels<E, KP, true>(p, o, bh, backward, st);
   else delta_kernels<E, KP, false>(p, o, bh, backward, st);

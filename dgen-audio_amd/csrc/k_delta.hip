@@ -2,6 +2,8 @@
 // kernels).
 #include "k_delta.h"
 
+#include <cmath>
+
 namespace dgen {
 
 namespace {
@@ -28,18 +30,23 @@ bool heads_writable(int64_t sb, int64_t st, int64_t sh, int64_t B, int64_t T, in
 
 DeltaPlan delta_plan(const dgen_hip_delta& a, bool backward) {
   DeltaPlan o = {};
-  if ((!backward && a.T <= kStepFrames) || a.batch == 0) return o;
-  const int64_t bh = a.batch * a.heads;
+  if (delta_steps(a, backward) || a.batch == 0) return o;
+  const int64_t bh = a.batch * a.heads, K = a.K <= 32 ? 32 : a.K <= 64 ? 64 : 128;
   o.chunks = (a.T + kC - 1) / kC;
   o.segs = 1;
   // 64 values a workgroup of eight waves where that fills the CUs
   o.vb = a.V > 32 && bh * ((a.V + 63) / 64) >= 192 ? 64 : 32;
   o.nvb = (a.V + o.vb - 1) / o.vb;
-  if (bh * o.nvb < 192) {
-    // (a segment costs its chunks twice, and a step of the carry)
-    o.segs = std::min<int64_t>((512 + bh * o.nvb - 1) / (bh * o.nvb), o.chunks / 8);
-    if (o.segs < 4) o.segs = 1;
-  }
+  // Segments go through their chunks twice, the second time with their transitions
+  // too, and each is a step of the carry: three times the work, so that they pay
+  // where the card is a third full at most (with 128 channels, whose steps of the
+  // carry are dearer, less).  The square root of the chunks balances both walks.
+  // One piece and segments, us, forward, fp32 64 x 64: 1 head of 512 frames 50 and
+  // 34, of 65536 4294 and 186, 24 heads of 1024 89 and 66, of 512 52 and 50; bf16
+  // 128 x 128: 8 heads of 2048 130 and 78, of 512 44 and 50, 24 of 1024 80 and 93.
+  const bool wide = K > 64;
+  if (bh * o.nvb <= (wide ? 40 : 96) && o.chunks >= (wide ? 12 : 8))
+    o.segs = std::min<int64_t>((int64_t)((wide ? 1.5 : 3.) * std::sqrt((double)o.chunks)), 512 / (bh * o.nvb));
   o.per = (o.chunks + o.segs - 1) / o.segs;
   o.segs = (o.chunks + o.per - 1) / o.per;
   int64_t at = 0;
@@ -48,7 +55,7 @@ DeltaPlan delta_plan(const dgen_hip_delta& a, bool backward) {
     at += align256(floats * 4);
     return p;
   };
-  const int64_t n = bh * o.chunks, K = a.K <= 32 ? 32 : a.K <= 64 ? 64 : 128, V = o.nvb * o.vb;
+  const int64_t n = bh * o.chunks, V = o.nvb * o.vb;
   o.X = take(n * kC * kC);
   o.M = take(n * kC * kC);
   if (backward) o.XT = take(n * kC * kC);
@@ -94,8 +101,7 @@ int delta_run(const dgen_hip_delta& a, bool backward, hipStream_t st, bool dry) 
            heads_writable(h.stride_b, h.stride_t, h.stride_h, a.batch, a.T, heads, n);
   };
   DGEN_REQUIRE(readable(a.q) && readable(a.k) && readable(a.v), "%s: q, k or v: null, or a negative stride, or more than 2^23 between frames", what);
-  DGEN_REQUIRE(((a.g.data && a.beta.data) || empty) && seq_readable(a.g) && seq_readable(a.beta), "%s: g or beta: null, or a negative stride, or more than 2^23 between frames",
-               what);
+  DGEN_REQUIRE(((a.g.data && a.beta.data) || empty) && seq_readable(a.g) && seq_readable(a.beta), "%s: g or beta: null, or a negative stride", what);
   if (!backward) {
     DGEN_REQUIRE(writable(a.y, a.heads, a.V), "%s: y: null, overlapping, or frames too far apart", what);
   } else {
