@@ -34,10 +34,9 @@
 // Chunks of 64 frames: a chunk costs 4 K V 64 operations for the memory, a share
 // that does not depend on its length, and 64 (K + V) a frame within it, which does;
 // at K = V = 128 the two are alike, and its triangles fit next to the memory.  Blocks
-// of 64 values and eight waves where that fills the card, else of 32 and four:
-// a chunk's keys are read and turned once for twice the values (chain of 32 x
-// 1000 x 8 heads of 128, forward: 225 us, 212 in blocks of 32; adjoints: 345 and
-// 386; both in one launch 503).
+// of 32 values and four waves, two of them a CU: of 64 and eight, one a CU, they
+// read and turn a chunk's keys half as often, and yet wait longer (400 heads of
+// 1000 frames, 128 x 128: 469 against 403 us in bf16, 1264 against 972 in fp32).
 //
 // Precision: operands that are bf16 go to the bf16 instructions as they are.
 // Numbers held in 32 bits (memories, adjoints, U, dR, X) are split into three
@@ -47,11 +46,11 @@
 // (2^-17 against 2^-9).  fp32 operands go to the fp32 instructions.
 //
 // What bounds it: 32 x 1000 x 8 heads of K = V = 128 in bf16 read and write 281 MB
-// (55 us at 5.1 TB/s) in 0.26 ms; prepare has 67 and the chain 222 us when profiled.
+// (55 us at 5.1 TB/s) in 0.25 ms; prepare has 68 and the chain 216 us when profiled.
 // The matrix instructions are busy for a fifth of it, vector instructions (parts,
-// turning) for 45 %; the rest is waits at three barriers a chunk with one
-// workgroup of eight waves a CU (130 KB of LDS).  Backward 463 MB (91 us) take
-// 0.94 ms: prepare 76, the two chains 503, gradients 500 us.  The kept memories
+// turning) for 45 %; the rest is waits at three barriers a chunk with two
+// workgroups of four waves a CU (73 KB of LDS).  Backward 463 MB (91 us) take
+// 0.90 ms: prepare 75, the two chains 470, gradients 511 us.  The kept memories
 // and adjoints are 0.8 GB more, written and read again; a chain that took the
 // gradients as it goes would need all of V in one workgroup, 256 of them here,
 // and the sums over V in its registers.  A call of few frames goes frame by frame
@@ -64,11 +63,12 @@
 namespace dgen {
 
 constexpr int kC = 64;           // frames of a chunk
+constexpr int kVB = 32;          // values of a block
 constexpr int kVecs = 10;        // numbers of a chunk's frames
 
 // How a call is cut, and the places of its parts in the workspace.
 struct DeltaPlan {
-  int64_t chunks, vb, nvb, segs, per;  // vb: values of a workgroup, per: chunks of a segment
+  int64_t chunks, nvb, segs, per;  // nvb: blocks of values, per: chunks of a segment
   int64_t X, M, XT, vec, S, dS, U, dR, ends, gends, bytes;
 };
 // Whether a call goes frame by frame: a chunk costs its 64 frames (32 sequences of 8
@@ -530,7 +530,7 @@ __global__ __launch_bounds__(kThreads) void k_delta_prepare(DeltaP<E> p) {
 // --------------------------------------------------------------------- chain
 enum Mode { kOut, kEnds, kKeep };
 
-// A workgroup's sequence and head, block of VB values and segment of chunks.
+// A workgroup's sequence and head, block of kVB values and segment of chunks.
 struct Place {
   int b, h, hk, bh, vb, seg;
 };
@@ -548,23 +548,16 @@ __device__ __forceinline__ Place place_of(const DeltaP<E>& p, int blocks, uint32
 
 // A wave's part: rows 16 w of a chunk's frames with two tiles of values, and
 // NKT x NVT tiles of the memory.
-template <int KP, int VB>
+template <int KP>
 struct Split {
-  static constexpr int NF = KP / 32, NV = 2, NT = KP / 32, NVT = NT < VB / 16 ? NT : VB / 16, NKT = NT / NVT;
-  int lane, w, l16, g4, v;  // v: first value of the two tiles
-  int wave;
+  static constexpr int NF = KP / 32, NV = 2, NT = KP / 32, NVT = NT < 2 ? NT : 2, NKT = NT / NVT;
+  int lane, w, l16, g4;
   __device__ __forceinline__ Split() {
-    // (later rows have more products: a SIMD's two waves take early and late ones)
-    lane = threadIdx.x & 63, wave = wave_index(), w = wave & 4 ? 7 - wave : wave, l16 = lane & 15, g4 = lane >> 4;
-    v = (wave >> 2) * 32;
+    lane = threadIdx.x & 63, w = wave_index(), l16 = lane & 15, g4 = lane >> 4;
   }
   // the memory's tiles: first channel and value
-  __device__ __forceinline__ int tile_k(int i) const { return (wave * NT / (VB / 16) + i) * 16; }
-  __device__ __forceinline__ int tile_v(int j) const { return (wave * NT % (VB / 16) + j) * 16; }
-  // the fragments of its rows that this wave writes, where two have the same rows
-  static constexpr int NW = VB == 32 ? NF : (NF + 1) / 2;
-  __device__ __forceinline__ int written(int i) const { return VB == 32 ? i : 2 * i + (wave >> 2); }
-  __device__ __forceinline__ bool writes(int f) const { return VB == 32 || (f & 1) == (wave >> 2); }
+  __device__ __forceinline__ int tile_k(int i) const { return (w * NT / 2 + i) * 16; }
+  __device__ __forceinline__ int tile_v(int j) const { return (w * NT % 2 + j) * 16; }
 };
 // f(i, j, e, k, v) over the memory's tiles and a lane's four channels of each.
 #define DGEN_TILES(...)                                                         \
@@ -659,23 +652,23 @@ __device__ __forceinline__ void store_values(const Frames<E>& a, int t, int T, i
 }
 // Zeros in the chunks from c0 on.
 template <class E>
-__device__ __forceinline__ void store_zeros(const Heads<E>& a, const Place& at, int c0, int c1, int T, int v0, int V, int VB) {
+__device__ __forceinline__ void store_zeros(const Heads<E>& a, const Place& at, int c0, int c1, int T, int v0, int V) {
   const int t0 = c0 * kC, n = min(c1 * kC, T) - t0;
-  for (int i = threadIdx.x; i < n * VB; i += blockDim.x)
-    if (v0 + i % VB < V) a.row(at.b, t0 + i / VB, at.h)[v0 + i % VB] = from_f32<E>(0.f);
+  for (int i = threadIdx.x; i < n * kVB; i += blockDim.x)
+    if (v0 + i % kVB < V) a.row(at.b, t0 + i / kVB, at.h)[v0 + i % kVB] = from_f32<E>(0.f);
 }
 
-template <class E, int KP, int VB, Mode MODE>
+template <class E, int KP, Mode MODE>
 struct ChainLds {
-  Tile<E, kState, VB, KP> s;
-  Tile<E, kState, VB, kC> r, wr;
-  Tile<E, kResult, MODE == kOut ? VB : 1, kC> u;
+  Tile<E, kState, kVB, KP> s;
+  Tile<E, kState, kVB, kC> r, wr;
+  Tile<E, kResult, MODE == kOut ? kVB : 1, kC> u;
   Tile<E, 1, KP, kC> kt;
 };
 // The memory's states along a segment's chunks.
-template <class E, int KP, int VB, Mode MODE, bool WHOLE>
-__device__ __forceinline__ void delta_chain(const DeltaP<E>& p, ChainLds<E, KP, VB, MODE>& L, uint32_t block, uint32_t blocks) {
-  using W = Split<KP, VB>;
+template <class E, int KP, Mode MODE, bool WHOLE>
+__device__ __forceinline__ void delta_chain(const DeltaP<E>& p, ChainLds<E, KP, MODE>& L, uint32_t block, uint32_t blocks) {
+  using W = Split<KP>;
   constexpr int NF = W::NF, NV = W::NV, NKT = W::NKT, NVT = W::NVT;
   auto &s = L.s;
   auto &r = L.r, &wr = L.wr;
@@ -683,13 +676,13 @@ __device__ __forceinline__ void delta_chain(const DeltaP<E>& p, ChainLds<E, KP, 
   auto& kt = L.kt;
   const W me;
   const int l16 = me.l16, g4 = me.g4;
-  const int nvb = MODE == kEnds ? p.nvb + (KP + VB - 1) / VB : p.nvb;
+  const int nvb = MODE == kEnds ? p.nvb + (KP + kVB - 1) / kVB : p.nvb;
   const Place at = place_of(p, nvb, block, blocks);
   const int live = live_of(p.lengths, at.b, p.T);
   // (ends: the transition is the state's own columns, from the identity on and
   // with nothing written)
   const bool unit = MODE == kEnds && at.vb >= p.nvb;
-  const int v0 = (unit ? at.vb - p.nvb : at.vb) * VB;
+  const int v0 = (unit ? at.vb - p.nvb : at.vb) * kVB;
   const int64_t end = ((int64_t)at.bh * p.segs + at.seg) * KP;
   const int ld = p.Vp + KP;
   floatx4 S[NKT][NVT] = {};
@@ -706,10 +699,10 @@ __device__ __forceinline__ void delta_chain(const DeltaP<E>& p, ChainLds<E, KP, 
 #pragma unroll
     for (int j = 0; j < NVT; ++j) s.put4(me.tile_v(j) + l16, me.tile_k(i) + 4 * g4, S[i][j]);
   const int c0 = at.seg * p.per, c1 = min(c0 + p.per, p.chunks), cl = min(max((live + kC - 1) / kC, c0), c1);
-  const int row = 16 * me.w + l16, rows = 16 * me.w + 4 * g4, col = v0 + me.v + l16;
+  const int row = 16 * me.w + l16, rows = 16 * me.w + 4 * g4, col = v0 + l16;
   Raw<E> kr[NF], qr[MODE == kOut ? NF : 1];
   Quad<E> vr[NV];
-  const int trow = rows + (l16 & 3), tcol = v0 + me.v + (l16 & ~3);  // (turned)
+  const int trow = rows + (l16 & 3), tcol = v0 + (l16 & ~3);  // (turned)
   auto load = [&](int c) {
     const int t0 = c * kC, n = live - t0;
     load_rows<WHOLE>(frames_of(p.k, at.b, at.hk, t0, n), row, g4, p.K, kr);
@@ -754,15 +747,15 @@ __device__ __forceinline__ void delta_chain(const DeltaP<E>& p, ChainLds<E, KP, 
     Wide<E, kState> o[2][NV];
     floatx4 ks[2][1][NV] = {}, qs[1][NV] = {};  // (keys: even and odd fragments apart)
 #pragma unroll
-    for (int v = 0; v < NV; ++v) o[0][v] = s.frag(me.v + 16 * v + l16, g4 * 8);
+    for (int v = 0; v < NV; ++v) o[0][v] = s.frag(16 * v + l16, g4 * 8);
 #pragma unroll
     for (int f = 0; f < NF; ++f)
-      if (me.writes(f)) kt.put_column(f * 32 + g4 * 8, row, kf[f]);
+      kt.put_column(f * 32 + g4 * 8, row, kf[f]);
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
       if (f + 1 < NF)
 #pragma unroll
-        for (int v = 0; v < NV; ++v) o[(f + 1) & 1][v] = s.frag(me.v + 16 * v + l16, (f + 1) * 32 + g4 * 8);
+        for (int v = 0; v < NV; ++v) o[(f + 1) & 1][v] = s.frag(16 * v + l16, (f + 1) * 32 + g4 * 8);
       loads_first();
       const Wide<E, 1> a[1] = {kf[f]};
       mma(ks[f & 1], a, o[f & 1]);
@@ -774,7 +767,7 @@ __device__ __forceinline__ void delta_chain(const DeltaP<E>& p, ChainLds<E, KP, 
     }
 #pragma unroll
     for (int v = 0; v < NV; ++v)
-      r.put4(me.v + 16 * v + l16, rows, beta * (val[v] - read * (ks[0][0][v] + ks[1][0][v])));
+      r.put4(16 * v + l16, rows, beta * (val[v] - read * (ks[0][0][v] + ks[1][0][v])));
     load(min(c + 1, cl - 1));  // (the next chunk's, in flight through this one's products)
     lds_barrier();
     // U = X r
@@ -784,15 +777,15 @@ __device__ __forceinline__ void delta_chain(const DeltaP<E>& p, ChainLds<E, KP, 
       if (f > me.w / 2) break;
       Wide<E, kState> x[NV];
 #pragma unroll
-      for (int v = 0; v < NV; ++v) x[v] = r.frag(me.v + 16 * v + l16, f * 32 + g4 * 8);
+      for (int v = 0; v < NV; ++v) x[v] = r.frag(16 * v + l16, f * 32 + g4 * 8);
       loads_first();
       const Wide<E, kState> a[1] = {wide<E, kState>(xf[f])};
       mma(U, a, x);
     }
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      wr.put4(me.v + 16 * v + l16, rows, U[0][v] * write);
-      if constexpr (MODE == kOut) u.put4(me.v + 16 * v + l16, rows, U[0][v]);
+      wr.put4(16 * v + l16, rows, U[0][v] * write);
+      if constexpr (MODE == kOut) u.put4(16 * v + l16, rows, U[0][v]);
       if constexpr (MODE == kKeep)
         *reinterpret_cast<floatx4*>(p.U + ci * kC * p.Vp + (uint32_t)((rows >> 2) * p.Vp + col + 16 * v) * 4) = U[0][v];
     }
@@ -806,7 +799,7 @@ __device__ __forceinline__ void delta_chain(const DeltaP<E>& p, ChainLds<E, KP, 
         if (f > me.w / 2) break;
         Wide<E, kResult> x[NV];
 #pragma unroll
-        for (int v = 0; v < NV; ++v) x[v] = u.frag(me.v + 16 * v + l16, f * 32 + g4 * 8);
+        for (int v = 0; v < NV; ++v) x[v] = u.frag(16 * v + l16, f * 32 + g4 * 8);
         loads_first();
         const Wide<E, kResult> a[1] = {wide<E, kResult>(mf[f])};
         mma(qs, a, x);
@@ -836,7 +829,7 @@ __device__ __forceinline__ void delta_chain(const DeltaP<E>& p, ChainLds<E, KP, 
     lds_barrier();
   }
   if constexpr (MODE == kOut) {
-    store_zeros(p.y, at, cl, c1, p.T, v0, p.V, VB);
+    store_zeros(p.y, at, cl, c1, p.T, v0, p.V);
     if (p.state_out && at.seg == p.segs - 1) {
       DGEN_TILES(if (k + e < p.K && v < p.V) p.state_out[((int64_t)at.bh * p.K + k + e) * p.V + v] = S[i][j][e];)
     }
@@ -850,10 +843,10 @@ __device__ __forceinline__ void delta_chain(const DeltaP<E>& p, ChainLds<E, KP, 
   }
 }
 
-template <class E, int KP, int VB, bool WHOLE>
-__global__ __launch_bounds__(VB * 8) void k_delta_forward(DeltaP<E> p) {
-  __shared__ ChainLds<E, KP, VB, kOut> lds;
-  delta_chain<E, KP, VB, kOut, WHOLE>(p, lds, blockIdx.x, gridDim.x);
+template <class E, int KP, bool WHOLE>
+__global__ __launch_bounds__(kThreads) void k_delta_forward(DeltaP<E> p) {
+  __shared__ ChainLds<E, KP, kOut> lds;
+  delta_chain<E, KP, kOut, WHOLE>(p, lds, blockIdx.x, gridDim.x);
 }
 
 // The states that enter the segments (BACK: the adjoints after them) from the
@@ -937,34 +930,34 @@ __global__ __launch_bounds__(kThreads) void k_delta_carry(DeltaP<E> p, bool both
   else delta_carry<E, KP, true>(p, blockIdx.x - n, s);
 }
 
-template <class E, int KP, int VB>
+template <class E, int KP>
 struct BackLds {
   // (the adjoints' parts are read in a chunk's first products alone: what the
   // later ones take lies in their place)
   union {
-    Tile<E, kState, VB, KP> s;
-    Tile<E, kState, VB, kC> d[2];
+    Tile<E, kState, kVB, KP> s;
+    Tile<E, kState, kVB, kC> d[2];
   } x;
-  Tile<E, 1, VB, kC> dyt;
-  Tile<E, kState, VB, kC> qdy;
+  Tile<E, 1, kVB, kC> dyt;
+  Tile<E, kState, kVB, kC> qdy;
   Tile<E, 1, KP, kC> kt, qt;
 };
 // The adjoints of the memory's states, against time.  Leaves dv, and dR.
-template <class E, int KP, int VB, Mode MODE, bool WHOLE>
-__device__ __forceinline__ void delta_back(const DeltaP<E>& p, BackLds<E, KP, VB>& L, uint32_t block, uint32_t blocks) {
-  using W = Split<KP, VB>;
+template <class E, int KP, Mode MODE, bool WHOLE>
+__device__ __forceinline__ void delta_back(const DeltaP<E>& p, BackLds<E, KP>& L, uint32_t block, uint32_t blocks) {
+  using W = Split<KP>;
   constexpr int NF = W::NF, NV = W::NV, NKT = W::NKT, NVT = W::NVT;
   auto& x = L.x;
   auto& dyt = L.dyt;
   auto& qdy = L.qdy;
   auto &kt = L.kt, &qt = L.qt;
-  Tile<E, kState, VB, KP>& s = x.s;
-  Tile<E, kState, VB, kC>&du = x.d[0], &dr = x.d[1];
+  Tile<E, kState, kVB, KP>& s = x.s;
+  Tile<E, kState, kVB, kC>&du = x.d[0], &dr = x.d[1];
   const W me;
   const int l16 = me.l16, g4 = me.g4;
   const Place at = place_of(p, p.nvb, block, blocks);
   const int live = live_of(p.lengths, at.b, p.T);
-  const int v0 = at.vb * VB;
+  const int v0 = at.vb * kVB;
   const int64_t end = ((int64_t)at.bh * p.segs + at.seg) * KP;
   floatx4 S[NKT][NVT] = {};
   if (MODE == kKeep && p.segs > 1) {
@@ -975,20 +968,15 @@ __device__ __forceinline__ void delta_back(const DeltaP<E>& p, BackLds<E, KP, VB
 #pragma unroll
     for (int j = 0; j < NVT; ++j) s.put4(me.tile_v(j) + l16, me.tile_k(i) + 4 * g4, S[i][j]);
   const int c0 = at.seg * p.per, c1 = min(c0 + p.per, p.chunks), cl = min(max((live + kC - 1) / kC, c0), c1);
-  const int row = 16 * me.w + l16, rows = 16 * me.w + 4 * g4, col = v0 + me.v + l16;
-  if constexpr (MODE == kKeep) store_zeros(p.dv, at, cl, c1, p.T, v0, p.V, VB);
-  Raw<E> kr[NF], qr[W::NW];
+  const int row = 16 * me.w + l16, rows = 16 * me.w + 4 * g4, col = v0 + l16;
+  if constexpr (MODE == kKeep) store_zeros(p.dv, at, cl, c1, p.T, v0, p.V);
+  Raw<E> kr[NF], qr[NF];
   Quad<E> dyr[NV];
-  const int trow = rows + (l16 & 3), tcol = v0 + me.v + (l16 & ~3);  // (turned)
+  const int trow = rows + (l16 & 3), tcol = v0 + (l16 & ~3);  // (turned)
   auto load = [&](int c) {
     const int t0 = c * kC, n = live - t0;
     load_rows<WHOLE>(frames_of(p.k, at.b, at.hk, t0, n), row, g4, p.K, kr);
-    {
-      const Frames<const E> a = frames_of(p.q, at.b, at.hk, t0, n);
-      const E* x = a.p + (uint32_t)min(row, a.n - 1) * a.step;
-#pragma unroll
-      for (int i = 0; i < W::NW; ++i) load_raw<WHOLE>(qr[i], x, me.written(i) * 32 + g4 * 8, p.K);
-    }
+    load_rows<WHOLE>(frames_of(p.q, at.b, at.hk, t0, n), row, g4, p.K, qr);
     load_values<WHOLE>(frames_of(p.dy, at.b, at.h, t0, n), trow, tcol, p.V, dyr);
   };
   if (c0 < cl) load(cl - 1);
@@ -1019,28 +1007,24 @@ __device__ __forceinline__ void delta_back(const DeltaP<E>& p, BackLds<E, KP, VB
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
       kf[f] = exact_of<WHOLE>(kr[f], f * 32 + g4 * 8, p.K, row < n);
-      if (me.writes(f)) kt.put_column(f * 32 + g4 * 8, row, kf[f]);
+      kt.put_column(f * 32 + g4 * 8, row, kf[f]);
     }
 #pragma unroll
-    for (int i = 0; i < W::NW; ++i) {
-      const int f = me.written(i);
-      const Wide<E, 1> x = exact_of<WHOLE>(qr[i], f * 32 + g4 * 8, p.K, row < n);
-      if (f < NF) qt.put_column(f * 32 + g4 * 8, row, x);
-    }
+    for (int f = 0; f < NF; ++f) qt.put_column(f * 32 + g4 * 8, row, exact_of<WHOLE>(qr[f], f * 32 + g4 * 8, p.K, row < n));
 #pragma unroll
     for (int v = 0; v < NV; ++v) dy[v] = turn(quad_of<WHOLE>(dyr[v], tcol + 16 * v, p.V, trow < n), l16);
     // the adjoint of U: what the writes reach after the chunk, then within it
     floatx4 part[2][1][NV] = {}, U[1][NV];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      dyt.put4(me.v + 16 * v + l16, rows, dy[v]);
-      qdy.put4(me.v + 16 * v + l16, rows, dy[v] * readq);
+      dyt.put4(16 * v + l16, rows, dy[v]);
+      qdy.put4(16 * v + l16, rows, dy[v] * readq);
     }
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
       Wide<E, kState> o[NV];
 #pragma unroll
-      for (int v = 0; v < NV; ++v) o[v] = s.frag(me.v + 16 * v + l16, f * 32 + g4 * 8);
+      for (int v = 0; v < NV; ++v) o[v] = s.frag(16 * v + l16, f * 32 + g4 * 8);
       loads_first();
       const Wide<E, 1> a[1] = {kf[f]};
       mma(part[f & 1], a, o);
@@ -1057,13 +1041,13 @@ __device__ __forceinline__ void delta_back(const DeltaP<E>& p, BackLds<E, KP, VB
       if (f < me.w / 2) continue;
       Wide<E, 1> x[NV];
 #pragma unroll
-      for (int v = 0; v < NV; ++v) x[v] = dyt.frag(me.v + 16 * v + l16, f * 32 + g4 * 8);
+      for (int v = 0; v < NV; ++v) x[v] = dyt.frag(16 * v + l16, f * 32 + g4 * 8);
       loads_first();
       const Wide<E, kState> a[1] = {wide<E, kState>(mf[f])};
       mma(U, a, x);
     }
 #pragma unroll
-    for (int v = 0; v < NV; ++v) du.put4(me.v + 16 * v + l16, rows, U[0][v]);
+    for (int v = 0; v < NV; ++v) du.put4(16 * v + l16, rows, U[0][v]);
     lds_barrier();
     // dR = X^T dU
     floatx4 R[1][NV] = {};
@@ -1072,13 +1056,13 @@ __device__ __forceinline__ void delta_back(const DeltaP<E>& p, BackLds<E, KP, VB
       if (f < me.w / 2) continue;
       Wide<E, kState> x[NV];
 #pragma unroll
-      for (int v = 0; v < NV; ++v) x[v] = du.frag(me.v + 16 * v + l16, f * 32 + g4 * 8);
+      for (int v = 0; v < NV; ++v) x[v] = du.frag(16 * v + l16, f * 32 + g4 * 8);
       loads_first();
       const Wide<E, kState> a[1] = {wide<E, kState>(xf[f])};
       mma(R, a, x);
     }
 #pragma unroll
-    for (int v = 0; v < NV; ++v) dr.put4(me.v + 16 * v + l16, rows, -R[0][v] * beta * read);
+    for (int v = 0; v < NV; ++v) dr.put4(16 * v + l16, rows, -R[0][v] * beta * read);
     if constexpr (MODE == kKeep) {
       floatx4 dv[NV];
 #pragma unroll
@@ -1121,14 +1105,14 @@ __device__ __forceinline__ void delta_back(const DeltaP<E>& p, BackLds<E, KP, VB
 // Both ways at once, as neither waits for the other: the first `forward`
 // workgroups with time, the others against it.  kEnds: the segments' ends (those
 // with time alone in a call that is not backward).
-template <class E, int KP, int VB, Mode MODE, bool WHOLE>
-__global__ __launch_bounds__(VB * 8) void k_delta_both(DeltaP<E> p, uint32_t forward) {
+template <class E, int KP, Mode MODE, bool WHOLE>
+__global__ __launch_bounds__(kThreads) void k_delta_both(DeltaP<E> p, uint32_t forward) {
   __shared__ union {
-    ChainLds<E, KP, VB, MODE> chain;
-    BackLds<E, KP, VB> back;
+    ChainLds<E, KP, MODE> chain;
+    BackLds<E, KP> back;
   } lds;
-  if (blockIdx.x < forward) delta_chain<E, KP, VB, MODE, WHOLE>(p, lds.chain, blockIdx.x, forward);
-  else delta_back<E, KP, VB, MODE, WHOLE>(p, lds.back, blockIdx.x - forward, gridDim.x - forward);
+  if (blockIdx.x < forward) delta_chain<E, KP, MODE, WHOLE>(p, lds.chain, blockIdx.x, forward);
+  else delta_back<E, KP, MODE, WHOLE>(p, lds.back, blockIdx.x - forward, gridDim.x - forward);
 }
 
 // -------------------------------------------------------------------- grads
@@ -1491,26 +1475,24 @@ __global__ __launch_bounds__(kThreads) void k_delta_step(DeltaP<E> p) {
 
 // ------------------------------------------------------------------ launches
 
-template <class E, int KP, int VB, bool WHOLE>
+template <class E, int KP, bool WHOLE>
 void delta_chains(const DeltaP<E>& p, const DeltaPlan& o, int64_t bh, bool backward, hipStream_t st) {
   auto grid = [](int64_t n) { return dim3((unsigned)n); };
-  constexpr int n = VB * 8;
   const int64_t blocks = bh * o.nvb * o.segs, carry = bh * (p.Vp / 16);
   if (o.segs > 1) {
-    const int64_t ends = bh * o.segs * (o.nvb + (KP + VB - 1) / VB);
-    k_delta_both<E, KP, VB, kEnds, WHOLE><<<grid(ends + (backward ? blocks : 0)), n, 0, st>>>(p, (uint32_t)ends);
+    const int64_t ends = bh * o.segs * (o.nvb + (KP + kVB - 1) / kVB);
+    k_delta_both<E, KP, kEnds, WHOLE><<<grid(ends + (backward ? blocks : 0)), kThreads, 0, st>>>(p, (uint32_t)ends);
     k_delta_carry<E, KP><<<grid(backward ? 2 * carry : carry), kThreads, 0, st>>>(p, backward);
   }
-  if (backward) k_delta_both<E, KP, VB, kKeep, WHOLE><<<grid(2 * blocks), n, 0, st>>>(p, (uint32_t)blocks);
-  else k_delta_forward<E, KP, VB, WHOLE><<<grid(blocks), n, 0, st>>>(p);
+  if (backward) k_delta_both<E, KP, kKeep, WHOLE><<<grid(2 * blocks), kThreads, 0, st>>>(p, (uint32_t)blocks);
+  else k_delta_forward<E, KP, WHOLE><<<grid(blocks), kThreads, 0, st>>>(p);
 }
 
 template <class E, int KP, bool WHOLE>
 void delta_kernels(const DeltaP<E>& p, const DeltaPlan& o, int64_t bh, bool backward, hipStream_t st) {
   auto grid = [](int64_t n) { return dim3((unsigned)n); };
   k_delta_prepare<E, KP, WHOLE><<<grid(bh * o.chunks), kThreads, 0, st>>>(p);
-  if (o.vb == 64) delta_chains<E, KP, 64, WHOLE>(p, o, bh, backward, st);
-  else delta_chains<E, KP, 32, WHOLE>(p, o, bh, backward, st);
+  delta_chains<E, KP, WHOLE>(p, o, bh, backward, st);
   if (backward) {
     const dim3 n = grid(bh / p.shared * o.chunks);
     p.shared > 1 ? k_delta_grads<E, KP, WHOLE, true><<<n, kGradThreads, 0, st>>>(p)
@@ -1531,7 +1513,7 @@ void delta_launch(const dgen_hip_delta& a, bool backward, hipStream_t st) {
   p.lengths = a.lengths, p.state = a.state, p.state_out = a.state_out;
   p.scale = a.scale, p.normalize = a.normalize;
   p.T = (int)a.T, p.H = (int)a.heads, p.shared = (int)(a.heads / a.key_heads), p.K = (int)a.K, p.V = (int)a.V;
-  p.Vp = (int)(o.nvb * o.vb);
+  p.Vp = (int)(o.nvb * kVB);
   p.chunks = (int)o.chunks, p.nvb = (int)o.nvb, p.segs = (int)o.segs, p.per = (int)o.per;
   auto at = [&](int64_t off) { return (float*)((char*)a.workspace + off); };
   p.X = at(o.X), p.M = at(o.M), p.XT = backward ? at(o.XT) : nullptr, p.vec = at(o.vec), p.S = at(o.S), p.dS = at(o.dS), p.U = at(o.U), p.dR = at(o.dR);

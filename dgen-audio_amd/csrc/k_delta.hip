@@ -34,9 +34,7 @@ DeltaPlan delta_plan(const dgen_hip_delta& a, bool backward) {
   const int64_t bh = a.batch * a.heads, K = a.K <= 32 ? 32 : a.K <= 64 ? 64 : 128;
   o.chunks = (a.T + kC - 1) / kC;
   o.segs = 1;
-  // 64 values a workgroup of eight waves where that fills the CUs
-  o.vb = a.V > 32 && bh * ((a.V + 63) / 64) >= 192 ? 64 : 32;
-  o.nvb = (a.V + o.vb - 1) / o.vb;
+  o.nvb = (a.V + kVB - 1) / kVB;
   // Segments go through their chunks twice, the second time with their transitions
   // too, and each is a step of the carry: three times the work, so that they pay
   // where the card is a third full at most (with 128 channels, whose steps of the
@@ -55,7 +53,7 @@ DeltaPlan delta_plan(const dgen_hip_delta& a, bool backward) {
     at += align256(floats * 4);
     return p;
   };
-  const int64_t n = bh * o.chunks, V = o.nvb * o.vb;
+  const int64_t n = bh * o.chunks, V = o.nvb * kVB;
   o.X = take(n * kC * kC);
   o.M = take(n * kC * kC);
   if (backward) o.XT = take(n * kC * kC);
