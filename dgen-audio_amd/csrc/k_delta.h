@@ -240,6 +240,37 @@ struct Tile {
   }
 };
 
+// A chunk's keys (or queries), written by rows and read by columns: four frames of
+// one channel a lane, of 16 channels from k on.  bf16 stays in rows and is turned
+// by the LDS as it is read (of 16 lanes, lane l reads four channels of row l / 4
+// and is given channel l of the four rows).
+template <class E, int KP>
+struct Turned {
+  static constexpr bool kFloat = std::is_same<E, float>::value;
+  Tile<E, 1, kFloat ? KP : kC, kFloat ? kC : KP> t;
+
+  __device__ __forceinline__ void put(int row, int k, const Wide<E, 1>& w) {
+    if constexpr (kFloat) t.put_column(k, row, w);
+    else t.put_row(row, k, w);
+  }
+  __device__ __forceinline__ bf16x4 four(int k, int row, int l16) const {
+    typedef __attribute__((address_space(3))) bf16x4 Lds;
+    return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((Lds*)&t.d[0][t.at(row + (l16 >> 2), k + 4 * (l16 & 3))]);
+  }
+  __device__ __forceinline__ Wide<E, 1> frag(int k, int row, int l16) const {
+    if constexpr (kFloat) {
+      return t.frag(k + l16, row);
+    } else {
+      const bf16x4 a = four(k, row, l16), b = four(k, row + 4, l16);
+      return {{__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7)}};
+    }
+  }
+  __device__ __forceinline__ floatx4 first4(int k, int row, int l16) const {
+    if constexpr (kFloat) return t.first4(k + l16, row);
+    else return __builtin_convertvector(four(k, row, l16), floatx4);
+  }
+};
+
 // Elements [at, at + 8) of a row of n as they are read, without branches and with
 // nothing done to them, so that they can be in flight until they are used: a piece
 // past the end is read from the row's last eight, and shifted or dropped then.
@@ -663,7 +694,7 @@ struct ChainLds {
   Tile<E, kState, kVB, KP> s;
   Tile<E, kState, kVB, kC> r, wr;
   Tile<E, kResult, MODE == kOut ? kVB : 1, kC> u;
-  Tile<E, 1, KP, kC> kt;
+  Turned<E, KP> kt;
 };
 // The memory's states along a segment's chunks.
 template <class E, int KP, Mode MODE, bool WHOLE>
@@ -750,7 +781,7 @@ __device__ __forceinline__ void delta_chain(const DeltaP<E>& p, ChainLds<E, KP, 
     for (int v = 0; v < NV; ++v) o[0][v] = s.frag(16 * v + l16, g4 * 8);
 #pragma unroll
     for (int f = 0; f < NF; ++f)
-      kt.put_column(f * 32 + g4 * 8, row, kf[f]);
+      kt.put(row, f * 32 + g4 * 8, kf[f]);
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
       if (f + 1 < NF)
@@ -816,7 +847,7 @@ __device__ __forceinline__ void delta_chain(const DeltaP<E>& p, ChainLds<E, KP, 
       Wide<E, 1> a[NKT];
       Wide<E, kState> x[NVT];
 #pragma unroll
-      for (int i = 0; i < NKT; ++i) a[i] = kt.frag(me.tile_k(i) + l16, f * 32 + g4 * 8);
+      for (int i = 0; i < NKT; ++i) a[i] = kt.frag(me.tile_k(i), f * 32 + g4 * 8, l16);
 #pragma unroll
       for (int j = 0; j < NVT; ++j) x[j] = wr.frag(me.tile_v(j) + l16, f * 32 + g4 * 8);
       loads_first();
@@ -940,7 +971,7 @@ struct BackLds {
   } x;
   Tile<E, 1, kVB, kC> dyt;
   Tile<E, kState, kVB, kC> qdy;
-  Tile<E, 1, KP, kC> kt, qt;
+  Turned<E, KP> kt, qt;
 };
 // The adjoints of the memory's states, against time.  Leaves dv, and dR.
 template <class E, int KP, Mode MODE, bool WHOLE>
@@ -1007,10 +1038,10 @@ __device__ __forceinline__ void delta_back(const DeltaP<E>& p, BackLds<E, KP>& L
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
       kf[f] = exact_of<WHOLE>(kr[f], f * 32 + g4 * 8, p.K, row < n);
-      kt.put_column(f * 32 + g4 * 8, row, kf[f]);
+      kt.put(row, f * 32 + g4 * 8, kf[f]);
     }
 #pragma unroll
-    for (int f = 0; f < NF; ++f) qt.put_column(f * 32 + g4 * 8, row, exact_of<WHOLE>(qr[f], f * 32 + g4 * 8, p.K, row < n));
+    for (int f = 0; f < NF; ++f) qt.put(row, f * 32 + g4 * 8, exact_of<WHOLE>(qr[f], f * 32 + g4 * 8, p.K, row < n));
 #pragma unroll
     for (int v = 0; v < NV; ++v) dy[v] = turn(quad_of<WHOLE>(dyr[v], tcol + 16 * v, p.V, trow < n), l16);
     // the adjoint of U: what the writes reach after the chunk, then within it
@@ -1084,7 +1115,7 @@ __device__ __forceinline__ void delta_back(const DeltaP<E>& p, BackLds<E, KP>& L
       Wide<E, 1> a[NKT];
       Wide<E, kState> x[NVT];
 #pragma unroll
-      for (int i = 0; i < NKT; ++i) a[i] = f < 2 ? qt.frag(me.tile_k(i) + l16, at8) : kt.frag(me.tile_k(i) + l16, at8);
+      for (int i = 0; i < NKT; ++i) a[i] = f < 2 ? qt.frag(me.tile_k(i), at8, l16) : kt.frag(me.tile_k(i), at8, l16);
 #pragma unroll
       for (int j = 0; j < NVT; ++j) x[j] = f < 2 ? qdy.frag(me.tile_v(j) + l16, at8) : dr.frag(me.tile_v(j) + l16, at8);
       loads_first();
@@ -1128,7 +1159,7 @@ struct GradLds {
     } a;
     Tile<E, kGradParts, kC, kC> m[2];
   };
-  Tile<E, 1, KP, kC> kt, qt;
+  Turned<E, KP> kt, qt;
   alignas(16) float vec[kVecs * kC], dots[2][3][kC];
   float db[kC], over[8];
 };
@@ -1141,7 +1172,7 @@ __global__ __launch_bounds__(kGradThreads) void k_delta_grads(DeltaP<E> p) {
   const int G = p.H / p.shared, c = blockIdx.x % (uint32_t)p.chunks, bg = blockIdx.x / (uint32_t)p.chunks;
   const int b = bg / G, hk = bg % G, t0 = c * kC, live = live_of(p.lengths, b, p.T) - t0;
   const int lane = threadIdx.x & 63, wave = wave_index(), half = wave >> 2, w = half ? 7 - wave : wave, l16 = lane & 15, g4 = lane >> 4;
-  const int row = 16 * w + l16, rows = 16 * w + 4 * g4, k0 = half * (KP / 2) + l16;
+  const int row = 16 * w + l16, rows = 16 * w + 4 * g4, k0 = half * (KP / 2);
   if (live <= 0) {
     for (int i = threadIdx.x; i < kC * p.K; i += kGradThreads) {
       const int t = t0 + i / p.K, k = i % p.K;
@@ -1158,12 +1189,12 @@ __global__ __launch_bounds__(kGradThreads) void k_delta_grads(DeltaP<E> p) {
   {
     // (the waves of the same rows take the keys and the queries)
     const E* x = half ? p.q.row(b, tc, hk) : p.k.row(b, tc, hk);
-    Tile<E, 1, KP, kC>& to = half ? L.qt : L.kt;
+    Turned<E, KP>& to = half ? L.qt : L.kt;
     Wide<E, 1> o[NF];
 #pragma unroll
     for (int f = 0; f < NF; ++f) o[f] = load_exact<WHOLE>(x, f * 32 + g4 * 8, p.K, on);
 #pragma unroll
-    for (int f = 0; f < NF; ++f) to.put_column(f * 32 + g4 * 8, row, o[f]);
+    for (int f = 0; f < NF; ++f) to.put(row, f * 32 + g4 * 8, o[f]);
   }
   // Sum over the 16 lanes of a row.
   auto row_total = [](floatx4 v) {
@@ -1270,7 +1301,7 @@ __global__ __launch_bounds__(kGradThreads) void k_delta_grads(DeltaP<E> p) {
       dqz[0][k] *= into;
       dqz[1][k] *= -into;
       wr[0][k] *= rest;
-      written += L.kt.first4(k0 + 16 * k, rows) * wr[0][k];
+      written += L.kt.first4(k0 + 16 * k, rows, l16) * wr[0][k];
     }
     {
       // over the chunk's end: what the entering state and the chunk's writes have there
@@ -1307,7 +1338,7 @@ __global__ __launch_bounds__(kGradThreads) void k_delta_grads(DeltaP<E> p) {
       const Wide<E, kGradParts> o[2] = {L.m[0].frag(row, col), L.m[1].frag(row, col)};
       Wide<E, 1> x[NK];
 #pragma unroll
-      for (int k = 0; k < NK; ++k) x[k] = L.kt.frag(k0 + 16 * k, col);
+      for (int k = 0; k < NK; ++k) x[k] = L.kt.frag(k0 + 16 * k, col, l16);
       loads_first();
       mma(dqz, o, x);
     }
@@ -1327,7 +1358,7 @@ __global__ __launch_bounds__(kGradThreads) void k_delta_grads(DeltaP<E> p) {
         const Wide<E, kGradParts> o[1] = {L.m[y].frag(row, col)};
         Wide<E, 1> x[NK];
 #pragma unroll
-        for (int k = 0; k < NK; ++k) x[k] = y ? L.kt.frag(k0 + 16 * k, col) : L.qt.frag(k0 + 16 * k, col);
+        for (int k = 0; k < NK; ++k) x[k] = y ? L.kt.frag(k0 + 16 * k, col, l16) : L.qt.frag(k0 + 16 * k, col, l16);
         loads_first();
         mma(wr, o, x);
       }
@@ -1335,8 +1366,8 @@ __global__ __launch_bounds__(kGradThreads) void k_delta_grads(DeltaP<E> p) {
     floatx4 q = {0, 0, 0, 0}, kr = {0, 0, 0, 0}, kw = {0, 0, 0, 0};
 #pragma unroll
     for (int k = 0; k < NK; ++k) {
-      const floatx4 kk = L.kt.first4(k0 + 16 * k, rows);
-      q += L.qt.first4(k0 + 16 * k, rows) * dqz[0][k];
+      const floatx4 kk = L.kt.first4(k0 + 16 * k, rows, l16);
+      q += L.qt.first4(k0 + 16 * k, rows, l16) * dqz[0][k];
       kr += kk * dqz[1][k];
       kw += kk * wr[0][k];
       if constexpr (SHARED) DQ[k] += dqz[0][k];
@@ -1381,9 +1412,9 @@ __global__ __launch_bounds__(kGradThreads) void k_delta_grads(DeltaP<E> p) {
   E *oq = p.dq.row(b, t0 + trow, hk), *ok = p.dk.row(b, t0 + trow, hk);
 #pragma unroll
   for (int k = 0; k < NK; ++k) {
-    const int col = k0 + 16 * k, at = (col & ~15) + (l16 & ~3);
-    floatx4 x = turn(rootq * (SHARED ? DQ[SHARED ? k : 0] : dqz[0][k]) - L.qt.first4(col, rows) * backq, l16);
-    floatx4 y = turn(rootk * DK[k] - L.kt.first4(col, rows) * backk, l16);
+    const int col = k0 + 16 * k, at = col + (l16 & ~3);
+    floatx4 x = turn(rootq * (SHARED ? DQ[SHARED ? k : 0] : dqz[0][k]) - L.qt.first4(col, rows, l16) * backq, l16);
+    floatx4 y = turn(rootk * DK[k] - L.kt.first4(col, rows, l16) * backk, l16);
     if (trow >= live) x = y = floatx4{0.f, 0.f, 0.f, 0.f};
     const float xs[4] = {x[0], x[1], x[2], x[3]}, ys[4] = {y[0], y[1], y[2], y[3]};
     if (t0 + trow >= p.T) continue;
