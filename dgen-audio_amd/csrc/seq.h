@@ -1,4 +1,5 @@
-// Shared by the sequence operators (k_norm, k_conv, k_scan, k_glu): element
+// Shared by the sequence operators (k_norm, k_conv, k_scan, k_glu, k_delta,
+// k_block) and the optimiser's step (k_adamw): element
 // types, their loads and stores, and the sums that their backward passes end
 // with.
 #pragma once
