@@ -65,16 +65,18 @@ namespace dgen {
 constexpr int kC = 64;           // frames of a chunk
 constexpr int kVB = 32;          // values of a block
 constexpr int kVecs = 10;        // numbers of a chunk's frames
+constexpr int kStepFrames = 16;  // calls of so few go frame by frame
 
 // How a call is cut, and the places of its parts in the workspace.
 struct DeltaPlan {
   int64_t chunks, nvb, segs, per;  // nvb: blocks of values, per: chunks of a segment
   int64_t X, M, XT, vec, S, dS, U, dR, ends, gends, bytes;
 };
-// Whether a call goes frame by frame: a chunk costs its 64 frames (32 sequences of 8
-// heads of 128: 30 us in bf16, 55 in fp32), a frame 2 us.
+// Whether a call goes frame by frame: a chunk costs its 64 frames, a frame its sums
+// over the memory (32 sequences of 8 heads of 128: 28 us in bf16 and 48 in fp32 for
+// a chunk, 1.5 for a frame; 1 sequence of 4 heads of 64: 17 and 19, and 0.8).
 inline bool delta_steps(const dgen_hip_delta& a, bool backward) {
-  return !backward && a.T <= (a.type == DGEN_HIP_BF16 ? 12 : 16);
+  return !backward && a.T <= kStepFrames;
 }
 DeltaPlan delta_plan(const dgen_hip_delta&, bool backward);
 void delta_enqueue_f32(const dgen_hip_delta&, bool backward, hipStream_t);
@@ -1425,11 +1427,13 @@ __global__ __launch_bounds__(kGradThreads) void k_delta_grads(DeltaP<E> p) {
 
 // --------------------------------------------------------------- few frames
 // Frame by frame: 32 values of one head a workgroup, a thread holds four of
-// them for KP / 32 of the keys' channels.
+// them for KP / 32 of the keys' channels.  Bound by the sums' vector instructions
+// (the next frame's operands loaded ahead were no faster).
 template <class E, int KP>
 __global__ __launch_bounds__(kThreads) void k_delta_step(DeltaP<E> p) {
   constexpr int NR = KP / 32;
-  __shared__ float kq[2][2][KP], red[2][4][8][12];
+  __shared__ float kq[2][2][KP];
+  __shared__ alignas(16) float red[2][4][8][12];
   const int nvb = (p.V + 31) / 32, vb = blockIdx.x % (uint32_t)nvb, bh = blockIdx.x / (uint32_t)nvb;
   const int b = bh / p.H, h = bh % p.H, hk = h / p.shared, live = live_of(p.lengths, b, p.T);
   const int lane = threadIdx.x & 63, w = wave_index(), l8 = lane & 7, rt = threadIdx.x >> 3;
@@ -1461,7 +1465,7 @@ __global__ __launch_bounds__(kThreads) void k_delta_step(DeltaP<E> p) {
     load_four(p.v.row(b, t, h) + v, left, val);
     __syncthreads();
     // k.S, q.S, k.q, k.k and q.q in one go
-    float o[11] = {};
+    float o[12] = {};
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
       const float k = kq[at][0][rt + 32 * i], q = kq[at][1][rt + 32 * i];
@@ -1469,11 +1473,15 @@ __global__ __launch_bounds__(kThreads) void k_delta_step(DeltaP<E> p) {
       for (int e = 0; e < 4; ++e) o[e] = fmaf(k, S[i][e], o[e]), o[4 + e] = fmaf(q, S[i][e], o[4 + e]);
       o[8] = fmaf(k, q, o[8]), o[9] = fmaf(k, k, o[9]), o[10] = fmaf(q, q, o[10]);
     }
+    // (each exchange halves the sums a lane goes on with)
+    float six[6], three[3];
 #pragma unroll
-    for (int e = 0; e < 11; ++e) {
-      o[e] += dpp<0x128>(o[e]);  // (lanes 8 apart)
-      o[e] = swap_add32(swap_add16(o[e], o[e]), swap_add16(o[e], o[e]));
-      if (lane < 8) red[at][w][l8][e] = o[e];
+    for (int e = 0; e < 6; ++e) six[e] = swap_add32(o[e], o[e + 6]);
+#pragma unroll
+    for (int e = 0; e < 3; ++e) {
+      three[e] = swap_add16(six[e], six[e + 3]);
+      three[e] += dpp<0x128>(three[e]);  // (lanes 8 apart)
+      if (!(lane & 8)) red[at][w][l8][3 * (lane >> 4) + e] = three[e];
     }
     __syncthreads();
 #pragma unroll

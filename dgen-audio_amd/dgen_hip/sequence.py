@@ -555,7 +555,7 @@ def _delta_parts(q, k, v, g, beta, scale, normalize, state, lengths):
 
 
 _NO_DELTA_GRADS = (0,) * 22
-_DELTA_FRAMES = 12  # longer calls may take scratch
+_DELTA_FRAMES = 16  # longer calls take scratch
 
 
 def gated_delta_rule(q, k, v, g, beta, scale: Optional[float] = None, normalize: bool = True, state=None, state_out=None,
@@ -574,8 +574,7 @@ def gated_delta_rule(q, k, v, g, beta, scale: Optional[float] = None, normalize:
     Products are formed in float32's accuracy for float32, and in that of
     bfloat16's exact values and float32 sums for bfloat16, states as accurate
     as float32 ones.  A value that is not finite spoils its head's results from
-    up to 63 frames before it on; short calls (up to 12
-    frames, of float32 up to 16) go frame by frame."""
+    up to 63 frames before it on; calls of up to 16 frames go frame by frame."""
     dev, states, head, ins = _delta_parts(q, k, v, g, beta, scale, normalize, state, lengths)
     B, T, H, V = shape = v.shape
     if out is None:

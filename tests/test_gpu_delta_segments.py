@@ -1,7 +1,7 @@
 """How the gated delta rule cuts its calls: by segments of chunks (from 8 chunks
 on, from 12 with more than 64 keys' channels, as many as the square root of the
-chunks suggests or the card takes) and frame by frame (up to 12 frames of
-bfloat16, 16 of float32), on both sides of each rule, against the definition in
+chunks suggests or the card takes) and frame by frame (up to 16 frames),
+on both sides of each rule, against the definition in
 64 bits.  Needs a GPU.
 
 Tolerances are those of test_gpu_delta_rule, twice over: with segments the memory
