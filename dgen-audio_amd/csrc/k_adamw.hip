@@ -19,7 +19,8 @@ namespace dgen {
 
 namespace {
 
-constexpr int kTensors = 40, kThreads = 256, kRuns = 4, kPer = kThreads * 4 * kRuns;
+// (as many tensors as a launch's 4096 bytes of arguments hold)
+constexpr int kTensors = 52, kSquares = 200, kThreads = 256, kRuns = 4, kPer = kThreads * 4 * kRuns;
 
 struct Tensor {
   const float *p, *m, *v;
@@ -40,12 +41,13 @@ struct StepP {
 static_assert(sizeof(StepP) <= 4096, "a launch's arguments");
 
 struct SquaresP {
-  const void* g[kTensors];
-  int64_t n[kTensors];
-  uint32_t first[kTensors + 1];
+  const void* g[kSquares];
+  int64_t n[kSquares];
+  uint32_t first[kSquares + 1];
   int count;
   float* parts;
 };
+static_assert(sizeof(SquaresP) <= 4096, "a launch's arguments");
 
 // The tensor that a workgroup works on.
 __device__ __forceinline__ int tensor_of(const uint32_t* first, int count) {
@@ -236,14 +238,14 @@ int adamw_run(const dgen_hip_adamw& a, hipStream_t st, bool dry) {
     return 0;
   }
   const bool half = a.grad_type == DGEN_HIP_BF16;
-  // Runs of up to kTensors tensors that have elements (and fewer workgroups
+  // Runs of up to `most` tensors that have elements (and fewer workgroups
   // than a launch takes).
-  auto runs = [&](auto take, auto launch) {
+  auto runs = [&](int most, auto take, auto launch) {
     uint32_t at = 0;
     int k = 0;
     for (int64_t i = 0; i <= a.count; ++i) {
       const int64_t g = i < a.count ? groups_of(a.tensors[i].n) : 0;
-      if (k && (i == a.count || k == kTensors || at + g >= (1 << 22))) {
+      if (k && (i == a.count || k == most || at + g >= (1 << 22))) {
         launch(k, at);
         k = 0, at = 0;
       }
@@ -254,7 +256,7 @@ int adamw_run(const dgen_hip_adamw& a, hipStream_t st, bool dry) {
     SquaresP q;
     q.parts = (float*)a.workspace;
     runs(
-        [&](int k, uint32_t at, const dgen_hip_adamw_tensor& t) { q.g[k] = t.grad, q.n[k] = t.n, q.first[k] = at; },
+        kSquares, [&](int k, uint32_t at, const dgen_hip_adamw_tensor& t) { q.g[k] = t.grad, q.n[k] = t.n, q.first[k] = at; },
         [&](int k, uint32_t groups) {
           q.count = k;
           half ? k_squares<bf16><<<groups, kThreads, 0, st>>>(q) : k_squares<float><<<groups, kThreads, 0, st>>>(q);
@@ -274,6 +276,7 @@ int adamw_run(const dgen_hip_adamw& a, hipStream_t st, bool dry) {
   }
   s.bound = (float)a.max_norm, s.norm = a.max_norm > 0 ? a.norm : nullptr;
   runs(
+      kTensors,
       [&](int k, uint32_t at, const dgen_hip_adamw_tensor& t) {
         s.t[k] = {t.param, t.m, t.v, t.grad, t.param_out, t.m_out, t.v_out, (bf16*)t.copy, t.n};
         s.first[k] = at;

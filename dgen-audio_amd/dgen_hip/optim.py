@@ -1,6 +1,6 @@
 """The optimiser's step on device tensors (include/dgen_hip.h, "optimiser step
 on device tensors"): AdamW over all of a model's tensors in one launch for each
-forty of them.
+fifty-two of them.
 
 ``adamw`` is one step from tensors to tensors; :class:`AdamW` keeps a model's
 moments and steps in place.  Tensors are contiguous torch tensors on one GPU;

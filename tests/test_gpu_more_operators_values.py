@@ -11,7 +11,7 @@ torch = pytest.importorskip("torch")
 from dgen_hip import optim  # noqa: E402
 from dgen_hip import sequence as Q  # noqa: E402
 from test_gpu_delta_rule import INPUTS, data, on_gpu, rule, wide  # noqa: E402
-from test_gpu_sequence import F64, TYPES, Data  # noqa: E402
+from test_gpu_sequence import F64, TYPES, Data, close  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 NAN, INF = float("nan"), float("inf")
@@ -199,3 +199,13 @@ def test_keys_that_are_alike_and_long_memories(gpu, ty):
     assert ((after.cpu().double() - left).abs() <= tol * big).all()
     assert ((y.cpu().double() - want).abs() <= (tol + (24 * 2.0 ** -16 if ty == torch.bfloat16 else 0.0)) * big
             + (2.0 ** -8 * want.abs() if ty == torch.bfloat16 else 0.0)).all()
+
+
+@pytest.mark.parametrize("count", [52, 53, 200, 201, 417])
+def test_as_many_tensors_as_a_launch_takes_and_more(gpu, count):
+    from test_gpu_adamw import ARGS, check, formula, tensors
+    p, g, m, v = tensors(count, [(1 + i % 5,) for i in range(count)])
+    want = formula(p, g, m, v, 3, max_norm=1e-3, **ARGS)
+    norm = optim.adamw(p, g, m, v, 3, max_norm=1e-3, **ARGS)
+    check((p, m, v), want)
+    close(norm, want[3].cpu(), 70, "norm")
