@@ -67,3 +67,37 @@ def test_few_frames(gpu, T, ty):
     big = max(want.abs().max().item(), left.abs().max().item(), 1.0)
     close(y, want, ops_of(T, K, ty), f"y {name_of(ty)}", big)
     close(after, left, ops_of(T, K), "state", max(big, 4.0))
+
+
+@pytest.mark.parametrize("ty", TYPES)
+def test_segments_captured(gpu, ty):
+    """A captured forward and backward pass in segments, replayed on other inputs
+    with eager calls of the same between."""
+    B, T, G, H, K, V = 2, 800, 1, 2, 32, 48
+    x, _, s, d = data(B, T, G, H, K, V, ty, True, slow=True)
+    a, dy = on_gpu(x, s=s), d.normal(B, T, H, V, type=ty).cuda()
+    after = torch.empty(B, H, K, V, device="cuda")
+
+    def run():
+        return (Q.gated_delta_rule(**a, state_out=after), after, *Q.gated_delta_rule_backward(dy, **a))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for k in range(4):
+        other = data(B, T, G, H, K, V, ty, True, slow=True, seed=k + 1)
+        for name, t in other[0].items():
+            a[name].copy_(t)
+        a["state"].copy_(other[2])
+        graph.replay()
+        got = [t.clone() for t in out]
+        for t in out:
+            t.fill_(float("nan"))
+        torch.cuda.synchronize()
+        want = run()
+        assert all(torch.equal(p, q) for p, q in zip(got, want)), k
