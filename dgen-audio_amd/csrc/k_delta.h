@@ -39,11 +39,11 @@
 // 1000 frames, 128 x 128: 469 against 403 us in bf16, 1264 against 972 in fp32).
 //
 // Precision: operands that are bf16 go to the bf16 instructions as they are.
-// Numbers held in 32 bits (memories, adjoints, U, dR, X) are split into three
+// Numbers held in 32 bits (memories, adjoints, U, dR, X, M) are split into three
 // bf16 parts, whose products of up to 2^-16 are kept: 24 bits, as fp32 products
 // have, at a sixth to a third of the bf16 rate, still above the fp32 instructions'.
-// Where only y, rounded to bf16, is left of a product two parts are taken
-// (2^-17 against 2^-9).  fp32 operands go to the fp32 instructions.
+// That goes for y too, which may be what is left of larger numbers when it is
+// rounded to bf16.  fp32 operands go to the fp32 instructions.
 //
 // What bounds it: 32 x 1000 x 8 heads of K = V = 128 in bf16 read and write 281 MB
 // (55 us at 5.1 TB/s) in 0.25 ms; prepare has 68 and the chain 216 us when profiled.
@@ -92,9 +92,8 @@ typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 constexpr int kThreads = 256;
 constexpr float kUnitEps = 1e-6f;
 
-// Parts of fp32 numbers in bf16 products: of what goes into the memory, and of
-// what goes into results that are rounded to bf16.
-constexpr int kState = 3, kResult = 2;
+// Parts of fp32 numbers in bf16 products.
+constexpr int kState = 3;
 
 // ------------------------------------------------------- fragments, products
 // Eight consecutive elements of one row, as the matrix instructions take them
@@ -166,18 +165,6 @@ __device__ __forceinline__ floatx8 whole_of(const Wide<bf16, P>& w) {
 }
 template <int P>
 __device__ __forceinline__ floatx8 whole_of(const Wide<float, P>& w) { return w.p; }
-// The first Q parts.
-template <int Q, int P>
-__device__ __forceinline__ Wide<bf16, Q> first(const Wide<bf16, P>& w) {
-  Wide<bf16, Q> o;
-#pragma unroll
-  for (int i = 0; i < Q; ++i) o.p[i] = w.p[i];
-  return o;
-}
-template <int Q, int P>
-__device__ __forceinline__ Wide<float, Q> first(const Wide<float, P>& w) {
-  return Wide<float, Q>{w.p};
-}
 
 // A matrix in LDS whose rows are fragments' rows, split into parts as it is
 // written.  A row's 16-byte pieces are permuted by the row, so that the sixteen
@@ -695,7 +682,7 @@ template <class E, int KP, Mode MODE>
 struct ChainLds {
   Tile<E, kState, kVB, KP> s;
   Tile<E, kState, kVB, kC> r, wr;
-  Tile<E, kResult, MODE == kOut ? kVB : 1, kC> u;
+  Tile<E, kState, MODE == kOut ? kVB : 1, kC> u;
   Turned<E, KP> kt;
 };
 // The memory's states along a segment's chunks.
@@ -794,8 +781,7 @@ __device__ __forceinline__ void delta_chain(const DeltaP<E>& p, ChainLds<E, KP, 
       mma(ks[f & 1], a, o[f & 1]);
       if constexpr (MODE == kOut) {
         const Wide<E, 1> b[1] = {qf[f]};
-        const Wide<E, kResult> x[NV] = {first<kResult>(o[f & 1][0]), first<kResult>(o[f & 1][1])};
-        mma(qs, b, x);
+        mma(qs, b, o[f & 1]);
       }
     }
 #pragma unroll
@@ -830,11 +816,11 @@ __device__ __forceinline__ void delta_chain(const DeltaP<E>& p, ChainLds<E, KP, 
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
         if (f > me.w / 2) break;
-        Wide<E, kResult> x[NV];
+        Wide<E, kState> x[NV];
 #pragma unroll
         for (int v = 0; v < NV; ++v) x[v] = u.frag(16 * v + l16, f * 32 + g4 * 8);
         loads_first();
-        const Wide<E, kResult> a[1] = {wide<E, kResult>(mf[f])};
+        const Wide<E, kState> a[1] = {wide<E, kState>(mf[f])};
         mma(qs, a, x);
       }
       store_values(frames_of(p.y, at.b, at.h, t0, n), trow, p.T - t0, tcol, p.V, l16, qs[0]);
