@@ -23,9 +23,15 @@
 // each chunk and dR of r; the gradients of q, k, g and beta are then a launch
 // with a workgroup per chunk, from products over the values:
 //   dq^ = e^G dy S^T + (d dy U^T) k^,  dk^ = -beta (e^G dR S^T + (d dR U^T) k^)
-//   + e^(G(end) - G) U D^T + the transposes of these,
-//   dg(i) = sum over j >= i of q^.dq^ + k^.(dk^ as read) - k^.(dk^ as written), with
-//   <S, D> and the writes over the chunk's end,  dbeta = dR.(v - S'^T k^).
+//   + e^(G(end) - G) U D^T + the transposes of these,  dbeta = dR.(v - S'^T k^).
+// A gate's gradient is the sum of what passes it:
+//   dg(m) = sum over j < m <= i of (M o dy U^T - A o dR U^T)(i, j)   frame to frame,
+//   over i >= m of e^G(i) (scale q^.S dy - beta k^.S dR)(i)          from the entering memory,
+//   over j < m of e^(G(end) - G(j)) k^.D U(j),  and e^G(end) <S, D>  over the chunk's end.
+// Each term has the decay e^g(m) in it, so the sum is as exact as its terms
+// however much the gate forgets.  (The differences of q^.dq^ + k^.dk^ as read and
+// k^.dk^ as written add up to the same, but terms that do not pass the gate cancel
+// there: at g = -16 nothing but their rounding was left.)
 // Few heads and a long axis: the chunks are cut into segments.  A segment is an
 // affine map of the memory, so each is run from zero and, with the identity as
 // its memory and nothing written, as a transition; a short chain over the
@@ -70,7 +76,7 @@ constexpr int kStepFrames = 16;  // calls of so few go frame by frame
 // How a call is cut, and the places of its parts in the workspace.
 struct DeltaPlan {
   int64_t chunks, nvb, segs, per;  // nvb: blocks of values, per: chunks of a segment
-  int64_t X, M, XT, vec, S, dS, U, dR, ends, gends, bytes;
+  int64_t X, M, XT, A, vec, S, dS, U, dR, ends, gends, bytes;
 };
 // Whether a call goes frame by frame: a chunk costs its 64 frames, a frame its sums
 // over the memory (32 sequences of 8 heads of 128: 28 us in bf16 and 48 in fp32 for
@@ -380,8 +386,8 @@ struct DeltaP {
   // what is between).
   int Vp;
   // [B H][chunks]: inverse, queries' products with keys [64][64], Vec [kVecs][64];
-  // backward: XT, X transposed, and M transposed in its own place
-  float *X, *M, *XT, *vec;
+  // backward: XT, X transposed, and M and A transposed in their own places
+  float *X, *M, *XT, *A, *vec;
   // backward: states entering and adjoints after a chunk [KP / 4][Vp][4], [16][Vp][4]:
   // a lane's four rows of a product are one store
   float *S, *dS, *U, *dR;
@@ -455,14 +461,14 @@ __global__ __launch_bounds__(kThreads) void k_delta_prepare(DeltaP<E> p) {
   float* Mp = p.M + ci * kC * kC;
 #pragma unroll
   for (int tj = 0; tj < 4; ++tj) {
-    floatx4 kk = {0, 0, 0, 0}, qk = {0, 0, 0, 0};
+    floatx4 kk = {0, 0, 0, 0}, qk = {0, 0, 0, 0}, a = {0, 0, 0, 0};
     floatx4 acc[2][1] = {};
     const int j = 16 * tj + l16;
     if (tj <= w) {
 #pragma unroll
       for (int f = 0; f < NF; ++f) {
-        const Wide<E, 1> a[2] = {kf[f], qf[f]}, o[1] = {kt.frag(j, f * 32 + g4 * 8)};
-        mma(acc, a, o);
+        const Wide<E, 1> both[2] = {kf[f], qf[f]}, o[1] = {kt.frag(j, f * 32 + g4 * 8)};
+        mma(acc, both, o);
       }
       kk = acc[0][0], qk = acc[1][0];
     }
@@ -470,13 +476,14 @@ __global__ __launch_bounds__(kThreads) void k_delta_prepare(DeltaP<E> p) {
     for (int r = 0; r < 4; ++r) {
       const int i = 16 * w + 4 * g4 + r;
       const float d = j <= i ? exp_accurate((gh[i] - gh[j]) + (gl[i] - gl[j])) : 0.f;
-      A[i][j] = j < i ? kk[r] * (rk[i] * rk[j]) * d * bt[i] : 0.f;
+      A[i][j] = a[r] = j < i ? kk[r] * (rk[i] * rk[j]) * d * bt[i] : 0.f;
       qk[r] = j <= i ? qk[r] * (rq[i] * rk[j] * p.scale) * d : 0.f;
     }
     // (the quarter above the diagonal, whose products are left out, is not stored)
     if (w < 2 && tj >= 2) continue;
     if (p.XT) {
       *reinterpret_cast<floatx4*>(Mp + j * kC + 16 * w + 4 * g4) = qk;
+      *reinterpret_cast<floatx4*>(p.A + ci * kC * kC + j * kC + 16 * w + 4 * g4) = a;
     } else {
 #pragma unroll
       for (int r = 0; r < 4; ++r) Mp[(16 * w + 4 * g4 + r) * kC + j] = qk[r];
@@ -1148,8 +1155,8 @@ struct GradLds {
     Tile<E, kGradParts, kC, kC> m[2];
   };
   Turned<E, KP> kt, qt;
-  alignas(16) float vec[kVecs * kC], dots[2][3][kC];
-  float db[kC], over[8];
+  alignas(16) float vec[kVecs * kC], dots[2][5][kC];
+  float db[kC], over[8], cross[8][kC];
 };
 
 // Eight waves: 16 rows (frames) and half the keys' channels each.
@@ -1283,21 +1290,62 @@ __global__ __launch_bounds__(kGradThreads) void k_delta_grads(DeltaP<E> p) {
     const floatx4 rest = load_vec(vec + kRest * kC + rows);
     rootk = load_vec(vec + kRootK * kC + rows);
     rootq = load_vec(vec + kRootQ * kC + rows) * p.scale;
-    floatx4 written = {0, 0, 0, 0};
+    // M (of the second half A), as m lies in the registers
+    const float* const tri = (half ? p.A : p.M) + ci * kC * kC + (uint32_t)(l16 * kC + rows);
+    floatx4 t[4];
+#pragma unroll
+    for (int tj = 0; tj < 4; ++tj)
+      if (tj <= w) t[tj] = load_vec(tri + tj * 16 * kC);
+    // each frame's share of the gates' gradients: reads of the entering memory,
+    // and writes over the chunk's end
+    floatx4 enter = {0, 0, 0, 0}, enterk = {0, 0, 0, 0}, written = {0, 0, 0, 0};
 #pragma unroll
     for (int k = 0; k < NK; ++k) {
       dqz[0][k] *= into;
       dqz[1][k] *= -into;
       wr[0][k] *= rest;
-      written += L.kt.first4(k0 + 16 * k, rows, l16) * wr[0][k];
+      const floatx4 kk = L.kt.first4(k0 + 16 * k, rows, l16);
+      enter += L.qt.first4(k0 + 16 * k, rows, l16) * dqz[0][k];
+      enterk += kk * dqz[1][k];
+      written += kk * wr[0][k];
+    }
+    enter = row_total(enter * rootq + beta * rootk * enterk), written = row_total(written * rootk);
+    if (l16 == 0) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) L.dots[half][3][rows + e] = enter[e], L.dots[half][4][rows + e] = written[e];
     }
     {
-      // over the chunk's end: what the entering state and the chunk's writes have there
-      const floatx4 t = written * rootk;
-      const float over = wave_sum(sd * vec[kInto * kC + kC - 1] + ((t[0] + t[1]) + (t[2] + t[3])));
+      const float over = wave_sum(sd * vec[kInto * kC + kC - 1]);
       if (lane == 0) L.over[wave] = over;
       rv += __shfl_xor(rv, 16, 64), rv += __shfl_xor(rv, 32, 64);
       if (half == 0 && g4 == 0) L.db[row] = rv;
+    }
+    {
+      // frame to frame: a row's sum over the columns before the lane's, added over
+      // the rows from the lane's frame on
+      floatx4 before = {0, 0, 0, 0};
+      float cross = 0.f;
+#pragma unroll
+      for (int tj = 0; tj < 4; ++tj) {
+        if (tj > w) continue;
+        floatx4 x = m[0][tj] * (half ? -t[tj] : t[tj]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = tj < w || l16 <= 4 * g4 + e ? x[e] : 0.f;
+        const floatx4 all = row_total(x);
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float c = x[e];
+          c += dpp<0x111>(c), c += dpp<0x112>(c), c += dpp<0x114>(c), c += dpp<0x118>(c);  // (lanes 1, 2, 4 and 8 before)
+          c = before[e] + dpp<0x111>(c);
+          if (tj < w || l16 <= 4 * g4 + e) sum += c;
+        }
+        before += all;
+        sum = swap_add32(sum, sum);
+        sum = swap_add16(sum, sum);
+        cross = g4 == tj ? sum : cross;
+      }
+      L.cross[wave][lane] = cross;
     }
     // the two triangular matrices by rows, then by columns
 #pragma unroll
@@ -1373,15 +1421,20 @@ __global__ __launch_bounds__(kGradThreads) void k_delta_grads(DeltaP<E> p) {
     kw = (load_vec(&L.dots[0][2][rows]) + load_vec(&L.dots[1][2][rows])) * rootk;
     qdq += q, kdk += beta * kr + kw;
     if (wave == 0) {
-      const float rk = vec[kRootK * kC + lane], bt = vec[kBeta * kC + lane], rq = vec[kRootQ * kC + lane] * p.scale;
-      const float read = (L.dots[0][1][lane] + L.dots[1][1][lane]) * rk;
-      float a = (L.dots[0][0][lane] + L.dots[1][0][lane]) * rq + bt * read - (L.dots[0][2][lane] + L.dots[1][2][lane]) * rk;
+      const float read = (L.dots[0][1][lane] + L.dots[1][1][lane]) * vec[kRootK * kC + lane];
+      float a = L.dots[0][3][lane] + L.dots[1][3][lane], out = L.dots[0][4][lane] + L.dots[1][4][lane];
 #pragma unroll
       for (int k = 1; k < 64; k *= 2) {
-        const float o = __shfl_down(a, k, 64);
-        if (lane + k < 64) a += o;
+        const float later = __shfl_down(a, k, 64), earlier = __shfl_up(out, k, 64);
+        a += lane + k < 64 ? later : 0.f;
+        out += lane >= k ? earlier : 0.f;
       }
-      a += ((L.over[0] + L.over[1]) + (L.over[2] + L.over[3])) + ((L.over[4] + L.over[5]) + (L.over[6] + L.over[7]));
+      out = __shfl_up(out, 1, 64);
+      a += lane > 0 ? out : 0.f;
+      float cross = 0.f, over = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) cross += L.cross[k][lane], over += L.over[k];
+      a += cross + over;
       const int t = t0 + lane;
       if (t < p.T) {
         const bool in = lane < live;
@@ -1541,7 +1594,7 @@ void delta_launch(const dgen_hip_delta& a, bool backward, hipStream_t st) {
   p.Vp = (int)(o.nvb * kVB);
   p.chunks = (int)o.chunks, p.nvb = (int)o.nvb, p.segs = (int)o.segs, p.per = (int)o.per;
   auto at = [&](int64_t off) { return (float*)((char*)a.workspace + off); };
-  p.X = at(o.X), p.M = at(o.M), p.XT = backward ? at(o.XT) : nullptr, p.vec = at(o.vec), p.S = at(o.S), p.dS = at(o.dS), p.U = at(o.U), p.dR = at(o.dR);
+  p.X = at(o.X), p.M = at(o.M), p.XT = backward ? at(o.XT) : nullptr, p.A = at(o.A), p.vec = at(o.vec), p.S = at(o.S), p.dS = at(o.dS), p.U = at(o.U), p.dR = at(o.dR);
   p.ends = at(o.ends), p.gends = at(o.gends);
   const int64_t bh = a.batch * a.heads;
   if (delta_steps(a, backward))

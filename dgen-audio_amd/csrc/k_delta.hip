@@ -56,7 +56,7 @@ DeltaPlan delta_plan(const dgen_hip_delta& a, bool backward) {
   const int64_t n = bh * o.chunks, V = o.nvb * kVB;
   o.X = take(n * kC * kC);
   o.M = take(n * kC * kC);
-  if (backward) o.XT = take(n * kC * kC);
+  if (backward) o.XT = take(n * kC * kC), o.A = take(n * kC * kC);
   o.vec = take(n * kVecs * kC);
   if (backward) {
     o.S = take(n * K * V);

@@ -603,7 +603,7 @@ def gated_delta_rule_backward(dy, q, k, v, g, beta, scale: Optional[float] = Non
     """Gradients of ``gated_delta_rule``; the state counts as given.  Those of
     shared queries and keys are the sums over the heads that share them.  For
     its own length the call keeps the memory's states and their adjoints every
-    64 frames: (2 K + 128) V + 12928 floats a head, K and V rounded up to 32,
+    64 frames: (2 K + 128) V + 17024 floats a head, K and V rounded up to 32,
     64 or 128 and to 32."""
     dev, _, head, ins = _delta_parts(q, k, v, g, beta, scale, normalize, state, lengths)
     r = DeltaGrads(*(torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v, g, beta)))
