@@ -217,8 +217,10 @@ class RecurrentDecoder:
         u, v, ab, g, beta = kept
         t = Q.gated_delta_rule_backward(ds.unflatten(-1, (c.heads, c.inner // c.heads)), *self._heads(v), g, beta, state=memory,
                                         lengths=lengths)
-        da = -t.dg * torch.exp(P[p + "log_A"]) * torch.sigmoid(ab[..., :c.heads] + P[p + "dt_bias"])
-        G[p + "log_A"], G[p + "dt_bias"] = (t.dg * g).sum((0, 1)), da.sum((0, 1))
+        # (a gate that lets nothing through has no gradient, however steep the way to it: -infinity's is not 0 times that)
+        shut = t.dg == 0
+        da = torch.where(shut, 0.0, -t.dg * torch.exp(P[p + "log_A"]) * torch.sigmoid(ab[..., :c.heads] + P[p + "dt_bias"]))
+        G[p + "log_A"], G[p + "dt_bias"] = torch.where(shut, 0.0, t.dg * g).sum((0, 1)), da.sum((0, 1))
         dy, G[p + "ab"] = _mm_grads(torch.cat([da, t.dbeta * beta * (1 - beta)], -1).to(c.dtype), y, P[p + "ab"])
         du, G[p + "conv"], G[p + "conv_bias"] = Q.causal_conv_backward(
             torch.cat([t.dq.flatten(2), t.dk.flatten(2), t.dv.flatten(2)], -1), u, P[p + "conv"], P[p + "conv_bias"],
