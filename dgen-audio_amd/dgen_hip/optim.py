@@ -145,7 +145,12 @@ class AdamW:
 
     @torch.no_grad()
     def step(self, grads: Sequence[torch.Tensor]) -> Optional[torch.Tensor]:
-        """One step; the gradients' norm where it is held to a bound."""
+        """One step; the gradients' norm where it is held to a bound.  A step that
+        is refused does not count."""
         self.count += 1
-        return adamw(self.params, grads, self.exp_avg, self.exp_avg_sq, self.count, self.lr, self.betas, self.eps,
-                     self.weight_decay, self.max_norm, self.copies)
+        try:
+            return adamw(self.params, grads, self.exp_avg, self.exp_avg_sq, self.count, self.lr, self.betas, self.eps,
+                         self.weight_decay, self.max_norm, self.copies)
+        except Exception:
+            self.count -= 1
+            raise
