@@ -130,7 +130,7 @@ def _library() -> ctypes.CDLL:
 class AdamW:
     """AdamW over a model's float32 tensors, in place: their moments, the count
     of steps, and ``copies`` (bfloat16, one for each tensor or None) that are
-    kept equal to the rounded parameters.  The count lies on the device, so a
+    kept equal to the rounded parameters, from the start on.  The count lies on the device, so a
     captured step counts on when it is replayed."""
 
     def __init__(self, params: Sequence[torch.Tensor], lr: float = 1e-3, betas: tuple[float, float] = (0.9, 0.999),
@@ -139,9 +139,23 @@ class AdamW:
         self.params, self.copies = list(params), None if copies is None else list(copies)
         if not self.params:
             raise ValueError("params: no tensors")
+        if self.copies is not None:
+            self._fill()
         self.lr, self.betas, self.eps, self.weight_decay, self.max_norm = lr, betas, eps, weight_decay, max_norm
         self.exp_avg, self.exp_avg_sq = ([torch.zeros_like(p) for p in self.params] for _ in range(2))
         self.count = torch.zeros((), dtype=torch.int64, device=self.params[0].device)
+
+    @torch.no_grad()
+    def _fill(self) -> None:
+        """The copies, for a pass before the first step."""
+        if len(self.copies) != len(self.params):
+            raise ValueError(f"copies: {len(self.params)} tensors expected, got {len(self.copies)}")
+        for k, (p, c) in enumerate(zip(self.params, self.copies)):
+            if c is not None and (not isinstance(c, torch.Tensor) or c.dtype is not torch.bfloat16 or c.shape != p.shape):
+                raise Q._wrong(f"copies[{k}]", c, f"{tuple(p.shape)} {torch.bfloat16}")
+        for p, c in zip(self.params, self.copies):
+            if c is not None:
+                c.copy_(p)
 
     @torch.no_grad()
     def step(self, grads: Sequence[torch.Tensor]) -> Optional[torch.Tensor]:

@@ -31,3 +31,20 @@ def test_a_refused_step_does_not_count(gpu):
         assert int(one.count) == int(two.count) == k + 1
     for x, y in zip((*one.params, *one.exp_avg, *one.exp_avg_sq), (*two.params, *two.exp_avg, *two.exp_avg_sq)):
         assert torch.equal(x, y)
+
+
+def test_copies_are_the_rounded_parameters_from_the_start():
+    """They are what a pass before the first step reads."""
+    p = [torch.linspace(-1, 1, 12).view(3, 4).requires_grad_(), torch.full((), 0.1), torch.zeros(0, 2)]
+    copies = [torch.full(t.shape, 9.0, dtype=torch.bfloat16) for t in p]
+    copies[1] = None
+    optim.AdamW(p, copies=copies)
+    assert torch.equal(copies[0], p[0].detach().bfloat16()) and copies[2].shape == (0, 2)
+
+
+def test_copies_that_do_not_fit_are_refused_and_left():
+    p = [torch.ones(3, 4), torch.ones(5)]
+    for wrong in ([torch.zeros(3, 4), None], [torch.zeros(4, dtype=torch.bfloat16), None], [None], [None, None, None], [3, None]):
+        with pytest.raises(ValueError):
+            optim.AdamW(p, copies=wrong)
+        assert all(not isinstance(t, torch.Tensor) or not t.any() for t in wrong)
