@@ -7,7 +7,9 @@
 // that one launch takes up to kTensors of any size and a captured step keeps
 // them; a workgroup takes 4096 elements of one tensor, all its loads in flight
 // before the first store.  The gradients' norm is a launch before: a sum of
-// squares per workgroup, added in a fixed order.  241 M parameters with bf16
+// squares per workgroup, added in a fixed order, in 64 bits: the squares of
+// gradients past 1e19 are no numbers in 32, and it is such gradients that the
+// bound is for.  241 M parameters with bf16
 // gradients, bounded, and bf16 copies: 6.76 GB in 1.38 ms (4.9 TB/s), the squares
 // 128 us of them, the steps 1.2 ms; 7.8 M of 32 tensors: 233 MB in 51 us.
 #include <cmath>
@@ -34,9 +36,9 @@ struct StepP {
   Tensor t[kTensors];
   uint32_t first[kTensors + 1];  // a tensor's first workgroup
   int count;
-  float b1, c1, b2, c2, decay, lr, rate, root, eps, ln1, ln2, bound;
+  float b1, c1, b2, c2, decay, lr, rate, root, eps, ln1, ln2;
   const int64_t* step;
-  const float* norm;
+  const double* factor;  // of the gradients
 };
 static_assert(sizeof(StepP) <= 4096, "a launch's arguments");
 
@@ -45,7 +47,7 @@ struct SquaresP {
   int64_t n[kSquares];
   uint32_t first[kSquares + 1];
   int count;
-  float* parts;
+  double* parts;
 };
 static_assert(sizeof(SquaresP) <= 4096, "a launch's arguments");
 
@@ -65,7 +67,8 @@ __global__ __launch_bounds__(kThreads) void k_squares(SquaresP a) {
   const int k = tensor_of(a.first, a.count);
   const int64_t at = (int64_t)(blockIdx.x - a.first[k]) * kPer + threadIdx.x * 4;
   const G* g = (const G*)a.g[k];
-  float x[kRuns][4], sum = 0.f;
+  float x[kRuns][4];
+  double sum = 0.0;
 #pragma unroll
   for (int r = 0; r < kRuns; ++r) {
     const int64_t i = at + r * kThreads * 4, left = a.n[k] - i;
@@ -74,27 +77,29 @@ __global__ __launch_bounds__(kThreads) void k_squares(SquaresP a) {
 #pragma unroll
   for (int r = 0; r < kRuns; ++r)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sum = fmaf(x[r][e], x[r][e], sum);
-  sum = wave_sum(sum);
-  __shared__ float red[kThreads / 64];
+    for (int e = 0; e < 4; ++e) sum = fma((double)x[r][e], (double)x[r][e], sum);
+#pragma unroll
+  for (int k = 32; k > 0; k >>= 1) sum += __shfl_xor(sum, k, 64);
+  __shared__ double red[kThreads / 64];
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
   __syncthreads();
   if (threadIdx.x == 0) a.parts[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// The parts' sum in 64 bits (as many as there are 4096 elements), and its root.
-__global__ __launch_bounds__(1024) void k_norm_of_squares(const float* __restrict__ parts, int64_t n,
-                                                          float* __restrict__ norm) {
+// The parts' sum (as many as there are 4096 elements), its root, and what the
+// gradients are multiplied by.
+__global__ __launch_bounds__(1024) void k_norm_of_squares(const double* __restrict__ parts, int64_t n, double bound,
+                                                          float* __restrict__ norm, double* __restrict__ factor) {
   double s = 0.0;
   int64_t i = threadIdx.x;
   for (; i + 7 * 1024 < n; i += 8 * 1024) {  // (eight loads in flight)
-    float x[8];
+    double x[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[k] = parts[i + k * 1024];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) s += (double)x[k];
+    for (int k = 0; k < 8; ++k) s += x[k];
   }
-  for (; i < n; i += 1024) s += (double)parts[i];
+  for (; i < n; i += 1024) s += parts[i];
   __shared__ double red[1024];
   red[threadIdx.x] = s;
   __syncthreads();
@@ -102,10 +107,16 @@ __global__ __launch_bounds__(1024) void k_norm_of_squares(const float* __restric
     if ((int)threadIdx.x < k) red[threadIdx.x] += red[threadIdx.x + k];
     __syncthreads();
   }
-  if (threadIdx.x == 0) *norm = (float)sqrt(red[0]);
+  if (threadIdx.x == 0) {
+    const double root = sqrt(red[0]), f = bound / (root + 1e-6);
+    *norm = (float)root;
+    *factor = f > 1.0 ? 1.0 : f;  // (a norm that is no number spoils all, as in the formula)
+  }
 }
 
-template <class G>
+// BOUND: the gradients are scaled, in 64 bits, as the factor may be below 2^-126
+// (without a bound those multiplications took 56 us where these take 51).
+template <class G, bool BOUND>
 __global__ __launch_bounds__(kThreads) void k_adamw(StepP a) {
   const int k = tensor_of(a.first, a.count);
   const Tensor t = a.t[k];
@@ -117,11 +128,7 @@ __global__ __launch_bounds__(kThreads) void k_adamw(StepP a) {
     rate = a.lr / -expm1f(n * a.ln1);
     root = rsqrtf(-expm1f(n * a.ln2));
   }
-  float factor = 1.f;
-  if (a.norm) {
-    factor = a.bound / (*a.norm + 1e-6f);
-    factor = factor > 1.f ? 1.f : factor;  // (a norm that is no number spoils all, as in the formula)
-  }
+  const double factor = BOUND ? *a.factor : 1.0;
   float p[kRuns][4], g[kRuns][4], m[kRuns][4], v[kRuns][4];
 #pragma unroll
   for (int r = 0; r < kRuns; ++r) {
@@ -138,7 +145,7 @@ __global__ __launch_bounds__(kThreads) void k_adamw(StepP a) {
     const int valid = left > 4 ? 4 : (int)left;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float x = g[r][e] * factor;
+      const float x = BOUND ? (float)((double)g[r][e] * factor) : g[r][e];
       m[r][e] = fmaf(a.c1, x, a.b1 * m[r][e]);
       v[r][e] = fmaf(a.c2, x * x, a.b2 * v[r][e]);
       p[r][e] = fmaf(-rate, m[r][e] / fmaf(sqrtf(v[r][e]), root, a.eps), a.decay * p[r][e]);
@@ -203,8 +210,9 @@ int check_apart(const dgen_hip_adamw& a, const char* name) try {
 
 }  // namespace
 
+// The factor, then the squares' sums.
 int64_t adamw_workspace(const dgen_hip_adamw& a) {
-  return a.max_norm > 0 ? align256(total_groups(a) * (int64_t)sizeof(float)) : 0;
+  return a.max_norm > 0 ? align256((1 + total_groups(a)) * (int64_t)sizeof(double)) : 0;
 }
 
 int adamw_run(const dgen_hip_adamw& a, hipStream_t st, bool dry) {
@@ -253,8 +261,9 @@ int adamw_run(const dgen_hip_adamw& a, hipStream_t st, bool dry) {
     }
   };
   if (a.max_norm > 0) {
+    double *const factor = (double*)a.workspace, *const parts = factor + 1;
     SquaresP q;
-    q.parts = (float*)a.workspace;
+    q.parts = parts;
     runs(
         kSquares, [&](int k, uint32_t at, const dgen_hip_adamw_tensor& t) { q.g[k] = t.grad, q.n[k] = t.n, q.first[k] = at; },
         [&](int k, uint32_t groups) {
@@ -262,7 +271,7 @@ int adamw_run(const dgen_hip_adamw& a, hipStream_t st, bool dry) {
           half ? k_squares<bf16><<<groups, kThreads, 0, st>>>(q) : k_squares<float><<<groups, kThreads, 0, st>>>(q);
           q.parts += groups;
         });
-    k_norm_of_squares<<<1, 1024, 0, st>>>((const float*)a.workspace, q.parts - (float*)a.workspace, a.norm);
+    k_norm_of_squares<<<1, 1024, 0, st>>>(parts, q.parts - parts, a.max_norm, a.norm, factor);
   }
   StepP s;
   s.b1 = (float)a.beta1, s.c1 = (float)(1 - a.beta1), s.b2 = (float)a.beta2, s.c2 = (float)(1 - a.beta2);
@@ -274,7 +283,7 @@ int adamw_run(const dgen_hip_adamw& a, hipStream_t st, bool dry) {
     s.rate = (float)(a.lr / (1 - std::pow(a.beta1, (double)a.step)));
     s.root = (float)(1 / std::sqrt(1 - std::pow(a.beta2, (double)a.step)));
   }
-  s.bound = (float)a.max_norm, s.norm = a.max_norm > 0 ? a.norm : nullptr;
+  s.factor = (const double*)a.workspace;
   runs(
       kTensors,
       [&](int k, uint32_t at, const dgen_hip_adamw_tensor& t) {
@@ -283,7 +292,10 @@ int adamw_run(const dgen_hip_adamw& a, hipStream_t st, bool dry) {
       },
       [&](int k, uint32_t groups) {
         s.count = k;
-        half ? k_adamw<bf16><<<groups, kThreads, 0, st>>>(s) : k_adamw<float><<<groups, kThreads, 0, st>>>(s);
+        if (a.max_norm > 0)
+          half ? k_adamw<bf16, true><<<groups, kThreads, 0, st>>>(s) : k_adamw<float, true><<<groups, kThreads, 0, st>>>(s);
+        else
+          half ? k_adamw<bf16, false><<<groups, kThreads, 0, st>>>(s) : k_adamw<float, false><<<groups, kThreads, 0, st>>>(s);
       });
   DGEN_LAUNCH_CHECK(what);
   return 0;
