@@ -13,6 +13,7 @@ decay and no bound on the gradients' norm.
 from __future__ import annotations
 
 import ctypes
+import operator
 import struct
 from typing import Optional, Sequence
 
@@ -61,6 +62,24 @@ def _table(lists, types, device) -> bytes:
     return b"".join(rows)
 
 
+def _list(x, name: str):
+    try:
+        return None if x is None else list(x)
+    except TypeError:
+        raise ValueError(f"{name}: a list of tensors expected, got {type(x).__name__}") from None
+
+
+def _whole(step) -> int:
+    """A count of steps that the descriptor holds (its size is tested there)."""
+    try:
+        n = int(step) if isinstance(step, float) and step.is_integer() else operator.index(step)
+    except TypeError:
+        n = -1
+    if not 0 <= n < 1 << 63:
+        raise ValueError(f"step {step!r}: a whole number from 1 on, or one int64 on the device, expected")
+    return n
+
+
 def adamw(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avg: Sequence[torch.Tensor],
           exp_avg_sq: Sequence[torch.Tensor], step, lr: float = 1e-3, betas: tuple[float, float] = (0.9, 0.999),
           eps: float = 1e-8, weight_decay: float = 1e-2, max_norm: Optional[float] = None,
@@ -78,10 +97,10 @@ def adamw(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avg
     one) receive the new params rounded, for the next pass.  With ``max_norm`` the gradients are scaled by min(1,
     max_norm / (norm + 1e-6)), and the result is their norm before that, on the
     device; else None."""
-    lists = [None if x is None else list(x) for x in (params, grads, exp_avg, exp_avg_sq, *(out or (params, exp_avg, exp_avg_sq)),
-                                                     copies)]
-    if len(lists) != 8:
+    out = (params, exp_avg, exp_avg_sq) if out is None else _list(out, "out")
+    if len(out) != 3:
         raise ValueError("out: three lists expected")
+    lists = [_list(x, name) for x, name in zip((params, grads, exp_avg, exp_avg_sq, *out, copies), _NAMES)]
     if not lists[0]:
         raise ValueError("params: no tensors")
     Q._type(lists[0][0], "params[0]")
@@ -94,14 +113,20 @@ def adamw(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avg
         if step.dtype is not torch.int64 or step.numel() != 1 or step.device != dev:
             raise Q._wrong("step", step, f"a number, or one int64 on {dev}")
         at, step = step.data_ptr(), 0
-    bound = 0.0 if max_norm is None else float(max_norm)
+    else:
+        step = _whole(step)
+    bound = 0.0 if max_norm is None else Q._number(max_norm, "max_norm")
     if max_norm is not None and not bound > 0:
         raise ValueError(f"max_norm {max_norm}: a positive number expected")
     norm = torch.empty((), dtype=torch.float32, device=dev) if bound else None
+    betas = _list(betas, "betas")
+    if betas is None or len(betas) != 2:
+        raise ValueError("betas: two numbers expected")
+    numbers = [Q._number(x, name) for x, name in zip((lr, *betas, eps, weight_decay), ("lr", "betas[0]", "betas[1]", "eps", "weight_decay"))]
     # (the rows of dgen_hip_adamw_tensor, copies before the number of elements)
     host = ctypes.create_string_buffer(rows, len(rows))
-    d = _ADAMW.pack(_ADAMW_SIZE, types[1], len(lists[0]), ctypes.addressof(host), lr, *betas, eps, weight_decay, bound,
-                    int(step), at, 0 if norm is None else norm.data_ptr())
+    d = _ADAMW.pack(_ADAMW_SIZE, types[1], len(lists[0]), ctypes.addressof(host), *numbers, bound, step, at,
+                    0 if norm is None else norm.data_ptr())
     _run(d, dev, norm is not None)
     return norm
 

@@ -152,6 +152,13 @@ def _wrong(name: str, t, want: str):
     return ValueError(f"{name}: {want} expected, got {got}")
 
 
+def _number(x, name: str) -> float:
+    try:
+        return float(x)
+    except (TypeError, ValueError, OverflowError):
+        raise ValueError(f"{name} {x!r}: a number expected") from None
+
+
 def _type(x, name: str) -> int:
     ty = _TYPES.get(x.dtype) if isinstance(x, torch.Tensor) and x.is_cuda else None
     if ty is None:
@@ -544,7 +551,7 @@ def _delta_parts(q, k, v, g, beta, scale, normalize, state, lengths):
     if keys[:2] != shape[:2]:
         raise _wrong("q", q, f"[{B}][{T}][key head][channel]")
     i, each, states = dev.index, shape[:3], (B, H, K, V)
-    head = (_DELTA_SIZE, ty, 1 if normalize else 0, float(K ** -0.5 if scale is None else scale) if K else 1.0, B, T, G, H, K, V,
+    head = (_DELTA_SIZE, ty, 1 if normalize else 0, (K ** -0.5 if scale is None else _number(scale, "scale")) if K else 1.0, B, T, G, H, K, V,
             dense(lengths, (B,), _INT32, i) or _dense(lengths, "lengths", (B,), torch.int32, dev),
             dense(state, states, _F32, i) or _dense(state, "state", states, f32, dev))
     return dev, states, head, (*(heads(q, keys, ty, i) or _heads(q, "q", keys, et, dev)),
@@ -637,6 +644,8 @@ def _block_parts(x, post_weight, pre_weight, gate, gate_activation, residual_sca
     act = _GATES.get(gate_activation)
     if act is None:
         raise ValueError(f"gate_activation {gate_activation!r}: one of {sorted(_GATES)}")
+    if post_weight is None or pre_weight is None:
+        raise ValueError("post_weight and pre_weight: both are needed")
     i, width, count, each, gp = dev.index, shape[-1:], _count(shape), 1, _NO_ROWS
     if gate is not None:
         its = shape
@@ -644,7 +653,7 @@ def _block_parts(x, post_weight, pre_weight, gate, gate_activation, residual_sca
             # one gate for all the rows of an axis
             each, its = max(1, shape[-2]), (*shape[:-2], 1, shape[-1])
         gp = rows(gate, its, ty, i) or _rows(gate, "gate", its, et, dev)
-    return (_BLOCK_SIZE, ty, st, act, count, shape[-1], each, eps,
+    return (_BLOCK_SIZE, ty, st, act, count, shape[-1], each, _number(eps, "eps"),
             dense(post_weight, width, _F32, i) or _dense(post_weight, "post_weight", width, f32, dev),
             dense(pre_weight, width, _F32, i) or _dense(pre_weight, "pre_weight", width, f32, dev),
             dense(residual_scale, width, _F32, i) or _dense(residual_scale, "residual_scale", width, f32, dev),
