@@ -92,8 +92,11 @@ class RecurrentDecoder:
 
         if cfg.mixer not in ("scan", "delta"):
             raise ValueError(f"mixer {cfg.mixer!r}: one of ['delta', 'scan']")
-        if cfg.mixer == "delta" and (E % cfg.heads or cfg.heads % cfg.key_heads):
-            raise ValueError(f"{E} channels, {cfg.heads} heads, {cfg.key_heads} key heads: each divides the one before")
+        if cfg.mixer == "delta":
+            if min(cfg.heads, cfg.key_heads) < 1 or E % cfg.heads or cfg.heads % cfg.key_heads:
+                raise ValueError(f"{E} channels, {cfg.heads} heads, {cfg.key_heads} key heads: each divides the one before")
+            if not 1 <= cfg.key <= 128 or not 1 <= E // cfg.heads <= 1024:
+                raise ValueError(f"{cfg.key} channels of a key head, {E // cfg.heads} of a head: 1 to 128 and 1 to 1024")
 
         def back(name, k):
             """A branch's projection to the stream; with a gate beside it, a norm
