@@ -254,14 +254,17 @@ class RecurrentDecoder:
             if keep and state is not None:  # (the calls below move it on in place)
                 start = (conv.clone(), memory.clone())
             s, kept = mixer(p, y1, conv, memory, lengths)
-            h2, r0, before = _mm(s, P[p + "out"]), r, h
+            # (what went into a join is kept where its gradient reads it)
+            h2, entering = _mm(s, P[p + "out"]), (h, r) if c.around and branch else (None, None)
             y2, r = self._join(h2, r1, p + "out", p + "norm2")
             g = Q.gated_mlp(y2, P[p + "gate"], P[p + "up"], activation=c.activation)
             h, branch = _mm(g, P[p + "down"]), p + "down"
             if keep:
-                saved.append((before, r0, y1, r1, s, kept, h2, y2, r, g, start))
+                saved.append((*entering, y1, r1, s, kept, h2 if c.around else None, y2, r, g, start))
         y, last = self._join(h, r, branch, "norm")
         Z = _mm(y, P["heads"]).float() + P["heads_bias"]
+        if not c.around:
+            h = r = None
         return (Z, (x, lengths, saved, h, r, y, last)) if keep else Z
 
     def backward(self, dZ, kept) -> dict[str, torch.Tensor]:
