@@ -275,7 +275,7 @@ class RecurrentDecoder:
         G["heads_bias"] = dZ.sum((0, 1))
         dy, G["heads"] = _mm_grads(dZ.to(c.dtype), y, P["heads"])
         # dr: of the stream; dh: of the branch that ends in it
-        dr, dh = self._join_backward(dy, None, h, r, last, f"{c.blocks - 1}.down", "norm", G)
+        dr, dh = self._join_backward(dy, None, h, r, last, f"{c.blocks - 1}.down" if c.blocks else None, "norm", G)
         for i in reversed(range(c.blocks)):
             p = f"{i}."
             before, r0, y1, r1, s, kept, h2, y2, r2, g, (conv, memory) = saved[i]

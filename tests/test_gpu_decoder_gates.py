@@ -1,10 +1,11 @@
-"""The control decoder's delta rule with heads that forget: their decays'
-gradients against the model in 64 bits, up to gates that are -infinity.  Needs a
+"""The control decoder at its ends: heads of the delta rule that forget, their decays'
+gradients against the model in 64 bits up to gates that are -infinity, and no blocks.  Needs a
 GPU."""
 import pytest
 
 torch = pytest.importorskip("torch")
 
+from test_gpu_decoder import norm  # noqa: E402
 from test_gpu_decoder_blocks import F64, small, wide_model  # noqa: E402
 
 pytestmark = pytest.mark.gpu
@@ -34,3 +35,21 @@ def test_heads_that_forget(gpu, log_A, lengths):
     if log_A >= 60.0:
         for i in range(2):
             assert grads[f"{i}.log_A"][1] == 0 and grads[f"{i}.dt_bias"][1] == 0
+
+
+@pytest.mark.parametrize("mixer", ["scan", "delta"])
+@pytest.mark.parametrize("around", [False, True])
+def test_a_decoder_of_no_blocks(gpu, mixer, around):
+    """Two projections and a norm: as the others, within the plain decoder's
+    bound."""
+    from dgen_hip.decoder import DecoderConfig, RecurrentDecoder
+    dec = RecurrentDecoder(DecoderConfig(controls=9, hidden=40, inner=72, blocks=0, dtype=torch.float32, mixer=mixer, around=around, heads=4))
+    x, dZ = torch.randn(2, 5, 2, generator=torch.Generator().manual_seed(1)), torch.randn(2, 5, 9, device="cuda")
+    Z, kept = dec.forward(x, keep=True)
+    grads = dec.backward(dZ, kept)
+    P = {k: v.cpu().to(F64).requires_grad_() for k, v in dec.params.items()}
+    want = norm(x.to(F64) @ P["in"], P["norm"]) @ P["heads"] + P["heads_bias"]
+    assert (Z.cpu().to(F64) - want).abs().max() <= 2e-4 * want.abs().max()
+    (want * dZ.cpu().to(F64)).sum().backward()
+    for k, p in P.items():
+        assert (grads[k].cpu().to(F64) - p.grad).abs().max() <= 2e-4 * p.grad.abs().max() + 1e-9, k
