@@ -37,6 +37,13 @@
 // its memory and nothing written, as a transition; a short chain over the
 // segments' ends gives the memories that enter them (k_delta.hip has when).
 //
+// A number that is not finite may not reach frames that its own does not: 0 times
+// it, above a triangle's diagonal, would.  Each chunk's r (backward dy and dU) is
+// looked through, eight products with 0 a lane; where a column has such a number, it
+// goes on without it, and the rows from that frame on (backward up to it) are made
+// NaN after each triangle.  A key, gate or strength that is none says so by its
+// frame's scale of what the key reads.
+//
 // Chunks of 64 frames: a chunk costs 4 K V 64 operations for the memory, a share
 // that does not depend on its length, and 64 (K + V) a frame within it, which does;
 // at K = V = 128 the two are alike, and its triangles fit next to the memory.  Blocks
@@ -63,6 +70,8 @@
 // with the memory in registers: 32 sequences of 8 heads, fp32, take 10 us for one
 // frame (34 MB: 6.7 us).
 #pragma once
+
+#include <cfloat>
 
 #include "seq.h"
 
@@ -227,6 +236,21 @@ struct Tile {
       for (int q = 0; q < P; ++q) w.p[q] = *reinterpret_cast<const bf16x8*>(&d[q][at(row, col)]);
     }
     return w;
+  }
+  // What four consecutive columns' parts add up to.
+  __device__ __forceinline__ floatx4 whole4(int row, int col) const {
+    const int i = at(row, col);
+    floatx4 x = {0, 0, 0, 0};
+#pragma unroll
+    for (int q = kParts - 1; q >= 0; --q) {
+      if constexpr (kFloat) x = *reinterpret_cast<const floatx4*>(&d[q][i]);
+      else x += __builtin_convertvector(*reinterpret_cast<const bf16x4*>(&d[q][i]), floatx4);
+    }
+    return x;
+  }
+  __device__ __forceinline__ void clear(int row, int col) {
+#pragma unroll
+    for (int q = 0; q < kParts; ++q) d[q][at(row, col)] = (T)0.f;
   }
   // Four consecutive columns of the first part.
   __device__ __forceinline__ floatx4 first4(int row, int col) const {
@@ -400,6 +424,61 @@ __device__ __forceinline__ int live_of(const int32_t* __restrict__ lengths, int 
   return n < 0 ? 0 : n < T ? n : T;
 }
 
+__device__ __forceinline__ bool is_finite(float x) { return fabsf(x) <= FLT_MAX; }
+// A chunk's columns with numbers that are not finite, and from which row on (BACK:
+// up to which, counted from the last).
+template <bool BACK>
+struct Spoilt {
+  alignas(16) int waves[4];
+  int from[4][kVB];
+
+  // Before a barrier: whether a wave's x has any.
+  __device__ __forceinline__ void note(const floatx4 (&x)[2], int w) {
+    float t = 0.f;
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t = fmaf(x[v][e], 0.f, t);
+    waves[w] = __ballot(!(t == 0.f)) != 0;
+  }
+  // After it: the notes, and whether there are any.
+  __device__ __forceinline__ int4 notes() const { return *reinterpret_cast<const int4*>(waves); }
+  static __device__ __forceinline__ bool any(int4 f) { return __builtin_amdgcn_readfirstlane(f.x | f.y | f.z | f.w) != 0; }
+  // If so, which is seldom: 0 in the place of the tile's, which is a
+  // wave's rows rows .. rows + 3 of columns l16 and 16 + l16.  `also`: numbers of
+  // the same rows that are left.
+  template <class E, int P>
+  __device__ __forceinline__ void settle(Tile<E, P, kVB, kC>& tile, const floatx4 (&also)[2], int w, int lane, int rows) {
+    const int l16 = lane & 15;
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      const floatx4 x = tile.whole4(16 * v + l16, rows);
+      int at = kC;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool in = is_finite(x[e]);
+        if (!in || (BACK && !is_finite(also[v][e]))) at = min(at, BACK ? kC - 1 - rows - e : rows + e);
+        if (!in) tile.clear(16 * v + l16, rows + e);
+      }
+      at = min(at, __shfl_xor(at, 16, 64));
+      at = min(at, __shfl_xor(at, 32, 64));
+      if (lane < 16) from[w][16 * v + lane] = at;
+    }
+    lds_barrier();
+  }
+  // x with `with` in the rows that are spoilt.
+  __device__ __forceinline__ void put(floatx4 (&x)[2], float with, int l16, int rows) const {
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      int first = kC;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) first = min(first, from[k][16 * v + l16]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[v][e] = (BACK ? kC - 1 - rows - e : rows + e) >= first ? with : x[v][e];
+    }
+  }
+};
+
 // ------------------------------------------------------------------- prepare
 // Per chunk and head: decays, norms, M and X.
 template <class E, int KP, bool WHOLE>
@@ -407,6 +486,7 @@ __global__ __launch_bounds__(kThreads) void k_delta_prepare(DeltaP<E> p) {
   constexpr int NF = KP / 32;
   __shared__ float A[kC][kC + 4], part[3][16][20];
   __shared__ float gh[kC], gl[kC], bt[kC], rk[kC], rq[kC];
+  __shared__ int bad[kC];  // frames whose row of A is not finite
   __shared__ union {
     Tile<E, 1, kC, KP> kt;
     float X[kC][kC + 4];  // (after the products)
@@ -431,6 +511,7 @@ __global__ __launch_bounds__(kThreads) void k_delta_prepare(DeltaP<E> p) {
     gh[lane] = (float)s;
     gl[lane] = (float)(s - (double)(float)s);
     bt[lane] = on ? p.beta.p[b * p.beta.b + (int64_t)(t0 + lane) * p.beta.t + h] : 0.f;
+    bad[lane] = 0;
   }
   const int row = 16 * w + l16;
   Wide<E, 1> kf[NF], qf[NF];
@@ -476,7 +557,9 @@ __global__ __launch_bounds__(kThreads) void k_delta_prepare(DeltaP<E> p) {
     for (int r = 0; r < 4; ++r) {
       const int i = 16 * w + 4 * g4 + r;
       const float d = j <= i ? exp_accurate((gh[i] - gh[j]) + (gl[i] - gl[j])) : 0.f;
-      A[i][j] = a[r] = j < i ? kk[r] * (rk[i] * rk[j]) * d * bt[i] : 0.f;
+      a[r] = j < i ? kk[r] * (rk[i] * rk[j]) * d * bt[i] : 0.f;
+      if (!is_finite(a[r])) a[r] = 0.f, bad[i] = 1;
+      A[i][j] = a[r];
       qk[r] = j <= i ? qk[r] * (rq[i] * rk[j] * p.scale) * d : 0.f;
     }
     // (the quarter above the diagonal, whose products are left out, is not stored)
@@ -541,7 +624,7 @@ __global__ __launch_bounds__(kThreads) void k_delta_prepare(DeltaP<E> p) {
     float* v = p.vec + ci * kVecs * kC + lane;
     const float into = exp_accurate(gh[lane] + gl[lane]);
     const float rest = exp_accurate((gh[kC - 1] - gh[lane]) + (gl[kC - 1] - gl[lane]));
-    v[kReadK * kC] = into * rk[lane];
+    v[kReadK * kC] = bad[lane] ? NAN : into * rk[lane];
     v[kWriteK * kC] = rest * rk[lane];
     v[kReadQ * kC] = into * rq[lane] * p.scale;
     v[kBeta * kC] = bt[lane];
@@ -691,6 +774,7 @@ struct ChainLds {
   Tile<E, kState, kVB, kC> r, wr;
   Tile<E, kState, MODE == kOut ? kVB : 1, kC> u;
   Turned<E, KP> kt;
+  Spoilt<false> bad;
 };
 // The memory's states along a segment's chunks.
 template <class E, int KP, Mode MODE, bool WHOLE>
@@ -792,26 +876,43 @@ __device__ __forceinline__ void delta_chain(const DeltaP<E>& p, ChainLds<E, KP, 
       }
     }
 #pragma unroll
-    for (int v = 0; v < NV; ++v)
-      r.put4(16 * v + l16, rows, beta * (val[v] - read * (ks[0][0][v] + ks[1][0][v])));
+    for (int v = 0; v < NV; ++v) val[v] = beta * (val[v] - read * (ks[0][0][v] + ks[1][0][v]));
+    L.bad.note(val, me.w);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) r.put4(16 * v + l16, rows, val[v]);
     load(min(c + 1, cl - 1));  // (the next chunk's, in flight through this one's products)
     lds_barrier();
     // U = X r
-    floatx4 U[1][NV] = {};
+    const int4 notes = L.bad.notes();
+    floatx4 U[1][NV];
+    auto solve = [&] {
 #pragma unroll
-    for (int f = 0; f < 2; ++f) {
-      if (f > me.w / 2) break;
-      Wide<E, kState> x[NV];
+      for (int v = 0; v < NV; ++v) U[0][v] = floatx4{0, 0, 0, 0};
 #pragma unroll
-      for (int v = 0; v < NV; ++v) x[v] = r.frag(16 * v + l16, f * 32 + g4 * 8);
-      loads_first();
-      const Wide<E, kState> a[1] = {wide<E, kState>(xf[f])};
-      mma(U, a, x);
+      for (int f = 0; f < 2; ++f) {
+        if (f > me.w / 2) break;
+        Wide<E, kState> x[NV];
+#pragma unroll
+        for (int v = 0; v < NV; ++v) x[v] = r.frag(16 * v + l16, f * 32 + g4 * 8);
+        loads_first();
+        const Wide<E, kState> a[1] = {wide<E, kState>(xf[f])};
+        mma(U, a, x);
+      }
+    };
+    solve();
+    const bool some = L.bad.any(notes);
+    if (some) {
+      L.bad.settle(r, val, me.w, me.lane, rows);
+      solve();
+      L.bad.put(U[0], 0.f, l16, rows);
     }
+    if constexpr (MODE == kOut)
+#pragma unroll
+      for (int v = 0; v < NV; ++v) u.put4(16 * v + l16, rows, U[0][v]);
+    if (some) L.bad.put(U[0], NAN, l16, rows);
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       wr.put4(16 * v + l16, rows, U[0][v] * write);
-      if constexpr (MODE == kOut) u.put4(16 * v + l16, rows, U[0][v]);
       if constexpr (MODE == kKeep)
         *reinterpret_cast<floatx4*>(p.U + ci * kC * p.Vp + (uint32_t)((rows >> 2) * p.Vp + col + 16 * v) * 4) = U[0][v];
     }
@@ -830,6 +931,7 @@ __device__ __forceinline__ void delta_chain(const DeltaP<E>& p, ChainLds<E, KP, 
         const Wide<E, kState> a[1] = {wide<E, kState>(mf[f])};
         mma(qs, a, x);
       }
+      if (some) L.bad.put(qs[0], NAN, l16, rows);
       store_values(frames_of(p.y, at.b, at.h, t0, n), trow, p.T - t0, tcol, p.V, l16, qs[0]);
     }
     // the memory over the chunk's end
@@ -967,6 +1069,7 @@ struct BackLds {
   Tile<E, 1, kVB, kC> dyt;
   Tile<E, kState, kVB, kC> qdy;
   Turned<E, KP> kt, qt;
+  Spoilt<true> bad;
 };
 // The adjoints of the memory's states, against time.  Leaves dv, and dR.
 template <class E, int KP, Mode MODE, bool WHOLE>
@@ -1057,11 +1160,17 @@ __device__ __forceinline__ void delta_back(const DeltaP<E>& p, BackLds<E, KP>& L
     }
 #pragma unroll
     for (int v = 0; v < NV; ++v) U[0][v] = (part[0][0][v] + part[1][0][v]) * write;
+    {
+      const floatx4 both[NV] = {dy[0] + U[0][0], dy[1] + U[0][1]};
+      L.bad.note(both, me.w);
+    }
 #pragma unroll
     for (int f = 0; f < 2; ++f)
       if (f >= me.w / 2) xf[f] = load_row(p.XT + ci * kC * kC + (uint32_t)(row * kC + g4 * 8) + f * 32);
     load(max(c - 1, c0));  // (the next chunk's, in flight through this one's products)
     lds_barrier();
+    const bool some = L.bad.any(L.bad.notes());
+    if (some) L.bad.settle(dyt, U[0], me.w, me.lane, rows);
 #pragma unroll
     for (int f = 0; f < 2; ++f) {
       if (f < me.w / 2) continue;
@@ -1072,6 +1181,7 @@ __device__ __forceinline__ void delta_back(const DeltaP<E>& p, BackLds<E, KP>& L
       const Wide<E, kState> a[1] = {wide<E, kState>(mf[f])};
       mma(U, a, x);
     }
+    if (some) L.bad.put(U[0], 0.f, l16, rows);
 #pragma unroll
     for (int v = 0; v < NV; ++v) du.put4(16 * v + l16, rows, U[0][v]);
     lds_barrier();
@@ -1087,6 +1197,7 @@ __device__ __forceinline__ void delta_back(const DeltaP<E>& p, BackLds<E, KP>& L
       const Wide<E, kState> a[1] = {wide<E, kState>(xf[f])};
       mma(R, a, x);
     }
+    if (some) L.bad.put(R[0], NAN, l16, rows);
 #pragma unroll
     for (int v = 0; v < NV; ++v) dr.put4(16 * v + l16, rows, -R[0][v] * beta * read);
     if constexpr (MODE == kKeep) {

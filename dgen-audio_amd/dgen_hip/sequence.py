@@ -580,8 +580,8 @@ def gated_delta_rule(q, k, v, g, beta, scale: Optional[float] = None, normalize:
     is K^-1/2 unless given.  The states ([batch][heads][K][V]) are float32.
     Products are formed in float32's accuracy for float32, and in that of
     bfloat16's exact values and float32 sums for bfloat16, states as accurate
-    as float32 ones.  A value that is not finite spoils its head's results from
-    up to 63 frames before it on; calls of up to 16 frames go frame by frame."""
+    as float32 ones.  An operand that is not finite spoils its head's results
+    from its frame on, one of v its own column of them, and none before."""
     dev, states, head, ins = _delta_parts(q, k, v, g, beta, scale, normalize, state, lengths)
     B, T, H, V = shape = v.shape
     if out is None:

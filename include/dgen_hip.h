@@ -1021,9 +1021,9 @@ int dgen_hip_block_norm_workspace(int device, const dgen_hip_block_norms* n, int
  * heads of v.  g is at most 0 (-infinity forgets everything; below -128 counts as
  * that), beta between 0 and 2.  S[-1] is `state` ([batch][heads][K][V] fp32) or
  * 0; `state_out` receives the last S (it may be `state` itself).
- * A value that is not finite spoils its head's results from up to 63 frames
- * before it on.  Frames of q, k, v, y and their gradients lie at most 2^23
- * elements apart.
+ * An operand that is not finite spoils its head's results from its frame on, one
+ * of v its own column of them, and none before.  Frames of q, k, v, y and their
+ * gradients lie at most 2^23 elements apart.
  * Backward: the state counts as given, no gradient reaches it, and no gradient
  * enters through state_out. */
 typedef struct dgen_hip_heads { /* [batch][T][heads][channels], contiguous channels */
