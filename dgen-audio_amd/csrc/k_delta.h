@@ -37,8 +37,8 @@
 // its memory and nothing written, as a transition; a short chain over the
 // segments' ends gives the memories that enter them (k_delta.hip has when).
 //
-// A number that is not finite may not reach frames that its own does not: 0 times
-// it, above a triangle's diagonal, would.  Each chunk's r (backward dy and dU) is
+// A number that is not finite may not reach results of frames before its own: 0
+// times it, above a triangle's diagonal, would.  Each chunk's r (backward dy and dU) is
 // looked through, eight products with 0 a lane; where a column has such a number, it
 // goes on without it, and the rows from that frame on (backward up to it) are made
 // NaN after each triangle.  A key, gate or strength that is none says so by its

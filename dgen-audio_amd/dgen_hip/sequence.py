@@ -608,7 +608,9 @@ def gated_delta_rule(q, k, v, g, beta, scale: Optional[float] = None, normalize:
 def gated_delta_rule_backward(dy, q, k, v, g, beta, scale: Optional[float] = None, normalize: bool = True, state=None,
                               lengths=None) -> DeltaGrads:
     """Gradients of ``gated_delta_rule``; the state counts as given.  Those of
-    shared queries and keys are the sums over the heads that share them.  For
+    shared queries and keys are the sums over the heads that share them.  A v
+    that is not finite spoils its head's gradients from its frame on (not dv), a
+    dy those up to its frame (and its own dq), another operand its head's.  For
     its own length the call keeps the memory's states and their adjoints every
     64 frames: (2 K + 128) V + 17024 floats a head, K and V rounded up to 32,
     64 or 128 and to 32."""

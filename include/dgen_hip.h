@@ -1025,7 +1025,9 @@ int dgen_hip_block_norm_workspace(int device, const dgen_hip_block_norms* n, int
  * of v its own column of them, and none before.  Frames of q, k, v, y and their
  * gradients lie at most 2^23 elements apart.
  * Backward: the state counts as given, no gradient reaches it, and no gradient
- * enters through state_out. */
+ * enters through state_out.  A v that is not finite spoils its head's gradients
+ * from its frame on (not dv), a dy those up to its frame (and its own dq), another
+ * operand its head's. */
 typedef struct dgen_hip_heads { /* [batch][T][heads][channels], contiguous channels */
   void* data;
   int64_t stride_b, stride_t, stride_h; /* in elements */
