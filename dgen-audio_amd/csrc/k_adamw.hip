@@ -147,7 +147,7 @@ __global__ __launch_bounds__(kThreads) void k_adamw(StepP a) {
     for (int e = 0; e < 4; ++e) {
       const float x = BOUND ? (float)((double)g[r][e] * factor) : g[r][e];
       m[r][e] = fmaf(a.c1, x, a.b1 * m[r][e]);
-      v[r][e] = fmaf(a.c2, x * x, a.b2 * v[r][e]);
+      v[r][e] = fmaf(a.c2 * x, x, a.b2 * v[r][e]);  // (x^2 alone may be past the largest number)
       p[r][e] = fmaf(-rate, m[r][e] / fmaf(sqrtf(v[r][e]), root, a.eps), a.decay * p[r][e]);
     }
     store_four(t.mo + i, valid, m[r]);

@@ -1,5 +1,5 @@
 """The bound on the gradients' norm (dgen_hip.optim) with gradients whose squares
-32 bits do not hold, against the formula in 64 bits with test_gpu_adamw's
+32 bits do not hold, and second moments of such, against the formula in 64 bits with test_gpu_adamw's
 tolerances.  Needs a GPU."""
 import pytest
 
@@ -41,3 +41,15 @@ def test_a_norm_past_the_largest_number(gpu):
     norm = optim.adamw(p, g, m, v, 3, max_norm=0.5, **ARGS)
     check((p, m, v), want)
     assert torch.isinf(norm) and want[3].to(F64) > torch.finfo(torch.float32).max
+
+
+@pytest.mark.parametrize("step", [1, 50])
+def test_second_moments_near_the_largest_number(gpu, step):
+    """(1 - beta2) g^2 is within 32 bits where g^2 is not."""
+    p, g, m, v = tensors(10, [(300,), (4100,)])
+    for t in g:
+        t[:] = t.sign() * 3e19
+    want = formula(p, g, m, v, step, **ARGS)
+    assert all(torch.isfinite(t.float()).all() for t in want[2]) and 3e19 ** 2 > torch.finfo(torch.float32).max
+    optim.adamw(p, g, m, v, step, **ARGS)
+    check((p, m, v), want)
