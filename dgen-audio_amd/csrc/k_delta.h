@@ -49,7 +49,8 @@
 // at K = V = 128 the two are alike, and its triangles fit next to the memory.  Blocks
 // of 32 values and four waves, two of them a CU: of 64 and eight, one a CU, they
 // read and turn a chunk's keys half as often, and yet wait longer (400 heads of
-// 1000 frames, 128 x 128: 469 against 403 us in bf16, 1264 against 972 in fp32).
+// 1000 frames, 128 x 128, when both were built: 469 against 403 us in bf16, 1264
+// against 972 in fp32).
 //
 // Precision: operands that are bf16 go to the bf16 instructions as they are.
 // Numbers held in 32 bits (memories, adjoints, U, dR, X, M) are split into three
@@ -59,16 +60,17 @@
 // rounded to bf16.  fp32 operands go to the fp32 instructions.
 //
 // What bounds it: 32 x 1000 x 8 heads of K = V = 128 in bf16 read and write 281 MB
-// (55 us at 5.1 TB/s) in 0.25 ms; prepare has 68 and the chain 216 us when profiled.
-// The matrix instructions are busy for a fifth of it, vector instructions (parts,
-// turning) for 45 %; the rest is waits at three barriers a chunk with two
-// workgroups of four waves a CU (73 KB of LDS).  Backward 463 MB (91 us) take
-// 0.90 ms: prepare 75, the two chains 470, gradients 511 us.  The kept memories
-// and adjoints are 0.8 GB more, written and read again; a chain that took the
-// gradients as it goes would need all of V in one workgroup, 256 of them here,
-// and the sums over V in its registers.  A call of few frames goes frame by frame
-// with the memory in registers: 32 sequences of 8 heads, fp32, take 10 us for one
-// frame (34 MB: 6.7 us).
+// (55 us at 5.1 TB/s) in 0.265 ms.  (Launches' own times are the profiler's, under
+// which they take longer than in a run of calls.)  Prepare has 71 us, the chain 231:
+// its vector instructions (parts, turning) issue for 53 % of that, the matrix
+// instructions are busy for 24 %, and of a wave's time a third is waiting for issue
+// and a quarter for memory or one of three barriers a chunk, with two workgroups of
+// four waves a CU (77 KB of LDS).  Backward 463 MB (91 us) take 0.95 ms: prepare 81,
+// the two chains 473, gradients 536 us.  The kept memories and adjoints are 0.8 GB
+// more, written and read again; a chain that took the gradients as it goes would
+// need all of V in one workgroup and the sums over V in its registers, which was
+// not built.  A call of few frames goes frame by frame with the memory in registers:
+// 32 sequences of 8 heads, fp32, take 10 us for one frame (34 MB: 6.7 us).
 #pragma once
 
 #include <cfloat>
@@ -88,8 +90,9 @@ struct DeltaPlan {
   int64_t X, M, XT, A, vec, S, dS, U, dR, ends, gends, bytes;
 };
 // Whether a call goes frame by frame: a chunk costs its 64 frames, a frame its sums
-// over the memory (32 sequences of 8 heads of 128: 28 us in bf16 and 48 in fp32 for
-// a chunk, 1.5 for a frame; 1 sequence of 4 heads of 64: 17 and 19, and 0.8).
+// over the memory (32 sequences of 8 heads of 128: 32 us in bf16 and 50 in fp32 for
+// a chunk, 9 and 1.4 for each frame; 1 sequence of 4 heads of 64: 18 and 20, and 9
+// and 0.6).
 inline bool delta_steps(const dgen_hip_delta& a, bool backward) {
   return !backward && a.T <= kStepFrames;
 }

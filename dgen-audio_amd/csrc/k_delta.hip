@@ -39,9 +39,11 @@ DeltaPlan delta_plan(const dgen_hip_delta& a, bool backward) {
   // too, and each is a step of the carry: three times the work, so that they pay
   // where the card is a third full at most (with 128 channels, whose steps of the
   // carry are dearer, less).  The square root of the chunks balances both walks.
-  // One piece and segments, us, forward, fp32 64 x 64: 1 head of 512 frames 50 and
-  // 34, of 65536 4294 and 186, 24 heads of 1024 89 and 66, of 512 52 and 50; bf16
-  // 128 x 128: 8 heads of 2048 130 and 78, of 512 44 and 50, 24 of 1024 80 and 93.
+  // One piece and segments, us, forward, fp32 64 x 64: 1 head of 512 frames 48 and
+  // 34, of 65536 3990 and 188, 24 heads of 1024 89 and 67, of 512 52 and 51; bf16
+  // 128 x 128: 8 heads of 2048 138 and 85, of 512 46 and 50, 24 of 1024 87 and 98.
+  // The limits do not go by the length: with more heads than these, segments would
+  // pay for far longer clips (11 heads of 65536 frames, 128 x 128: 4221 and 1435).
   const bool wide = K > 64;
   if (bh * o.nvb <= (wide ? 40 : 96) && o.chunks >= (wide ? 12 : 8))
     o.segs = std::min<int64_t>((int64_t)((wide ? 1.5 : 3.) * std::sqrt((double)o.chunks)), 512 / (bh * o.nvb));

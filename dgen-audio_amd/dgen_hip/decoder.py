@@ -302,7 +302,8 @@ def fit(decoder: RecurrentDecoder, x, target, steps: int, lr: float = 1e-3, leng
     may be anything); the losses of the steps.  Parameters are kept in 32 bits
     and rounded to their own type for each pass.  With ``weight_decay`` or
     ``max_norm`` (of all gradients) the steps are those of
-    :class:`dgen_hip.optim.AdamW`."""
+    :class:`dgen_hip.optim.AdamW`, whose decay takes every parameter alike: norms'
+    weights, scales, biases and the mixers' decays and steps too."""
     own = None
     if weight_decay is None and max_norm is None:
         master = {k: v.float().clone().requires_grad_() for k, v in decoder.params.items()}
