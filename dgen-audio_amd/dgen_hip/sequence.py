@@ -574,7 +574,8 @@ def gated_delta_rule(q, k, v, g, beta, scale: Optional[float] = None, normalize:
         S' = exp(g[t]) S[t-1];  S[t] = S' + k^[t] (beta[t] (v[t] - S'^T k^[t]))^T;  y[t] = scale S[t]^T q^[t]
 
     with k^ = k / sqrt(|k|^2 + 1e-6), q^ alike (``normalize`` false: k and q as
-    they are, which keeps S bounded only if the keys' lengths do).  g, the
+    they are, which keeps S bounded only if the keys' lengths do; squares are
+    summed in float32, which holds lengths below 1.8e19).  g, the
     decays' logarithms (at most 0; -inf forgets, and below -128 counts as
     that), and beta (between 0 and 2) are float32 [batch][time][heads]; scale
     is K^-1/2 unless given.  The states ([batch][heads][K][V]) are float32.
@@ -671,6 +672,7 @@ def block_norm(x, post_weight, residual, pre_weight, gate=None, gate_activation:
         s = residual_scale residual + activation(gate) p       the next residual
         y = s / sqrt(mean(s^2) + eps) pre_weight               the next block's input
 
+    Squares are summed in float32, which holds rows of a length below 1.8e19.
     gate has x's type and shape, or 1 in the axis before the last (a clip's
     gate for all its frames); its activation is "sigmoid" or "none".  gate and
     residual_scale [width] may be left out; eps is at least 1e-30.  ``out`` may

@@ -972,7 +972,8 @@ int dgen_hip_gated_mlp_workspace(int device, const dgen_hip_mlp* m, int backward
  * gate is a row for each of the rows, or one for every `gate_rows` of them
  * (a clip's gate for all its frames); act is the logistic function or nothing.
  * gate and scale are optional (left out: 1).  s is stored, rounded to its type,
- * and y is formed from the sum before that rounding.
+ * and y is formed from the sum before that rounding.  Squares are summed in fp32,
+ * which holds rows whose length is below 1.8e19.
  * Backward (dy, ds, x, residual, s, gate -> dx, dresidual, dgate, dpost, dpre,
  * dscale): from the stored s; ds (optional) is the gradient that reaches it from
  * elsewhere. */
@@ -1012,7 +1013,7 @@ int dgen_hip_block_norm_workspace(int device, const dgen_hip_block_norms* n, int
 /* Gated delta rule: a memory S [K][V] per sequence and head that decays, is read
  * with the key, written with what the value differs from that, and read with the
  * query.  With k^ = k / sqrt(|k|^2 + 1e-6), q^ likewise (normalize; else as
- * given):
+ * given; squares are summed in fp32, which holds lengths below 1.8e19):
  *   S'   = exp(g[t]) S[t-1]
  *   u    = beta[t] (v[t] - S'^T k^[t])
  *   S[t] = S' + k^[t] u^T
